@@ -357,6 +357,65 @@ int s2g_attention_bwd(const float* Q, const float* K, const float* V, const floa
                       const float* P, const float* dO, float* dS, float* dQ, float* dK, float* dV, const S2GAttn* dims,
                       void* stream);
 
+/* ---- causal attention over packed sequences, grouped heads (transformer.py of this repository: packed_attention).
+ * Element type of Q, K, V, out and their gradients: 0 fp32 (exact), 1 bf16, 2 fp16; sums in fp32.  Q [q_rows, heads,
+ * dim], K and V [k_rows, kv_heads, dim] with token and head strides in elements (multiples of 16 bytes, 16-byte aligned
+ * bases, dim a multiple of 8 and at most 128, heads / kv_heads at most 128); out, dQ [q_rows, heads, dim] and dK, dV
+ * [k_rows, kv_heads, dim] are contiguous.  Row i of a sequence with n_q queries and n_k keys sees keys j <= i + n_k -
+ * n_q (causal) or all of them; a row that sees none gives zeros and no gradient.  Rows of no sequence are not touched.
+ * The tile list has one entry per 128 rows (token, head of the group) of a sequence: ceil(n_q heads / kv_heads / 128)
+ * of them, in any order; k_tiles one per 128 keys.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
+ * exponentials, for the backward pass (may be NULL in fwd); delta has its size. */
+typedef struct S2GPackedTile {
+  int q_start, q_len, k_start, k_len, tile, pad[3];
+} S2GPackedTile;
+typedef struct S2GPacked {
+  int type, heads, kv_heads, dim, causal;
+  float scale;
+  long q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, do_ld, do_hd, q_rows, k_rows;
+} S2GPacked;
+int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, float* lse, const S2GPackedTile* tiles,
+                             int n_tiles, const S2GPacked* dims, void* stream);
+/* floats of `work` below: the rows of a key tile are dealt to `parts` workgroups (1 .. 64) that each leave a partial sum */
+long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int parts);
+int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
+                             float* delta, void* dQ, void* dK, void* dV, float* work, int parts, const S2GPackedTile* q_tiles,
+                             int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPacked* dims, void* stream);
+
+/* ---- attention of new tokens over a paged cache (paged_attention).  keys, values [pages, page_size, kv_heads, dim] with
+ * the strides below (page_size a power of two, 16 .. 65536); table [sequences, table_cols] int32: the page of tokens
+ * c page_size .. of a sequence; lengths [sequences] int32: tokens in the cache, the new ones among them; starts
+ * [sequences + 1] int32: rows of Q.  Query i of n new tokens sees keys j <= length - n + i (causal) or all.  lengths,
+ * table and starts are read on the device (a captured graph may update them): a length is cut to what the table and
+ * parts * part_keys cover, a page number outside [0, pages) is a page whose keys are absent.  max_new, max_length: upper
+ * bounds known to the host.  Keys are cut into `parts` of part_keys (a multiple of 128); by_rows: 128 rows per workgroup
+ * (chunks) instead of 32 (single tokens).  work: s2g_paged_attention_workspace(dims) floats. */
+typedef struct S2GPaged {
+  int type, sequences, heads, kv_heads, dim, causal, page_size, pages, table_cols, max_new, max_length, part_keys, parts, by_rows;
+  float scale;
+  long q_rows, q_ld, q_hd, page_ld, token_ld, head_ld;
+} S2GPaged;
+long s2g_paged_attention_workspace(const S2GPaged* dims);
+int s2g_paged_attention(const void* Q, const void* keys, const void* values, const int* table, const int* lengths,
+                        const int* starts, void* out, float* work, const S2GPaged* dims, void* stream);
+
+/* ---- rotary positions (apply_rotary): pair i of the first `rotary` features of every head turned by position *
+ * frequencies[i] radians (angles in double) and scaled by multiplier; pairs (2i, 2i + 1) if interleaved, else (i, i +
+ * rotary / 2).  backward: the turn by the negative angle.  q [rows, heads, dim], k [rows, kv_heads, dim] with strides;
+ * q_out, k_out contiguous.  dim at most 256. */
+typedef struct S2GRotary {
+  int type, heads, kv_heads, dim, rotary, interleaved, backward;
+  float multiplier;
+  long rows, q_ld, q_hd, k_ld, k_hd, v_ld, v_hd;
+} S2GRotary;
+int s2g_rotary(const void* q, const void* k, const int* positions, const double* frequencies, void* q_out, void* k_out,
+               const S2GRotary* dims, void* stream);
+/* The same on the way into a paged cache (append_rotary): token i of n new ones stands at position length - n + i; its
+ * turned k and its v are written to that position's page, its turned q to q_out.  Positions without a page are skipped. */
+int s2g_rotary_append(const void* q, const void* k, const void* v, const double* frequencies, void* q_out, void* keys,
+                      void* values, const int* table, const int* lengths, const int* starts, const S2GRotary* dims,
+                      const S2GPaged* paged, void* stream);
+
 /* ---- weight-clipping WGAN variant (reference wgan.py).  Hidden size 64 throughout (wgan.py:50, 96); buffers
  * are [rows, .] with sequence n owning rows [n T, n T + len_n).
  * One LSTM layer over all its steps (nn.LSTM(64, 64, ...) of wgan.py:58, 100): pin [rows, 256] = x W_ih^T + b_ih + b_hh

@@ -1,0 +1,322 @@
+// Attention of the last few tokens of every sequence over its keys and values in a paged cache.
+//
+// Sequence s has lens[s] tokens in the cache, the newest starts[s + 1] - starts[s] of which bring queries; query i of n
+// sees keys j <= len - n + i.  Token t of s lies in page table[s][t >> shift].  Rows are (token, head of the group), as
+// in packed_attention.hip, so the G query heads of a kv head read its keys and values once.
+//
+// Single tokens are bound by reading K and V: a workgroup takes 32 rows and a part of the keys, each wave streams tiles
+// of 32 keys of its own through LDS without ever waiting for the others, and the waves join at the end.  Chunks of new
+// tokens are bound by the products: a workgroup takes 128 rows, its waves share tiles of 64 keys.  Either way a long
+// axis is cut into parts of part_keys keys so that few rows still fill the chip; parts leave (O, m, l) in 32 bits and
+// s2g_k_paged_join adds them in order.  A sequence with a single part is written at once.
+//
+// Lengths and pages come from device memory (a captured decoding loop updates them there), so nothing read from it is
+// trusted: lengths are cut to what the table covers, a page number outside the pool is a page that is not there.
+#include "attn_rows.h"
+#include "paged_attention.h"
+
+struct PagedSeq {
+  int n, len, start, rows;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const int* lens, const int* starts, int s, const PagedDims& dm) {
+  PagedSeq q;
+  const int a = min(max(uniform(starts[s]), 0), (int)dm.q_rows), b = min(max(uniform(starts[s + 1]), a), (int)dm.q_rows);
+  q.start = a;
+  q.n = b - a;
+  q.len = (int)min((long)max(uniform(lens[s]), 0), (long)dm.cols << dm.page_shift);
+  q.len = min(q.len, dm.part_keys * dm.parts);
+  q.rows = min(q.n * dm.by.G, dm.max_rows);
+  return q;
+}
+// keys that the rows [row0, row0 + count) of a sequence see, at most
+__device__ __forceinline__ int keys_seen(const PagedSeq& q, int row, const PagedDims& dm) {
+  if (!dm.causal) return q.len;
+  return max(0, min(q.len, divide(min(row, q.rows - 1), dm.by) + q.len - q.n + 1));
+}
+
+// The page of key k0 + lane, -1 if there is none
+__device__ __forceinline__ int page_of(const int* table, int key, int len, const PagedDims& dm) {
+  int p = -1;
+  if (key < len) p = table[key >> dm.page_shift];
+  return (unsigned)p < (unsigned)dm.pages ? p : -1;
+}
+// One tile of KT keys from k0 on: wave instruction after wave instruction, each within one page (whose 16 tokens or more
+// it never crosses).  Keys beyond the length and of absent pages come as zeros.
+template <typename LT, int WAVES, typename T>
+__device__ __forceinline__ void fetch_pages(char* lds, const T* pool, int page, int k0, int len, const int* off, int wave,
+                                            const PagedDims& dm) {
+#pragma unroll
+  for (int i = 0; i < LT::NI; ++i) {
+    const int r = (i * WAVES + wave) * LT::RPI, pg = __builtin_amdgcn_readlane(page, r);
+    const int n = pg < 0 ? 0 : min(LT::RPI, len - (k0 + r)), in = (k0 + r) & ((1 << dm.page_shift) - 1);
+    const T* p = pool + (n > 0 ? pg * dm.page_ld + in * dm.ld : 0);
+    load_to_lds(buffer_of(p, n > 0 ? (int)(((n - 1) * dm.ld + dm.D) * (long)sizeof(T)) : 0), lds + (i * WAVES + wave) * 1024, off[i], 0);
+  }
+}
+template <typename LT, typename T>
+__device__ __forceinline__ void page_offsets(int* off, int wave, int lane, const PagedDims& dm) {
+#pragma unroll
+  for (int i = 0; i < LT::NI; ++i) {
+    const int c = LT::chunk_of(i, wave, lane);
+    off[i] = c * 16 < dm.D * (int)sizeof(T) ? (int)((lane / LT::CH) * dm.ld * (long)sizeof(T)) + c * 16 : OUT_OF_BUFFER;
+  }
+}
+
+// Where a row's result goes: the output if its sequence has one part, else part `part` of the workspace
+// ([row of all kv heads][part][D] sums, then [row][part] (m, l)).
+struct Joined {
+  float* sums;
+  float* ml;
+};
+__device__ __forceinline__ Joined workspace(float* ws, const PagedDims& dm) {
+  return {ws, ws + (long)dm.Hk * dm.q_rows * dm.by.G * dm.parts * dm.D};
+}
+__device__ __forceinline__ long ws_row(const PagedSeq& q, int kvh, int row, const PagedDims& dm) {
+  return ((long)kvh * dm.q_rows + q.start) * dm.by.G + row;
+}
+
+// --------------------------------------------------------------------------------------------------------- single tokens
+template <typename T, int DP>
+struct KeyTiles {                                              // tiles of 32 keys, one wave's own
+  static constexpr int PITCH = Shape<T, DP>::PITCH;
+  typedef Tile<T, PITCH, 32, 1> LT;
+  static constexpr int NW = 16 * LT::BYTES <= 131072 ? 4 : 2;  // K and V, twice, per wave
+  static constexpr int BYTES = 4 * NW * LT::BYTES;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_keys(
+    const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
+    const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
+  typedef KeyTiles<T, DP> KT;
+  typedef typename KT::LT LT;
+  constexpr int NW = KT::NW, DB = Shape<T, DP>::DB;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int kvh = blockIdx.x % dm.Hk, part = blockIdx.x / dm.Hk, tile = blockIdx.y, s = blockIdx.z;
+  const PagedSeq sq = paged_seq(lens, starts, s, dm);
+  if (tile * 32 >= sq.rows) return;
+  const int seen = keys_seen(sq, tile * 32 + 31, dm);
+  const int lo = part * dm.part_keys, hi = min(seen, lo + dm.part_keys);
+  if (lo >= hi && part > 0) return;
+  const bool alone = seen <= dm.part_keys;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int row = tile * 32 + (lane & 31), rr = min(row, sq.rows - 1);
+  const bool live = row < sq.rows;
+  const int tok = divide(rr, dm.by), head = kvh * dm.by.G + rr - tok * dm.by.G;
+  const int last = live ? (dm.causal ? sq.len - sq.n + tok : sq.len - 1) : -1;
+  const int w_lo = keys_seen(sq, tile * 32, dm) - 1;           // every row sees the keys up to here
+  table += (long)s * dm.cols;
+  const T* kb = keys + kvh * dm.hd;
+  const T* vb = values + kvh * dm.hd;
+
+  int off[LT::NI];
+  page_offsets<LT, T>(off, 0, lane, dm);
+  char* mine = lds + wave * 4 * LT::BYTES;
+  // tiles lo + 32 (wave + NW t), the pages of the one after next on their way with the next
+  int page = page_of(table, lo + 32 * wave + (lane & 31), hi, dm);
+  int k0 = lo + 32 * wave;
+  Rows<T, DP> r;
+  if (k0 < hi) {
+    fetch_pages<LT, 1>(mine, kb, page, k0, hi, off, 0, dm);
+    fetch_pages<LT, 1>(mine + LT::BYTES, vb, page, k0, hi, off, 0, dm);
+  }
+  int next = page_of(table, k0 + 32 * NW + (lane & 31), hi, dm);
+  r.begin(Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq, dm.D, live, half, dm.scale);
+  for (int t = 0; k0 < hi; ++t, k0 += 32 * NW) {
+    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
+    wait_loads();
+    const unsigned absent = (unsigned)__ballot(page < 0 && k0 + (lane & 31) < hi);
+    page = next;
+    if (k0 + 32 * NW < hi) {
+      char* nx = mine + ((t + 1) & 1) * 2 * LT::BYTES;
+      fetch_pages<LT, 1>(nx, kb, page, k0 + 32 * NW, hi, off, 0, dm);
+      fetch_pages<LT, 1>(nx + LT::BYTES, vb, page, k0 + 32 * NW, hi, off, 0, dm);
+      next = page_of(table, k0 + 64 * NW + (lane & 31), hi, dm);
+    }
+    r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
+  }
+  // ---- the waves' results joined: maxima and sums through LDS, then the scaled O
+  float* ml = reinterpret_cast<float*>(lds);                   // [NW][32] (m, l)
+  const float l = both_sum(r.l);
+  __syncthreads();
+  if (half == 0) {
+    ml[(wave * 32 + lane) * 2] = r.m;
+    ml[(wave * 32 + lane) * 2 + 1] = l;
+  }
+  __syncthreads();
+  float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[(w * 32 + (lane & 31)) * 2]);
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float mw = ml[(w * 32 + (lane & 31)) * 2];
+    sum += ml[(w * 32 + (lane & 31)) * 2 + 1] * (mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * r.c));
+  }
+  const float f = r.m == m ? 1.0f : __builtin_amdgcn_exp2f((r.m - m) * r.c);
+  constexpr int PAD = 32 * DB + 4;                             // floats per row
+  float* os = reinterpret_cast<float*>(lds) + NW * 64;
+  store_rows<T, DB>(os + (wave * 32 + (lane & 31)) * PAD, r.o, alone ? (sum == 0.0f ? 0.0f : f / sum) : f, 32 * DB, half, true);
+  const Joined j = workspace(ws, dm);
+  if (!alone && wave == 0 && half == 0 && live) {
+    float* p = j.ml + (ws_row(sq, kvh, row, dm) * dm.parts + part) * 2;
+    p[0] = m;
+    p[1] = sum;
+  }
+  __syncthreads();
+  const int n4 = dm.D >> 2, count = min(32, sq.rows - tile * 32) * n4;
+  for (int e = threadIdx.x; e < count; e += 64 * NW) {
+    const int y = e / n4, d = (e - y * n4) * 4;
+    fx4 a = *reinterpret_cast<const fx4*>(os + y * PAD + d);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      const fx4 b = *reinterpret_cast<const fx4*>(os + (w * 32 + y) * PAD + d);
+      a[0] += b[0]; a[1] += b[1]; a[2] += b[2]; a[3] += b[3];
+    }
+    const int ry = tile * 32 + y;
+    if (alone) {
+      const int tk = divide(ry, dm.by);
+      typename Vec<T>::v4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (T)a[i];
+      *reinterpret_cast<typename Vec<T>::v4*>(out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + ry - tk * dm.by.G) * dm.D + d) = v;
+    } else {
+      *reinterpret_cast<fx4*>(j.sums + (ws_row(sq, kvh, ry, dm) * dm.parts + part) * dm.D + d) = a;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- chunks
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void s2g_k_paged_attn_rows(
+    const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
+    const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
+  typedef Shape<T, DP> S;
+  typedef typename S::LT LT;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int kvh = blockIdx.x % dm.Hk, part = blockIdx.x / dm.Hk, s = blockIdx.z;
+  const PagedSeq sq = paged_seq(lens, starts, s, dm);
+  const int tile = blockIdx.y;
+  if (tile * 128 >= sq.rows) return;
+  const int seen = keys_seen(sq, tile * 128 + 127, dm);
+  const int lo = part * dm.part_keys, hi = min(seen, lo + dm.part_keys);
+  if (lo >= hi && part > 0) return;
+  const bool alone = seen <= dm.part_keys;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int w_row = tile * 128 + 32 * wave, row = w_row + (lane & 31), rr = min(row, sq.rows - 1);
+  const bool live = row < sq.rows;
+  const int tok = divide(rr, dm.by), head = kvh * dm.by.G + rr - tok * dm.by.G;
+  const int last = live ? (dm.causal ? sq.len - sq.n + tok : sq.len - 1) : -1;
+  const int w_lo = keys_seen(sq, w_row, dm) - 1, w_hi = w_row < sq.rows ? keys_seen(sq, w_row + 31, dm) - 1 : -1;
+  table += (long)s * dm.cols;
+  const T* kb = keys + kvh * dm.hd;
+  const T* vb = values + kvh * dm.hd;
+  int off[LT::NI];
+  page_offsets<LT, T>(off, wave, lane, dm);
+
+  const int kl = lane & (S::KT - 1);
+  int k0 = lo, page = page_of(table, k0 + kl, hi, dm);
+  if (k0 < hi) {
+    fetch_pages<LT, 4>(lds, kb, page, k0, hi, off, wave, dm);
+    fetch_pages<LT, 4>(lds + LT::BYTES, vb, page, k0, hi, off, wave, dm);
+  }
+  int next = page_of(table, k0 + S::KT + kl, hi, dm);
+  Rows<T, DP> r;
+  r.begin(Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq, dm.D, live, half, dm.scale);
+  for (int t = 0; k0 < hi; ++t, k0 += S::KT) {
+    const char* kt = lds + (t & 1) * 2 * LT::BYTES;
+    wait_loads();
+    const unsigned long long absent = __ballot(page < 0 && k0 + kl < hi);
+    page = next;
+    __syncthreads();
+    if (k0 + S::KT < hi) {
+      char* nx = lds + ((t + 1) & 1) * 2 * LT::BYTES;
+      fetch_pages<LT, 4>(nx, kb, page, k0 + S::KT, hi, off, wave, dm);
+      fetch_pages<LT, 4>(nx + LT::BYTES, vb, page, k0 + S::KT, hi, off, wave, dm);
+      next = page_of(table, k0 + 2 * S::KT + kl, hi, dm);
+    }
+    if (k0 > w_hi) continue;
+    const bool edge = k0 + S::KT - 1 > min(w_lo, hi - 1);
+    if (absent) {                                              // rare: 32 keys at a time, each with its own bits
+#pragma unroll
+      for (int b = 0; b < S::KB; ++b)
+        r.template step<1>(kt + 32 * b * S::PITCH * (int)sizeof(T), kt + LT::BYTES + 32 * b * S::PITCH * (int)sizeof(T), true,
+                           min(last, hi - 1) - k0 - 32 * b, (unsigned)(absent >> (32 * b)), lane);
+    } else {
+      r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, 0, lane);
+    }
+  }
+  const float l = both_sum(r.l);
+  if (alone) {
+    store_rows<T, S::DB>(out + (((long)sq.start + tok) * dm.H + head) * dm.D, r.o, l == 0.0f ? 0.0f : 1.0f / l, dm.D, half, live);
+  } else {
+    const Joined j = workspace(ws, dm);
+    const long at = ws_row(sq, kvh, rr, dm) * dm.parts + part;
+    store_rows<T, S::DB>(j.sums + at * dm.D, r.o, 1.0f, dm.D, half, live);
+    if (live && half == 0) {
+      j.ml[2 * at] = r.m;
+      j.ml[2 * at + 1] = l;
+    }
+  }
+}
+
+// One wave per row: its parts' sums brought to one maximum and added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void s2g_k_paged_join(const float* __restrict__ ws, const int* __restrict__ lens,
+                                                        const int* __restrict__ starts, T* __restrict__ out, int tile_rows,
+                                                        PagedDims dm) {
+  const int kvh = blockIdx.x % dm.Hk, s = blockIdx.z, lane = threadIdx.x & 63;
+  const int row = (blockIdx.x / dm.Hk) * 4 + uniform(threadIdx.x >> 6);
+  const PagedSeq sq = paged_seq(lens, starts, s, dm);
+  if (row >= sq.rows) return;
+  const int seen = keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm);     // as the row's workgroup saw it
+  const int parts = (seen + dm.part_keys - 1) / dm.part_keys;
+  if (parts <= 1) return;
+  const Joined j = workspace(const_cast<float*>(ws), dm);
+  const long at = ws_row(sq, kvh, row, dm) * dm.parts;
+  const float c = dm.scale * LOG2E;
+  float m = -INFINITY, l = 0.0f;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, j.ml[2 * (at + p)]);
+  float a[2] = {0.0f, 0.0f};
+  for (int p = 0; p < parts; ++p) {
+    const float mp = j.ml[2 * (at + p)], f = mp == m ? 1.0f : __builtin_amdgcn_exp2f((mp - m) * c);
+    l = fmaf(j.ml[2 * (at + p) + 1], f, l);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 64 * i < dm.D) a[i] = fmaf(j.sums[(at + p) * dm.D + lane + 64 * i], f, a[i]);
+  }
+  const int tk = divide(row, dm.by);
+  T* o = out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + row - tk * dm.by.G) * dm.D;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < dm.D) o[lane + 64 * i] = (T)(l == 0.0f ? 0.0f : a[i] / l);
+}
+
+// ----------------------------------------------------------------------------------------------------------------- host
+template <typename T, int DP>
+static int launch_paged(const void* Q, const void* keys, const void* values, const int* table, const int* lens,
+                        const int* starts, void* out, float* ws, int by_rows, const PagedDims& dm, hipStream_t st) {
+  static S2GLdsCap rcap, kcap;
+  const int tile_rows = by_rows ? 128 : 32, tiles = (dm.max_rows + tile_rows - 1) / tile_rows;
+  const dim3 grid((unsigned)dm.Hk * dm.parts, tiles, dm.n);
+  if (by_rows) {
+    const auto kernel = s2g_k_paged_attn_rows<T, DP>;
+    const int bytes = 4 * Shape<T, DP>::LT::BYTES;
+    if (s2g_lds_cap(rcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
+  } else {
+    const auto kernel = s2g_k_paged_attn_keys<T, DP>;
+    typedef KeyTiles<T, DP> KT;
+    const int join = KT::NW * (64 + 32 * (32 * Shape<T, DP>::DB + 4)) * (int)sizeof(float), bytes = KT::BYTES > join ? KT::BYTES : join;
+    if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
+  }
+  if (dm.parts > 1)
+    hipLaunchKernelGGL(s2g_k_paged_join<T>, dim3((unsigned)dm.Hk * ((dm.max_rows + 3) / 4), 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+extern "C" int PACKED_NAME(s2g_launch_paged)(const void* Q, const void* keys, const void* values, const int* table,
+                                             const int* lens, const int* starts, void* out, float* ws, int by_rows,
+                                             PagedDims dm, hipStream_t st) {
+  return PER_DIM(launch_paged, PACKED_T, Q, keys, values, table, lens, starts, out, ws, by_rows, dm, st);
+}

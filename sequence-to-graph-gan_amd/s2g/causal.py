@@ -1,0 +1,484 @@
+"""Host side of the causal-transformer operators: rotary positions, attention over packed sequences with grouped heads
+(and its gradient), and the paged key/value cache that serves single tokens and chunks.  Plans are laid out here from
+lengths the host knows; every product and reduction runs in libs2g kernels (include/s2g.h)."""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from .lib import S2GError, S2GPacked, S2GPaged, S2GRotary, call, get
+from .ops import ptr, stream_ptr
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+TILE = 128                       # rows, or keys, of one workgroup
+
+
+def _device(t: torch.Tensor):
+    """Launches go to the tensors' device, whichever is current."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _check(what: str, **tensors: Optional[torch.Tensor]) -> None:
+    """One GPU, one element type the kernels have."""
+    first = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise S2GError(f"{what}: {name} must be a GPU tensor (MI355X-only implementation, no CPU path)")
+        first = t if first is None else first
+        if t.dtype not in TYPES:
+            raise S2GError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+        if t.dtype != first.dtype or t.device != first.device:
+            raise S2GError(f"{what}: {name} ({t.dtype}, {t.device}) differs from {first.dtype}, {first.device}")
+
+
+def _strides(x: torch.Tensor) -> Tuple[int, int]:
+    """Token and head stride of [tokens, heads, dim]; those of a single token or head are what they would be."""
+    h = x.stride(1) if x.shape[1] > 1 else x.shape[2]
+    return (x.stride(0) if x.shape[0] > 1 else x.shape[1] * h), h
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it whose rows the kernels can fetch in 16-byte units."""
+    unit = 16 // x.element_size()
+    t, h = _strides(x)
+    if x.stride(2) == 1 and t % unit == 0 and h % unit == 0 and x.data_ptr() % 16 == 0 and max(t, h) < 1 << 22:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _dense(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+def _attention_shapes(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise S2GError(f"{what}: q, k and v must be [tokens, heads, dim]")
+    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise S2GError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} must agree, and q {tuple(q.shape)} share their dim")
+    _attention_heads(what, q.shape[1], k.shape[1], q.shape[2])
+
+
+def _attention_heads(what: str, H: int, Hk: int, D: int) -> None:
+    if Hk == 0 or H % Hk or not 1 <= H // Hk <= 128:
+        raise S2GError(f"{what}: {H} query heads must be 1 to 128 times the {Hk} key/value heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise S2GError(f"{what}: head dim must be a multiple of 8, at most 128, got {D}")
+
+
+def _scale(what: str, scale: Optional[float], D: int) -> float:
+    s = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < s < math.inf:
+        raise S2GError(f"{what}: scale must be positive and finite, got {scale}")
+    return s
+
+
+def _on_device(values, device) -> torch.Tensor:
+    """An int32 device copy of host integers, complete on return (any stream may use it)."""
+    if torch.cuda.is_current_stream_capturing():
+        raise S2GError("a batch layout cannot be made inside a graph capture: use it once before")
+    return torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32)).to(device)
+
+
+# ---------------------------------------------------------------------------------------------------------------- rotary
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: int = 4096, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(frequencies [rotary_dim / 2] in radians per position, float64; multiplier) for apply_rotary.
+    scaling, for contexts `factor` times as long as the original_length a model was trained at:
+      None      base^(-2i / rotary_dim)
+      "linear"  every frequency divided by factor
+      "base"    base raised to base factor^(rotary_dim / (rotary_dim - 2)): the slowest pair is stretched by factor, the
+                quickest not at all
+      "ramp"    by how often a pair turns within original_length: at most once, stretched by factor; 32 times or more,
+                left alone; between, blended; multiplier 0.1 log(factor) + 1"""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise S2GError(f"rotary_frequencies: rotary_dim must be even and positive, got {rotary_dim}")
+    if not base > 0 or not factor > 0:
+        raise S2GError("rotary_frequencies: base and factor must be positive")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    f, multiplier = base ** -i, 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "base":
+        if rotary_dim > 2:
+            f = (base * factor ** (rotary_dim / (rotary_dim - 2))) ** -i
+    elif scaling == "ramp":
+        turns = original_length * f / (2 * math.pi)
+        keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
+        f, multiplier = f * keep + f / factor * (1 - keep), 0.1 * math.log(factor) + 1.0
+    elif scaling is not None:
+        raise S2GError(f"rotary_frequencies: scaling must be None, 'linear', 'base' or 'ramp', got {scaling!r}")
+    return f.to(device), multiplier
+
+
+def _rotary_dims(what, q, k, v, frequencies, interleaved, multiplier, backward) -> S2GRotary:
+    D = q.shape[2]
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or frequencies.device != q.device or not frequencies.is_contiguous():
+        raise S2GError(f"{what}: frequencies must be a contiguous float64 vector on {q.device}")
+    if 2 * frequencies.numel() > D or D > 256:
+        raise S2GError(f"{what}: {2 * frequencies.numel()} rotary features of head dim {D} (at most 256)")
+    if not math.isfinite(multiplier):
+        raise S2GError(f"{what}: multiplier must be finite")
+    (ql, qh), (kl, kh), (vl, vh) = (_strides(x) if x is not None else (0, 0) for x in (q, k, v))
+    return S2GRotary(TYPES[q.dtype], q.shape[1], 0 if k is None else k.shape[1], D, 2 * frequencies.numel(), int(interleaved),
+                     int(backward), multiplier, q.shape[0], ql, qh, kl, kh, vl, vh)
+
+
+def _turn(q, k, positions, frequencies, interleaved, multiplier, backward):
+    q, k = _dense(q), None if k is None else _dense(k)
+    dims = _rotary_dims("apply_rotary", q, k, None, frequencies, interleaved, multiplier, backward)
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0]:
+        with _device(q):
+            call("s2g_rotary", ptr(q), ptr(k), ptr(positions), ptr(frequencies), ptr(qo), ptr(ko), ctypes.byref(dims), stream_ptr())
+    return qo, ko
+
+
+class RotaryFn(torch.autograd.Function):
+    """(q, k) turned by their tokens' positions; the gradient is the turn by the negative angles."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, interleaved, multiplier):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (interleaved, multiplier)
+        return _turn(q, k, positions, frequencies, interleaved, multiplier, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        positions, frequencies = ctx.saved_tensors
+        return (*_turn(dq, dk, positions, frequencies, *ctx.how, True), None, None, None, None)
+
+
+def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor,
+                 interleaved: bool = False, multiplier: float = 1.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Turns pair i of the first 2 len(frequencies) features of every head by positions[token] * frequencies[i] radians
+    and scales it by multiplier; further features pass through.  q [tokens, heads, dim], k [tokens, kv heads, dim] or
+    None, fp32 / bf16 / fp16 with any strides; positions int32 [tokens]; pairs are features (2i, 2i + 1) if interleaved,
+    else (i, i + len(frequencies)).  Returns new tensors; differentiable in q and k."""
+    _check("apply_rotary", q=q, k=k)
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise S2GError("apply_rotary: q and k must be [tokens, heads, dim] with the same tokens and dim")
+    if q.shape[1] == 0 or q.shape[2] == 0 or (k is not None and k.shape[1] == 0):
+        raise S2GError("apply_rotary: no heads, or heads without features")
+    if positions.shape != q.shape[:1] or positions.dtype != torch.int32 or positions.device != q.device or not positions.is_contiguous():
+        raise S2GError(f"apply_rotary: positions must be contiguous int32 [{q.shape[0]}] on {q.device}")
+    return RotaryFn.apply(q, k, positions, frequencies, bool(interleaved), float(multiplier))
+
+
+# ----------------------------------------------------------------------------------------------------- packed sequences
+class PackedSequences:
+    """The layout of a batch of sequences that lie one after another: `lengths` tokens each (zeros allowed), and
+    `key_lengths` keys each where those differ (the newest tokens of longer sequences: query i of n sees the first
+    key_length - n + i + 1 keys when causal).  Rows behind the last sequence belong to nobody.
+    starts, positions: int32 device tensors, the first row of every sequence (and the end), and every row's position in
+    its sequence's keys.  Made once per batch, and kept for forward and backward; the work lists of a grouping of heads
+    are laid out when it is first used."""
+
+    def __init__(self, lengths: Sequence[int], device="cuda", key_lengths: Optional[Sequence[int]] = None):
+        q = np.asarray(lengths, dtype=np.int64).reshape(-1)
+        k = q if key_lengths is None else np.asarray(key_lengths, dtype=np.int64).reshape(-1)
+        if q.shape != k.shape or q.size == 0 or q.min() < 0 or k.min() < 0 or q.sum() >= 1 << 30 or k.sum() >= 1 << 30:
+            raise S2GError("PackedSequences: lengths and key_lengths must be as many, not negative, below 2^30 in all")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise S2GError("PackedSequences: needs a GPU device")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.q_len, self.k_len = q, k
+        self.q_start, self.k_start = np.cumsum(q) - q, np.cumsum(k) - k
+        self.rows, self.key_rows = int(q.sum()), int(k.sum())
+        with torch.cuda.device(self.device):
+            self.starts = _on_device(np.append(self.q_start, self.rows), self.device)
+            self.positions = _on_device(np.arange(self.rows) - np.repeat(self.q_start - (k - q), q), self.device)
+        self._lists: Dict[Tuple[int, bool], Tuple[torch.Tensor, torch.Tensor]] = {}
+
+    def _list(self, of: np.ndarray, work: np.ndarray, seq: np.ndarray) -> torch.Tensor:
+        """One entry per tile, the longest first: what remains at the end of the launch is short."""
+        order = np.argsort(-work, kind="stable")
+        seq, tile = seq[order], of[order]
+        entry = np.zeros((seq.size, 8), dtype=np.int32)
+        entry[:, :5] = np.stack([self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile], 1)
+        return _on_device(entry, self.device)
+
+    def tiles(self, group: int, causal: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Work lists of the query and the key side for `group` query heads to a kv head."""
+        got = self._lists.get((group, causal))
+        if got is None:
+            out = []
+            for count in (self.q_len * group, self.k_len):
+                n = -(-count // TILE)
+                seq = np.repeat(np.arange(n.size), n)
+                tile = np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
+                if count is self.k_len:
+                    seen = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) if causal else np.zeros_like(tile)
+                    work = np.maximum(0, self.q_len[seq] - seen)
+                else:
+                    token = (np.minimum((tile + 1) * TILE, count[seq]) - 1) // group
+                    work = np.minimum(self.k_len[seq], token + 1 + (self.k_len - self.q_len)[seq]) if causal else self.k_len[seq]
+                out.append(self._list(tile, work, seq))
+            got = self._lists[group, causal] = (out[0], out[1])
+        return got
+
+
+def _parts_of_rows(n_blocks: int, rows: int) -> int:
+    """Workgroups per key tile of the backward pass: two to a compute unit, each with 8 row tiles or more."""
+    return max(1, min(-(-512 // max(1, n_blocks)), rows // 512, 16))
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, pack, causal, scale):
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        (R, H, D), (M, Hk, _) = q.shape, k.shape
+        G = H // Hk
+        dims = S2GPacked(TYPES[q.dtype], H, Hk, D, int(causal), scale, *_strides(q), *_strides(k), *_strides(v), H * D, D, R, M)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out[pack.rows:].zero_()
+        q_tiles, _ = pack.tiles(G, causal)
+        lse = torch.empty(Hk * R * G, dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad) else None
+        if q_tiles.shape[0]:
+            with _device(q):
+                call("s2g_packed_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(q_tiles), q_tiles.shape[0],
+                     ctypes.byref(dims), stream_ptr())
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.pack, ctx.how = pack, (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, out, lse = ctx.saved_tensors
+        pack, (causal, scale) = ctx.pack, ctx.how
+        (R, H, D), (M, Hk, _) = q.shape, k.shape
+        G, dev = H // Hk, q.device
+        do = _rows16(do)
+        dims = S2GPacked(TYPES[q.dtype], H, Hk, D, int(causal), scale, *_strides(q), *_strides(k), *_strides(v), *_strides(do), R, M)
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+        dq[pack.rows:].zero_()
+        dk[pack.key_rows:].zero_()
+        dv[pack.key_rows:].zero_()
+        q_tiles, k_tiles = pack.tiles(G, causal)
+        parts = _parts_of_rows(k_tiles.shape[0] * Hk, int(pack.q_len.max()) * G)
+        delta = torch.empty(Hk * R * G, dtype=torch.float32, device=dev)
+        work = torch.empty(get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), parts), dtype=torch.float32, device=dev)
+        with _device(q):
+            call("s2g_packed_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk),
+                 ptr(dv), ptr(work) if parts > 1 else None, parts, ptr(q_tiles), q_tiles.shape[0], ptr(k_tiles), k_tiles.shape[0],
+                 ctypes.byref(dims), stream_ptr())
+        return dq, dk, dv, None, None, None
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: PackedSequences, causal: bool = True,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v within every sequence of `pack`, row i of n queries and m keys seeing keys j <= i + m - n
+    (causal) or all of them.  q [tokens, heads, dim], k and v [keys, kv heads, dim], fp32 / bf16 / fp16, query head h
+    reading kv head h // (heads / kv heads); dim a multiple of 8 up to 128; scale: 1 / sqrt(dim).  A row that sees no key
+    gives zeros; rows behind the last sequence give zeros and have no gradient.  Differentiable in q, k and v, with the
+    same bits on every run."""
+    _check("packed_attention", q=q, k=k, v=v)
+    _attention_shapes("packed_attention", q, k, v)
+    if not isinstance(pack, PackedSequences) or pack.device != q.device:
+        raise S2GError(f"packed_attention: pack must be PackedSequences on {q.device}")
+    if q.shape[0] < pack.rows or k.shape[0] < pack.key_rows:
+        raise S2GError(f"packed_attention: the layout needs {pack.rows} queries and {pack.key_rows} keys, got {q.shape[0]} and {k.shape[0]}")
+    if q.shape[0] * q.shape[1] >= 1 << 30 or k.shape[0] >= 1 << 30:
+        raise S2GError("packed_attention: 2^30 rows or more")
+    return PackedAttentionFn.apply(q, k, v, pack, bool(causal), _scale("packed_attention", scale, q.shape[2]))
+
+
+# ---------------------------------------------------------------------------------------------------------- paged cache
+class PagedBatch:
+    """What a step of serving reads: for every sequence its row of the page table (int32 [sequences, columns], column c
+    the page of tokens c * page size ..), its length in the cache with the new tokens counted in, and how many of them are
+    new; the new tokens of all sequences lie one after another, `rows` in all.  table, lengths and starts live on the
+    device and may be rewritten there between launches (a captured decoding loop does `batch.lengths.add_(1)`), up to
+    max_length tokens a sequence; what the host knows is max_new, max_length and rows."""
+
+    def __init__(self, table, lengths: Sequence[int], new_lengths: Sequence[int], max_length: Optional[int] = None, device=None):
+        n, c = np.asarray(new_lengths, dtype=np.int64).reshape(-1), np.asarray(lengths, dtype=np.int64).reshape(-1)
+        if n.shape != c.shape or n.size == 0 or n.size > 65535 or n.min() < 0 or (c < n).any() or c.max() >= 1 << 30 or n.sum() >= 1 << 30:
+            raise S2GError("PagedBatch: lengths must be as many as new_lengths (1 to 65535), and none smaller")
+        if not isinstance(table, torch.Tensor):
+            table = torch.as_tensor(np.asarray(table, dtype=np.int32))
+        if table.dim() != 2 or table.shape[0] != n.size or table.dtype != torch.int32:
+            raise S2GError(f"PagedBatch: table must be int32 [{n.size}, columns]")
+        dev = table.device if table.is_cuda else torch.device(device or "cuda")
+        if dev.type != "cuda":
+            raise S2GError("PagedBatch: needs a GPU device")
+        if torch.cuda.is_current_stream_capturing():
+            raise S2GError("a batch layout cannot be made inside a graph capture")
+        self.table = table.to(dev).contiguous()
+        dev = self.table.device
+        self.lengths, self.starts = _on_device(c, dev), _on_device(np.append(0, np.cumsum(n)), dev)
+        self.sequences, self.rows, self.max_new = n.size, int(n.sum()), int(n.max())
+        self.max_length = int(c.max()) if max_length is None else int(max_length)
+        if self.max_length < c.max():
+            raise S2GError("PagedBatch: max_length is below a length")
+
+
+def _pool(what: str, keys: torch.Tensor, values: torch.Tensor) -> Tuple[int, int, int]:
+    if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or keys.stride(3) != 1:
+        raise S2GError(f"{what}: keys and values must be [pages, page size, kv heads, dim], alike in shape and strides, dim dense")
+    size = keys.shape[1]
+    if size < 16 or size > 65536 or size & (size - 1):
+        raise S2GError(f"{what}: page size must be a power of two, 16 to 65536, got {size}")
+    if keys.shape[0] == 0 or keys.shape[0] >= 1 << 31:
+        raise S2GError(f"{what}: {keys.shape[0]} pages")
+    return keys.stride(0), keys.stride(1), keys.stride(2)
+
+
+def _batch(what: str, batch: PagedBatch, q: torch.Tensor, keys: torch.Tensor) -> None:
+    if not isinstance(batch, PagedBatch) or batch.table.device != q.device:
+        raise S2GError(f"{what}: batch must be a PagedBatch on {q.device}")
+    if q.shape[0] < batch.rows:
+        raise S2GError(f"{what}: the batch has {batch.rows} new tokens, got {q.shape[0]}")
+    if batch.max_length > batch.table.shape[1] * keys.shape[1]:
+        raise S2GError(f"{what}: {batch.max_length} tokens do not fit {batch.table.shape[1]} pages of {keys.shape[1]}")
+    if batch.table.shape[1] * keys.shape[1] >= 1 << 30:
+        raise S2GError(f"{what}: the table covers 2^30 tokens or more")
+
+
+def _no_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise S2GError(f"{what} serves: it has no gradient (call it under torch.no_grad())")
+
+
+def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                  batch: PagedBatch, frequencies: torch.Tensor, interleaved: bool = False, multiplier: float = 1.0) -> torch.Tensor:
+    """The new tokens of a batch on their way into the cache, in one launch: q and k are turned as apply_rotary turns them,
+    by the tokens' positions in their sequences, k and v written to their pages (keys, values: [pages, page size, kv heads,
+    dim], in place), the turned q returned.  A token whose position has no page is not written.  Rows of q behind the
+    batch's come back as zeros.  No two sequences may own a page that both write to."""
+    _check("append_rotary", q=q, k=k, v=v, keys=keys, values=values)
+    _no_grad("append_rotary", q, k, v, keys, values)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or q.shape[1] == 0:
+        raise S2GError("append_rotary: q must be [tokens, heads, dim], k and v [tokens, kv heads, dim]")
+    page_ld, token_ld, head_ld = _pool("append_rotary", keys, values)
+    if tuple(keys.shape[2:]) != tuple(k.shape[1:]) or k.shape[1] == 0:
+        raise S2GError(f"append_rotary: pages hold heads {tuple(keys.shape[2:])}, k has {tuple(k.shape[1:])}")
+    _batch("append_rotary", batch, q, keys)
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    dims = _rotary_dims("append_rotary", q, k, v, frequencies, interleaved, multiplier, False)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out[batch.rows:].zero_()
+    if batch.rows:
+        paged = S2GPaged(sequences=batch.sequences, page_size=keys.shape[1], pages=keys.shape[0], table_cols=batch.table.shape[1],
+                         max_new=batch.max_new, page_ld=page_ld, token_ld=token_ld, head_ld=head_ld)
+        with _device(q):
+            call("s2g_rotary_append", ptr(q), ptr(k), ptr(v), ptr(frequencies), ptr(out), ptr(keys), ptr(values), ptr(batch.table),
+                 ptr(batch.lengths), ptr(batch.starts), ctypes.byref(dims), ctypes.byref(paged), stream_ptr())
+    return out
+
+
+def _cut(batch: PagedBatch, Hk: int, G: int) -> Tuple[bool, int, int]:
+    """(128 rows to a workgroup, keys per part, parts): parts of a long context fill the chip where rows do not."""
+    rows = batch.max_new * G
+    by_rows = rows > 64
+    blocks = batch.sequences * Hk * -(-rows // (TILE if by_rows else 32))
+    parts = max(1, min(512 // blocks, -(-batch.max_length // 512)))
+    keys = max(512, -(-batch.max_length // parts // 128) * 128)
+    return by_rows, keys, max(1, -(-batch.max_length // keys))
+
+
+def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, batch: PagedBatch, causal: bool = True,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of a batch's new tokens (q [tokens, heads, dim]) over what its sequences hold in the cache: query i of n
+    new tokens of a sequence of m sees keys j <= m - n + i (causal) or all m.  One token or thousands per sequence, mixed
+    at will; types, heads and scale as in packed_attention.  A page number outside the pool is a page whose keys are not
+    there; a query without keys gives zeros, and so do rows of q behind the batch's."""
+    _check("paged_attention", q=q, keys=keys, values=values)
+    _no_grad("paged_attention", q, keys, values)
+    page_ld, token_ld, head_ld = _pool("paged_attention", keys, values)
+    if q.dim() != 3 or q.shape[2] != keys.shape[3]:
+        raise S2GError(f"paged_attention: q must be [tokens, heads, {keys.shape[3]}]")
+    (R, H, D), Hk = q.shape, keys.shape[2]
+    _attention_heads("paged_attention", H, Hk, D)
+    unit = 16 // q.element_size()
+    if any(s % unit for s in (page_ld, token_ld, head_ld)) or keys.data_ptr() % 16 or values.data_ptr() % 16 or max(token_ld, head_ld) >= 1 << 22:
+        raise S2GError("paged_attention: pages must start, and be strided, at multiples of 16 bytes")
+    _batch("paged_attention", batch, q, keys)
+    s = _scale("paged_attention", scale, D)
+    if R * H >= 1 << 30:
+        raise S2GError("paged_attention: 2^30 rows or more")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out[batch.rows:].zero_()
+    if batch.rows:
+        q = _rows16(q)
+        by_rows, part_keys, parts = _cut(batch, Hk, H // Hk)
+        dims = S2GPaged(TYPES[q.dtype], batch.sequences, H, Hk, D, int(causal), keys.shape[1], keys.shape[0], batch.table.shape[1],
+                        batch.max_new, batch.max_length, part_keys, parts, int(by_rows), s, R, *_strides(q), page_ld, token_ld, head_ld)
+        work = torch.empty(max(0, get().s2g_paged_attention_workspace(ctypes.byref(dims))), dtype=torch.float32, device=q.device)
+        with _device(q):
+            call("s2g_paged_attention", ptr(q), ptr(keys), ptr(values), ptr(batch.table), ptr(batch.lengths), ptr(batch.starts),
+                 ptr(out), ptr(work) if parts > 1 else None, ctypes.byref(dims), stream_ptr())
+    return out
+
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages of one pool: `keys`, `values` [pages, page size, kv heads, dim].
+    Sequences come and go on the host; `extend` reserves room for new tokens and says where they lie."""
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype=torch.float32, device="cuda"):
+        if num_pages <= 0 or page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+            raise S2GError("PagedKVCache: needs pages, of a power of two of tokens, 16 to 65536")
+        _attention_heads("PagedKVCache", num_kv_heads, num_kv_heads, head_dim)
+        if dtype not in TYPES:
+            raise S2GError(f"PagedKVCache: float32, bfloat16 or float16, got {dtype}")
+        self.keys = torch.empty(num_pages, page_size, num_kv_heads, head_dim, dtype=dtype, device=device)
+        self.values = torch.empty_like(self.keys)
+        self.page_size = page_size
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: Dict[int, List[int]] = {}
+        self._length: Dict[int, int] = {}
+        self._next = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        self._next += 1
+        self._pages[self._next], self._length[self._next] = [], 0
+        return self._next
+
+    def length(self, sequence: int) -> int:
+        return self._length[self._known(sequence)]
+
+    def remove(self, sequence: int) -> None:
+        """Gives a sequence's pages back (to be used again by launches enqueued later on the same stream)."""
+        self._free.extend(reversed(self._pages.pop(self._known(sequence))))
+        del self._length[sequence]
+
+    def _known(self, sequence: int) -> int:
+        if sequence not in self._pages:
+            raise S2GError(f"PagedKVCache: no sequence {sequence}")
+        return sequence
+
+    def extend(self, sequences: Sequence[int], new_lengths: Sequence[int]) -> PagedBatch:
+        """Room for new_lengths[i] more tokens of sequences[i]; the batch of them for append_rotary and paged_attention.
+        Refuses, changing nothing, if the pool has too few pages."""
+        if len(sequences) != len(new_lengths) or len(set(sequences)) != len(sequences) or not sequences or min(new_lengths) < 0:
+            raise S2GError("PagedKVCache.extend: needs different sequences, each with its number of new tokens")
+        lengths = [self._length[self._known(s)] + int(n) for s, n in zip(sequences, new_lengths)]
+        need = [-(-m // self.page_size) - len(self._pages[s]) for s, m in zip(sequences, lengths)]
+        if sum(need) > len(self._free):
+            raise S2GError(f"PagedKVCache.extend: {sum(need)} pages needed, {len(self._free)} free")
+        for s, m, k in zip(sequences, lengths, need):
+            self._pages[s].extend(self._free.pop() for _ in range(k))
+            self._length[s] = m
+        table = np.zeros((len(sequences), max(1, max(len(self._pages[s]) for s in sequences))), dtype=np.int32)
+        for row, s in zip(table, sequences):
+            row[:len(self._pages[s])] = self._pages[s]
+        return PagedBatch(torch.from_numpy(table), lengths, new_lengths, device=self.keys.device)

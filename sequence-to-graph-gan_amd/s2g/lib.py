@@ -38,6 +38,22 @@ class S2GAttn(ctypes.Structure):
     _fields_ = [("N", I), ("H", I), ("T", I), ("D", I), ("ld", L), ("ldo", L), ("scale", F)]
 
 
+class S2GPacked(ctypes.Structure):
+    _fields_ = ([(k, I) for k in ("type", "heads", "kv_heads", "dim", "causal")] + [("scale", F)]
+                + [(k, L) for k in ("q_ld", "q_hd", "k_ld", "k_hd", "v_ld", "v_hd", "do_ld", "do_hd", "q_rows", "k_rows")])
+
+
+class S2GPaged(ctypes.Structure):
+    _fields_ = ([(k, I) for k in ("type", "sequences", "heads", "kv_heads", "dim", "causal", "page_size", "pages",
+                                  "table_cols", "max_new", "max_length", "part_keys", "parts", "by_rows")] + [("scale", F)]
+                + [(k, L) for k in ("q_rows", "q_ld", "q_hd", "page_ld", "token_ld", "head_ld")])
+
+
+class S2GRotary(ctypes.Structure):
+    _fields_ = ([(k, I) for k in ("type", "heads", "kv_heads", "dim", "rotary", "interleaved", "backward")]
+                + [("multiplier", F)] + [(k, L) for k in ("rows", "q_ld", "q_hd", "k_ld", "k_hd", "v_ld", "v_hd")])
+
+
 class S2GLstm64Stack(ctypes.Structure):
     _fields_ = ([("pin0", P)] + [(k, P * 3) for k in ("whh", "wih", "bsum", "gates", "cst", "hout", "mask", "hdrop")]
                 + [("tokens", P), ("tab", P), ("labels", P), ("tabl", P), ("V", I), ("n_classes", I)])
@@ -138,6 +154,13 @@ SIGNATURES = {
     "s2g_add_inplace": [P, P, L, P],
     "s2g_attention_fwd": [P, P, P, P, P, P, P, ctypes.POINTER(S2GAttn), P],
     "s2g_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, ctypes.POINTER(S2GAttn), P],
+    "s2g_packed_attention_fwd": [P, P, P, P, P, P, I, ctypes.POINTER(S2GPacked), P],
+    "s2g_packed_attention_bwd_workspace": [ctypes.POINTER(S2GPacked), I],
+    "s2g_packed_attention_bwd": [P] * 11 + [I, P, I, P, I, ctypes.POINTER(S2GPacked), P],
+    "s2g_paged_attention_workspace": [ctypes.POINTER(S2GPaged)],
+    "s2g_paged_attention": [P] * 8 + [ctypes.POINTER(S2GPaged), P],
+    "s2g_rotary": [P] * 6 + [ctypes.POINTER(S2GRotary), P],
+    "s2g_rotary_append": [P] * 10 + [ctypes.POINTER(S2GRotary), ctypes.POINTER(S2GPaged), P],
     "s2g_graph_features": [P, P, I, I, I, P, P, P, L, P],
     "s2g_graph_features_workspace": [I, I],
     "s2g_stream_create_cu_mask": [P, I, P],
@@ -163,6 +186,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn.restype = ctypes.c_int
     lib.s2g_graph_features_workspace.restype = ctypes.c_long      # a byte count
     lib.s2g_embed_grad_tokens_scratch.restype = ctypes.c_long     # a float count
+    lib.s2g_packed_attention_bwd_workspace.restype = ctypes.c_long
+    lib.s2g_paged_attention_workspace.restype = ctypes.c_long
     return lib
 
 

@@ -1,0 +1,180 @@
+"""Refusals and layouts of the causal-transformer operators that need no GPU: C entry points reject bad arguments before
+any launch, the bindings' structures match the header, batches and caches refuse what cannot be."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SIZES = {"int": 4, "float": 4, "long": 8}
+
+
+def fields(text):
+    """(name, type) of every member of a C structure's body."""
+    out = []
+    for line in re.sub(r"/\*.*?\*/", "", text, flags=re.S).split(";"):
+        line = line.split()
+        if line:
+            out += [(n.strip().split("[")[0], line[0]) for n in " ".join(line[1:]).split(",")]
+    return out
+
+
+@pytest.mark.parametrize("name", ["S2GPacked", "S2GPaged", "S2GRotary"])
+def test_structures_match_the_header(name):
+    from s2g import lib
+    body = {}
+    for path in ("include/s2g.h", "sequence-to-graph-gan_amd/csrc/causal_lib.hip"):
+        text = open(os.path.join(ROOT, path)).read()
+        body[path] = fields(re.search(r"struct %s \{(.*?)\}" % name, text, re.S).group(1))
+    a, b = body.values()
+    assert a == b, "the library's own copy"
+    cls = getattr(lib, name)
+    assert [f for f, _ in a] == [f for f, _ in cls._fields_]
+    for (f, t), (_, c) in zip(a, cls._fields_):
+        assert ctypes.sizeof(c) == SIZES[t], f
+
+
+def packed(**change):
+    from s2g.lib import S2GPacked
+    d = dict(type=1, heads=4, kv_heads=2, dim=64, causal=1, scale=0.125, q_ld=256, q_hd=64, k_ld=128, k_hd=64, v_ld=128, v_hd=64,
+             do_ld=256, do_hd=64, q_rows=10, k_rows=10)
+    d.update(change)
+    return ctypes.byref(S2GPacked(**d))
+
+
+def paged(**change):
+    from s2g.lib import S2GPaged
+    d = dict(type=1, sequences=2, heads=4, kv_heads=2, dim=64, causal=1, page_size=16, pages=8, table_cols=4, max_new=1, max_length=64,
+             part_keys=512, parts=1, by_rows=0, scale=0.125, q_rows=2, q_ld=256, q_hd=64, page_ld=2048, token_ld=128, head_ld=64)
+    d.update(change)
+    return ctypes.byref(S2GPaged(**d))
+
+
+def rotary(**change):
+    from s2g.lib import S2GRotary
+    d = dict(type=1, heads=4, kv_heads=2, dim=64, rotary=64, interleaved=0, backward=0, multiplier=1.0, rows=10, q_ld=256, q_hd=64,
+             k_ld=128, k_hd=64, v_ld=128, v_hd=64)
+    d.update(change)
+    return ctypes.byref(S2GRotary(**d))
+
+
+BAD_HEADS = [dict(type=3), dict(type=-1), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(dim=0), dict(dim=136), dict(dim=12),
+             dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(heads=258, kv_heads=2), dict(q_ld=257),
+             dict(q_hd=1 << 22), dict(q_rows=1 << 30)]
+
+
+def test_c_entry_points_refuse():
+    """Every pointer is a placeholder that is never read: all of these are turned down on the host."""
+    from s2g import lib
+    l, p = lib.load(), 4096
+    for change in BAD_HEADS + [dict(k_ld=4), dict(v_hd=2), dict(do_ld=-8), dict(k_rows=-1)]:
+        assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, packed(**change), None) == -1, change
+        assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, 1, p, 1, p, 1, packed(**change), None) == -1, change
+        assert l.s2g_packed_attention_bwd_workspace(packed(**change), 2) == -1, change
+    for i in (0, 1, 2, 3, 5):
+        args = [p, p, p, p, None, p]
+        args[i] = None
+        assert l.s2g_packed_attention_fwd(*args, 1, packed(), None) == -1, i
+    assert l.s2g_packed_attention_fwd(p + 2, p, p, p, None, p, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 0, packed(), None) == -1
+    assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, None, None) == -1
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, 2, p, 1, p, 1, packed(), None) == -1      # parts, no workspace
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, 65, p, 1, p, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_bwd_workspace(packed(), 3) == 2 * 3 * 10 * 2 * 64 and l.s2g_packed_attention_bwd_workspace(packed(), 1) == 0
+    for change in BAD_HEADS + [dict(sequences=0), dict(sequences=65536), dict(page_size=8), dict(page_size=24), dict(page_size=1 << 17),
+                               dict(pages=0), dict(table_cols=0), dict(table_cols=1 << 26), dict(max_new=0), dict(max_new=3),
+                               dict(part_keys=0), dict(part_keys=100), dict(parts=0), dict(parts=5000), dict(max_length=600), dict(token_ld=3),
+                               dict(head_ld=1), dict(page_ld=5)]:
+        assert l.s2g_paged_attention(p, p, p, p, p, p, p, p, paged(**change), None) == -1, change
+        assert l.s2g_paged_attention_workspace(paged(**change)) == -1, change
+    for i in range(7):
+        args = [p] * 8
+        args[i] = None
+        assert l.s2g_paged_attention(*args, paged(), None) == -1, i
+    assert l.s2g_paged_attention(p, p, p, p, p, p, p, None, paged(parts=2), None) == -1
+    assert l.s2g_paged_attention_workspace(paged(parts=2)) == 2 * 4 * 2 * 66 and l.s2g_paged_attention_workspace(paged()) == 0
+    for change in (dict(type=5), dict(rows=0), dict(rows=1 << 31), dict(heads=-1), dict(heads=0, kv_heads=0), dict(dim=0), dict(dim=257),
+                   dict(rotary=63), dict(rotary=66), dict(rotary=-2), dict(multiplier=float("inf")), dict(multiplier=float("nan"))):
+        assert l.s2g_rotary(p, p, p, p, p, p, rotary(**change), None) == -1, change
+        assert l.s2g_rotary_append(p, p, p, p, p, p, p, p, p, p, rotary(**change), paged(), None) == -1, change
+    for i in range(6):
+        args = [p] * 6
+        args[i] = None
+        assert l.s2g_rotary(*args, rotary(), None) == -1, i
+    for i in range(10):
+        args = [p] * 10
+        args[i] = None
+        assert l.s2g_rotary_append(*args, rotary(), paged(), None) == -1, i
+    for change in (dict(sequences=0), dict(page_size=15), dict(pages=0), dict(table_cols=0), dict(max_new=0), dict(max_new=11)):
+        assert l.s2g_rotary_append(*[p] * 10, rotary(), paged(**change), None) == -1, change
+
+
+def test_cpu_tensors_are_refused():
+    import transformer as M
+    from s2g.lib import S2GError
+    x = torch.zeros(4, 2, 32)
+    freq, _ = M.rotary_frequencies(32, device="cpu")
+    with pytest.raises(S2GError):
+        M.apply_rotary(x, x, torch.zeros(4, dtype=torch.int32), freq)
+    with pytest.raises(S2GError):
+        M.packed_attention(x, x, x, None)
+    with pytest.raises(S2GError):
+        M.paged_attention(x, x[None], x[None], None)
+    with pytest.raises(S2GError):
+        M.append_rotary(x, x, x, x[None], x[None], None, freq)
+    with pytest.raises(S2GError):
+        M.PackedSequences([3], "cpu")
+    for bad in ([], [-1], [1 << 30]):
+        with pytest.raises(S2GError):
+            M.PackedSequences(bad, "cuda:0")
+    with pytest.raises(S2GError):
+        M.PackedSequences([1, 2], "cuda:0", [1])
+    for lengths, new in (([], []), ([1], [2]), ([1, 2], [1]), ([3], [-1]), ([1 << 30], [1])):
+        with pytest.raises(S2GError):
+            M.PagedBatch(torch.zeros(1, 1, dtype=torch.int32), lengths, new)
+    with pytest.raises(S2GError):
+        M.PagedBatch(torch.zeros(2, 1, dtype=torch.int32), [1], [1])
+    for bad in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=4, base=0.0), dict(rotary_dim=4, factor=0.0), dict(rotary_dim=4, scaling="other")):
+        with pytest.raises(S2GError):
+            M.rotary_frequencies(**bad, device="cpu")
+    for bad in ((5, 2, None), (8, 3, 2), (8, 4, 3), (8, 4, 0)):
+        with pytest.raises(S2GError):
+            M.GroupedQueryAttention(*bad)
+
+
+def test_cache_bookkeeping():
+    """Pages are reserved on the host; the batch itself needs a GPU, so it is looked at before it is made."""
+    from s2g import causal
+    from s2g.lib import S2GError
+    made = []
+    whole, causal.PagedBatch = causal.PagedBatch, lambda table, lengths, new, device=None: made.append((table, lengths, new))
+    try:
+        cache = causal.PagedKVCache(6, 16, 2, 32, device="cpu")
+        a, b = cache.add(), cache.add()
+        cache.extend([a, b], [17, 0])
+        assert cache.free_pages == 4 and cache.length(a) == 17 and made[-1][0].shape == (2, 2)
+        cache.extend([b, a], [16, 15])
+        assert cache.free_pages == 3 and made[-1][1] == [16, 32]
+        cache.extend([a], [1])
+        assert cache.free_pages == 2
+        with pytest.raises(S2GError):
+            cache.extend([a, b], [16, 32])
+        assert cache.free_pages == 2 and cache.length(a) == 33 and cache.length(b) == 16
+        pages = set(made[-1][0].flatten().tolist())
+        cache.remove(a)
+        assert cache.free_pages == 5
+        c = cache.add()
+        cache.extend([c], [80])
+        assert cache.free_pages == 0 and pages <= set(made[-1][0].flatten().tolist())
+        for bad in (([a], [1]), ([b, b], [1, 1]), ([b], [1, 2]), ([b], [-1]), ([], [])):
+            with pytest.raises(S2GError):
+                cache.extend(*bad)
+        for bad in ((0, 16, 2, 32), (4, 8, 2, 32), (4, 24, 2, 32), (4, 16, 2, 12), (4, 16, 0, 32)):
+            with pytest.raises(S2GError):
+                causal.PagedKVCache(*bad, device="cpu")
+        with pytest.raises(S2GError):
+            causal.PagedKVCache(4, 16, 2, 32, dtype=torch.float64, device="cpu")
+    finally:
+        causal.PagedBatch = whole

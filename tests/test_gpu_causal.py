@@ -1,0 +1,465 @@
+"""Rotary positions, attention over packed sequences and over a paged cache, on the GPU, against 64-bit definitions with
+element-wise bounds (tests/causal_reference.py)."""
+import math
+
+import pytest
+import torch
+
+import causal_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+name = lambda t: str(t).split(".")[-1]  # noqa: E731
+
+
+def rand(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+# ------------------------------------------------------------------------------------------------------------- packed
+SHAPES = [(4, 4, 16), (4, 2, 64), (3, 1, 80), (8, 2, 128), (6, 2, 96), (12, 1, 32), (1, 1, 8), (5, 5, 72)]
+LENGTHS = [
+    ([1], None), ([0, 1, 0, 2], None), ([31, 32, 33], None), ([127, 128, 129, 65], None), ([300, 7, 511], None),
+    ([5, 40, 0, 3], [70, 40, 9, 200]),             # new tokens of longer sequences; one of none
+    ([50, 130, 9], [20, 129, 0]),                  # rows that see no key at all
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_packed_attention_and_gradient(dtype, shape, lengths):
+    import transformer as M
+    H, Hk, D = shape
+    n, m = lengths[0], lengths[1] or lengths[0]
+    g = gen(hash((H, Hk, D, sum(n), sum(m))) & 0xffff)
+    pack = M.PackedSequences(n, DEV, None if lengths[1] is None else m)
+    for causal in (True, False):
+        q, k, v, do = (rand(g, r, h, D, dtype=dtype) for r, h in ((sum(n), H), (sum(m), Hk), (sum(m), Hk), (sum(n), H)))
+        for x in (q, k, v):
+            x.requires_grad_()
+        out = M.packed_attention(q, k, v, pack, causal=causal)
+        want = ref.packed(q.detach(), k.detach(), v.detach(), n, m, causal, 1 / math.sqrt(D), do)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        for what, got, w in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), want):
+            ref.within(got, w, f"{what} causal={causal}")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_packed_attention_long(dtype):
+    """More than one part on the key side, many tiles, scores far from zero and a scale of its own."""
+    import transformer as M
+    g, n, (H, Hk, D) = gen(5), [2500, 17, 1100], (8, 1, 64)
+    q, do = rand(g, sum(n), H, D, dtype=dtype), rand(g, sum(n), H, D, dtype=dtype)
+    k, v = (3 * rand(g, sum(n), Hk, D, dtype=dtype) for _ in range(2))
+    k[::97] *= 4                                   # maxima that move late in a row
+    for x in (q, k, v):
+        x.requires_grad_()
+    pack = M.PackedSequences(n, DEV)
+    out = M.packed_attention(q, k, v, pack, scale=0.2)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    for what, got, w in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref.packed(q.detach(), k.detach(), v.detach(), n, n, True, 0.2, do)):
+        ref.within(got, w, what)
+    again = torch.autograd.grad(M.packed_attention(q, k, v, pack, scale=0.2), (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again)), "the same bits on every run"
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_packed_attention_views_and_rows_behind(dtype):
+    """Parts of one projection, transposed heads, a misaligned slice and a shared (expanded) key; what lies behind the
+    last sequence, NaN here, reaches nothing, and has no gradient."""
+    import transformer as M
+    g, n, (H, Hk, D) = gen(6), [40, 150], (4, 2, 32)
+    rows = sum(n) + 9
+    qkv = rand(g, rows, (H + 2 * Hk) * D, dtype=dtype)
+    qkv[sum(n):] = math.nan
+    do = rand(g, rows, H, D, dtype=dtype)
+    do[sum(n):] = math.nan
+    pack = M.PackedSequences(n, DEV)
+    odd = torch.empty(rows * Hk * D + 1, dtype=dtype, device=DEV)[1:].view(rows, Hk, D).copy_(qkv[:, (H + Hk) * D:].reshape(rows, Hk, D))
+    views = {
+        "projection": [x.unflatten(1, (-1, D)) for x in qkv.split([H * D, Hk * D, Hk * D], 1)],
+        "transposed": [x.unflatten(1, (-1, D)).transpose(0, 1).contiguous().transpose(0, 1) for x in qkv.split([H * D, Hk * D, Hk * D], 1)],
+        "misaligned": [qkv[:, :H * D].unflatten(1, (-1, D)), odd, odd],
+        "inner stride": [x.unflatten(1, (-1, D)).transpose(1, 2).contiguous().transpose(1, 2) for x in qkv.split([H * D, Hk * D, Hk * D], 1)],
+    }
+    for what, (q, k, v) in views.items():
+        q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+        out = M.packed_attention(q, k, v, pack)
+        grads = torch.autograd.grad(out, (q, k, v), do.transpose(0, 1).contiguous().transpose(0, 1) if what == "transposed" else do)
+        live = [x.detach()[:sum(n)] for x in (q, k, v)]
+        for name_, got, w in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref.packed(*live, n, n, True, 1 / math.sqrt(D), do[:sum(n)])):
+            ref.within(got[:sum(n)], w, f"{what} {name_}")
+            assert (got[sum(n):] == 0).all(), f"{what} {name_} behind the last sequence"
+    # one key head broadcast to two: the gradient of the shared one is the sum
+    one = rand(g, rows, 1, D, dtype=dtype)
+    q = views["projection"][0].detach()
+    leaf = one.clone().requires_grad_()
+    out = M.packed_attention(q, leaf.expand(rows, 2, D), leaf.expand(rows, 2, D), pack)
+    (got,) = torch.autograd.grad(out, leaf, do)
+    a = ref.packed(q[:sum(n)], one[:sum(n)].expand(-1, 2, -1), one[:sum(n)].expand(-1, 2, -1), n, n, True, 1 / math.sqrt(D), do[:sum(n)])
+    value, bound = (a[2][i] + a[3][i] for i in range(2))
+    # autograd adds dk to dv and then the two heads, in the inputs' type: three more roundings of the parts' sizes
+    parts = (a[2][0].abs() + a[3][0].abs()).sum(1, keepdim=True)
+    ref.within(got[:sum(n)], (value.sum(1, keepdim=True), bound.sum(1, keepdim=True) + 4 * ref.U[dtype] * parts), "shared head")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_packed_attention_gradient_against_differences(dtype):
+    import transformer as M
+    g, n, (H, Hk, D) = gen(7), [70, 33], (4, 2, 32)
+    q, k, v, do, dq_, dk_, dv_ = (rand(g, sum(n), h, D, dtype=dtype) for h in (H, Hk, Hk, H, H, Hk, Hk))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    pack = M.PackedSequences(n, DEV)
+    grads = torch.autograd.grad(M.packed_attention(*leaves, pack), leaves, do)
+    along = sum(float((a.double() * b.double()).sum()) for a, b in zip(grads, (dq_, dk_, dv_)))
+    e = 1e-4
+
+    def loss(sign):
+        moved = [x.detach().double() + sign * e * y.double() for x, y in zip(leaves, (dq_, dk_, dv_))]
+        return float((ref.packed(*moved, n, n, True, 1 / math.sqrt(D))[0][0] * do.double()).sum())
+
+    difference = (loss(1) - loss(-1)) / (2 * e)
+    # the three gradients' own bounds along the direction, and the difference's cut-off term (third derivatives ~ 1e2)
+    bounds = ref.packed(q.detach(), k.detach(), v.detach(), n, n, True, 1 / math.sqrt(D), do)[1:]
+    slack = sum(float((b[1] * y.double().abs()).sum()) for b, y in zip(bounds, (dq_, dk_, dv_)))
+    size = sum(float((b[0].abs() * y.double().abs()).sum()) for b, y in zip(bounds, (dq_, dk_, dv_)))
+    assert abs(along - difference) <= slack + 1e-6 * size, (along, difference, slack)
+
+
+def test_packed_attention_captured():
+    """Forward and backward in a graph, replayed with new inputs between eager work, on a stream of their own."""
+    import transformer as M
+    n, (H, Hk, D) = [300, 45, 129], (8, 1, 64)
+    pack = M.PackedSequences(n, DEV)
+    g = gen(8)
+    q, k, v, do = (rand(g, sum(n), h, D, dtype=torch.bfloat16) for h in (H, Hk, Hk, H))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def both():
+        out = M.packed_attention(*leaves, pack)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for turn in range(3):
+        with torch.no_grad():
+            for x in (q, k, v, do):
+                x.copy_(rand(g, *x.shape, dtype=x.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        for a, b in zip(got, both()):
+            assert torch.equal(a, b), turn
+
+
+# -------------------------------------------------------------------------------------------------------------- paged
+def cache_of(g, context, page, Hk, D, dtype, spare=3):
+    need = [-(-c // page) for c in context]
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=g, device=DEV).tolist()
+    table = torch.zeros(len(context), max(1, max(need)), dtype=torch.int32)
+    for i, m in enumerate(need):
+        table[i, :m] = torch.tensor(order[:m], dtype=torch.int32)
+        order = order[m:]
+    keys, values = (rand(g, pages, page, Hk, D, dtype=dtype) for _ in range(2))
+    return keys, values, table.to(DEV)
+
+
+def rows_of(pool, table, c):
+    return pool[table.long()].flatten(0, 1)[:c]
+
+
+def check_paged(q, keys, values, table, context, new, causal, scale, got):
+    H, Hk = q.shape[1], keys.shape[2]
+    r = 0
+    for i, (n, c) in enumerate(zip(new, context)):
+        k, v = rows_of(keys, table[i], c), rows_of(values, table[i], c)
+        for h in range(H):
+            (w,) = ref.head(q[r:r + n, h], k[:, h // (H // Hk)], v[:, h // (H // Hk)], c - n, causal, scale, q.dtype)
+            # parts and waves add their sums: a few more fp32 roundings of the sum of sizes, inside (m + 4) STEP
+            ref.within(got[r:r + n, h], w, f"sequence {i} head {h}")
+        r += n
+
+
+CONTEXTS = [
+    ([1], [1]), ([1, 1, 1], [1, 17, 777]), ([1, 0, 1], [5000, 40, 0 + 1]), ([3, 1, 16], [64, 1000, 16]),
+    ([40, 5, 200], [40, 3000, 517]), ([129, 1], [1300, 1025]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (8, 1, 64), (8, 2, 128), (6, 2, 96), (3, 1, 40), (40, 1, 32)], ids=str)
+@pytest.mark.parametrize("case", CONTEXTS, ids=str)
+def test_paged_attention(dtype, shape, case):
+    import transformer as M
+    (H, Hk, D), (new, context) = shape, case
+    for page, causal in ((16, True), (64, True), (32, False)):
+        g = gen(page + sum(context))
+        keys, values, table = cache_of(g, context, page, Hk, D, dtype)
+        for i, c in enumerate(context):            # what lies behind a sequence's end is stale, NaN here
+            if c % page:
+                keys[table[i, c // page].long(), c % page:] = math.nan
+                values[table[i, c // page].long(), c % page:] = math.nan
+        q = rand(g, sum(new), H, D, dtype=dtype)
+        got = M.paged_attention(q, keys, values, M.PagedBatch(table, context, new), causal=causal)
+        check_paged(q, keys, values, table, context, new, causal, 1 / math.sqrt(D), got)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_paged_attention_absent_pages(dtype):
+    """A page number outside the pool: its keys are not there; a sequence of such pages gives zeros."""
+    import transformer as M
+    g, (H, Hk, D), page = gen(11), (4, 2, 64), 16
+    for new in ([1, 1, 1], [100, 30, 2]):
+        context = [300, 200, 100]
+        keys, values, table = cache_of(g, context, page, Hk, D, dtype)
+        bad = table.clone()
+        bad[0, 3], bad[0, 7], bad[1, 0] = -1, keys.shape[0], 2 ** 31 - 1
+        bad[2] = -5
+        q = rand(g, sum(new), H, D, dtype=dtype)
+        got = M.paged_attention(q, keys, values, M.PagedBatch(bad, context, new))
+        r = 0
+        for i, (n, c) in enumerate(zip(new, context)):
+            k, v = rows_of(keys, table[i], c), rows_of(values, table[i], c)
+            there = ((bad[i] >= 0) & (bad[i] < keys.shape[0])).repeat_interleave(page)[:c]
+            for t in range(n):
+                seen = there & (torch.arange(c, device=DEV) <= c - n + t)
+                for h in range(H):
+                    if not bool(seen.any()):
+                        assert (got[r + t, h] == 0).all()
+                        continue
+                    (w,) = ref.head(q[r + t:r + t + 1, h], k[seen][:, h // 2], v[seen][:, h // 2], 0, False, 1 / math.sqrt(D), dtype)
+                    ref.within(got[r + t:r + t + 1, h], w, f"sequence {i} token {t} head {h}")
+            r += n
+
+
+def test_paged_attention_pool_beyond_32_bits():
+    """A pool of more than 2^31 elements, the sequence in its last pages."""
+    import transformer as M
+    g, (H, Hk, D), page = gen(12), (4, 2, 128), 64
+    pages = (1 << 31) // (page * Hk * D) + 40
+    keys = torch.empty(pages, page, Hk, D, dtype=torch.bfloat16, device=DEV)
+    values = torch.empty_like(keys)
+    keys[-20:] = rand(g, 20, page, Hk, D, dtype=torch.bfloat16)
+    values[-20:] = rand(g, 20, page, Hk, D, dtype=torch.bfloat16)
+    table = torch.arange(pages - 1, pages - 21, -1, device=DEV, dtype=torch.int32)[None]
+    for new in ([1], [300]):
+        q = rand(g, new[0], H, D, dtype=torch.bfloat16)
+        got = M.paged_attention(q, keys, values, M.PagedBatch(table, [1270], new))
+        check_paged(q, keys, values, table, [1270], new, True, 1 / math.sqrt(D), got)
+    k = rand(g, 5, Hk, D, dtype=torch.bfloat16)
+    freq, _ = M.rotary_frequencies(D, device=DEV)
+    M.append_rotary(q[:5], k, k, keys, values, M.PagedBatch(table, [1275], [5]), freq)
+    assert torch.equal(rows_of(values, table[0], 1275)[1270:], k)
+
+
+def test_paged_step_captured():
+    """A decoding step in a graph: lengths grow on the device between replays; two graphs over one cache."""
+    import transformer as M
+    g, (H, Hk, D), page = gen(13), (8, 2, 64), 16
+    context = [600, 33, 1200]
+    keys, values, table = cache_of(g, [c + 40 for c in context], page, Hk, D, torch.bfloat16)
+    freq, _ = M.rotary_frequencies(D, device=DEV)
+    batch = M.PagedBatch(table, context, [1, 1, 1], max_length=1240)
+    q, k, v = (rand(g, 3, h, D, dtype=torch.bfloat16) for h in (H, Hk, Hk))
+
+    def step(b):
+        return M.paged_attention(M.append_rotary(q, k, v, keys, values, b, freq), keys, values, b)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(batch)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(batch))
+    for turn in range(6):
+        for x in (q, k, v):
+            x.copy_(rand(g, *x.shape, dtype=x.dtype))
+        batch.lengths.add_(1)
+        graphs[turn % 2].replay()
+        torch.cuda.synchronize()
+        got = outs[turn % 2].clone()
+        fresh = M.PagedBatch(table, [c + turn + 1 for c in context], [1, 1, 1], max_length=1240)
+        assert torch.equal(got, step(fresh)), turn
+
+
+# ------------------------------------------------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims", [(16, 16), (128, 128), (96, 48), (80, 20), (6, 2), (64, 0), (33, 10), (256, 256), (128, 24)], ids=str)
+def test_rotary(dtype, interleaved, dims):
+    import transformer as M
+    D, R = dims
+    for rows, H, Hk, first in ((1, 3, 1, 0), (37, 5, 2, 1000000), (2500, 4, 4, -7)):
+        g = gen(D + R + rows)
+        qk = rand(g, rows, (H + Hk) * D, dtype=dtype)
+        q, k = (x.unflatten(1, (-1, D)).detach().requires_grad_() for x in qk.split([H * D, Hk * D], 1))
+        freq = (10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / max(R, 1))).to(DEV)
+        pos = torch.arange(rows, device=DEV, dtype=torch.int32) + first
+        out = M.apply_rotary(q, k, pos, freq, interleaved=interleaved, multiplier=1.25)
+        do = [rand(g, *x.shape, dtype=dtype) for x in out]
+        grads = torch.autograd.grad(out, (q, k), do)
+        for x, y, d, e in zip((q, k), out, do, grads):
+            ref.within(y.detach(), ref.turned(x.detach(), pos, freq, interleaved, 1.25), "turned")
+            ref.within(e, ref.turned(d, pos, freq, interleaved, 1.25, -1.0), "gradient")
+            assert torch.equal(y[..., R:], x[..., R:])
+        alone, none = M.apply_rotary(q.detach().transpose(1, 2).contiguous().transpose(1, 2), None, pos, freq, interleaved=interleaved, multiplier=1.25)
+        assert none is None and torch.equal(alone, out[0])
+
+
+def test_rotary_frequencies():
+    import transformer as M
+    plain, one = M.rotary_frequencies(64, device="cpu")
+    assert one == 1.0 and plain[0] == 1.0 and abs(float(plain[-1]) - 10000.0 ** (-62 / 64)) < 1e-18
+    assert torch.allclose(M.rotary_frequencies(64, scaling="linear", factor=4.0, device="cpu")[0], plain / 4, rtol=1e-15)
+    base, _ = M.rotary_frequencies(64, scaling="base", factor=4.0, device="cpu")
+    assert base[0] == 1.0 and abs(float(base[-1] / plain[-1]) - 0.25) < 1e-12
+    ramp, m = M.rotary_frequencies(64, scaling="ramp", factor=8.0, original_length=2048, device="cpu")
+    turns = 2048 * plain / (2 * math.pi)
+    assert torch.equal(ramp[turns >= 32], plain[turns >= 32]) and torch.allclose(ramp[turns <= 1], plain[turns <= 1] / 8)
+    assert abs(m - (1 + 0.1 * math.log(8))) < 1e-15 and (ramp <= plain).all() and (ramp >= plain / 8).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("dims", [(128, 128, True), (96, 48, False), (40, 20, True), (36, 10, False), (16, 16, False)], ids=str)
+def test_append_rotary(dtype, dims):
+    import transformer as M
+    (D, R, interleaved), H, Hk, page = dims, 6, 2, 16
+    g = gen(D + R)
+    for new, context in (([1, 1, 1], [40, 1, 16]), ([50, 0, 33, 1], [50, 20, 90, 17])):
+        keys, values, table = cache_of(g, context, page, Hk, D, dtype)
+        before = keys.clone(), values.clone()
+        rows = sum(new) + 3
+        q, k, v = (rand(g, rows, h, D, dtype=dtype) for h in (H, Hk, Hk))
+        freq = (10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)).to(DEV)
+        out = M.append_rotary(q, k, v, keys, values, M.PagedBatch(table, context, new), freq, interleaved=interleaved, multiplier=0.5)
+        assert (out[sum(new):] == 0).all()
+        written = torch.zeros(keys.shape[:2], dtype=torch.bool, device=DEV)
+        r = 0
+        for i, (n, c) in enumerate(zip(new, context)):
+            pos = torch.arange(c - n, c, device=DEV, dtype=torch.int32)
+            at = (table[i].long()[pos.long() // page], pos.long() % page)
+            ref.within(out[r:r + n], ref.turned(q[r:r + n], pos, freq, interleaved, 0.5), "q")
+            ref.within(keys[at], ref.turned(k[r:r + n], pos, freq, interleaved, 0.5), "k")
+            assert torch.equal(values[at], v[r:r + n])
+            written[at] = True
+            r += n
+        for pool, old in zip((keys, values), before):
+            assert torch.equal(pool[~written], old[~written]), "only the new tokens' places are written"
+        bad = table.clone()
+        bad[:, 0] = torch.tensor([-1, 10 ** 6, -2, 2 ** 31 - 1][:len(new)], dtype=torch.int32, device=DEV)
+        for pool, old in zip((keys, values), before):
+            pool.copy_(old)
+        M.append_rotary(q, k, v, keys, values, M.PagedBatch(bad, context, new), freq)
+        absent = torch.cat([table[i, :1].long() for i in range(len(new))])
+        assert torch.equal(keys[absent], before[0][absent]) and torch.equal(values[absent], before[1][absent])
+
+
+# ----------------------------------------------------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_model_trains_and_serves(dtype):
+    """The module over packed sequences against itself over the cache: a prompt in chunks, then token by token."""
+    import transformer as M
+    torch.manual_seed(3)
+    E, H, Hk = 128, 4, 2
+    net = M.GroupedQueryAttention(E, H, Hk, rotary_dim=16, scaling="ramp", factor=4.0, original_length=64, dtype=dtype).to(DEV)
+    lengths = [90, 7, 41]
+    g = gen(21)
+    x = rand(g, sum(lengths), E)
+    pack = M.PackedSequences(lengths, DEV)
+    with torch.no_grad():
+        whole = net(x, pack)
+    cache = net.new_cache(12, page_size=16)
+    ids = [cache.add() for _ in lengths]
+    start, left, parts = [0, 90, 97], list(lengths), [[] for _ in lengths]
+    for chunk in ([40, 3, 1], [49, 0, 39], [1, 1, 1], [0, 1, 0], [0, 1, 0], [0, 1, 0]):
+        batch = cache.extend(ids, chunk)
+        new = torch.cat([x[s:s + n] for s, n in zip(start, chunk)])
+        y = net.step(new, cache, batch).split(chunk)
+        for i, n in enumerate(chunk):
+            parts[i].append(y[i])
+            start[i] += n
+    served = torch.cat([torch.cat(p) for p in parts])
+    # the same rotation and scores: outputs differ by the weights' rounding (twice a step of the type) through fc_out
+    size = float(whole.abs().max())
+    assert float((served - whole).abs().max()) <= (8 * ref.U[dtype] if dtype != torch.float32 else 2e-5) * max(1.0, size) * 2
+    assert cache.free_pages == 12 - 6 - 1 - 3
+    cache.remove(ids[0])
+    assert cache.free_pages == 12 - 1 - 3
+    # and the gradients of a training step exist and follow the loss along them
+    loss = (net(x, pack) ** 2).sum()
+    loss.backward()
+    grads = [p.grad for p in net.parameters()]
+    assert all(p is not None and bool(torch.isfinite(p).all()) for p in grads)
+
+
+def test_other_stream():
+    """Operators enqueue on the current stream: work on a side stream sees what that stream wrote."""
+    import transformer as M
+    g, n = gen(31), [500, 300]
+    pack = M.PackedSequences(n, DEV)
+    q, k, v = (rand(g, sum(n), h, 64, dtype=torch.bfloat16) for h in (8, 2, 2))
+    want = M.packed_attention(q * 2, k, v, pack)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = M.packed_attention(q * 2, k, v, pack)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_refusals_on_gpu_tensors():
+    import transformer as M
+    from s2g.lib import S2GError
+    pack = M.PackedSequences([4], DEV)
+    x = lambda r, h, d, t=torch.float32: torch.zeros(r, h, d, dtype=t, device=DEV)  # noqa: E731
+    for bad in ((x(4, 3, 32), x(4, 2, 32), x(4, 2, 32)), (x(4, 2, 12), x(4, 2, 12), x(4, 2, 12)), (x(4, 2, 136),) * 3,
+                (x(3, 2, 32), x(4, 2, 32), x(4, 2, 32)), (x(4, 2, 32), x(3, 2, 32), x(3, 2, 32)), (x(4, 2, 32), x(4, 2, 32), x(4, 2, 64)),
+                (x(4, 2, 32), x(4, 2, 32, torch.bfloat16), x(4, 2, 32)), (x(4, 2, 32, torch.float64),) * 3):
+        with pytest.raises(S2GError):
+            M.packed_attention(*bad, pack)
+    ok = x(4, 2, 32)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(S2GError):
+            M.packed_attention(ok, ok, ok, pack, scale=scale)
+    table = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    pool = torch.zeros(4, 16, 2, 32, device=DEV)
+    batch = M.PagedBatch(table, [10], [4])
+    freq, _ = M.rotary_frequencies(32, device=DEV)
+    M.paged_attention(ok, pool, pool.clone(), batch)
+    for keys in (torch.zeros(4, 12, 2, 32, device=DEV), torch.zeros(4, 16, 2, 40, device=DEV), torch.zeros(4, 16, 3, 32, device=DEV),
+                 pool.bfloat16(), pool[..., ::2], torch.zeros(0, 16, 2, 32, device=DEV)):
+        with pytest.raises(S2GError):
+            M.paged_attention(ok, keys, keys.clone(), batch)
+        with pytest.raises(S2GError):
+            M.append_rotary(ok, ok, ok, keys, keys.clone(), batch, freq)
+    with pytest.raises(S2GError):
+        M.paged_attention(ok, pool, pool, M.PagedBatch(table, [40], [4]))           # beyond the table
+    with pytest.raises(S2GError):
+        M.paged_attention(ok[:3], pool, pool, batch)
+    with pytest.raises(S2GError):
+        M.paged_attention(ok.clone().requires_grad_(), pool, pool, batch)
+    pos = torch.arange(4, dtype=torch.int32, device=DEV)
+    for args in ((ok, ok, pos.long(), freq), (ok, ok, pos[:3], freq), (ok, ok, pos, freq.float()), (ok, x(3, 2, 32), pos, freq),
+                 (x(4, 2, 16), None, pos, freq), (x(4, 1, 300), None, pos, freq)):
+        with pytest.raises(S2GError):
+            M.apply_rotary(*args)

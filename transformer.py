@@ -19,6 +19,9 @@ if _PKG not in sys.path:
 
 from s2g import ops  # noqa: E402
 from s2g.attention import AddLayerNormFn, LinearActFn, MulMaskFn, MultiheadAttentionFn, dropout_multiplier  # noqa: E402
+from s2g.causal import (PackedSequences, PagedBatch, PagedKVCache, append_rotary, apply_rotary, packed_attention,  # noqa: E402,F401
+                        paged_attention, rotary_frequencies)
+from s2g.lib import S2GError  # noqa: E402
 
 
 def create_causal_mask(seq_len):
@@ -143,3 +146,52 @@ class CustomTransformerEncoderLayer(nn.TransformerEncoderLayer):
         if self.batch_first:
             src = src.transpose(0, 1)
         return src
+
+
+class GroupedQueryAttention(nn.Module):
+    """Causal self-attention with rotary positions and grouped heads over packed sequences, for training on ragged batches
+    and for serving from a paged cache: num_heads query heads share num_kv_heads key/value heads.  Projections are fp32;
+    rotation and attention run in `dtype`.  The first rotary_dim features of every head are turned (all of them by default),
+    with the frequencies of rotary_frequencies(rotary_dim, base, scaling, factor, original_length)."""
+
+    def __init__(self, embed_size, num_heads, num_kv_heads=None, rotary_dim=None, interleaved=False, base=10000.0, scaling=None,
+                 factor=1.0, original_length=4096, dtype=torch.float32):
+        super(GroupedQueryAttention, self).__init__()
+        self.num_heads, self.num_kv_heads = num_heads, num_heads if num_kv_heads is None else num_kv_heads
+        self.head_dim = embed_size // num_heads
+        if self.head_dim * num_heads != embed_size or self.num_kv_heads <= 0 or num_heads % self.num_kv_heads:
+            raise S2GError("GroupedQueryAttention: heads must divide the embedding size, kv heads the heads")
+        self.interleaved, self.dtype = interleaved, dtype
+        self.in_proj = nn.Linear(embed_size, (num_heads + 2 * self.num_kv_heads) * self.head_dim)
+        self.fc_out = nn.Linear(embed_size, embed_size)
+        self._frequencies, self.multiplier = rotary_frequencies(self.head_dim if rotary_dim is None else rotary_dim, base, scaling,
+                                                                factor, original_length, device="cpu")
+
+    def _turns(self, device):
+        # float64 whatever the module's parameters are cast to
+        if self._frequencies.device != device:
+            self._frequencies = self._frequencies.to(device)
+        return self._frequencies
+
+    def _project(self, x):
+        qkv = LinearActFn.apply(x, self.in_proj.weight, self.in_proj.bias, 0).to(self.dtype)
+        return qkv.view(x.shape[0], -1, self.head_dim).split([self.num_heads, self.num_kv_heads, self.num_kv_heads], 1)
+
+    def _out(self, y):
+        return LinearActFn.apply(y.reshape(y.shape[0], -1).float(), self.fc_out.weight, self.fc_out.bias, 0)
+
+    def forward(self, x, pack):
+        """x [tokens, embed_size], the sequences of `pack` one after another."""
+        q, k, v = self._project(x)
+        q, k = apply_rotary(q, k, pack.positions, self._turns(x.device), self.interleaved, self.multiplier)
+        return self._out(packed_attention(q, k, v, pack))
+
+    def new_cache(self, num_pages, page_size=64):
+        return PagedKVCache(num_pages, page_size, self.num_kv_heads, self.head_dim, self.dtype, self.in_proj.weight.device)
+
+    @torch.no_grad()
+    def step(self, x, cache, batch):
+        """The new tokens x [tokens, embed_size] of `batch` (cache.extend) into the cache, and their attention over it."""
+        q, k, v = self._project(x)
+        q = append_rotary(q, k, v, cache.keys, cache.values, batch, self._turns(x.device), self.interleaved, self.multiplier)
+        return self._out(paged_attention(q, cache.keys, cache.values, batch))
