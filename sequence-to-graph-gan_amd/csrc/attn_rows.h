@@ -21,9 +21,10 @@ __device__ __forceinline__ void tile_offsets(int* off, long ld, int D, int wave,
 }
 template <typename LT, typename T>
 __device__ __forceinline__ void fetch_rows(char* lds, const T* p, long ld, int D, int rows, const int* off, int wave) {
-  const auto b = buffer_of(p, (int)(((rows - 1) * ld + D) * (long)sizeof(T)));
+  const ix4 b = buffer_of(p, (int)(((rows - 1) * ld + D) * (long)sizeof(T)));
+  const unsigned to = lds_address(lds);
 #pragma unroll
-  for (int i = 0; i < LT::NI; ++i) load_to_lds(b, lds + (i * 4 + wave) * 1024, off[i], 0);
+  for (int i = 0; i < LT::NI; ++i) load_to_lds(b, to + (i * 4 + wave) * 1024, off[i]);
 }
 
 // 8 elements of a row straight from memory: zeros beyond the row's D elements or where !ok
@@ -73,9 +74,9 @@ struct Rows {
     m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = 8.0f / c;
   }
   // KB blocks of 32 keys from LDS.  edge: some row of the wave does not see all of them (`last`: the last one that this
-  // lane's row sees, counted from the tile's first); absent: keys (bits, of the first 32) that are not there.
+  // lane's row sees, counted from the tile's first); absent: keys (bits) that are not there.
   template <int KB>
-  __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned absent, int lane) {
+  __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {
     const int half = lane >> 5;
     // S^T = K Q^T: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's own registers and
     // one exchange between the halves
@@ -95,8 +96,12 @@ struct Rows {
     }
     if (absent) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if ((absent >> (reg_row(i) + 4 * half)) & 1) st[0][i] = -INFINITY;
+      for (int b = 0; b < KB; ++b) {
+        const unsigned bits = (unsigned)(absent >> (32 * b)) >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if ((bits >> reg_row(i)) & 1) st[b][i] = -INFINITY;
+      }
     }
     float mx = st[0][0];
 #pragma unroll

@@ -125,7 +125,7 @@ int s2g_paged_attention(const void* Q, const void* keys, const void* values, con
   if (!Q || !keys || !values || !table || !lengths || !starts || !out || paged_dims(dims, &d) != 0 || (d.parts > 1 && !work)) return -1;
   if (!aligned16(Q) || !aligned16(keys) || !aligned16(values) || !aligned16(out) || !aligned16(work)) return -1;
   const int tile = dims->by_rows ? 128 : 32;
-  if ((d.max_rows + tile - 1) / tile > 65535 || (long)d.Hk * d.parts >= (1L << 31) || (long)d.Hk * ((d.max_rows + 3) / 4) >= (1L << 31)) return -1;
+  if ((d.max_rows + tile - 1) / tile > 65535 || (long)d.Hk * d.parts >= (1L << 31) || (long)d.Hk * d.max_rows >= (1L << 31)) return -1;
   return BY_TYPE(dims->type, s2g_launch_paged, Q, keys, values, table, lengths, starts, out, work, dims->by_rows, d, (hipStream_t)stream);
 }
 

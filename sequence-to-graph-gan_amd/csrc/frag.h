@@ -106,8 +106,6 @@ __device__ __forceinline__ int divide(int r, DivBy d) {
   return q;
 }
 
-typedef __attribute__((address_space(3))) void lds_void;
-
 // A tile of ROWS rows of PITCH elements in LDS, filled by buffer_load ... lds of 16 bytes per lane.  One wave instruction
 // fills 1 KB of consecutive LDS, so the layout is [row][chunk of 16 bytes] without padding, and bank conflicts are
 // kept away by WHERE a chunk sits: chunk c of row r is stored at c ^ key(r).  Rows read in step with each other
@@ -168,16 +166,30 @@ struct Tile {
   }
 };
 
-// A raw buffer over `bytes` bytes at p: lanes whose offset lies beyond it fetch zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+// A raw buffer over `bytes` bytes at p (both the same in all lanes): lanes whose offset lies beyond it fetch zeros.
+__device__ __forceinline__ ix4 buffer_of(const void* p, int bytes) {
+  const unsigned long a = (unsigned long)p;
+  return (ix4){__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)),
+               __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
 #define OUT_OF_BUFFER 0x7fffff00       // an offset beyond every buffer made here
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t b, char* lds, int lane_offset, int offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_void*)lds, 16, lane_offset, offset, 0, 0);
+// 16 bytes per lane to consecutive LDS from `lds` on (an LDS byte address).  In assembly because the compiler, which
+// cannot tell the tile being filled from the one being read, waits for the loads of the builtin before every transposed
+// read: the next tile would never be in flight.  No register is written; wait_loads() is the wait.
+__device__ __forceinline__ void load_to_lds(ix4 b, unsigned lds, int lane_offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(lane_offset), "s"(b) : "memory", "m0");
 }
-// this wave's loads have arrived, and its LDS reads are done (the next loads may take the place of what they read)
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane((int)(unsigned long)(const __attribute__((address_space(3))) void*)p);
+}
+// this wave's loads have arrived, and its LDS reads are done (the next loads may take the place of what they read).  The
+// builtin, not assembly: the compiler then knows that its own loads have arrived too, and waits no second time in the loop.
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);      // vmcnt(0) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
 
 // wave-uniform values: tells the compiler to keep them in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }

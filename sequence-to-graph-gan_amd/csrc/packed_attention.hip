@@ -18,7 +18,7 @@
 
 // -------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ out,
                                                              float* __restrict__ lse, const PackedTile* __restrict__ tiles,
                                                              PackedDims dm) {
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void s2g_k_packed_attn_fwd(const T* __restrict
 // ------------------------------------------------------------------------------------------------- backward, query side
 // D of every row, and dQ: lanes are rows, as in the forward pass
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, const T* __restrict__ out,
                                                                const T* __restrict__ dO, const float* __restrict__ lse,
                                                                float* __restrict__ delta, T* __restrict__ dQ,
@@ -210,15 +210,15 @@ __global__ __launch_bounds__(256, 1) void s2g_k_packed_attn_bwd_kv(const T* __re
   const T* gb = dO + (long)w.q_start * dm.ldo + kvh * G * dm.ho;
   const long lb = ((long)kvh * dm.q_rows + w.q_start) * G;
   auto fetch = [&](int t, int into) {
-    char* to = lds + into * 2 * LT::BYTES;
+    const unsigned to = lds_address(lds) + into * 2 * LT::BYTES;
     const int r0 = t * S::KT, tok0 = divide(r0, dm.by);
-    const auto qr = buffer_of(qb + tok0 * dm.ldq, 0x7ffffe00), gr = buffer_of(gb + tok0 * dm.ldo, 0x7ffffe00);
+    const ix4 qr = buffer_of(qb + tok0 * dm.ldq, 0x7ffffe00), gr = buffer_of(gb + tok0 * dm.ldo, 0x7ffffe00);
 #pragma unroll
     for (int i = 0; i < LT::NI; ++i) {
       const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
       const bool ok = r < rows && ch < dm.D * (int)sizeof(T);
-      load_to_lds(qr, to + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER, 0);
-      load_to_lds(gr, to + LT::BYTES + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER, 0);
+      load_to_lds(qr, to + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+      load_to_lds(gr, to + LT::BYTES + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
     }
   };
   float st_next = 0.0f;

@@ -34,23 +34,24 @@ __device__ __forceinline__ int keys_seen(const PagedSeq& q, int row, const Paged
   return max(0, min(q.len, divide(min(row, q.rows - 1), dm.by) + q.len - q.n + 1));
 }
 
-// The page of key k0 + lane, -1 if there is none
+// What the table says of key `key`'s page.  The load is unconditional (of a key that exists, or the first) and is looked
+// at only when its tile is fetched, an iteration later: a test here would wait for it, and for every load before it.
 __device__ __forceinline__ int page_of(const int* table, int key, int len, const PagedDims& dm) {
-  int p = -1;
-  if (key < len) p = table[key >> dm.page_shift];
-  return (unsigned)p < (unsigned)dm.pages ? p : -1;
+  return table[key < len ? key >> dm.page_shift : 0];
 }
+__device__ __forceinline__ bool in_pool(int page, const PagedDims& dm) { return (unsigned)page < (unsigned)dm.pages; }
 // One tile of KT keys from k0 on: wave instruction after wave instruction, each within one page (whose 16 tokens or more
 // it never crosses).  Keys beyond the length and of absent pages come as zeros.
 template <typename LT, int WAVES, typename T>
 __device__ __forceinline__ void fetch_pages(char* lds, const T* pool, int page, int k0, int len, const int* off, int wave,
                                             const PagedDims& dm) {
+  const unsigned to = lds_address(lds);
 #pragma unroll
   for (int i = 0; i < LT::NI; ++i) {
     const int r = (i * WAVES + wave) * LT::RPI, pg = __builtin_amdgcn_readlane(page, r);
-    const int n = pg < 0 ? 0 : min(LT::RPI, len - (k0 + r)), in = (k0 + r) & ((1 << dm.page_shift) - 1);
-    const T* p = pool + (n > 0 ? pg * dm.page_ld + in * dm.ld : 0);
-    load_to_lds(buffer_of(p, n > 0 ? (int)(((n - 1) * dm.ld + dm.D) * (long)sizeof(T)) : 0), lds + (i * WAVES + wave) * 1024, off[i], 0);
+    const int n = in_pool(pg, dm) ? max(0, min(LT::RPI, len - (k0 + r))) : 0, in = (k0 + r) & ((1 << dm.page_shift) - 1);
+    const T* p = pool + pg * dm.page_ld + in * dm.ld;                    // not touched if n is 0
+    load_to_lds(buffer_of(p, n > 0 ? (int)(((n - 1) * dm.ld + dm.D) * (long)sizeof(T)) : 0), to + (i * WAVES + wave) * 1024, off[i]);
   }
 }
 template <typename LT, typename T>
@@ -61,6 +62,11 @@ __device__ __forceinline__ void page_offsets(int* off, int wave, int lane, const
     off[i] = c * 16 < dm.D * (int)sizeof(T) ? (int)((lane / LT::CH) * dm.ld * (long)sizeof(T)) + c * 16 : OUT_OF_BUFFER;
   }
 }
+
+// The part that the i-th workgroup of a sequence takes: turned by one from sequence to sequence.  Workgroups are dealt to
+// the XCDs and their engines in turn, so the parts that short sequences lack would otherwise all fall to the same ones
+// (64 sequences of 300 to 8200 tokens in 8 parts: 300 us, turned 250).
+__device__ __forceinline__ int part_of(int i, int by, int parts) { return (i + by) % parts; }
 
 // Where a row's result goes: the output if its sequence has one part, else part `part` of the workspace
 // ([row of all kv heads][part][D] sums, then [row][part] (m, l)).
@@ -92,7 +98,7 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
   typedef typename KT::LT LT;
   constexpr int NW = KT::NW, DB = Shape<T, DP>::DB;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int kvh = blockIdx.x % dm.Hk, part = blockIdx.x / dm.Hk, tile = blockIdx.y, s = blockIdx.z;
+  const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(blockIdx.x / dm.Hk, s + tile, dm.parts);
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
   if (tile * 32 >= sq.rows) return;
   const int seen = keys_seen(sq, tile * 32 + 31, dm);
@@ -125,7 +131,7 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
   for (int t = 0; k0 < hi; ++t, k0 += 32 * NW) {
     const char* kt = mine + (t & 1) * 2 * LT::BYTES;
     wait_loads();
-    const unsigned absent = (unsigned)__ballot(page < 0 && k0 + (lane & 31) < hi);
+    const unsigned absent = (unsigned)__ballot(!in_pool(page, dm) && k0 + (lane & 31) < hi);
     page = next;
     if (k0 + 32 * NW < hi) {
       char* nx = mine + ((t + 1) & 1) * 2 * LT::BYTES;
@@ -187,15 +193,14 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
 
 // ---------------------------------------------------------------------------------------------------------------- chunks
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void s2g_k_paged_attn_rows(
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_rows(
     const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int kvh = blockIdx.x % dm.Hk, part = blockIdx.x / dm.Hk, s = blockIdx.z;
+  const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(blockIdx.x / dm.Hk, s + tile, dm.parts);
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
-  const int tile = blockIdx.y;
   if (tile * 128 >= sq.rows) return;
   const int seen = keys_seen(sq, tile * 128 + 127, dm);
   const int lo = part * dm.part_keys, hi = min(seen, lo + dm.part_keys);
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(256) void s2g_k_paged_attn_rows(
   for (int t = 0; k0 < hi; ++t, k0 += S::KT) {
     const char* kt = lds + (t & 1) * 2 * LT::BYTES;
     wait_loads();
-    const unsigned long long absent = __ballot(page < 0 && k0 + kl < hi);
+    const unsigned long long absent = __ballot(!in_pool(page, dm) && k0 + kl < hi);
     page = next;
     __syncthreads();
     if (k0 + S::KT < hi) {
@@ -236,14 +241,7 @@ __global__ __launch_bounds__(256) void s2g_k_paged_attn_rows(
     }
     if (k0 > w_hi) continue;
     const bool edge = k0 + S::KT - 1 > min(w_lo, hi - 1);
-    if (absent) {                                              // rare: 32 keys at a time, each with its own bits
-#pragma unroll
-      for (int b = 0; b < S::KB; ++b)
-        r.template step<1>(kt + 32 * b * S::PITCH * (int)sizeof(T), kt + LT::BYTES + 32 * b * S::PITCH * (int)sizeof(T), true,
-                           min(last, hi - 1) - k0 - 32 * b, (unsigned)(absent >> (32 * b)), lane);
-    } else {
-      r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, 0, lane);
-    }
+    r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, absent, lane);
   }
   const float l = both_sum(r.l);
   if (alone) {
@@ -259,36 +257,64 @@ __global__ __launch_bounds__(256) void s2g_k_paged_attn_rows(
   }
 }
 
-// One wave per row: its parts' sums brought to one maximum and added in order.
-template <typename T>
+// WAVES waves per row (4 where there are many parts, else 1 and four rows to a workgroup): each brings its share of the
+// parts to the row's maximum, eight at a time (a loop of single loads would wait for memory at every part), and the waves'
+// sums are added in order.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void s2g_k_paged_join(const float* __restrict__ ws, const int* __restrict__ lens,
                                                         const int* __restrict__ starts, T* __restrict__ out, int tile_rows,
                                                         PagedDims dm) {
-  const int kvh = blockIdx.x % dm.Hk, s = blockIdx.z, lane = threadIdx.x & 63;
-  const int row = (blockIdx.x / dm.Hk) * 4 + uniform(threadIdx.x >> 6);
+  __shared__ float sum[4][132];
+  const int lane = threadIdx.x & 63, id = uniform(threadIdx.x >> 6), wave = id % WAVES;
+  const int kvh = blockIdx.x % dm.Hk, row = blockIdx.x / dm.Hk * (4 / WAVES) + id / WAVES, s = blockIdx.z;
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
-  if (row >= sq.rows) return;
-  const int seen = keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm);     // as the row's workgroup saw it
+  const int seen = row < sq.rows ? keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm) : 0;   // as the row's workgroup saw it
   const int parts = (seen + dm.part_keys - 1) / dm.part_keys;
-  if (parts <= 1) return;
+  if (parts <= 1) return;                       // all waves of the row, and of the workgroup where they share one
   const Joined j = workspace(const_cast<float*>(ws), dm);
   const long at = ws_row(sq, kvh, row, dm) * dm.parts;
+  const float* ml = j.ml + 2 * at;
+  const float* sums = j.sums + at * dm.D;
   const float c = dm.scale * LOG2E;
-  float m = -INFINITY, l = 0.0f;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, j.ml[2 * (at + p)]);
-  float a[2] = {0.0f, 0.0f};
-  for (int p = 0; p < parts; ++p) {
-    const float mp = j.ml[2 * (at + p)], f = mp == m ? 1.0f : __builtin_amdgcn_exp2f((mp - m) * c);
-    l = fmaf(j.ml[2 * (at + p) + 1], f, l);
+  float m = -INFINITY;
+  for (int p = lane; p < parts; p += 64) m = fmaxf(m, ml[2 * p]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < dm.D) a[i] = fmaf(j.sums[(at + p) * dm.D + lane + 64 * i], f, a[i]);
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const int f0 = min(lane, dm.D - 1), f1 = min(lane + 64, dm.D - 1);
+  float l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+  for (int p0 = wave; p0 < parts; p0 += 8 * WAVES) {
+    float mp[8], lp[8], x0[8], x1[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = min(p0 + WAVES * i, parts - 1);
+      mp[i] = ml[2 * p];
+      lp[i] = ml[2 * p + 1];
+      x0[i] = sums[(long)p * dm.D + f0];
+      x1[i] = sums[(long)p * dm.D + f1];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (p0 + WAVES * i < parts) {
+        const float f = mp[i] == m ? 1.0f : __builtin_amdgcn_exp2f((mp[i] - m) * c);
+        l = fmaf(lp[i], f, l);
+        a0 = fmaf(x0[i], f, a0);
+        a1 = fmaf(x1[i], f, a1);
+      }
+  }
+  if constexpr (WAVES > 1) {
+    sum[wave][lane] = a0;
+    sum[wave][lane + 64] = a1;
+    if (lane == 0) sum[wave][128] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    a0 = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+    a1 = (sum[0][lane + 64] + sum[1][lane + 64]) + (sum[2][lane + 64] + sum[3][lane + 64]);
+    l = (sum[0][128] + sum[1][128]) + (sum[2][128] + sum[3][128]);
   }
   const int tk = divide(row, dm.by);
   T* o = out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + row - tk * dm.by.G) * dm.D;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < dm.D) o[lane + 64 * i] = (T)(l == 0.0f ? 0.0f : a[i] / l);
+  if (lane < dm.D) o[lane] = (T)(l == 0.0f ? 0.0f : a0 / l);
+  if (lane + 64 < dm.D) o[lane + 64] = (T)(l == 0.0f ? 0.0f : a1 / l);
 }
 
 // ----------------------------------------------------------------------------------------------------------------- host
@@ -310,8 +336,10 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   }
-  if (dm.parts > 1)
-    hipLaunchKernelGGL(s2g_k_paged_join<T>, dim3((unsigned)dm.Hk * ((dm.max_rows + 3) / 4), 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
+  if (dm.parts > 16)
+    hipLaunchKernelGGL((s2g_k_paged_join<T, 4>), dim3((unsigned)dm.Hk * dm.max_rows, 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
+  else if (dm.parts > 1)
+    hipLaunchKernelGGL((s2g_k_paged_join<T, 1>), dim3((unsigned)dm.Hk * ((dm.max_rows + 3) / 4), 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 

@@ -323,6 +323,7 @@ class PagedBatch:
         self.lengths, self.starts = _on_device(c, dev), _on_device(np.append(0, np.cumsum(n)), dev)
         self.sequences, self.rows, self.max_new = n.size, int(n.sum()), int(n.max())
         self.max_length = int(c.max()) if max_length is None else int(max_length)
+        self._length, self._new, self._cuts = c, n, {}
         if self.max_length < c.max():
             raise S2GError("PagedBatch: max_length is below a length")
 
@@ -381,14 +382,38 @@ def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch
     return out
 
 
-def _cut(batch: PagedBatch, Hk: int, G: int) -> Tuple[bool, int, int]:
-    """(128 rows to a workgroup, keys per part, parts): parts of a long context fill the chip where rows do not."""
-    rows = batch.max_new * G
-    by_rows = rows > 64
-    blocks = batch.sequences * Hk * -(-rows // (TILE if by_rows else 32))
-    parts = max(1, min(512 // blocks, -(-batch.max_length // 512)))
-    keys = max(512, -(-batch.max_length // parts // 128) * 128)
-    return by_rows, keys, max(1, -(-batch.max_length // keys))
+def _cut(batch: PagedBatch, Hk: int, G: int, D: int, size: int) -> Tuple[bool, int, int]:
+    """(128 rows to a workgroup, keys per part, parts).  One workgroup per (row tile, kv head, part) that exists.  Either all
+    of them are resident at once (counting on 85 % of the places, as they are not dealt quite evenly) and take as long as a
+    part; or they come in turn, which takes the whole work and, at the end, about 0.6 of a part.  Beginning and ending cost
+    a workgroup about 256 keys' time, a part's sums of 128 rows another 4 to write and to join.  (64 sequences of 300 to 8200
+    tokens, 8 kv heads of 128 bf16: parts of 512 / 1024 / 2048 / 8192 keys 253 / 232 / 212 / 236 us.)  From the lengths as
+    they were when the batch was made, and kept with it."""
+    got = batch._cuts.get((Hk, G, D, size))
+    if got is None:
+        rows = np.maximum(batch._new, 0) * G
+        by_rows = batch.max_new * G > 64
+        tiles = -(-rows // (TILE if by_rows else 32)) * Hk
+        width = 32 if D <= 32 else 64 if D <= 64 else 128
+        resident = 256 if by_rows else 256 * max(1, 131072 // (16 * 32 * width * size))
+        work = int((tiles * batch._length).sum())
+        best, k = None, 128
+        while True:
+            blocks = int((tiles * -(-batch._length // k)).sum())
+            if blocks <= 0.85 * resident:
+                cost = min(k, batch.max_length) + 256
+            else:
+                cost = (work + 256 * blocks) / resident + 0.6 * min(k, batch.max_length)
+            if by_rows and k < batch.max_length:
+                cost += 4 * blocks * width * 256 / resident / 128
+            if best is None or cost < best[0]:
+                best = cost, k
+            if k >= batch.max_length:
+                break
+            k += max(128, k // 8 // 128 * 128)
+        k = max(best[1], -(-batch.max_length // 4096 // 128) * 128)
+        got = batch._cuts[Hk, G, D, size] = by_rows, k, max(1, -(-batch.max_length // k))
+    return got
 
 
 def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, batch: PagedBatch, causal: bool = True,
@@ -415,7 +440,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, b
     out[batch.rows:].zero_()
     if batch.rows:
         q = _rows16(q)
-        by_rows, part_keys, parts = _cut(batch, Hk, H // Hk)
+        by_rows, part_keys, parts = _cut(batch, Hk, H // Hk, D, q.element_size())
         dims = S2GPaged(TYPES[q.dtype], batch.sequences, H, Hk, D, int(causal), keys.shape[1], keys.shape[0], batch.table.shape[1],
                         batch.max_new, batch.max_length, part_keys, parts, int(by_rows), s, R, *_strides(q), page_ld, token_ld, head_ld)
         work = torch.empty(max(0, get().s2g_paged_attention_workspace(ctypes.byref(dims))), dtype=torch.float32, device=q.device)
