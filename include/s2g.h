@@ -364,10 +364,12 @@ int s2g_attention_bwd(const float* Q, const float* K, const float* V, const floa
  * [k_rows, kv_heads, dim] are contiguous.  Row i of a sequence with n_q queries and n_k keys sees keys j <= i + n_k -
  * n_q (causal) or all of them; a row that sees none gives zeros and no gradient.  Rows of no sequence are not touched.
  * The tile list has one entry per 128 rows (token, head of the group) of a sequence: ceil(n_q heads / kv_heads / 128)
- * of them, in any order; k_tiles one per 128 keys.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
+ * of them, in any order.  k_tiles: one per 128 keys with slot -1 and all rows (row_lo 0, row_hi n_q heads / kv_heads), or
+ * several that share its rows out among them (bounds multiples of 64), with consecutive slots of their own; each tile so
+ * cut has an entry in cut_tiles, row_lo the number and slot the first of its slots.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
  * exponentials, for the backward pass (may be NULL in fwd); delta has its size. */
 typedef struct S2GPackedTile {
-  int q_start, q_len, k_start, k_len, tile, pad[3];
+  int q_start, q_len, k_start, k_len, tile, row_lo, row_hi, slot;
 } S2GPackedTile;
 typedef struct S2GPacked {
   int type, heads, kv_heads, dim, causal;
@@ -376,11 +378,12 @@ typedef struct S2GPacked {
 } S2GPacked;
 int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, float* lse, const S2GPackedTile* tiles,
                              int n_tiles, const S2GPacked* dims, void* stream);
-/* floats of `work` below: the rows of a key tile are dealt to `parts` workgroups (1 .. 64) that each leave a partial sum */
-long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int parts);
+/* floats of `work` below for so many slots */
+long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int slots);
 int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
-                             float* delta, void* dQ, void* dK, void* dV, float* work, int parts, const S2GPackedTile* q_tiles,
-                             int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPacked* dims, void* stream);
+                             float* delta, void* dQ, void* dK, void* dV, float* work, const S2GPackedTile* q_tiles,
+                             int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPackedTile* cut_tiles,
+                             int n_cut_tiles, const S2GPacked* dims, void* stream);
 
 /* ---- attention of new tokens over a paged cache (paged_attention).  keys, values [pages, page_size, kv_heads, dim] with
  * the strides below (page_size a power of two, 16 .. 65536); table [sequences, table_cols] int32: the page of tokens

@@ -7,7 +7,7 @@
 
 // mirror include/s2g.h
 struct S2GPackedTile {
-  int q_start, q_len, k_start, k_len, tile, pad[3];
+  int q_start, q_len, k_start, k_len, tile, row_lo, row_hi, slot;
 };
 struct S2GPacked {
   int type, heads, kv_heads, dim, causal;
@@ -30,7 +30,7 @@ static_assert(sizeof(S2GPackedTile) == sizeof(PackedTile) && sizeof(PackedTile) 
 #define DECLARE(sfx)                                                                                                    \
   extern "C" int s2g_launch_packed_fwd_##sfx(const void*, const void*, const void*, void*, float*, const PackedTile*, int, PackedDims, hipStream_t); \
   extern "C" int s2g_launch_packed_bwd_##sfx(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, \
-                                             void*, float*, int, const PackedTile*, int, const PackedTile*, int, PackedDims, hipStream_t); \
+                                             void*, float*, const PackedTile*, int, const PackedTile*, int, const PackedTile*, int, PackedDims, hipStream_t); \
   extern "C" int s2g_launch_paged_##sfx(const void*, const void*, const void*, const int*, const int*, const int*, void*, float*, int, PagedDims, hipStream_t);
 DECLARE(f32)
 DECLARE(bf16)
@@ -71,24 +71,26 @@ int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* 
   return BY_TYPE(dims->type, s2g_launch_packed_fwd, Q, K, V, out, lse, reinterpret_cast<const PackedTile*>(tiles), n_tiles, d, (hipStream_t)stream);
 }
 
-long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int parts) {
+long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int slots) {
   PackedDims d;
-  if (packed_dims(dims, &d) != 0 || parts < 1 || parts > 64) return -1;
-  return parts == 1 ? 0 : 2L * parts * d.k_rows * d.Hk * d.D;
+  if (packed_dims(dims, &d) != 0 || slots < 0) return -1;
+  return 256L * slots * d.Hk * d.D;
 }
 
 int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
-                             float* delta, void* dQ, void* dK, void* dV, float* work, int parts, const S2GPackedTile* q_tiles,
-                             int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPacked* dims, void* stream) {
+                             float* delta, void* dQ, void* dK, void* dV, float* work, const S2GPackedTile* q_tiles,
+                             int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPackedTile* cut_tiles,
+                             int n_cut_tiles, const S2GPacked* dims, void* stream) {
   PackedDims d;
   if (!Q || !K || !V || !out || !dO || !lse || !delta || !dQ || !dK || !dV || packed_dims(dims, &d) != 0) return -1;
-  if (parts < 1 || parts > 64 || (parts > 1 && !work) || n_q_tiles < 0 || n_k_tiles < 0 || (n_q_tiles && !q_tiles) || (n_k_tiles && !k_tiles)) return -1;
-  if ((long)n_q_tiles * d.Hk >= (1L << 31) || (long)n_k_tiles * d.Hk * parts >= (1L << 31)) return -1;
+  if (n_q_tiles < 0 || n_k_tiles < 0 || n_cut_tiles < 0 || (n_q_tiles && !q_tiles) || (n_k_tiles && !k_tiles) || (n_cut_tiles && (!cut_tiles || !work))) return -1;
+  if ((long)n_q_tiles * d.Hk >= (1L << 31) || (long)n_k_tiles * d.Hk >= (1L << 31) || (long)n_cut_tiles * d.Hk >= (1L << 31)) return -1;
   const void* all[] = {Q, K, V, out, dO, dQ, dK, dV, work};
   for (const void* p : all)
     if (!aligned16(p)) return -1;
-  return BY_TYPE(dims->type, s2g_launch_packed_bwd, Q, K, V, out, dO, lse, delta, dQ, dK, dV, work, parts,
-                 reinterpret_cast<const PackedTile*>(q_tiles), n_q_tiles, reinterpret_cast<const PackedTile*>(k_tiles), n_k_tiles, d, (hipStream_t)stream);
+  return BY_TYPE(dims->type, s2g_launch_packed_bwd, Q, K, V, out, dO, lse, delta, dQ, dK, dV, work,
+                 reinterpret_cast<const PackedTile*>(q_tiles), n_q_tiles, reinterpret_cast<const PackedTile*>(k_tiles), n_k_tiles,
+                 reinterpret_cast<const PackedTile*>(cut_tiles), n_cut_tiles, d, (hipStream_t)stream);
 }
 
 static int page_shift(int page_size) {

@@ -7,7 +7,8 @@ struct PackedTile {
   int q_start, q_len;      // the sequence's tokens in Q, out and dO
   int k_start, k_len;      // and in K and V
   int tile;                // which 128 rows / keys of the sequence
-  int pad[3];
+  int row_lo, row_hi;      // key side: the rows to go through, of all that the kv head has
+  int slot;                // key side: -1, or where in the workspace these rows' share goes
 };
 
 struct PackedDims {

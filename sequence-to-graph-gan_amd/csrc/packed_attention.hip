@@ -15,6 +15,7 @@
 // b / Hk: with 8 kv heads each XCD (workgroups are dealt to the 8 XCDs in turn) keeps to one head's K and V.
 #include "attn_rows.h"
 #include "packed_attention.h"
+#include <type_traits>
 
 // -------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP>
@@ -169,42 +170,111 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 }
 
 // --------------------------------------------------------------------------------------------------- backward, key side
-// dK and dV of 128 keys: lanes are keys, the rows of the kv head's G query heads come by in tiles.  Few key tiles make
-// few workgroups, so a tile's rows may be cut into `parts` ranges, each leaving a 32-bit partial result that
+// dK and dV of 128 keys: lanes are keys, the rows of the kv head's G query heads come by in tiles.  The first keys of a
+// long sequence are seen by all its rows: where such a tile is more than its share of the work, or the tiles are too few
+// for the chip, the host cuts a tile's rows into ranges, each leaving a 32-bit partial result in a slot of its own that
 // s2g_k_packed_attn_sum adds in a fixed order: no atomics, the same bits every time.
+//
+// The sums of dK and dV of 32 keys, with their K and V, leave room for one wave to a SIMD at 96 or 128 16-bit features,
+// and one wave alone keeps the matrix unit idle while it makes P and dS.  There 8 waves share the work: waves 0 .. 3 take
+// S and dV, waves 4 .. 7 S, dP and dK of the same keys, 40 products where 32 would do, but two waves to a SIMD
+// (DKV_SPLIT_FIGURES).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void s2g_k_packed_attn_bwd_kv(const T* __restrict__ Q, const T* __restrict__ K,
-                                                                const T* __restrict__ V, const T* __restrict__ dO,
-                                                                const float* __restrict__ lse,
-                                                                const float* __restrict__ delta, T* __restrict__ dK,
-                                                                T* __restrict__ dV, float* __restrict__ partial, int parts,
-                                                                const PackedTile* __restrict__ tiles, PackedDims dm) {
+struct KeySide {
+  static constexpr bool SPLIT = sizeof(T) == 2 && DP > 64;
+  static constexpr int WAVES = SPLIT ? 8 : 4;
+  typedef Tile<T, Shape<T, DP>::PITCH, Shape<T, DP>::KT, WAVES> LT;
+};
+
+template <typename T, int DP, bool DV, bool DK>
+struct KeySums {
   typedef Shape<T, DP> S;
-  typedef typename S::LT LT;
+  typedef typename KeySide<T, DP>::LT LT;
   typedef typename Vec<T>::v8 v8;
+  v8 k[S::KS], v[DK ? S::KS : 1];
+  fx16 dv[DV ? S::DB : 1], dk[DK ? S::DB : 1];
+
+  __device__ __forceinline__ void begin(const T* kp, const T* vp, int D, bool live, int half) {
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s) {
+      k[s] = row8(kp, 16 * s + 8 * half, D, live);
+      if constexpr (DK) v[s] = row8(vp, 16 * s + 8 * half, D, live);
+    }
+#pragma unroll
+    for (int d = 0; d < S::DB; ++d) {
+      if constexpr (DV) dv[d] = zero16();
+      if constexpr (DK) dk[d] = zero16();
+    }
+  }
+  // a tile of rows: Q, dO, (L, D); edge: some of them do not see some of the wave's keys (`first`: the first that sees this
+  // lane's, counted from the tile's first)
+  __device__ __forceinline__ void step(const char* qt, const char* gt, const float* sl, float c, bool edge, int first, int lane) {
+    const int half = lane >> 5, col = lane & 31;
+#pragma unroll
+    for (int b = 0; b < S::KB; ++b) {
+      fx16 p = zero16(), ds = zero16();
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) p = mma(LT::along(qt, 32 * b + col, s, half), k[s], p);
+      if constexpr (DK)
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) ds = mma(LT::along(gt, 32 * b + col, s, half), v[s], ds);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const fx4 L = *reinterpret_cast<const fx4*>(sl + 32 * b + 8 * g + 4 * half);
+        fx4 D;
+        if constexpr (DK) D = *reinterpret_cast<const fx4*>(sl + S::KT + 32 * b + 8 * g + 4 * half);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * g + j;
+          p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -L[j]));
+          if constexpr (DK) ds[i] = p[i] * (ds[i] - D[j]);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + reg_row(i) + 4 * half < first) p[i] = 0.0f, ds[i] = 0.0f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (DV) {
+          const v8 pt = operand<T>(p, s);
+#pragma unroll
+          for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
+        }
+        if constexpr (DK) {
+          const v8 dt = operand<T>(ds, s);
+#pragma unroll
+          for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
+        }
+      }
+    }
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * (KeySide<T, DP>::WAVES), sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_kv(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
+    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dK, T* __restrict__ dV,
+    float* __restrict__ partial, const PackedTile* __restrict__ tiles, PackedDims dm) {
+  typedef Shape<T, DP> S;
+  typedef typename KeySide<T, DP>::LT LT;
+  constexpr int WAVES = KeySide<T, DP>::WAVES;
   extern __shared__ __attribute__((aligned(1024))) char lds[];       // Q, dO, Q, dO, then 2 x (L, D)
   float* stats = reinterpret_cast<float*>(lds + 4 * LT::BYTES);
-  const int kvh = blockIdx.x % dm.Hk, part = (blockIdx.x / dm.Hk) % parts;
-  const PackedTile w = tiles[blockIdx.x / (dm.Hk * parts)];
+  const int kvh = blockIdx.x % dm.Hk;
+  const PackedTile w = tiles[blockIdx.x / dm.Hk];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
-  const int G = dm.by.G, rows = w.q_len * G, key = w.tile * 128 + 32 * wave + (lane & 31);
+  const int G = dm.by.G, rows = w.q_len * G, w_key = w.tile * 128 + 32 * (wave & 3), key = w_key + (lane & 31);
   const bool live = key < w.k_len;
   const long krow = (long)w.k_start + min(key, w.k_len - 1);
-  v8 k[S::KS], v[S::KS];
-#pragma unroll
-  for (int s = 0; s < S::KS; ++s) {
-    k[s] = row8(K + krow * dm.ldk + kvh * dm.hk, 16 * s + 8 * half, dm.D, live);
-    v[s] = row8(V + krow * dm.ldv + kvh * dm.hv, 16 * s + 8 * half, dm.D, live);
-  }
   // the first row that sees this key, the wave's first and last, the workgroup's first
   const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
   const int first = !live ? 0x7fffffff : max(0, key - shift) * G;
-  const int w_key = w.tile * 128 + 32 * wave;
   const int w_lo = w_key < w.k_len ? max(0, w_key - shift) * G : 0x7fffffff, w_hi = max(0, min(w_key + 31, w.k_len - 1) - shift) * G;
   const bool ragged = w_key + 31 >= w.k_len;
-  const int b_lo = max(0, w.tile * 128 - shift) * G;
-  const int all0 = b_lo / S::KT, all = max(0, (rows + S::KT - 1) / S::KT - all0);
-  const int t0 = all0 + (int)((long)all * part / parts), t1 = all0 + (int)((long)all * (part + 1) / parts);
+  const int b_lo = max(max(0, w.tile * 128 - shift) * G, w.row_lo);
+  const int t0 = b_lo / S::KT, t1 = (min(rows, w.row_hi) + S::KT - 1) / S::KT;     // row_lo, row_hi: whole tiles
 
   const T* qb = Q + (long)w.q_start * dm.ldq + kvh * G * dm.hq;
   const T* gb = dO + (long)w.q_start * dm.ldo + kvh * G * dm.ho;
@@ -217,93 +287,90 @@ __global__ __launch_bounds__(256, 1) void s2g_k_packed_attn_bwd_kv(const T* __re
     for (int i = 0; i < LT::NI; ++i) {
       const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
       const bool ok = r < rows && ch < dm.D * (int)sizeof(T);
-      load_to_lds(qr, to + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
-      load_to_lds(gr, to + LT::BYTES + (i * 4 + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+      load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+      load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
     }
   };
   float st_next = 0.0f;
-  auto stat = [&](int t) {                                            // threads 0 .. KT: L, then D of the tile's rows
+  auto stat = [&](int t) {                                            // threads 0 .. 2 KT: L, then D of the tile's rows
     const int r = t * S::KT + (threadIdx.x & (S::KT - 1));
     st_next = 0.0f;
     if (threadIdx.x < 2 * S::KT && r < rows) st_next = (threadIdx.x < S::KT ? lse : delta)[lb + r];
   };
-  fx16 dk[S::DB], dv[S::DB];
-#pragma unroll
-  for (int d = 0; d < S::DB; ++d) dk[d] = zero16(), dv[d] = zero16();
   const float c = dm.scale * LOG2E;
+  const T* kp = K + krow * dm.ldk + kvh * dm.hk;
+  const T* vp = V + krow * dm.ldv + kvh * dm.hv;
+  const long orow = (krow * dm.Hk + kvh) * dm.D;
+  float* slot = partial + (((long)w.slot * dm.Hk + kvh) * 256 + 32 * (wave & 3) + (lane & 31)) * dm.D;    // dK, then dV
   if (t0 < t1) {
     stat(t0);
     fetch(t0, t0 & 1);
   }
-  for (int t = t0; t < t1; ++t) {
-    const char* qt = lds + (t & 1) * 2 * LT::BYTES;
-    const char* gt = qt + LT::BYTES;
-    float* sl = stats + (t & 1) * 2 * S::KT;
-    wait_loads();
-    if (threadIdx.x < 2 * S::KT) sl[threadIdx.x] = st_next;
-    __syncthreads();
-    if (t + 1 < t1) {
-      stat(t + 1);
-      fetch(t + 1, (t + 1) & 1);
-    }
-    const int r0 = t * S::KT;
-    if (r0 + S::KT <= w_lo) continue;                                // none of these rows sees this wave's keys
-    const bool edge = ragged || r0 < w_hi;
-#pragma unroll
-    for (int b = 0; b < S::KB; ++b) {
-      fx16 p = zero16(), ds = zero16();
-#pragma unroll
-      for (int s = 0; s < S::KS; ++s) p = mma(LT::along(qt, 32 * b + (lane & 31), s, half), k[s], p);
-#pragma unroll
-      for (int s = 0; s < S::KS; ++s) ds = mma(LT::along(gt, 32 * b + (lane & 31), s, half), v[s], ds);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const fx4 L = *reinterpret_cast<const fx4*>(sl + 32 * b + 8 * g + 4 * half);
-        const fx4 D = *reinterpret_cast<const fx4*>(sl + S::KT + 32 * b + 8 * g + 4 * half);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * g + j;
-          p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -L[j]));
-          ds[i] = p[i] * (ds[i] - D[j]);
-          if (edge && r0 + 32 * b + reg_row(i) + 4 * half < first) p[i] = 0.0f, ds[i] = 0.0f;
-        }
+  // every wave goes through the same tiles and barriers, whichever of the sums are its own
+  auto all_tiles = [&](auto& sums, auto dk_mine, auto dv_mine) {
+    sums.begin(kp, vp, dm.D, live, half);
+    for (int t = t0; t < t1; ++t) {
+      const char* qt = lds + (t & 1) * 2 * LT::BYTES;
+      float* sl = stats + (t & 1) * 2 * S::KT;
+      wait_loads();
+      if (threadIdx.x < 2 * S::KT) sl[threadIdx.x] = st_next;
+      __syncthreads();
+      if (t + 1 < t1) {
+        stat(t + 1);
+        fetch(t + 1, (t + 1) & 1);
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const v8 pt = operand<T>(p, s), dt = operand<T>(ds, s);
-#pragma unroll
-        for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
-#pragma unroll
-        for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
-      }
+      const int r0 = t * S::KT;
+      if (r0 + S::KT <= w_lo) continue;                              // none of these rows sees this wave's keys
+      sums.step(qt, qt + LT::BYTES, sl, c, ragged || r0 < w_hi, first - r0, lane);
     }
-  }
-  const long orow = (krow * dm.Hk + kvh) * dm.D;
-  if (parts == 1) {
-    store_rows<T, S::DB>(dK + orow, dk, dm.scale, dm.D, half, live);
-    store_rows<T, S::DB>(dV + orow, dv, 1.0f, dm.D, half, live);
+    if constexpr (dk_mine.value) {
+      if (w.slot < 0) store_rows<T, S::DB>(dK + orow, sums.dk, dm.scale, dm.D, half, live);
+      else store_rows<T, S::DB>(slot, sums.dk, dm.scale, dm.D, half, live);
+    }
+    if constexpr (dv_mine.value) {
+      if (w.slot < 0) store_rows<T, S::DB>(dV + orow, sums.dv, 1.0f, dm.D, half, live);
+      else store_rows<T, S::DB>(slot + 128 * dm.D, sums.dv, 1.0f, dm.D, half, live);
+    }
+  };
+  if constexpr (KeySide<T, DP>::SPLIT) {
+    if (wave < 4) {
+      KeySums<T, DP, true, false> sums;
+      all_tiles(sums, std::false_type{}, std::true_type{});
+    } else {
+      KeySums<T, DP, false, true> sums;
+      all_tiles(sums, std::true_type{}, std::false_type{});
+    }
   } else {
-    const long plane = (long)dm.k_rows * dm.Hk * dm.D;
-    store_rows<T, S::DB>(partial + 2 * part * plane + orow, dk, dm.scale, dm.D, half, live);
-    store_rows<T, S::DB>(partial + (2 * part + 1) * plane + orow, dv, 1.0f, dm.D, half, live);
+    KeySums<T, DP, true, true> sums;
+    all_tiles(sums, std::true_type{}, std::true_type{});
   }
 }
 
+// one cut tile (its entry's row_lo: the number of its slots) and kv head: blockIdx.y / 4 0 dK, 1 dV, and 32 of its keys
 template <typename T>
-__global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __restrict__ partial, int parts, long plane,
-                                                             T* __restrict__ dK, T* __restrict__ dV) {
+__global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __restrict__ partial, T* __restrict__ dK,
+                                                             T* __restrict__ dV, const PackedTile* __restrict__ tiles,
+                                                             PackedDims dm) {
   typedef typename Vec<T>::v4 v4;
-  const long at = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= 2 * plane) return;
-  fx4 s = *reinterpret_cast<const fx4*>(partial + at);
-  for (int p = 1; p < parts; ++p) {
-    const fx4 x = *reinterpret_cast<const fx4*>(partial + 2 * p * plane + at);
-    s[0] += x[0]; s[1] += x[1]; s[2] += x[2]; s[3] += x[3];
-  }
-  v4 y;
+  const int kvh = blockIdx.x % dm.Hk;
+  const PackedTile w = tiles[blockIdx.x / dm.Hk];
+  const int n4 = dm.D >> 2, y0 = 32 * (blockIdx.y & 3), count = min(32, w.k_len - w.tile * 128 - y0) * n4;
+  const long next = (long)dm.Hk * 256 * dm.D;
+  const float* from = partial + (((long)w.slot * dm.Hk + kvh) * 256 + 32 * blockIdx.y) * dm.D;
+  T* to = blockIdx.y >> 2 ? dV : dK;
+  for (int e = threadIdx.x; e < count; e += 256) {
+    const int y = e / n4, d = (e - y * n4) * 4;
+    fx4 s = *reinterpret_cast<const fx4*>(from + y * dm.D + d);
+#pragma unroll 4
+    for (int p = 1; p < w.row_lo; ++p) {
+      const fx4 x = *reinterpret_cast<const fx4*>(from + p * next + y * dm.D + d);
+      s[0] += x[0]; s[1] += x[1]; s[2] += x[2]; s[3] += x[3];
+    }
+    v4 r;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = (T)s[j];
-  *reinterpret_cast<v4*>((at < plane ? dK : dV - plane) + at) = y;
+    for (int j = 0; j < 4; ++j) r[j] = (T)s[j];
+    *reinterpret_cast<v4*>(to + (((long)w.k_start + w.tile * 128 + y0 + y) * dm.Hk + kvh) * dm.D + d) = r;
+  }
 }
 
 // ----------------------------------------------------------------------------------------------------------------- host
@@ -319,8 +386,8 @@ static int launch_fwd(const void* Q, const void* K, const void* V, void* out, fl
 }
 template <typename T, int DP>
 static int launch_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
-                      float* delta, void* dQ, void* dK, void* dV, float* partial, int parts, const PackedTile* qt, int nqt,
-                      const PackedTile* kt, int nkt, const PackedDims& dm, hipStream_t st) {
+                      float* delta, void* dQ, void* dK, void* dV, float* partial, const PackedTile* qt, int nqt,
+                      const PackedTile* kt, int nkt, const PackedTile* cut, int ncut, const PackedDims& dm, hipStream_t st) {
   typedef typename Shape<T, DP>::LT LT;
   const int qb = 4 * LT::BYTES, kb = 4 * LT::BYTES + 4 * Shape<T, DP>::KT * (int)sizeof(float);
   static S2GLdsCap qcap, kcap;
@@ -330,14 +397,11 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
   if (nqt > 0)
     hipLaunchKernelGGL(kq, dim3((unsigned)nqt * dm.Hk), dim3(256), qb, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out,
                        (const T*)dO, lse, delta, (T*)dQ, qt, dm);
-  if (nkt > 0) {
-    hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk * parts), dim3(256), kb, st, (const T*)Q, (const T*)K, (const T*)V,
-                       (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, parts, kt, dm);
-    if (parts > 1) {
-      const long plane = (long)dm.k_rows * dm.Hk * dm.D;
-      hipLaunchKernelGGL(s2g_k_packed_attn_sum<T>, dim3((unsigned)((2 * plane / 4 + 255) / 256)), dim3(256), 0, st, partial, parts, plane, (T*)dK, (T*)dV);
-    }
-  }
+  if (nkt > 0)
+    hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk), dim3(64 * KeySide<T, DP>::WAVES), kb, st, (const T*)Q, (const T*)K,
+                       (const T*)V, (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
+  if (ncut > 0)
+    hipLaunchKernelGGL(s2g_k_packed_attn_sum<T>, dim3((unsigned)ncut * dm.Hk, 8), dim3(256), 0, st, partial, (T*)dK, (T*)dV, cut, dm);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
@@ -347,7 +411,8 @@ extern "C" int PACKED_NAME(s2g_launch_packed_fwd)(const void* Q, const void* K, 
 }
 extern "C" int PACKED_NAME(s2g_launch_packed_bwd)(const void* Q, const void* K, const void* V, const void* out,
                                                   const void* dO, const float* lse, float* delta, void* dQ, void* dK,
-                                                  void* dV, float* partial, int parts, const PackedTile* qt, int nqt,
-                                                  const PackedTile* kt, int nkt, PackedDims dm, hipStream_t st) {
-  return PER_DIM(launch_bwd, PACKED_T, Q, K, V, out, dO, lse, delta, dQ, dK, dV, partial, parts, qt, nqt, kt, nkt, dm, st);
+                                                  void* dV, float* partial, const PackedTile* qt, int nqt,
+                                                  const PackedTile* kt, int nkt, const PackedTile* cut, int ncut,
+                                                  PackedDims dm, hipStream_t st) {
+  return PER_DIM(launch_bwd, PACKED_T, Q, K, V, out, dO, lse, delta, dQ, dK, dV, partial, qt, nqt, kt, nkt, cut, ncut, dm, st);
 }

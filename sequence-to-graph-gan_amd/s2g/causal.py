@@ -201,39 +201,59 @@ class PackedSequences:
         with torch.cuda.device(self.device):
             self.starts = _on_device(np.append(self.q_start, self.rows), self.device)
             self.positions = _on_device(np.arange(self.rows) - np.repeat(self.q_start - (k - q), q), self.device)
-        self._lists: Dict[Tuple[int, bool], Tuple[torch.Tensor, torch.Tensor]] = {}
+        self._lists: dict = {}
 
-    def _list(self, of: np.ndarray, work: np.ndarray, seq: np.ndarray) -> torch.Tensor:
-        """One entry per tile, the longest first: what remains at the end of the launch is short."""
-        order = np.argsort(-work, kind="stable")
-        seq, tile = seq[order], of[order]
-        entry = np.zeros((seq.size, 8), dtype=np.int32)
-        entry[:, :5] = np.stack([self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile], 1)
+    def _tiles(self, count: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
+        """(sequence, which) of every tile of `count` rows or keys a sequence."""
+        n = -(-count // TILE)
+        return np.repeat(np.arange(n.size), n), np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
+
+    def _list(self, seq, tile, row_lo, row_hi, slot) -> torch.Tensor:
+        entry = np.empty((seq.size, 8), dtype=np.int32)
+        for i, column in enumerate((self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile, row_lo, row_hi, slot)):
+            entry[:, i] = column
         return _on_device(entry, self.device)
 
-    def tiles(self, group: int, causal: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Work lists of the query and the key side for `group` query heads to a kv head."""
+    def query_tiles(self, group: int, causal: bool) -> torch.Tensor:
+        """Work list of the query side for `group` query heads to a kv head: the longest first, so that what remains at the
+        end of the launch is short."""
         got = self._lists.get((group, causal))
         if got is None:
-            out = []
-            for count in (self.q_len * group, self.k_len):
-                n = -(-count // TILE)
-                seq = np.repeat(np.arange(n.size), n)
-                tile = np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
-                if count is self.k_len:
-                    seen = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) if causal else np.zeros_like(tile)
-                    work = np.maximum(0, self.q_len[seq] - seen)
-                else:
-                    token = (np.minimum((tile + 1) * TILE, count[seq]) - 1) // group
-                    work = np.minimum(self.k_len[seq], token + 1 + (self.k_len - self.q_len)[seq]) if causal else self.k_len[seq]
-                out.append(self._list(tile, work, seq))
-            got = self._lists[group, causal] = (out[0], out[1])
+            count = self.q_len * group
+            seq, tile = self._tiles(count)
+            work = self.k_len[seq]
+            if causal:
+                last = (np.minimum((tile + 1) * TILE, count[seq]) - 1) // group
+                work = np.minimum(work, last + 1 + (self.k_len - self.q_len)[seq])
+            order = np.argsort(-work, kind="stable")
+            got = self._lists[group, causal] = self._list(seq[order], tile[order], 0, 0, -1)
         return got
 
-
-def _parts_of_rows(n_blocks: int, rows: int) -> int:
-    """Workgroups per key tile of the backward pass: two to a compute unit, each with 8 row tiles or more."""
-    return max(1, min(-(-512 // max(1, n_blocks)), rows // 512, 16))
+    def key_tiles(self, group: int, causal: bool, kv_heads: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
+        """Work list of the key side, the tiles that are cut, and how many slots they need.  A tile is as much work as it has
+        rows; none is left with more than half of what falls to a compute unit, but 512 rows are not worth a slot."""
+        got = self._lists.get((group, causal, kv_heads))
+        if got is None:
+            seq, tile = self._tiles(self.k_len)
+            rows = (self.q_len * group)[seq]
+            first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // 64 * 64 if causal else np.zeros_like(rows)
+            work = np.maximum(0, rows - first)
+            most = max(512, -(-int(work.sum()) * kv_heads // 512 // 64) * 64)
+            parts = np.maximum(1, -(-work // most))
+            each = -(-work // parts // 64) * 64                      # whole tiles of rows
+            of = np.repeat(np.arange(parts.size), parts)
+            nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
+            lo = np.minimum(first[of] + nth * each[of], rows[of])
+            hi = np.minimum(lo + each[of], rows[of])
+            is_cut = parts[of] > 1
+            slot = np.where(is_cut, np.cumsum(is_cut) - 1, -1)
+            order = np.argsort(lo - hi, kind="stable")
+            cut = np.flatnonzero(parts > 1)
+            start = np.cumsum(parts) - parts
+            got = self._lists[group, causal, kv_heads] = (
+                self._list(seq[of][order], tile[of][order], np.where(is_cut, lo, 0)[order], np.where(is_cut, hi, rows[of])[order], slot[order]),
+                self._list(seq[cut], tile[cut], parts[cut], 0, slot[start[cut]]), int(is_cut.sum()))
+        return got
 
 
 class PackedAttentionFn(torch.autograd.Function):
@@ -245,7 +265,7 @@ class PackedAttentionFn(torch.autograd.Function):
         dims = S2GPacked(TYPES[q.dtype], H, Hk, D, int(causal), scale, *_strides(q), *_strides(k), *_strides(v), H * D, D, R, M)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         out[pack.rows:].zero_()
-        q_tiles, _ = pack.tiles(G, causal)
+        q_tiles = pack.query_tiles(G, causal)
         lse = torch.empty(Hk * R * G, dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad) else None
         if q_tiles.shape[0]:
             with _device(q):
@@ -268,14 +288,13 @@ class PackedAttentionFn(torch.autograd.Function):
         dq[pack.rows:].zero_()
         dk[pack.key_rows:].zero_()
         dv[pack.key_rows:].zero_()
-        q_tiles, k_tiles = pack.tiles(G, causal)
-        parts = _parts_of_rows(k_tiles.shape[0] * Hk, int(pack.q_len.max()) * G)
+        q_tiles, (k_tiles, cut, slots) = pack.query_tiles(G, causal), pack.key_tiles(G, causal, Hk)
         delta = torch.empty(Hk * R * G, dtype=torch.float32, device=dev)
-        work = torch.empty(get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), parts), dtype=torch.float32, device=dev)
+        work = torch.empty(get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots), dtype=torch.float32, device=dev)
         with _device(q):
             call("s2g_packed_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk),
-                 ptr(dv), ptr(work) if parts > 1 else None, parts, ptr(q_tiles), q_tiles.shape[0], ptr(k_tiles), k_tiles.shape[0],
-                 ctypes.byref(dims), stream_ptr())
+                 ptr(dv), ptr(work) if slots else None, ptr(q_tiles), q_tiles.shape[0], ptr(k_tiles), k_tiles.shape[0], ptr(cut),
+                 cut.shape[0], ctypes.byref(dims), stream_ptr())
         return dq, dk, dv, None, None, None
 
 

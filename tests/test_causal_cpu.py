@@ -71,7 +71,7 @@ def test_c_entry_points_refuse():
     l, p = lib.load(), 4096
     for change in BAD_HEADS + [dict(k_ld=4), dict(v_hd=2), dict(do_ld=-8), dict(k_rows=-1)]:
         assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, packed(**change), None) == -1, change
-        assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, 1, p, 1, p, 1, packed(**change), None) == -1, change
+        assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, None, 0, packed(**change), None) == -1, change
         assert l.s2g_packed_attention_bwd_workspace(packed(**change), 2) == -1, change
     for i in (0, 1, 2, 3, 5):
         args = [p, p, p, p, None, p]
@@ -80,9 +80,9 @@ def test_c_entry_points_refuse():
     assert l.s2g_packed_attention_fwd(p + 2, p, p, p, None, p, 1, packed(), None) == -1
     assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 0, packed(), None) == -1
     assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, None, None) == -1
-    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, 2, p, 1, p, 1, packed(), None) == -1      # parts, no workspace
-    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, 65, p, 1, p, 1, packed(), None) == -1
-    assert l.s2g_packed_attention_bwd_workspace(packed(), 3) == 2 * 3 * 10 * 2 * 64 and l.s2g_packed_attention_bwd_workspace(packed(), 1) == 0
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, p, 1, packed(), None) == -1      # cut tiles, no workspace
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, p, 1, p, 1, None, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_bwd_workspace(packed(), 3) == 3 * 256 * 2 * 64 and l.s2g_packed_attention_bwd_workspace(packed(), -1) == -1
     for change in BAD_HEADS + [dict(sequences=0), dict(sequences=65536), dict(page_size=8), dict(page_size=24), dict(page_size=1 << 17),
                                dict(pages=0), dict(table_cols=0), dict(table_cols=1 << 26), dict(max_new=0), dict(max_new=3),
                                dict(part_keys=0), dict(part_keys=100), dict(parts=0), dict(parts=5000), dict(max_length=600), dict(token_ld=3),
@@ -178,3 +178,36 @@ def test_cache_bookkeeping():
             causal.PagedKVCache(4, 16, 2, 32, dtype=torch.float64, device="cpu")
     finally:
         causal.PagedBatch = whole
+
+
+def test_key_tiles_cover_every_row_once():
+    """The key side's work list: every row that sees a tile is in exactly one of its entries, slots are consecutive."""
+    import numpy as np
+    from s2g import causal
+    old, causal._on_device = causal._on_device, lambda values, device: torch.from_numpy(np.array(values, dtype=np.int32))
+    try:
+        for q, k in (([5000, 1, 130], None), ([3], [900]), ([700, 0, 40], [100, 300, 2048]), ([1] * 200, None)):
+            pack = object.__new__(causal.PackedSequences)
+            pack.q_len, pack.k_len = np.array(q), np.array(k or q)
+            pack.q_start, pack.k_start = np.cumsum(pack.q_len) - pack.q_len, np.cumsum(pack.k_len) - pack.k_len
+            pack.device, pack._lists = "cpu", {}
+            for group, heads, is_causal in ((1, 1, True), (8, 2, True), (3, 1, False)):
+                tiles, cut, slots = pack.key_tiles(group, is_causal, heads)
+                spans, used = {}, []
+                for qs, ql, ks, kl, t, lo, hi, slot in tiles.tolist():
+                    assert lo % 64 == 0 and (hi % 64 == 0 or hi == ql * group)
+                    spans.setdefault((ks, kl, t), []).append((lo, hi))
+                    used += [slot] if slot >= 0 else []
+                assert sorted(used) == list(range(slots))
+                assert len(spans) == sum(-(-m // 128) for m in pack.k_len)
+                named = sorted(x for e in cut.tolist() for x in range(e[7], e[7] + e[5]))
+                assert named == list(range(slots))
+                for (ks, kl, t), parts in spans.items():
+                    i = [j for j in range(len(pack.k_len)) if pack.k_start[j] == ks and pack.k_len[j] == kl][0]
+                    rows = int(pack.q_len[i]) * group
+                    first = max(0, t * 128 - (kl - int(pack.q_len[i]))) * group if is_causal else 0
+                    parts.sort()
+                    assert parts[0][0] <= first or first >= rows
+                    assert all(a[1] == b[0] for a, b in zip(parts, parts[1:])) and (parts[-1][1] == rows or first >= rows)
+    finally:
+        causal._on_device = old
