@@ -21,7 +21,7 @@ __device__ __forceinline__ void tile_offsets(int* off, long ld, int D, int wave,
 }
 template <typename LT, typename T>
 __device__ __forceinline__ void fetch_rows(char* lds, const T* p, long ld, int D, int rows, const int* off, int wave) {
-  const ix4 b = buffer_of(p, (int)(((rows - 1) * ld + D) * (long)sizeof(T)));
+  const ix4 b = buffer_of(p, rows > 0 ? (int)(((rows - 1) * ld + D) * (long)sizeof(T)) : 0);
   const unsigned to = lds_address(lds);
 #pragma unroll
   for (int i = 0; i < LT::NI; ++i) load_to_lds(b, to + (i * 4 + wave) * 1024, off[i]);
@@ -57,12 +57,18 @@ __device__ __forceinline__ void store_rows(U* p, const fx16* acc, float f, int D
     }
 }
 
+// fp16 weights below 2^-14 lose bits, and a long row's weights are that small: there all of them are taken 2^RAISE times
+// as large (the sums alike, so it cancels), as much as the largest term, 2^SLACK, leaves room for.
+template <typename T> struct Weights { static constexpr float RAISE = 0.0f, SLACK = 8.0f; };
+template <> struct Weights<_Float16> { static constexpr float RAISE = 11.0f, SLACK = 4.0f; };
+
 // The running softmax of 32 rows of one wave: lane l holds row l % 32 (both halves of the wave; each its own keys).
 template <typename T, int DP>
 struct Rows {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
-  typename Vec<T>::v8 q[S::KS];
+  typedef typename Vec<T>::v8 v8;
+  v8 q[S::KS];
   fx16 o[S::DB];
   float m, l, c, slack;
 
@@ -71,28 +77,51 @@ struct Rows {
     for (int s = 0; s < S::KS; ++s) q[s] = row8(qp, 16 * s + 8 * half, D, live);
 #pragma unroll
     for (int d = 0; d < S::DB; ++d) o[d] = zero16();
-    m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = 8.0f / c;
+    m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c;
   }
-  // KB blocks of 32 keys from LDS.  edge: some row of the wave does not see all of them (`last`: the last one that this
-  // lane's row sees, counted from the tile's first); absent: keys (bits) that are not there.
-  template <int KB>
-  __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {
-    const int half = lane >> 5;
-    // S^T = K Q^T: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's own registers and
-    // one exchange between the halves
-    fx16 st[KB];
+  // S^T = K Q^T of KB blocks of 32 keys: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's
+  // own registers and one exchange between the halves.  `beside(i)` is called for the i-th product: what it does fills the
+  // 32 cycles that the matrix unit takes.  The order is laid down here (16-bit types), LDS reads two products ahead: left
+  // to itself the compiler reads one ahead, or hoists so many that registers spill.
+  template <int KB, typename F>
+  __device__ __forceinline__ void scores(fx16* st, const char* kt, int lane, F beside) const {
+    constexpr int N = KB * S::KS;
+    const int row = lane & 31, half = lane >> 5;
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      st[b] = zero16();
+    for (int b = 0; b < KB; ++b) st[b] = zero16();
+    if constexpr (sizeof(T) == 2) {
+      v8 a[3];
+      a[0] = LT::along(kt, row, 0, half);
+      if (N > 1) a[1] = LT::along(kt, row + 32 * (1 / S::KS), 1 % S::KS, half);
 #pragma unroll
-      for (int s = 0; s < S::KS; ++s) st[b] = mma(LT::along(kt, 32 * b + (lane & 31), s, half), q[s], st[b]);
+      for (int i = 0; i < N; ++i) {
+        if (i + 2 < N) a[(i + 2) % 3] = LT::along(kt, row + 32 * ((i + 2) / S::KS), (i + 2) % S::KS, half);
+        st[i / S::KS] = mma(a[i % 3], q[i % S::KS], st[i / S::KS]);
+        beside(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        st[i / S::KS] = mma(LT::along(kt, row + 32 * (i / S::KS), i % S::KS, half), q[i % S::KS], st[i / S::KS]);
+        beside(i);
+      }
     }
+  }
+  // Scores st into sums.  edge: some row of the wave does not see all of the keys (`last`: the last one that this lane's
+  // row sees, counted from the tile's first); absent: keys (bits) that are not there.  NEXT: the scores of the next tile,
+  // kt, are made meanwhile, so that the matrix unit has work while this tile's 2^x are taken.
+  template <int KB, bool NEXT>
+  __device__ __forceinline__ void add(fx16* st, fx16* next, const char* kt, const char* vt, bool edge, int last,
+                                      unsigned long long absent, int lane) {
+    const int half = lane >> 5;
     if (edge) {
+      const int at = hidden(last - 4 * half);
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * b + reg_row(i) + 4 * half > last) st[b][i] = -INFINITY;
+          if (32 * b + reg_row(i) > at) st[b][i] = -INFINITY;
     }
     if (absent) {
 #pragma unroll
@@ -109,8 +138,8 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[b][i]);
     mx = both_max(mx);
-    // the sums are rescaled only where a row's maximum has grown by a factor of 2^8: until then its terms stay below
-    // 2^8 and nothing is lost, every term being rounded relative to its own size
+    // the sums are rescaled only where a row's maximum has grown by a factor of 2^SLACK: until then its terms stay below
+    // that and nothing is lost, every term being rounded relative to its own size
     if (__any(mx > m + slack)) {
       const float mn = fmaxf(m, mx), a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
@@ -120,20 +149,61 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= a;
     }
-    const float base = m == -INFINITY ? 0.0f : m * c;
+    const float base = (m == -INFINITY ? 0.0f : m * c) - Weights<T>::RAISE;
+    v8 p[2 * KB];
+    const auto weigh = [&](int e) {                      // two weights; four pairs make an operand
+      const int b = e >> 3, i = 2 * (e & 7);
+      st[b][i] = __builtin_amdgcn_exp2f(fmaf(st[b][i], c, -base));
+      st[b][i + 1] = __builtin_amdgcn_exp2f(fmaf(st[b][i + 1], c, -base));
+      p[e >> 2][i & 7] = (T)st[b][i];
+      p[e >> 2][(i & 7) + 1] = (T)st[b][i + 1];
+      l = add_two(l, p[e >> 2], st[b], i);
+    };
+    constexpr int PAIRS = 8 * KB, N = KB * S::KS;
+    if constexpr (NEXT) {
+      scores<KB>(next, kt, lane, [&](int i) {
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+        for (int e = i * PAIRS / N; e < (i + 1) * PAIRS / N; ++e) weigh(e);
+      });
+    } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[b][i] = __builtin_amdgcn_exp2f(fmaf(st[b][i], c, -base));
-        l += st[b][i];
+      for (int e = 0; e < PAIRS; ++e) weigh(e);
+    }
+    // O^T += V^T P^T, the weights straight from the registers they are in
+    if constexpr (sizeof(T) == 2) {
+      constexpr int M = 2 * KB * S::DB;
+      v8 a[3];
+      a[0] = LT::across(vt, 0, 0, lane);
+      a[1] = LT::across(vt, 1 % S::DB, 1 / S::DB, lane);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        if (i + 2 < M) a[(i + 2) % 3] = LT::across(vt, (i + 2) % S::DB, (i + 2) / S::DB, lane);
+        o[i % S::DB] = mma(a[i % 3], p[i / S::DB], o[i % S::DB]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    // O^T += V^T P^T, the weights (rounded to the inputs' type) straight from the registers they are in
+    } else {
 #pragma unroll
-    for (int s = 0; s < 2 * KB; ++s) {
-      const typename Vec<T>::v8 p = operand<T>(st[s >> 1], s & 1);
+      for (int s = 0; s < 2 * KB; ++s)
 #pragma unroll
-      for (int d = 0; d < S::DB; ++d) o[d] = mma(LT::across(vt, d, s, lane), p, o[d]);
+        for (int d = 0; d < S::DB; ++d) o[d] = mma(LT::across(vt, d, s, lane), p[s], o[d]);
     }
   }
+  template <int KB>
+  __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {
+    fx16 st[KB];
+    scores<KB>(st, kt, lane, [](int) {});
+    add<KB, false>(st, nullptr, nullptr, vt, edge, last, absent, lane);
+  }
+  // log2 of the row's sum of exponentials, given the sum over both halves
+  __device__ __forceinline__ float log_sum(float sum) const { return fmaf(m, c, __builtin_amdgcn_logf(sum)) - Weights<T>::RAISE; }
+
+ private:
+  // a row's sum is that of the rounded weights, as its products take them, where one instruction (v_dot2) does it
+  static __device__ __forceinline__ float add_two(float l, bx8 p, const fx16&, int i) {
+    typedef __bf16 bx2 __attribute__((ext_vector_type(2)));
+    const bx2 one = {(__bf16)1.0f, (__bf16)1.0f}, two = {p[i & 7], p[(i & 7) + 1]};
+    return __builtin_amdgcn_fdot2_f32_bf16(two, one, l, false);
+  }
+  static __device__ __forceinline__ float add_two(float l, hx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
+  static __device__ __forceinline__ float add_two(float l, fx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
 };

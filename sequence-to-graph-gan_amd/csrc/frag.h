@@ -73,6 +73,13 @@ __device__ __forceinline__ fx16 zero16() {
 // the result row of register i
 __device__ __forceinline__ constexpr int reg_row(int i) { return (i & 3) + 8 * (i >> 2); }
 
+// x, of which the compiler knows nothing: comparing it with constants stays that (it would rather move x to the constants'
+// side and keep the 32 sums in registers throughout a loop)
+__device__ __forceinline__ int hidden(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // a value of this lane and of lane ^ 32: v_permlane32_swap leaves the lower half's in one register, the upper half's in
 // the other
 struct Halves {

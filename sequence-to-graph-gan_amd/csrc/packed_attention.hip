@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
                                                              PackedDims dm) {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];       // K, V, K, V
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int kvh = blockIdx.x % dm.Hk;
   const PackedTile w = tiles[blockIdx.x / dm.Hk];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
@@ -50,30 +50,48 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   int ko[LT::NI], vo[LT::NI];
   tile_offsets<LT, T>(ko, dm.ldk, dm.D, wave, lane);
   tile_offsets<LT, T>(vo, dm.ldv, dm.D, wave, lane);
+  // 32 keys at a time: while one half of a tile is summed, the scores of the next half are made.  So the tiles of K lie 32
+  // keys ahead of those of V.  LDS: K even, K odd, V even, V odd; two turns of the loop, so that every LDS address is a
+  // register and a constant.
+  const auto fetch = [&](const T* p, long ld, int key, int place, const int* off) {
+    fetch_rows<LT>(lds + place * LT::BYTES, p + (long)key * ld, ld, dm.D, min(S::KT, w.k_len - key), off, wave);
+  };
+  constexpr int HALF = 32 * S::PITCH * (int)sizeof(T);
+  fx16 one, two;
+  const int mine = w_hi < 0 ? 0 : w_hi / S::KT + 1;         // tiles that some row of this wave sees
   if (nt > 0) {
-    fetch_rows<LT>(lds, kp, dm.ldk, dm.D, min(S::KT, w.k_len), ko, wave);
-    fetch_rows<LT>(lds + LT::BYTES, vp, dm.ldv, dm.D, min(S::KT, w.k_len), vo, wave);
-  }
-  for (int t = 0; t < nt; ++t) {
-    char* kt = lds + (t & 1) * 2 * LT::BYTES;
-    const char* vt = kt + LT::BYTES;
+    fetch(kp, dm.ldk, 0, 1, ko);                            // the first 32 keys
+    fetch(kp, dm.ldk, 32, 0, ko);
+    fetch(vp, dm.ldv, 0, 2, vo);
     wait_loads();
-    __syncthreads();            // tile t is here, and everyone is done with tile t - 1, whose place tile t + 1 takes
-    if (t + 1 < nt) {
-      char* nx = lds + ((t + 1) & 1) * 2 * LT::BYTES;
-      const int k1 = (t + 1) * S::KT, n = min(S::KT, w.k_len - k1);
-      fetch_rows<LT>(nx, kp + (long)k1 * dm.ldk, dm.ldk, dm.D, n, ko, wave);
-      fetch_rows<LT>(nx + LT::BYTES, vp + (long)k1 * dm.ldv, dm.ldv, dm.D, n, vo, wave);
-    }
+    __syncthreads();
+    r.template scores<1>(&one, lds + LT::BYTES, lane, [](int) {});
+  }
+  const auto turn = [&](int t, auto parity) {
+    constexpr int P = decltype(parity)::value;
+    wait_loads();
+    __syncthreads();            // this turn's K and V are here; everyone is done with the last turn's
     const int k0 = t * S::KT;
-    if (k0 > w_hi) continue;    // none of this wave's rows sees this tile
-    r.template step<S::KB>(kt, vt, k0 + S::KT - 1 > w_lo, last - k0, 0, lane);
+    if (t + 1 < nt) {
+      fetch(kp, dm.ldk, k0 + S::KT + 32, 1 - P, ko);
+      fetch(vp, dm.ldv, k0 + S::KT, 3 - P, vo);
+    }
+    if (t >= mine) return;
+    const char* kt = lds + P * LT::BYTES;                   // behind the last key: scores that nobody takes
+    const char* vt = lds + (2 + P) * LT::BYTES;
+    r.template add<1, true>(&one, &two, kt, vt, k0 + 31 > w_lo, last - k0, 0, lane);
+    if constexpr (S::KB == 2) r.template add<1, true>(&two, &one, kt + HALF, vt + HALF, k0 + 63 > w_lo, last - k0 - 32, 0, lane);
+    else one = two;
+  };
+  for (int t = 0; t < nt; t += 2) {
+    turn(t, std::integral_constant<int, 0>{});
+    if (t + 1 < nt) turn(t + 1, std::integral_constant<int, 1>{});
   }
   const float l = both_sum(r.l);
   store_rows<T, S::DB>(out + (qrow * dm.H + head) * dm.D, r.o, l == 0.0f ? 0.0f : 1.0f / l, dm.D, half, live);
   // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
   if (lse && live && half == 0)
-    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : fmaf(r.m, r.c, __builtin_amdgcn_logf(l));
+    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
 }
 
 // ------------------------------------------------------------------------------------------------- backward, query side
@@ -154,9 +172,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 #pragma unroll
       for (int s = 0; s < S::KS; ++s) dp = mma(LT::along(vt, 32 * b + (lane & 31), s, half), g[s], dp);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], c, -L)) * (dp[i] - dl);
-        if (edge && k0 + 32 * b + reg_row(i) + 4 * half > last) st[i] = 0.0f;
+      for (int i = 0; i < 16; ++i) st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], c, -L)) * (dp[i] - dl);
+      if (edge) {
+        const int at = hidden(last - k0 - 4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + reg_row(i) > at) st[i] = 0.0f;
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -231,9 +252,10 @@ struct KeySums {
         }
       }
       if (edge) {
+        const int at = hidden(first - 4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * b + reg_row(i) + 4 * half < first) p[i] = 0.0f, ds[i] = 0.0f;
+          if (32 * b + reg_row(i) < at) p[i] = 0.0f, ds[i] = 0.0f;
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
