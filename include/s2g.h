@@ -365,7 +365,7 @@ int s2g_attention_bwd(const float* Q, const float* K, const float* V, const floa
  * n_q (causal) or all of them; a row that sees none gives zeros and no gradient.  Rows of no sequence are not touched.
  * The tile list has one entry per 128 rows (token, head of the group) of a sequence: ceil(n_q heads / kv_heads / 128)
  * of them, in any order.  k_tiles: one per 128 keys with slot -1 and all rows (row_lo 0, row_hi n_q heads / kv_heads), or
- * several that share its rows out among them (bounds multiples of 64), with consecutive slots of their own; each tile so
+ * several that share its rows out among them (bounds multiples of 128), with consecutive slots of their own; each tile so
  * cut has an entry in cut_tiles, row_lo the number and slot the first of its slots.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
  * exponentials, for the backward pass (may be NULL in fwd); delta has its size. */
 typedef struct S2GPackedTile {

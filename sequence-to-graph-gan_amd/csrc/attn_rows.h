@@ -7,6 +7,7 @@ struct Shape {
   static constexpr int PITCH = DP == 96 ? 128 : DP;
   static constexpr int KT = sizeof(T) == 2 ? 64 : 32;        // keys (rows, in the key-side backward pass) per LDS tile
   static constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  static constexpr int AHEAD = 2;
   typedef Tile<T, PITCH, KT, 4> LT;
 };
 
@@ -80,33 +81,13 @@ struct Rows {
     m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c;
   }
   // S^T = K Q^T of KB blocks of 32 keys: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's
-  // own registers and one exchange between the halves.  `beside(i)` is called for the i-th product: what it does fills the
-  // 32 cycles that the matrix unit takes.  The order is laid down here (16-bit types), LDS reads two products ahead: left
-  // to itself the compiler reads one ahead, or hoists so many that registers spill.
+  // own registers and one exchange between the halves
   template <int KB, typename F>
   __device__ __forceinline__ void scores(fx16* st, const char* kt, int lane, F beside) const {
-    constexpr int N = KB * S::KS;
-    const int row = lane & 31, half = lane >> 5;
 #pragma unroll
     for (int b = 0; b < KB; ++b) st[b] = zero16();
-    if constexpr (sizeof(T) == 2) {
-      v8 a[3];
-      a[0] = LT::along(kt, row, 0, half);
-      if (N > 1) a[1] = LT::along(kt, row + 32 * (1 / S::KS), 1 % S::KS, half);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + 2 < N) a[(i + 2) % 3] = LT::along(kt, row + 32 * ((i + 2) / S::KS), (i + 2) % S::KS, half);
-        st[i / S::KS] = mma(a[i % 3], q[i % S::KS], st[i / S::KS]);
-        beside(i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        st[i / S::KS] = mma(LT::along(kt, row + 32 * (i / S::KS), i % S::KS, half), q[i % S::KS], st[i / S::KS]);
-        beside(i);
-      }
-    }
+    products<T, KB * S::KS, S::AHEAD>([&](int i) { return LT::along(kt, (lane & 31) + 32 * (i / S::KS), i % S::KS, lane >> 5); },
+                            [&](int i, const v8& a) { st[i / S::KS] = mma(a, q[i % S::KS], st[i / S::KS]); }, beside);
   }
   // Scores st into sums.  edge: some row of the wave does not see all of the keys (`last`: the last one that this lane's
   // row sees, counted from the tile's first); absent: keys (bits) that are not there.  NEXT: the scores of the next tile,
@@ -170,23 +151,8 @@ struct Rows {
       for (int e = 0; e < PAIRS; ++e) weigh(e);
     }
     // O^T += V^T P^T, the weights straight from the registers they are in
-    if constexpr (sizeof(T) == 2) {
-      constexpr int M = 2 * KB * S::DB;
-      v8 a[3];
-      a[0] = LT::across(vt, 0, 0, lane);
-      a[1] = LT::across(vt, 1 % S::DB, 1 / S::DB, lane);
-#pragma unroll
-      for (int i = 0; i < M; ++i) {
-        if (i + 2 < M) a[(i + 2) % 3] = LT::across(vt, (i + 2) % S::DB, (i + 2) / S::DB, lane);
-        o[i % S::DB] = mma(a[i % 3], p[i / S::DB], o[i % S::DB]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 2 * KB; ++s)
-#pragma unroll
-        for (int d = 0; d < S::DB; ++d) o[d] = mma(LT::across(vt, d, s, lane), p[s], o[d]);
-    }
+    products<T, 2 * KB * S::DB, S::AHEAD>([&](int i) { return LT::across(vt, i % S::DB, i / S::DB, lane); },
+                                [&](int i, const v8& a) { o[i % S::DB] = mma(a, p[i / S::DB], o[i % S::DB]); }, [](int) {});
   }
   template <int KB>
   __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {

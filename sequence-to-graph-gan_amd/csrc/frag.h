@@ -198,5 +198,30 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
+// N products in a row: load(i) fetches the LDS operand of product i, use(i, a) makes it, beside(i) is arithmetic that fills
+// the 32 cycles a 16-bit product takes.  For 16-bit types the order is laid down here, LDS reads AHEAD products ahead: left
+// to itself the compiler reads one ahead, or hoists so many that registers spill.  fp32 products take eight times as long.
+template <typename T, int N, int AHEAD, typename L, typename U, typename B>
+__device__ __forceinline__ void products(L load, U use, B beside) {
+  if constexpr (sizeof(T) == 2) {
+    typename Vec<T>::v8 a[AHEAD + 1];
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < N; ++i) a[i] = load(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + AHEAD < N) a[(i + AHEAD) % (AHEAD + 1)] = load(i + AHEAD);
+      use(i, a[i % (AHEAD + 1)]);
+      beside(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      use(i, load(i));
+      beside(i);
+    }
+  }
+}
+
 // wave-uniform values: tells the compiler to keep them in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }

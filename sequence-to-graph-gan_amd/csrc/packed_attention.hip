@@ -196,35 +196,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 // for the chip, the host cuts a tile's rows into ranges, each leaving a 32-bit partial result in a slot of its own that
 // s2g_k_packed_attn_sum adds in a fixed order: no atomics, the same bits every time.
 //
-// The sums of dK and dV of 32 keys, with their K and V, leave room for one wave to a SIMD at 96 or 128 16-bit features,
-// and one wave alone keeps the matrix unit idle while it makes P and dS.  There 8 waves share the work: waves 0 .. 3 take
-// S and dV, waves 4 .. 7 S, dP and dK of the same keys, 40 products where 32 would do, but two waves to a SIMD
-// (DKV_SPLIT_FIGURES).
+// Two forms.  Up to 64 16-bit features, and in fp32, a wave takes 32 keys.  Beyond, the sums of dK and dV of 32 keys with
+// their K and V leave room for only one wave to a SIMD, which keeps the matrix unit idle while it makes P and dS; so there
+// two waves share 32 keys (s2g_k_packed_attn_bwd_kv2).
 template <typename T, int DP>
-struct KeySide {
-  static constexpr bool SPLIT = sizeof(T) == 2 && DP > 64;
-  static constexpr int WAVES = SPLIT ? 8 : 4;
-  typedef Tile<T, Shape<T, DP>::PITCH, Shape<T, DP>::KT, WAVES> LT;
-};
-
-template <typename T, int DP, bool DV, bool DK>
 struct KeySums {
   typedef Shape<T, DP> S;
-  typedef typename KeySide<T, DP>::LT LT;
+  typedef typename S::LT LT;
   typedef typename Vec<T>::v8 v8;
-  v8 k[S::KS], v[DK ? S::KS : 1];
-  fx16 dv[DV ? S::DB : 1], dk[DK ? S::DB : 1];
+  v8 k[S::KS], v[S::KS];
+  fx16 dv[S::DB], dk[S::DB];
 
   __device__ __forceinline__ void begin(const T* kp, const T* vp, int D, bool live, int half) {
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) {
       k[s] = row8(kp, 16 * s + 8 * half, D, live);
-      if constexpr (DK) v[s] = row8(vp, 16 * s + 8 * half, D, live);
+      v[s] = row8(vp, 16 * s + 8 * half, D, live);
     }
 #pragma unroll
     for (int d = 0; d < S::DB; ++d) {
-      if constexpr (DV) dv[d] = zero16();
-      if constexpr (DK) dk[d] = zero16();
+      dv[d] = zero16();
+      dk[d] = zero16();
     }
   }
   // a tile of rows: Q, dO, (L, D); edge: some of them do not see some of the wave's keys (`first`: the first that sees this
@@ -236,19 +228,17 @@ struct KeySums {
       fx16 p = zero16(), ds = zero16();
 #pragma unroll
       for (int s = 0; s < S::KS; ++s) p = mma(LT::along(qt, 32 * b + col, s, half), k[s], p);
-      if constexpr (DK)
 #pragma unroll
-        for (int s = 0; s < S::KS; ++s) ds = mma(LT::along(gt, 32 * b + col, s, half), v[s], ds);
+      for (int s = 0; s < S::KS; ++s) ds = mma(LT::along(gt, 32 * b + col, s, half), v[s], ds);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const fx4 L = *reinterpret_cast<const fx4*>(sl + 32 * b + 8 * g + 4 * half);
-        fx4 D;
-        if constexpr (DK) D = *reinterpret_cast<const fx4*>(sl + S::KT + 32 * b + 8 * g + 4 * half);
+        const fx4 D = *reinterpret_cast<const fx4*>(sl + S::KT + 32 * b + 8 * g + 4 * half);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * g + j;
           p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -L[j]));
-          if constexpr (DK) ds[i] = p[i] * (ds[i] - D[j]);
+          ds[i] = p[i] * (ds[i] - D[j]);
         }
       }
       if (edge) {
@@ -259,52 +249,47 @@ struct KeySums {
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if constexpr (DV) {
-          const v8 pt = operand<T>(p, s);
+        const v8 pt = operand<T>(p, s), dt = operand<T>(ds, s);
 #pragma unroll
-          for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
-        }
-        if constexpr (DK) {
-          const v8 dt = operand<T>(ds, s);
+        for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
 #pragma unroll
-          for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
-        }
+        for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
       }
     }
   }
 };
 
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * (KeySide<T, DP>::WAVES), sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_kv(
-    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
-    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dK, T* __restrict__ dV,
-    float* __restrict__ partial, const PackedTile* __restrict__ tiles, PackedDims dm) {
-  typedef Shape<T, DP> S;
-  typedef typename KeySide<T, DP>::LT LT;
-  constexpr int WAVES = KeySide<T, DP>::WAVES;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];       // Q, dO, Q, dO, then 2 x (L, D)
-  float* stats = reinterpret_cast<float*>(lds + 4 * LT::BYTES);
-  const int kvh = blockIdx.x % dm.Hk;
-  const PackedTile w = tiles[blockIdx.x / dm.Hk];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
-  const int G = dm.by.G, rows = w.q_len * G, w_key = w.tile * 128 + 32 * (wave & 3), key = w_key + (lane & 31);
-  const bool live = key < w.k_len;
-  const long krow = (long)w.k_start + min(key, w.k_len - 1);
-  // the first row that sees this key, the wave's first and last, the workgroup's first
-  const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
-  const int first = !live ? 0x7fffffff : max(0, key - shift) * G;
-  const int w_lo = w_key < w.k_len ? max(0, w_key - shift) * G : 0x7fffffff, w_hi = max(0, min(w_key + 31, w.k_len - 1) - shift) * G;
-  const bool ragged = w_key + 31 >= w.k_len;
-  const int b_lo = max(max(0, w.tile * 128 - shift) * G, w.row_lo);
-  const int t0 = b_lo / S::KT, t1 = (min(rows, w.row_hi) + S::KT - 1) / S::KT;     // row_lo, row_hi: whole tiles
-
-  const T* qb = Q + (long)w.q_start * dm.ldq + kvh * G * dm.hq;
-  const T* gb = dO + (long)w.q_start * dm.ldo + kvh * G * dm.ho;
-  const long lb = ((long)kvh * dm.q_rows + w.q_start) * G;
-  auto fetch = [&](int t, int into) {
-    const unsigned to = lds_address(lds) + into * 2 * LT::BYTES;
-    const int r0 = t * S::KT, tok0 = divide(r0, dm.by);
-    const ix4 qr = buffer_of(qb + tok0 * dm.ldq, 0x7ffffe00), gr = buffer_of(gb + tok0 * dm.ldo, 0x7ffffe00);
+// What both forms know of a wave's 32 keys and of the rows that see them
+struct KeyWork {
+  PackedTile w;
+  int kvh, rows, first, w_lo, w_hi, t0, t1;
+  bool live, ragged;
+  long krow, lrow;
+  // ROWS rows to a tile; `group`: which 32 of the tile's 128 keys
+  template <int ROWS>
+  __device__ __forceinline__ void begin(const PackedTile* tiles, int group, int lane, const PackedDims& dm) {
+    kvh = blockIdx.x % dm.Hk;
+    w = tiles[blockIdx.x / dm.Hk];
+    const int G = dm.by.G, w_key = w.tile * 128 + 32 * group, key = w_key + (lane & 31);
+    rows = w.q_len * G;
+    live = key < w.k_len;
+    krow = (long)w.k_start + min(key, w.k_len - 1);
+    lrow = ((long)kvh * dm.q_rows + w.q_start) * G;
+    // the first row that sees this key, the wave's first and last, the tiles of rows that see some key of the workgroup
+    const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
+    first = !live ? 0x7fffffff : max(0, key - shift) * G;
+    w_lo = w_key < w.k_len ? max(0, w_key - shift) * G : 0x7fffffff;
+    w_hi = max(0, min(w_key + 31, w.k_len - 1) - shift) * G;
+    ragged = w_key + 31 >= w.k_len;
+    t0 = max(max(0, w.tile * 128 - shift) * G, w.row_lo) / ROWS;           // row_lo, row_hi: whole tiles
+    t1 = (min(rows, w.row_hi) + ROWS - 1) / ROWS;
+  }
+  // Q and dO of the ROWS rows from r0 on, side by side: the group's heads of a token, then the next token
+  template <typename LT, int WAVES, typename T>
+  __device__ __forceinline__ void fetch(unsigned to, int r0, const T* Q, const T* dO, int wave, int lane, const PackedDims& dm) const {
+    const int G = dm.by.G, tok0 = divide(r0, dm.by);
+    const ix4 qr = buffer_of(Q + ((long)w.q_start + tok0) * dm.ldq + kvh * G * dm.hq, 0x7ffffe00);
+    const ix4 gr = buffer_of(dO + ((long)w.q_start + tok0) * dm.ldo + kvh * G * dm.ho, 0x7ffffe00);
 #pragma unroll
     for (int i = 0; i < LT::NI; ++i) {
       const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
@@ -312,59 +297,209 @@ __global__ __launch_bounds__(64 * (KeySide<T, DP>::WAVES), sizeof(T) == 2 ? 2 : 
       load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
       load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
     }
+  }
+  template <typename T, int DB>
+  __device__ __forceinline__ void store(T* out, float* partial, int second, const fx16* acc, float f, int group, int lane, const PackedDims& dm) const {
+    if (w.slot < 0) store_rows<T, DB>(out + (krow * dm.Hk + kvh) * dm.D, acc, f, dm.D, lane >> 5, live);
+    else store_rows<T, DB>(partial + (((long)w.slot * dm.Hk + kvh) * 256 + 128 * second + 32 * group + (lane & 31)) * dm.D, acc, f, dm.D, lane >> 5, live);
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_kv(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
+    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dK, T* __restrict__ dV,
+    float* __restrict__ partial, const PackedTile* __restrict__ tiles, PackedDims dm) {
+  typedef Shape<T, DP> S;
+  typedef typename S::LT LT;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];       // Q, dO, Q, dO, then 2 x (L, D)
+  float* stats = reinterpret_cast<float*>(lds + 4 * LT::BYTES);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  KeyWork kw;
+  kw.begin<S::KT>(tiles, wave, lane, dm);
+  const auto fetch = [&](int t) {
+    kw.fetch<LT, 4>(lds_address(lds) + (t & 1) * 2 * LT::BYTES, t * S::KT, Q, dO, wave, lane, dm);
   };
   float st_next = 0.0f;
-  auto stat = [&](int t) {                                            // threads 0 .. 2 KT: L, then D of the tile's rows
+  const auto stat = [&](int t) {                                      // threads 0 .. 2 KT: L, then D of the tile's rows
     const int r = t * S::KT + (threadIdx.x & (S::KT - 1));
     st_next = 0.0f;
-    if (threadIdx.x < 2 * S::KT && r < rows) st_next = (threadIdx.x < S::KT ? lse : delta)[lb + r];
+    if (threadIdx.x < 2 * S::KT && r < kw.rows) st_next = (threadIdx.x < S::KT ? lse : delta)[kw.lrow + r];
   };
   const float c = dm.scale * LOG2E;
-  const T* kp = K + krow * dm.ldk + kvh * dm.hk;
-  const T* vp = V + krow * dm.ldv + kvh * dm.hv;
-  const long orow = (krow * dm.Hk + kvh) * dm.D;
-  float* slot = partial + (((long)w.slot * dm.Hk + kvh) * 256 + 32 * (wave & 3) + (lane & 31)) * dm.D;    // dK, then dV
+  if (kw.t0 < kw.t1) {
+    stat(kw.t0);
+    fetch(kw.t0);
+  }
+  KeySums<T, DP> sums;
+  sums.begin(K + kw.krow * dm.ldk + kw.kvh * dm.hk, V + kw.krow * dm.ldv + kw.kvh * dm.hv, dm.D, kw.live, lane >> 5);
+  for (int t = kw.t0; t < kw.t1; ++t) {
+    const char* qt = lds + (t & 1) * 2 * LT::BYTES;
+    float* sl = stats + (t & 1) * 2 * S::KT;
+    wait_loads();
+    if (threadIdx.x < 2 * S::KT) sl[threadIdx.x] = st_next;
+    __syncthreads();
+    if (t + 1 < kw.t1) {
+      stat(t + 1);
+      fetch(t + 1);
+    }
+    const int r0 = t * S::KT;
+    if (r0 + S::KT <= kw.w_lo) continue;                              // none of these rows sees this wave's keys
+    sums.step(qt, qt + LT::BYTES, sl, c, kw.ragged || r0 < kw.w_hi, kw.first - r0, lane);
+  }
+  kw.store<T, S::DB>(dK, partial, 0, sums.dk, dm.scale, wave, lane, dm);
+  kw.store<T, S::DB>(dV, partial, 1, sums.dv, 1.0f, wave, lane, dm);
+}
+
+// Two waves to 32 keys: wave g of the first four makes S, P and dV, wave 4 + g dP, dS and dK.  P goes from one to the other
+// through LDS, raised by 2^14 and rounded to fp16 (half a step is 2^-11 of it: an eighth of what rounding dS to bf16 adds,
+// and it is nothing at all where fp16 is the type and dV takes the same weights).  The first four are a tile of 64 rows
+// ahead, so that neither waits for the other within one.
+template <typename T, int DP>
+struct PairSums {
+  typedef Shape<T, DP> S;
+  typedef Tile<T, S::PITCH, 64, 8> LT;
+  typedef typename Vec<T>::v8 v8;
+  static constexpr float RAISE = 14.0f, LOWER = 1.0f / 16384.0f;
+  v8 k[S::KS];                                     // K of the first four, V of the others
+  fx16 sum[S::DB];
+
+  __device__ __forceinline__ void begin(const T* p, int D, bool live, int half) {
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s) k[s] = row8(p, 16 * s + 8 * half, D, live);
+#pragma unroll
+    for (int d = 0; d < S::DB; ++d) sum[d] = zero16();
+  }
+  template <typename B>
+  __device__ __forceinline__ void rows_by_keys(const char* tile, int b, fx16& to, int lane, B beside) const {
+    to = zero16();
+    products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(tile, 32 * b + (lane & 31), i, lane >> 5); },
+                                 [&](int i, const v8& a) { to = mma(a, k[i], to); }, beside);
+  }
+  __device__ __forceinline__ void add(const char* tile, int b, const v8* x, int lane) {
+    products<T, 2 * S::DB, S::AHEAD>([&](int i) { return LT::across(tile, i % S::DB, 2 * b + i / S::DB, lane); },
+                                     [&](int i, const v8& a) { sum[i % S::DB] = mma(a, x[i / S::DB], sum[i % S::DB]); }, [](int) {});
+  }
+  // f(0 .. 3) over the S::KS products that they stand beside
+  template <typename F>
+  static __device__ __forceinline__ auto spread(F f) {
+    return [f](int i) {
+#pragma unroll
+      for (int g = 4 * i / S::KS; g < 4 * (i + 1) / S::KS; ++g) f(g);
+    };
+  }
+  static __device__ __forceinline__ void mask(fx16& x, int first, int lane) {
+    const int at = hidden(first - 4 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (reg_row(i) < at) x[i] = 0.0f;
+  }
+  // 64 rows: P to `share` ([block][2][lane] of 16 bytes), dV^T += dO^T P
+  __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, hx8* share, float c, bool edge, int first, int lane) {
+    fx16 p, next;
+    rows_by_keys(qt, 0, p, lane, [](int) {});
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const auto weigh = [&](int g) {
+        const fx4 l = *reinterpret_cast<const fx4*>(L + 32 * b + 8 * g + 4 * (lane >> 5));
+#pragma unroll
+        for (int i = 4 * g; i < 4 * g + 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, RAISE - l[i & 3]));
+      };
+      if (b == 0) rows_by_keys(qt, 1, next, lane, spread(weigh));
+      else
+#pragma unroll
+        for (int g = 0; g < 4; ++g) weigh(g);
+      if (edge) mask(p, first - 32 * b, lane);
+      const hx8 h[2] = {operand<_Float16>(p, 0), operand<_Float16>(p, 1)};
+      share[(2 * b) * 64 + lane] = h[0];
+      share[(2 * b + 1) * 64 + lane] = h[1];
+      const v8 x[2] = {operand<T>(p, 0), operand<T>(p, 1)};
+      add(gt, b, x, lane);
+      p = next;
+    }
+  }
+  // the same 64 rows, P taken from `share`: dK^T += Q^T dS
+  __device__ __forceinline__ void slopes(const char* qt, const char* gt, const float* D, const hx8* share, bool edge, int first, int lane) {
+    fx16 ds, next;
+    rows_by_keys(gt, 0, ds, lane, [](int) {});
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const hx8 h[2] = {share[(2 * b) * 64 + lane], share[(2 * b + 1) * 64 + lane]};
+      const auto slope = [&](int g) {
+        const fx4 d = *reinterpret_cast<const fx4*>(D + 32 * b + 8 * g + 4 * (lane >> 5));
+#pragma unroll
+        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = (float)h[i >> 3][i & 7] * (fmaf(ds[i], LOWER, -d[i & 3]));
+      };
+      if (b == 0) rows_by_keys(gt, 1, next, lane, spread(slope));
+      else
+#pragma unroll
+        for (int g = 0; g < 4; ++g) slope(g);
+      if (edge) mask(ds, first - 32 * b, lane);
+      const v8 x[2] = {operand<T>(ds, 0), operand<T>(ds, 1)};
+      add(qt, b, x, lane);
+      ds = next;
+    }
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
+    const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dK, T* __restrict__ dV,
+    float* __restrict__ partial, const PackedTile* __restrict__ tiles, PackedDims dm) {
+  typedef PairSums<T, DP> P;
+  typedef typename P::LT LT;
+  constexpr int DB = Shape<T, DP>::DB;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];       // 3 x (Q, dO), 2 x 4 x P, 3 x (L, D)
+  hx8* shares = reinterpret_cast<hx8*>(lds + 6 * LT::BYTES);
+  float* stats = reinterpret_cast<float*>(lds + 6 * LT::BYTES + 32768);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), group = wave & 3;
+  KeyWork kw;
+  kw.begin<64>(tiles, group, lane, dm);
+  const int t0 = kw.t0, t1 = kw.t1;
+  const auto fetch = [&](int t) {
+    kw.fetch<LT, 8>(lds_address(lds) + (t - t0) % 3 * 2 * LT::BYTES, t * 64, Q, dO, wave, lane, dm);
+  };
+  float st_next = 0.0f;
+  const auto stat = [&](int t) {                                      // threads 0 .. 127: L, then D of the tile's rows
+    const int r = t * 64 + (threadIdx.x & 63);
+    st_next = 0.0f;
+    if (threadIdx.x < 128 && r < kw.rows) st_next = (threadIdx.x < 64 ? lse : delta)[kw.lrow + r] * (threadIdx.x < 64 ? 1.0f : P::LOWER);
+  };
+  const float c = dm.scale * LOG2E;
   if (t0 < t1) {
     stat(t0);
-    fetch(t0, t0 & 1);
+    fetch(t0);
   }
-  // every wave goes through the same tiles and barriers, whichever of the sums are its own
-  auto all_tiles = [&](auto& sums, auto dk_mine, auto dv_mine) {
-    sums.begin(kp, vp, dm.D, live, half);
-    for (int t = t0; t < t1; ++t) {
-      const char* qt = lds + (t & 1) * 2 * LT::BYTES;
-      float* sl = stats + (t & 1) * 2 * S::KT;
+  P sums;
+  if (wave < 4) sums.begin(K + kw.krow * dm.ldk + kw.kvh * dm.hk, dm.D, kw.live, lane >> 5);
+  else sums.begin(V + kw.krow * dm.ldv + kw.kvh * dm.hv, dm.D, kw.live, lane >> 5);
+  // turn t: the first four at tile t, the others at tile t - 1, tile t + 1 on its way
+  const auto turns = [&](auto first_four) {
+    for (int t = t0; t <= t1; ++t) {
       wait_loads();
-      if (threadIdx.x < 2 * S::KT) sl[threadIdx.x] = st_next;
+      if (threadIdx.x < 128 && t < t1) stats[(t - t0) % 3 * 128 + threadIdx.x] = st_next;
       __syncthreads();
       if (t + 1 < t1) {
         stat(t + 1);
-        fetch(t + 1, (t + 1) & 1);
+        fetch(t + 1);
       }
-      const int r0 = t * S::KT;
-      if (r0 + S::KT <= w_lo) continue;                              // none of these rows sees this wave's keys
-      sums.step(qt, qt + LT::BYTES, sl, c, ragged || r0 < w_hi, first - r0, lane);
-    }
-    if constexpr (dk_mine.value) {
-      if (w.slot < 0) store_rows<T, S::DB>(dK + orow, sums.dk, dm.scale, dm.D, half, live);
-      else store_rows<T, S::DB>(slot, sums.dk, dm.scale, dm.D, half, live);
-    }
-    if constexpr (dv_mine.value) {
-      if (w.slot < 0) store_rows<T, S::DB>(dV + orow, sums.dv, 1.0f, dm.D, half, live);
-      else store_rows<T, S::DB>(slot + 128 * dm.D, sums.dv, 1.0f, dm.D, half, live);
+      const int mine = first_four.value ? t : t - 1, r0 = mine * 64;
+      if (t0 == t1 || mine < t0 || mine >= t1 || r0 + 64 <= kw.w_lo) continue;       // none of these rows sees this wave's keys
+      const char* qt = lds + (mine - t0) % 3 * 2 * LT::BYTES;
+      const float* st = stats + (mine - t0) % 3 * 128;
+      hx8* share = shares + ((mine & 1) * 4 + group) * 256;
+      const bool edge = kw.ragged || r0 < kw.w_hi;
+      if constexpr (first_four.value) sums.weights(qt, qt + LT::BYTES, st, share, c, edge, kw.first - r0, lane);
+      else sums.slopes(qt, qt + LT::BYTES, st + 64, share, edge, kw.first - r0, lane);
     }
   };
-  if constexpr (KeySide<T, DP>::SPLIT) {
-    if (wave < 4) {
-      KeySums<T, DP, true, false> sums;
-      all_tiles(sums, std::false_type{}, std::true_type{});
-    } else {
-      KeySums<T, DP, false, true> sums;
-      all_tiles(sums, std::true_type{}, std::false_type{});
-    }
+  if (wave < 4) {
+    turns(std::true_type{});
+    kw.store<T, DB>(dV, partial, 1, sums.sum, P::LOWER, group, lane, dm);
   } else {
-    KeySums<T, DP, true, true> sums;
-    all_tiles(sums, std::true_type{}, std::true_type{});
+    turns(std::false_type{});
+    kw.store<T, DB>(dK, partial, 0, sums.sum, dm.scale, group, lane, dm);
   }
 }
 
@@ -411,17 +546,25 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
                       float* delta, void* dQ, void* dK, void* dV, float* partial, const PackedTile* qt, int nqt,
                       const PackedTile* kt, int nkt, const PackedTile* cut, int ncut, const PackedDims& dm, hipStream_t st) {
   typedef typename Shape<T, DP>::LT LT;
-  const int qb = 4 * LT::BYTES, kb = 4 * LT::BYTES + 4 * Shape<T, DP>::KT * (int)sizeof(float);
+  constexpr bool PAIR = sizeof(T) == 2 && DP > 64;
+  const int qb = 4 * LT::BYTES;
   static S2GLdsCap qcap, kcap;
   const auto kq = s2g_k_packed_attn_bwd_q<T, DP>;
-  const auto kk = s2g_k_packed_attn_bwd_kv<T, DP>;
-  if (s2g_lds_cap(qcap, reinterpret_cast<const void*>(kq), qb) != 0 || s2g_lds_cap(kcap, reinterpret_cast<const void*>(kk), kb) != 0) return -2;
-  if (nqt > 0)
-    hipLaunchKernelGGL(kq, dim3((unsigned)nqt * dm.Hk), dim3(256), qb, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out,
-                       (const T*)dO, lse, delta, (T*)dQ, qt, dm);
-  if (nkt > 0)
-    hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk), dim3(64 * KeySide<T, DP>::WAVES), kb, st, (const T*)Q, (const T*)K,
-                       (const T*)V, (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
+  if (s2g_lds_cap(qcap, reinterpret_cast<const void*>(kq), qb) != 0) return -2;
+  const auto key_side = [&](auto kk, int threads, int bytes) {
+    if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kk), bytes) != 0) return -2;
+    if (nqt > 0)
+      hipLaunchKernelGGL(kq, dim3((unsigned)nqt * dm.Hk), dim3(256), qb, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out,
+                         (const T*)dO, lse, delta, (T*)dQ, qt, dm);
+    if (nkt > 0)
+      hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk), dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V,
+                         (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
+    return 0;
+  };
+  int rc;
+  if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, 6 * PairSums<T, DP>::LT::BYTES + 32768 + 3 * 128 * (int)sizeof(float));
+  else rc = key_side(s2g_k_packed_attn_bwd_kv<T, DP>, 256, 4 * LT::BYTES + 4 * Shape<T, DP>::KT * (int)sizeof(float));
+  if (rc != 0) return rc;
   if (ncut > 0)
     hipLaunchKernelGGL(s2g_k_packed_attn_sum<T>, dim3((unsigned)ncut * dm.Hk, 8), dim3(256), 0, st, partial, (T*)dK, (T*)dV, cut, dm);
   return hipGetLastError() == hipSuccess ? 0 : -2;

@@ -236,11 +236,11 @@ class PackedSequences:
         if got is None:
             seq, tile = self._tiles(self.k_len)
             rows = (self.q_len * group)[seq]
-            first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // 64 * 64 if causal else np.zeros_like(rows)
+            first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // TILE * TILE if causal else np.zeros_like(rows)
             work = np.maximum(0, rows - first)
-            most = max(512, -(-int(work.sum()) * kv_heads // 512 // 64) * 64)
+            most = max(512, -(-int(work.sum()) * kv_heads // 512 // TILE) * TILE)
             parts = np.maximum(1, -(-work // most))
-            each = -(-work // parts // 64) * 64                      # whole tiles of rows
+            each = -(-work // parts // TILE) * TILE                      # whole tiles of rows
             of = np.repeat(np.arange(parts.size), parts)
             nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
             lo = np.minimum(first[of] + nth * each[of], rows[of])

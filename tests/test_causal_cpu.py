@@ -195,7 +195,7 @@ def test_key_tiles_cover_every_row_once():
                 tiles, cut, slots = pack.key_tiles(group, is_causal, heads)
                 spans, used = {}, []
                 for qs, ql, ks, kl, t, lo, hi, slot in tiles.tolist():
-                    assert lo % 64 == 0 and (hi % 64 == 0 or hi == ql * group)
+                    assert lo % 128 == 0 and (hi % 128 == 0 or hi == ql * group)
                     spans.setdefault((ks, kl, t), []).append((lo, hi))
                     used += [slot] if slot >= 0 else []
                 assert sorted(used) == list(range(slots))
