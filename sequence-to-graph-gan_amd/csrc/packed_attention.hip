@@ -284,18 +284,37 @@ struct KeyWork {
     t0 = max(max(0, w.tile * 128 - shift) * G, w.row_lo) / ROWS;           // row_lo, row_hi: whole tiles
     t1 = (min(rows, w.row_hi) + ROWS - 1) / ROWS;
   }
-  // Q and dO of the ROWS rows from r0 on, side by side: the group's heads of a token, then the next token
-  template <typename LT, int WAVES, typename T>
-  __device__ __forceinline__ void fetch(unsigned to, int r0, const T* Q, const T* dO, int wave, int lane, const PackedDims& dm) const {
+  // Q and dO of a tile of rows from r0 on, side by side: the group's heads of a token, then the next token.  Where whole
+  // tokens fill the tiles (`off`, made once by offsets()) a tile is fetched as the one before; other groups divide anew.
+  template <typename LT, typename T>
+  __device__ __forceinline__ void offsets(int* off, long ld, long hd, int wave, int lane, const PackedDims& dm) const {
+#pragma unroll
+    for (int i = 0; i < LT::NI; ++i) {
+      const int r = LT::row_of(i, wave, lane), tk = divide(r, dm.by), ch = LT::chunk_of(i, wave, lane) * 16;
+      off[i] = ch < dm.D * (int)sizeof(T) ? (int)((tk * ld + (r - tk * dm.by.G) * hd) * (long)sizeof(T)) + ch : OUT_OF_BUFFER;
+    }
+  }
+  template <typename LT, int WAVES, int ROWS, typename T>
+  __device__ __forceinline__ void fetch(unsigned to, int r0, const T* Q, const T* dO, const int* qoff, const int* goff, int wave,
+                                        int lane, const PackedDims& dm) const {
     const int G = dm.by.G, tok0 = divide(r0, dm.by);
     const ix4 qr = buffer_of(Q + ((long)w.q_start + tok0) * dm.ldq + kvh * G * dm.hq, 0x7ffffe00);
     const ix4 gr = buffer_of(dO + ((long)w.q_start + tok0) * dm.ldo + kvh * G * dm.ho, 0x7ffffe00);
+    if (ROWS % G == 0) {
 #pragma unroll
-    for (int i = 0; i < LT::NI; ++i) {
-      const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
-      const bool ok = r < rows && ch < dm.D * (int)sizeof(T);
-      load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
-      load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+      for (int i = 0; i < LT::NI; ++i) {
+        const bool ok = LT::row_of(i, wave, lane) < rows - r0;
+        load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? qoff[i] : OUT_OF_BUFFER);
+        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? goff[i] : OUT_OF_BUFFER);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LT::NI; ++i) {
+        const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
+        const bool ok = r < rows && ch < dm.D * (int)sizeof(T);
+        load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+      }
     }
   }
   template <typename T, int DB>
@@ -317,8 +336,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   KeyWork kw;
   kw.begin<S::KT>(tiles, wave, lane, dm);
+  int qoff[LT::NI], goff[LT::NI];
+  kw.offsets<LT, T>(qoff, dm.ldq, dm.hq, wave, lane, dm);
+  kw.offsets<LT, T>(goff, dm.ldo, dm.ho, wave, lane, dm);
   const auto fetch = [&](int t) {
-    kw.fetch<LT, 4>(lds_address(lds) + (t & 1) * 2 * LT::BYTES, t * S::KT, Q, dO, wave, lane, dm);
+    kw.fetch<LT, 4, S::KT>(lds_address(lds) + (t & 1) * 2 * LT::BYTES, t * S::KT, Q, dO, qoff, goff, wave, lane, dm);
   };
   float st_next = 0.0f;
   const auto stat = [&](int t) {                                      // threads 0 .. 2 KT: L, then D of the tile's rows
@@ -403,7 +425,7 @@ struct PairSums {
       const auto weigh = [&](int g) {
         const fx4 l = *reinterpret_cast<const fx4*>(L + 32 * b + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-        for (int i = 4 * g; i < 4 * g + 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, RAISE - l[i & 3]));
+        for (int i = 4 * g; i < 4 * g + 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, l[i & 3]));
       };
       if (b == 0) rows_by_keys(qt, 1, next, lane, spread(weigh));
       else
@@ -428,7 +450,7 @@ struct PairSums {
       const auto slope = [&](int g) {
         const fx4 d = *reinterpret_cast<const fx4*>(D + 32 * b + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = (float)h[i >> 3][i & 7] * (fmaf(ds[i], LOWER, -d[i & 3]));
+        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = fmaf((float)h[i >> 3][i & 7], fmaf(ds[i], LOWER, d[i & 3]), 0.0f);     // v_fma_mix
       };
       if (b == 0) rows_by_keys(gt, 1, next, lane, spread(slope));
       else
@@ -457,37 +479,43 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
   KeyWork kw;
   kw.begin<64>(tiles, group, lane, dm);
   const int t0 = kw.t0, t1 = kw.t1;
-  const auto fetch = [&](int t) {
-    kw.fetch<LT, 8>(lds_address(lds) + (t - t0) % 3 * 2 * LT::BYTES, t * 64, Q, dO, wave, lane, dm);
+  int qoff[LT::NI], goff[LT::NI];
+  kw.offsets<LT, T>(qoff, dm.ldq, dm.hq, wave, lane, dm);
+  kw.offsets<LT, T>(goff, dm.ldo, dm.ho, wave, lane, dm);
+  const auto fetch = [&](int t, int place) {
+    kw.fetch<LT, 8, 64>(lds_address(lds) + place * 2 * LT::BYTES, t * 64, Q, dO, qoff, goff, wave, lane, dm);
   };
   float st_next = 0.0f;
-  const auto stat = [&](int t) {                                      // threads 0 .. 127: L, then D of the tile's rows
+  const auto stat = [&](int t) {                                      // threads 0 .. 127: RAISE - L, then -LOWER D of the tile's rows
     const int r = t * 64 + (threadIdx.x & 63);
     st_next = 0.0f;
-    if (threadIdx.x < 128 && r < kw.rows) st_next = (threadIdx.x < 64 ? lse : delta)[kw.lrow + r] * (threadIdx.x < 64 ? 1.0f : P::LOWER);
+    if (threadIdx.x < 128 && r < kw.rows) st_next = threadIdx.x < 64 ? P::RAISE - lse[kw.lrow + r] : -P::LOWER * delta[kw.lrow + r];
   };
   const float c = dm.scale * LOG2E;
   if (t0 < t1) {
     stat(t0);
-    fetch(t0);
+    fetch(t0, 0);
   }
   P sums;
   if (wave < 4) sums.begin(K + kw.krow * dm.ldk + kw.kvh * dm.hk, dm.D, kw.live, lane >> 5);
   else sums.begin(V + kw.krow * dm.ldv + kw.kvh * dm.hv, dm.D, kw.live, lane >> 5);
   // turn t: the first four at tile t, the others at tile t - 1, tile t + 1 on its way
   const auto turns = [&](auto first_four) {
-    for (int t = t0; t <= t1; ++t) {
+    int at = 0;                                                       // (t - t0) % 3
+    for (int t = t0; t < t1 + (t0 < t1); ++t) {
+      const int next = at == 2 ? 0 : at + 1, before = at == 0 ? 2 : at - 1;
       wait_loads();
-      if (threadIdx.x < 128 && t < t1) stats[(t - t0) % 3 * 128 + threadIdx.x] = st_next;
+      if (threadIdx.x < 128 && t < t1) stats[at * 128 + threadIdx.x] = st_next;
       __syncthreads();
       if (t + 1 < t1) {
         stat(t + 1);
-        fetch(t + 1);
+        fetch(t + 1, next);
       }
-      const int mine = first_four.value ? t : t - 1, r0 = mine * 64;
-      if (t0 == t1 || mine < t0 || mine >= t1 || r0 + 64 <= kw.w_lo) continue;       // none of these rows sees this wave's keys
-      const char* qt = lds + (mine - t0) % 3 * 2 * LT::BYTES;
-      const float* st = stats + (mine - t0) % 3 * 128;
+      const int mine = first_four.value ? t : t - 1, r0 = mine * 64, place = first_four.value ? at : before;
+      at = next;
+      if (mine < t0 || mine >= t1 || r0 + 64 <= kw.w_lo) continue;   // none of these rows sees this wave's keys
+      const char* qt = lds + place * 2 * LT::BYTES;
+      const float* st = stats + place * 128;
       hx8* share = shares + ((mine & 1) * 4 + group) * 256;
       const bool edge = kw.ragged || r0 < kw.w_hi;
       if constexpr (first_four.value) sums.weights(qt, qt + LT::BYTES, st, share, c, edge, kw.first - r0, lane);
