@@ -367,7 +367,8 @@ int s2g_attention_bwd(const float* Q, const float* K, const float* V, const floa
  * of them, in any order.  k_tiles: one per 128 keys with slot -1 and all rows (row_lo 0, row_hi n_q heads / kv_heads), or
  * several that share its rows out among them (bounds multiples of 128), with consecutive slots of their own; each tile so
  * cut has an entry in cut_tiles, row_lo the number and slot the first of its slots.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
- * exponentials, for the backward pass (may be NULL in fwd); delta has its size. */
+ * exponentials, and rest, like out, what rounding to a 16-bit type took from it, are for the backward pass (either may be
+ * NULL in fwd; fp32 has no rest); delta has lse's size. */
 typedef struct S2GPackedTile {
   int q_start, q_len, k_start, k_len, tile, row_lo, row_hi, slot;
 } S2GPackedTile;
@@ -376,11 +377,11 @@ typedef struct S2GPacked {
   float scale;
   long q_ld, q_hd, k_ld, k_hd, v_ld, v_hd, do_ld, do_hd, q_rows, k_rows;
 } S2GPacked;
-int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, float* lse, const S2GPackedTile* tiles,
+int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const S2GPackedTile* tiles,
                              int n_tiles, const S2GPacked* dims, void* stream);
 /* floats of `work` below for so many slots */
 long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int slots);
-int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
+int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* rest, const void* dO, const float* lse,
                              float* delta, void* dQ, void* dK, void* dV, float* work, const S2GPackedTile* q_tiles,
                              int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPackedTile* cut_tiles,
                              int n_cut_tiles, const S2GPacked* dims, void* stream);

@@ -28,8 +28,8 @@ struct S2GRotary {
 static_assert(sizeof(S2GPackedTile) == sizeof(PackedTile) && sizeof(PackedTile) == 32, "S2GPackedTile");
 
 #define DECLARE(sfx)                                                                                                    \
-  extern "C" int s2g_launch_packed_fwd_##sfx(const void*, const void*, const void*, void*, float*, const PackedTile*, int, PackedDims, hipStream_t); \
-  extern "C" int s2g_launch_packed_bwd_##sfx(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, \
+  extern "C" int s2g_launch_packed_fwd_##sfx(const void*, const void*, const void*, void*, void*, float*, const PackedTile*, int, PackedDims, hipStream_t); \
+  extern "C" int s2g_launch_packed_bwd_##sfx(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, \
                                              void*, float*, const PackedTile*, int, const PackedTile*, int, const PackedTile*, int, PackedDims, hipStream_t); \
   extern "C" int s2g_launch_paged_##sfx(const void*, const void*, const void*, const int*, const int*, const int*, void*, float*, int, PagedDims, hipStream_t);
 DECLARE(f32)
@@ -63,12 +63,12 @@ static int packed_dims(const S2GPacked* a, PackedDims* d) {
 
 extern "C" {
 
-int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, float* lse, const S2GPackedTile* tiles,
+int s2g_packed_attention_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const S2GPackedTile* tiles,
                              int n_tiles, const S2GPacked* dims, void* stream) {
   PackedDims d;
   if (!Q || !K || !V || !out || !tiles || n_tiles <= 0 || packed_dims(dims, &d) != 0) return -1;
-  if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(out) || (long)n_tiles * d.Hk >= (1L << 31)) return -1;
-  return BY_TYPE(dims->type, s2g_launch_packed_fwd, Q, K, V, out, lse, reinterpret_cast<const PackedTile*>(tiles), n_tiles, d, (hipStream_t)stream);
+  if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(out) || !aligned16(rest) || (long)n_tiles * d.Hk >= (1L << 31)) return -1;
+  return BY_TYPE(dims->type, s2g_launch_packed_fwd, Q, K, V, out, rest, lse, reinterpret_cast<const PackedTile*>(tiles), n_tiles, d, (hipStream_t)stream);
 }
 
 long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int slots) {
@@ -77,7 +77,7 @@ long s2g_packed_attention_bwd_workspace(const S2GPacked* dims, int slots) {
   return 256L * slots * d.Hk * d.D;
 }
 
-int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
+int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const void* out, const void* rest, const void* dO, const float* lse,
                              float* delta, void* dQ, void* dK, void* dV, float* work, const S2GPackedTile* q_tiles,
                              int n_q_tiles, const S2GPackedTile* k_tiles, int n_k_tiles, const S2GPackedTile* cut_tiles,
                              int n_cut_tiles, const S2GPacked* dims, void* stream) {
@@ -85,10 +85,11 @@ int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const 
   if (!Q || !K || !V || !out || !dO || !lse || !delta || !dQ || !dK || !dV || packed_dims(dims, &d) != 0) return -1;
   if (n_q_tiles < 0 || n_k_tiles < 0 || n_cut_tiles < 0 || (n_q_tiles && !q_tiles) || (n_k_tiles && !k_tiles) || (n_cut_tiles && (!cut_tiles || !work))) return -1;
   if ((long)n_q_tiles * d.Hk >= (1L << 31) || (long)n_k_tiles * d.Hk >= (1L << 31) || (long)n_cut_tiles * d.Hk >= (1L << 31)) return -1;
-  const void* all[] = {Q, K, V, out, dO, dQ, dK, dV, work};
+  if (dims->type != 0 && !rest) return -1;
+  const void* all[] = {Q, K, V, out, rest, dO, dQ, dK, dV, work};
   for (const void* p : all)
     if (!aligned16(p)) return -1;
-  return BY_TYPE(dims->type, s2g_launch_packed_bwd, Q, K, V, out, dO, lse, delta, dQ, dK, dV, work,
+  return BY_TYPE(dims->type, s2g_launch_packed_bwd, Q, K, V, out, rest, dO, lse, delta, dQ, dK, dV, work,
                  reinterpret_cast<const PackedTile*>(q_tiles), n_q_tiles, reinterpret_cast<const PackedTile*>(k_tiles), n_k_tiles,
                  reinterpret_cast<const PackedTile*>(cut_tiles), n_cut_tiles, d, (hipStream_t)stream);
 }

@@ -21,7 +21,7 @@
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ out,
-                                                             float* __restrict__ lse, const PackedTile* __restrict__ tiles,
+                                                             T* __restrict__ rest, float* __restrict__ lse, const PackedTile* __restrict__ tiles,
                                                              PackedDims dm) {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
@@ -87,8 +87,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     turn(t, std::integral_constant<int, 0>{});
     if (t + 1 < nt) turn(t + 1, std::integral_constant<int, 1>{});
   }
-  const float l = both_sum(r.l);
-  store_rows<T, S::DB>(out + (qrow * dm.H + head) * dm.D, r.o, l == 0.0f ? 0.0f : 1.0f / l, dm.D, half, live);
+  const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l;
+  const long orow = (qrow * dm.H + head) * dm.D;
+  store_rows<T, S::DB>(out + orow, r.o, f, dm.D, half, live);
+  // what rounding took from O: with it the backward pass has D = dO . O nearly exactly, where dP - D is a small difference
+  // (a row's first keys: D from the rounded O alone puts 60 % on the error of dQ and dK of short sequences)
+  if (sizeof(T) == 2 && rest) {
+#pragma unroll
+    for (int d = 0; d < S::DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[d][i] = r.o[d][i] * f - (float)(T)(r.o[d][i] * f);
+    store_rows<T, S::DB>(rest + orow, r.o, 1.0f, dm.D, half, live);
+  }
   // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
   if (lse && live && half == 0)
     lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
@@ -99,7 +109,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, const T* __restrict__ out,
-                                                               const T* __restrict__ dO, const float* __restrict__ lse,
+                                                               const T* __restrict__ rest, const T* __restrict__ dO, const float* __restrict__ lse,
                                                                float* __restrict__ delta, T* __restrict__ dQ,
                                                                const PackedTile* __restrict__ tiles, PackedDims dm) {
   typedef Shape<T, DP> S;
@@ -128,6 +138,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     const v8 y = row8(out + orow, at, dm.D, live);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)y[j], dl);
+    if constexpr (sizeof(T) == 2) {
+      const v8 x = row8(rest + orow, at, dm.D, live);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)x[j], dl);
+    }
   }
   dl = both_sum(dl);
   if (live && half == 0) delta[lrow] = dl;
@@ -560,17 +575,17 @@ __global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __rest
 
 // ----------------------------------------------------------------------------------------------------------------- host
 template <typename T, int DP>
-static int launch_fwd(const void* Q, const void* K, const void* V, void* out, float* lse, const PackedTile* tiles, int nt,
+static int launch_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
                       const PackedDims& dm, hipStream_t st) {
   const int bytes = 4 * Shape<T, DP>::LT::BYTES;
   static S2GLdsCap cap;
   const auto kernel = s2g_k_packed_attn_fwd<T, DP>;
   if (s2g_lds_cap(cap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)nt * dm.Hk), dim3(256), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, lse, tiles, dm);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)nt * dm.Hk), dim3(256), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 template <typename T, int DP>
-static int launch_bwd(const void* Q, const void* K, const void* V, const void* out, const void* dO, const float* lse,
+static int launch_bwd(const void* Q, const void* K, const void* V, const void* out, const void* rest, const void* dO, const float* lse,
                       float* delta, void* dQ, void* dK, void* dV, float* partial, const PackedTile* qt, int nqt,
                       const PackedTile* kt, int nkt, const PackedTile* cut, int ncut, const PackedDims& dm, hipStream_t st) {
   typedef typename Shape<T, DP>::LT LT;
@@ -583,7 +598,7 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kk), bytes) != 0) return -2;
     if (nqt > 0)
       hipLaunchKernelGGL(kq, dim3((unsigned)nqt * dm.Hk), dim3(256), qb, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out,
-                         (const T*)dO, lse, delta, (T*)dQ, qt, dm);
+                         (const T*)rest, (const T*)dO, lse, delta, (T*)dQ, qt, dm);
     if (nkt > 0)
       hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk), dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V,
                          (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
@@ -598,14 +613,14 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
-extern "C" int PACKED_NAME(s2g_launch_packed_fwd)(const void* Q, const void* K, const void* V, void* out, float* lse,
+extern "C" int PACKED_NAME(s2g_launch_packed_fwd)(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse,
                                                   const PackedTile* tiles, int nt, PackedDims dm, hipStream_t st) {
-  return PER_DIM(launch_fwd, PACKED_T, Q, K, V, out, lse, tiles, nt, dm, st);
+  return PER_DIM(launch_fwd, PACKED_T, Q, K, V, out, rest, lse, tiles, nt, dm, st);
 }
 extern "C" int PACKED_NAME(s2g_launch_packed_bwd)(const void* Q, const void* K, const void* V, const void* out,
-                                                  const void* dO, const float* lse, float* delta, void* dQ, void* dK,
+                                                  const void* rest, const void* dO, const float* lse, float* delta, void* dQ, void* dK,
                                                   void* dV, float* partial, const PackedTile* qt, int nqt,
                                                   const PackedTile* kt, int nkt, const PackedTile* cut, int ncut,
                                                   PackedDims dm, hipStream_t st) {
-  return PER_DIM(launch_bwd, PACKED_T, Q, K, V, out, dO, lse, delta, dQ, dK, dV, partial, qt, nqt, kt, nkt, cut, ncut, dm, st);
+  return PER_DIM(launch_bwd, PACKED_T, Q, K, V, out, rest, dO, lse, delta, dQ, dK, dV, partial, qt, nqt, kt, nkt, cut, ncut, dm, st);
 }

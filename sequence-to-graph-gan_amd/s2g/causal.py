@@ -266,19 +266,22 @@ class PackedAttentionFn(torch.autograd.Function):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         out[pack.rows:].zero_()
         q_tiles = pack.query_tiles(G, causal)
-        lse = torch.empty(Hk * R * G, dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad) else None
+        lse = rest = None
+        if any(ctx.needs_input_grad):
+            lse = torch.empty(Hk * R * G, dtype=torch.float32, device=q.device)
+            rest = torch.empty_like(out) if q.dtype != torch.float32 else None
         if q_tiles.shape[0]:
             with _device(q):
-                call("s2g_packed_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(q_tiles), q_tiles.shape[0],
+                call("s2g_packed_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), ptr(q_tiles), q_tiles.shape[0],
                      ctypes.byref(dims), stream_ptr())
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.pack, ctx.how = pack, (causal, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         pack, (causal, scale) = ctx.pack, ctx.how
         (R, H, D), (M, Hk, _) = q.shape, k.shape
         G, dev = H // Hk, q.device
@@ -292,7 +295,7 @@ class PackedAttentionFn(torch.autograd.Function):
         delta = torch.empty(Hk * R * G, dtype=torch.float32, device=dev)
         work = torch.empty(get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots), dtype=torch.float32, device=dev)
         with _device(q):
-            call("s2g_packed_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk),
+            call("s2g_packed_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk),
                  ptr(dv), ptr(work) if slots else None, ptr(q_tiles), q_tiles.shape[0], ptr(k_tiles), k_tiles.shape[0], ptr(cut),
                  cut.shape[0], ctypes.byref(dims), stream_ptr())
         return dq, dk, dv, None, None, None

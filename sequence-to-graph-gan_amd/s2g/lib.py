@@ -154,9 +154,9 @@ SIGNATURES = {
     "s2g_add_inplace": [P, P, L, P],
     "s2g_attention_fwd": [P, P, P, P, P, P, P, ctypes.POINTER(S2GAttn), P],
     "s2g_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, ctypes.POINTER(S2GAttn), P],
-    "s2g_packed_attention_fwd": [P, P, P, P, P, P, I, ctypes.POINTER(S2GPacked), P],
+    "s2g_packed_attention_fwd": [P] * 7 + [I, ctypes.POINTER(S2GPacked), P],
     "s2g_packed_attention_bwd_workspace": [ctypes.POINTER(S2GPacked), I],
-    "s2g_packed_attention_bwd": [P] * 11 + [P, I, P, I, P, I, ctypes.POINTER(S2GPacked), P],
+    "s2g_packed_attention_bwd": [P] * 12 + [P, I, P, I, P, I, ctypes.POINTER(S2GPacked), P],
     "s2g_paged_attention_workspace": [ctypes.POINTER(S2GPaged)],
     "s2g_paged_attention": [P] * 8 + [ctypes.POINTER(S2GPaged), P],
     "s2g_rotary": [P] * 6 + [ctypes.POINTER(S2GRotary), P],

@@ -70,18 +70,19 @@ def test_c_entry_points_refuse():
     from s2g import lib
     l, p = lib.load(), 4096
     for change in BAD_HEADS + [dict(k_ld=4), dict(v_hd=2), dict(do_ld=-8), dict(k_rows=-1)]:
-        assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, packed(**change), None) == -1, change
-        assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, None, 0, packed(**change), None) == -1, change
+        assert l.s2g_packed_attention_fwd(p, p, p, p, None, None, p, 1, packed(**change), None) == -1, change
+        assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, None, 0, packed(**change), None) == -1, change
         assert l.s2g_packed_attention_bwd_workspace(packed(**change), 2) == -1, change
-    for i in (0, 1, 2, 3, 5):
-        args = [p, p, p, p, None, p]
+    for i in (0, 1, 2, 3, 6):
+        args = [p, p, p, p, None, None, p]
         args[i] = None
         assert l.s2g_packed_attention_fwd(*args, 1, packed(), None) == -1, i
-    assert l.s2g_packed_attention_fwd(p + 2, p, p, p, None, p, 1, packed(), None) == -1
-    assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 0, packed(), None) == -1
-    assert l.s2g_packed_attention_fwd(p, p, p, p, None, p, 1, None, None) == -1
-    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, p, 1, packed(), None) == -1      # cut tiles, no workspace
-    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, p, 1, p, 1, None, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_fwd(p + 2, p, p, p, None, None, p, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_fwd(p, p, p, p, None, None, p, 0, packed(), None) == -1
+    assert l.s2g_packed_attention_fwd(p, p, p, p, None, None, p, 1, None, None) == -1
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, p, 1, packed(), None) == -1      # cut tiles, no workspace
+    assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, p, p, 1, p, 1, None, 1, packed(), None) == -1
+    assert l.s2g_packed_attention_bwd(p, p, p, p, None, p, p, p, p, p, p, p, p, 1, p, 1, None, 0, packed(), None) == -1       # bf16, no rest
     assert l.s2g_packed_attention_bwd_workspace(packed(), 3) == 3 * 256 * 2 * 64 and l.s2g_packed_attention_bwd_workspace(packed(), -1) == -1
     for change in BAD_HEADS + [dict(sequences=0), dict(sequences=65536), dict(page_size=8), dict(page_size=24), dict(page_size=1 << 17),
                                dict(pages=0), dict(table_cols=0), dict(table_cols=1 << 26), dict(max_new=0), dict(max_new=3),
