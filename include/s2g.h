@@ -367,7 +367,7 @@ int s2g_attention_bwd(const float* Q, const float* K, const float* V, const floa
  * of them, in any order.  k_tiles: one per 128 keys with slot -1 and all rows (row_lo 0, row_hi n_q heads / kv_heads), or
  * several that share its rows out among them (bounds multiples of 128), with consecutive slots of their own; each tile so
  * cut has an entry in cut_tiles, row_lo the number and slot the first of its slots.  lse [kv_heads][q_rows][heads / kv_heads]: log2 of the row's sum of
- * exponentials, and rest, like out, what rounding to a 16-bit type took from it, are for the backward pass (either may be
+ * exponentials, and rest, like out, what rounding to a 16-bit type took from rows of few keys, are for the backward pass (either may be
  * NULL in fwd; fp32 has no rest); delta has lse's size. */
 typedef struct S2GPackedTile {
   int q_start, q_len, k_start, k_len, tile, row_lo, row_hi, slot;

@@ -17,6 +17,8 @@
 #include "packed_attention.h"
 #include <type_traits>
 
+#define FEW_KEYS 128
+
 // -------------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
@@ -90,14 +92,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l;
   const long orow = (qrow * dm.H + head) * dm.D;
   store_rows<T, S::DB>(out + orow, r.o, f, dm.D, half, live);
-  // what rounding took from O: with it the backward pass has D = dO . O nearly exactly, where dP - D is a small difference
-  // (a row's first keys: D from the rounded O alone puts 60 % on the error of dQ and dK of short sequences)
-  if (sizeof(T) == 2 && rest) {
+  // what rounding took from O: with it the backward pass has D = dO . O nearly exactly where dP - D is a small difference.
+  // Only rows of few keys need it: of n like keys, D's error is 1 / sqrt(n) of what rounding dS adds.  (Without it dQ and dK
+  // of short fp16 sequences are off by 1.57 times the result's own rounding, with it by 1.45.)
+  if (sizeof(T) == 2 && rest && w_lo < FEW_KEYS) {
 #pragma unroll
     for (int d = 0; d < S::DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) r.o[d][i] = r.o[d][i] * f - (float)(T)(r.o[d][i] * f);
-    store_rows<T, S::DB>(rest + orow, r.o, 1.0f, dm.D, half, live);
+    store_rows<T, S::DB>(rest + orow, r.o, 1.0f, dm.D, half, live && last < FEW_KEYS);
   }
   // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
   if (lse && live && half == 0)
@@ -128,6 +131,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   const T* kp = K + (long)w.k_start * dm.ldk + kvh * dm.hk;
   const T* vp = V + (long)w.k_start * dm.ldv + kvh * dm.hv;
 
+  const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
+  const int last = live ? min(w.k_len - 1, tok + shift) : -1;
+  const int w_lo = min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave, rows - 1), dm.by) + shift);
+  const int w_hi = w.tile * 128 + 32 * wave < rows ? min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave + 31, rows - 1), dm.by) + shift) : -1;
+  const int b_hi = min(w.k_len - 1, divide(min(w.tile * 128 + 127, rows - 1), dm.by) + shift);
+  const int nt = b_hi < 0 ? 0 : b_hi / S::KT + 1;
+
   v8 q[S::KS], g[S::KS];
   float dl = 0.0f;
 #pragma unroll
@@ -138,22 +148,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     const v8 y = row8(out + orow, at, dm.D, live);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)y[j], dl);
-    if constexpr (sizeof(T) == 2) {
-      const v8 x = row8(rest + orow, at, dm.D, live);
+    if (sizeof(T) == 2 && w_lo < FEW_KEYS) {
+      const v8 x = row8(rest + orow, at, dm.D, live && last < FEW_KEYS);
 #pragma unroll
       for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)x[j], dl);
     }
   }
   dl = both_sum(dl);
-  if (live && half == 0) delta[lrow] = dl;
   const float L = live ? lse[lrow] : INFINITY, c = dm.scale * LOG2E;
-
-  const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
-  const int last = live ? min(w.k_len - 1, tok + shift) : -1;
-  const int w_lo = min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave, rows - 1), dm.by) + shift);
-  const int w_hi = w.tile * 128 + 32 * wave < rows ? min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave + 31, rows - 1), dm.by) + shift) : -1;
-  const int b_hi = min(w.k_len - 1, divide(min(w.tile * 128 + 127, rows - 1), dm.by) + shift);
-  const int nt = b_hi < 0 ? 0 : b_hi / S::KT + 1;
 
   int ko[LT::NI], vo[LT::NI];
   tile_offsets<LT, T>(ko, dm.ldk, dm.D, wave, lane);
@@ -186,6 +188,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
       for (int s = 0; s < S::KS; ++s) st = mma(LT::along(kt, 32 * b + (lane & 31), s, half), q[s], st);
 #pragma unroll
       for (int s = 0; s < S::KS; ++s) dp = mma(LT::along(vt, 32 * b + (lane & 31), s, half), g[s], dp);
+      // a row that sees one key only has D = dP there, to the last bit: its scores have no gradient
+      if (b == 0 && k0 == 0 && last == 0) dl = dp[0];
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], c, -L)) * (dp[i] - dl);
       if (edge) {
@@ -202,6 +206,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
       }
     }
   }
+  if (live && half == 0) delta[lrow] = dl;
   store_rows<T, S::DB>(dQ + orow, dq, dm.scale, dm.D, half, live);
 }
 
@@ -389,14 +394,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 }
 
 // Two waves to 32 keys: wave g of the first four makes S, P and dV, wave 4 + g dP, dS and dK.  P goes from one to the other
-// through LDS, raised by 2^14 and rounded to fp16 (half a step is 2^-11 of it: an eighth of what rounding dS to bf16 adds,
-// and it is nothing at all where fp16 is the type and dV takes the same weights).  The first four are a tile of 64 rows
-// ahead, so that neither waits for the other within one.
+// through LDS, raised by 2^14.  For bf16 it goes as fp16: half a step is 2^-11 of it, an eighth of what rounding dS to bf16
+// adds; for fp16 that would be as much as rounding dS adds, so there it goes in 32 bits, and a tile is half as many rows.
+// The first four are a tile ahead, so that neither waits for the other within one.
 template <typename T, int DP>
 struct PairSums {
   typedef Shape<T, DP> S;
-  typedef Tile<T, S::PITCH, 64, 8> LT;
+  static constexpr bool WIDE = std::is_same<T, _Float16>::value;
+  static constexpr int BLOCKS = WIDE ? 1 : 2, ROWS = 32 * BLOCKS;
+  typedef Tile<T, S::PITCH, ROWS, 8> LT;
   typedef typename Vec<T>::v8 v8;
+  static constexpr int UNITS = WIDE ? 4 : 2, SHARE = BLOCKS * UNITS * 64;      // 16-byte units of P of 32 rows per lane; of a tile
+  static constexpr int BYTES = 6 * LT::BYTES + 8 * SHARE * 16 + 3 * 2 * ROWS * (int)sizeof(float);
   static constexpr float RAISE = 14.0f, LOWER = 1.0f / 16384.0f;
   v8 k[S::KS];                                     // K of the first four, V of the others
   fx16 sum[S::DB];
@@ -431,49 +440,66 @@ struct PairSums {
     for (int i = 0; i < 16; ++i)
       if (reg_row(i) < at) x[i] = 0.0f;
   }
-  // 64 rows: P to `share` ([block][2][lane] of 16 bytes), dV^T += dO^T P
-  __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, hx8* share, float c, bool edge, int first, int lane) {
+  static __device__ __forceinline__ void give(fx4* share, const fx16& p, int lane) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) share[u * 64 + lane] = (fx4){p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]};
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) share[u * 64 + lane] = __builtin_bit_cast(fx4, operand<_Float16>(p, u));
+    }
+  }
+  // P of register i out of what was given
+  static __device__ __forceinline__ float given(const fx4* x, int i) {
+    if constexpr (WIDE) return x[i >> 2][i & 3];
+    else {
+      const hx8 h = __builtin_bit_cast(hx8, x[i >> 3]);
+      return (float)h[i & 7];
+    }
+  }
+  // a tile of rows: P to `share` ([block][unit][lane] of 16 bytes), dV^T += dO^T P
+  __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, fx4* share, float c, bool edge, int first, int lane) {
     fx16 p, next;
     rows_by_keys(qt, 0, p, lane, [](int) {});
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < BLOCKS; ++b) {
       const auto weigh = [&](int g) {
         const fx4 l = *reinterpret_cast<const fx4*>(L + 32 * b + 8 * g + 4 * (lane >> 5));
 #pragma unroll
         for (int i = 4 * g; i < 4 * g + 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, l[i & 3]));
       };
-      if (b == 0) rows_by_keys(qt, 1, next, lane, spread(weigh));
+      if (b + 1 < BLOCKS) rows_by_keys(qt, 1, next, lane, spread(weigh));
       else
 #pragma unroll
         for (int g = 0; g < 4; ++g) weigh(g);
       if (edge) mask(p, first - 32 * b, lane);
-      const hx8 h[2] = {operand<_Float16>(p, 0), operand<_Float16>(p, 1)};
-      share[(2 * b) * 64 + lane] = h[0];
-      share[(2 * b + 1) * 64 + lane] = h[1];
+      give(share + b * UNITS * 64, p, lane);
       const v8 x[2] = {operand<T>(p, 0), operand<T>(p, 1)};
       add(gt, b, x, lane);
       p = next;
     }
   }
-  // the same 64 rows, P taken from `share`: dK^T += Q^T dS
-  __device__ __forceinline__ void slopes(const char* qt, const char* gt, const float* D, const hx8* share, bool edge, int first, int lane) {
+  // the same rows, P taken from `share`: dK^T += Q^T dS
+  __device__ __forceinline__ void slopes(const char* qt, const char* gt, const float* D, const fx4* share, bool edge, int first, int lane) {
     fx16 ds, next;
     rows_by_keys(gt, 0, ds, lane, [](int) {});
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const hx8 h[2] = {share[(2 * b) * 64 + lane], share[(2 * b + 1) * 64 + lane]};
+    for (int b = 0; b < BLOCKS; ++b) {
+      fx4 x[UNITS];
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) x[u] = share[(b * UNITS + u) * 64 + lane];
       const auto slope = [&](int g) {
         const fx4 d = *reinterpret_cast<const fx4*>(D + 32 * b + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = fmaf((float)h[i >> 3][i & 7], fmaf(ds[i], LOWER, d[i & 3]), 0.0f);     // v_fma_mix
+        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = fmaf(given(x, i), fmaf(ds[i], LOWER, d[i & 3]), 0.0f);     // v_fma_mix
       };
-      if (b == 0) rows_by_keys(gt, 1, next, lane, spread(slope));
+      if (b + 1 < BLOCKS) rows_by_keys(gt, 1, next, lane, spread(slope));
       else
 #pragma unroll
         for (int g = 0; g < 4; ++g) slope(g);
       if (edge) mask(ds, first - 32 * b, lane);
-      const v8 x[2] = {operand<T>(ds, 0), operand<T>(ds, 1)};
-      add(qt, b, x, lane);
+      const v8 y[2] = {operand<T>(ds, 0), operand<T>(ds, 1)};
+      add(qt, b, y, lane);
       ds = next;
     }
   }
@@ -486,25 +512,25 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
     float* __restrict__ partial, const PackedTile* __restrict__ tiles, PackedDims dm) {
   typedef PairSums<T, DP> P;
   typedef typename P::LT LT;
-  constexpr int DB = Shape<T, DP>::DB;
+  constexpr int DB = Shape<T, DP>::DB, ROWS = P::ROWS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];       // 3 x (Q, dO), 2 x 4 x P, 3 x (L, D)
-  hx8* shares = reinterpret_cast<hx8*>(lds + 6 * LT::BYTES);
-  float* stats = reinterpret_cast<float*>(lds + 6 * LT::BYTES + 32768);
+  fx4* shares = reinterpret_cast<fx4*>(lds + 6 * LT::BYTES);
+  float* stats = reinterpret_cast<float*>(shares + 8 * P::SHARE);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), group = wave & 3;
   KeyWork kw;
-  kw.begin<64>(tiles, group, lane, dm);
+  kw.begin<ROWS>(tiles, group, lane, dm);
   const int t0 = kw.t0, t1 = kw.t1;
   int qoff[LT::NI], goff[LT::NI];
   kw.offsets<LT, T>(qoff, dm.ldq, dm.hq, wave, lane, dm);
   kw.offsets<LT, T>(goff, dm.ldo, dm.ho, wave, lane, dm);
   const auto fetch = [&](int t, int place) {
-    kw.fetch<LT, 8, 64>(lds_address(lds) + place * 2 * LT::BYTES, t * 64, Q, dO, qoff, goff, wave, lane, dm);
+    kw.fetch<LT, 8, ROWS>(lds_address(lds) + place * 2 * LT::BYTES, t * ROWS, Q, dO, qoff, goff, wave, lane, dm);
   };
   float st_next = 0.0f;
-  const auto stat = [&](int t) {                                      // threads 0 .. 127: RAISE - L, then -LOWER D of the tile's rows
-    const int r = t * 64 + (threadIdx.x & 63);
+  const auto stat = [&](int t) {                                      // threads 0 .. 2 ROWS: RAISE - L, then -LOWER D of the tile's rows
+    const int r = t * ROWS + (threadIdx.x & (ROWS - 1));
     st_next = 0.0f;
-    if (threadIdx.x < 128 && r < kw.rows) st_next = threadIdx.x < 64 ? P::RAISE - lse[kw.lrow + r] : -P::LOWER * delta[kw.lrow + r];
+    if (threadIdx.x < 2 * ROWS && r < kw.rows) st_next = threadIdx.x < ROWS ? P::RAISE - lse[kw.lrow + r] : -P::LOWER * delta[kw.lrow + r];
   };
   const float c = dm.scale * LOG2E;
   if (t0 < t1) {
@@ -520,21 +546,21 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
     for (int t = t0; t < t1 + (t0 < t1); ++t) {
       const int next = at == 2 ? 0 : at + 1, before = at == 0 ? 2 : at - 1;
       wait_loads();
-      if (threadIdx.x < 128 && t < t1) stats[at * 128 + threadIdx.x] = st_next;
+      if (threadIdx.x < 2 * ROWS && t < t1) stats[at * 2 * ROWS + threadIdx.x] = st_next;
       __syncthreads();
       if (t + 1 < t1) {
         stat(t + 1);
         fetch(t + 1, next);
       }
-      const int mine = first_four.value ? t : t - 1, r0 = mine * 64, place = first_four.value ? at : before;
+      const int mine = first_four.value ? t : t - 1, r0 = mine * ROWS, place = first_four.value ? at : before;
       at = next;
-      if (mine < t0 || mine >= t1 || r0 + 64 <= kw.w_lo) continue;   // none of these rows sees this wave's keys
+      if (mine < t0 || mine >= t1 || r0 + ROWS <= kw.w_lo) continue;   // none of these rows sees this wave's keys
       const char* qt = lds + place * 2 * LT::BYTES;
-      const float* st = stats + place * 128;
-      hx8* share = shares + ((mine & 1) * 4 + group) * 256;
+      const float* st = stats + place * 2 * ROWS;
+      fx4* share = shares + ((mine & 1) * 4 + group) * P::SHARE;
       const bool edge = kw.ragged || r0 < kw.w_hi;
       if constexpr (first_four.value) sums.weights(qt, qt + LT::BYTES, st, share, c, edge, kw.first - r0, lane);
-      else sums.slopes(qt, qt + LT::BYTES, st + 64, share, edge, kw.first - r0, lane);
+      else sums.slopes(qt, qt + LT::BYTES, st + ROWS, share, edge, kw.first - r0, lane);
     }
   };
   if (wave < 4) {
@@ -605,7 +631,7 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
     return 0;
   };
   int rc;
-  if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, 6 * PairSums<T, DP>::LT::BYTES + 32768 + 3 * 128 * (int)sizeof(float));
+  if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, PairSums<T, DP>::BYTES);
   else rc = key_side(s2g_k_packed_attn_bwd_kv<T, DP>, 256, 4 * LT::BYTES + 4 * Shape<T, DP>::KT * (int)sizeof(float));
   if (rc != 0) return rc;
   if (ncut > 0)

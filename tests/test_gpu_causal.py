@@ -112,6 +112,29 @@ def test_packed_attention_views_and_rows_behind(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_packed_attention_of_one_key(dtype, shape):
+    """A row that sees a single key returns its value, and its scores have no gradient: zeros, not small numbers."""
+    import transformer as M
+    H, Hk, D = shape
+    g, n, m = gen(9), [1, 1, 1, 2, 1], [1, 1, 1, 1, 1]
+    pack = M.PackedSequences(n, DEV, m)
+    q, k, v, do = (rand(g, r, h, D, dtype=dtype).requires_grad_() for r, h in ((6, H), (5, Hk), (5, Hk), (6, H)))
+    out = M.packed_attention(q, k, v, pack)
+    of = [0, 1, 2, None, 3, 4]                     # the first of two rows over one key sees none
+    for r, j in enumerate(of):
+        want = torch.zeros(H, D, dtype=dtype, device=DEV) if j is None else v[j].repeat_interleave(H // Hk, 0)
+        # one weight p: p v, 1 / p and their product are rounded in fp32, half a step each; a 16-bit v then comes out itself
+        assert ((out[r] - want).abs() <= (3.1 * 2.0 ** -24 if dtype == torch.float32 else 0.0) * want.abs()).all(), r
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    assert (dq == 0).all() and (dk == 0).all()
+    for r, j in enumerate(of):
+        if j is not None:
+            ref.within(dv[j], [x(do[r].detach().double().view(Hk, H // Hk, D)) for x in
+                               (lambda y: y.sum(1), lambda y: 4 * ref.U[dtype] * y.abs().sum(1))], f"dv {j}")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
 def test_packed_attention_gradient_against_differences(dtype):
     import transformer as M
     g, n, (H, Hk, D) = gen(7), [70, 33], (4, 2, 32)
