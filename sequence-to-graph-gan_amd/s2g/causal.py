@@ -3,7 +3,6 @@
 lengths the host knows; every product and reduction runs in libs2g kernels (include/s2g.h)."""
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -19,11 +18,13 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 TILE = 128                       # rows, or keys, of one workgroup
 
 
-def _device(t: torch.Tensor):
-    """Launches go to the tensors' device, whichever is current."""
-    if t.device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(device: int, name: str, *args) -> None:
+    """A kernel call on the tensors' device, whichever is current, and on its current stream."""
+    if device == torch._C._cuda_getDevice():
+        call(name, *args, stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_ptr())
 
 
 def _check(what: str, **tensors: Optional[torch.Tensor]) -> None:
@@ -47,13 +48,33 @@ def _strides(x: torch.Tensor) -> Tuple[int, int]:
     return (x.stride(0) if x.shape[0] > 1 else x.shape[1] * h), h
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy of it whose rows the kernels can fetch in 16-byte units."""
+def _fetchable(x: torch.Tensor) -> bool:
+    """Rows that the kernels can fetch in 16-byte units, as far as their strides go."""
     unit = 16 // x.element_size()
     t, h = _strides(x)
-    if x.stride(2) == 1 and t % unit == 0 and h % unit == 0 and x.data_ptr() % 16 == 0 and max(t, h) < 1 << 22:
-        return x
+    return x.stride(2) == 1 and t % unit == 0 and h % unit == 0 and max(t, h) < 1 << 22
+
+
+def _once(backward):
+    """once_differentiable, whose bookkeeping (10 us a call) is needed only where a graph of the gradient is being made."""
+    slow = once_differentiable(backward)
+
+    def choose(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return choose
+
+
+def _new(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _copy(x: torch.Tensor) -> torch.Tensor:
     return x.clone(memory_format=torch.contiguous_format)
+
+
+def _layout(*tensors) -> tuple:
+    """What the checks of a call and its plan go by: shapes, strides, types, devices; never addresses or values."""
+    return tuple([(t.dtype, t.shape, t.stride(), t.get_device()) for t in tensors])
 
 
 def _dense(x: torch.Tensor) -> torch.Tensor:
@@ -120,27 +141,47 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return f.to(device), multiplier
 
 
-def _rotary_dims(what, q, k, v, frequencies, interleaved, multiplier, backward) -> S2GRotary:
-    D = q.shape[2]
-    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or frequencies.device != q.device or not frequencies.is_contiguous():
-        raise S2GError(f"{what}: frequencies must be a contiguous float64 vector on {q.device}")
-    if 2 * frequencies.numel() > D or D > 256:
-        raise S2GError(f"{what}: {2 * frequencies.numel()} rotary features of head dim {D} (at most 256)")
+def _frequencies(what: str, frequencies: torch.Tensor, device: int, D: int) -> int:
+    """How many features `frequencies` turn."""
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or frequencies.get_device() != device or not frequencies.is_contiguous():
+        raise S2GError(f"{what}: frequencies must be a contiguous float64 vector on the tensors' device")
+    R = 2 * frequencies.numel()
+    if R > D or D > 256:
+        raise S2GError(f"{what}: {R} rotary features of head dim {D} (at most 256)")
+    return R
+
+
+def _rotary_dims(q, k, v, R, interleaved, multiplier, backward) -> S2GRotary:
     if not math.isfinite(multiplier):
-        raise S2GError(f"{what}: multiplier must be finite")
+        raise S2GError("rotary positions: multiplier must be finite")
     (ql, qh), (kl, kh), (vl, vh) = (_strides(x) if x is not None else (0, 0) for x in (q, k, v))
-    return S2GRotary(TYPES[q.dtype], q.shape[1], 0 if k is None else k.shape[1], D, 2 * frequencies.numel(), int(interleaved),
-                     int(backward), multiplier, q.shape[0], ql, qh, kl, kh, vl, vh)
+    return S2GRotary(TYPES[q.dtype], q.shape[1], 0 if k is None else k.shape[1], q.shape[2], R, int(interleaved), int(backward), multiplier,
+                     q.shape[0], ql, qh, kl, kh, vl, vh)
+
+
+class _TurnPlan:
+    """The kernel's arguments for q and k laid out like these, checked once."""
+    kept: dict = {}
+
+    def __init__(self, q, k, R, interleaved, multiplier, backward):
+        self.copy = q.stride(2) != 1 or (k is not None and k.stride(2) != 1)
+        self.rows, self.device = q.shape[0], q.get_device()
+        self.args = ctypes.byref(_rotary_dims(q, k, None, R, interleaved, multiplier, backward))
 
 
 def _turn(q, k, positions, frequencies, interleaved, multiplier, backward):
-    q, k = _dense(q), None if k is None else _dense(k)
-    dims = _rotary_dims("apply_rotary", q, k, None, frequencies, interleaved, multiplier, backward)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if q.shape[0]:
-        with _device(q):
-            call("s2g_rotary", ptr(q), ptr(k), ptr(positions), ptr(frequencies), ptr(qo), ptr(ko), ctypes.byref(dims), stream_ptr())
+    how = (frequencies.numel(), interleaved, multiplier, backward)
+    key = (_layout(q) if k is None else _layout(q, k), how)
+    plan = _TurnPlan.kept.get(key)
+    if plan is None:
+        if len(_TurnPlan.kept) >= 256:                 # batches of ever new sizes
+            _TurnPlan.kept.clear()
+        plan = _TurnPlan.kept[key] = _TurnPlan(q, k, 2 * how[0], *how[1:])
+    if plan.copy:
+        return _turn(_dense(q), None if k is None else _dense(k), positions, frequencies, interleaved, multiplier, backward)
+    qo, ko = _new(q), None if k is None else _new(k)
+    if plan.rows:
+        _launch(plan.device, "s2g_rotary", q.data_ptr(), ptr(k), positions.data_ptr(), frequencies.data_ptr(), qo.data_ptr(), ptr(ko), plan.args)
     return qo, ko
 
 
@@ -154,7 +195,7 @@ class RotaryFn(torch.autograd.Function):
         return _turn(q, k, positions, frequencies, interleaved, multiplier, False)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
         return (*_turn(dq, dk, positions, frequencies, *ctx.how, True), None, None, None, None)
@@ -173,6 +214,9 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise S2GError("apply_rotary: no heads, or heads without features")
     if positions.shape != q.shape[:1] or positions.dtype != torch.int32 or positions.device != q.device or not positions.is_contiguous():
         raise S2GError(f"apply_rotary: positions must be contiguous int32 [{q.shape[0]}] on {q.device}")
+    _frequencies("apply_rotary", frequencies, q.get_device(), q.shape[2])
+    if not torch.is_grad_enabled() or not (q.requires_grad or (k is not None and k.requires_grad)):
+        return _turn(q, k, positions, frequencies, bool(interleaved), float(multiplier), False)
     return RotaryFn.apply(q, k, positions, frequencies, bool(interleaved), float(multiplier))
 
 
@@ -201,7 +245,7 @@ class PackedSequences:
         with torch.cuda.device(self.device):
             self.starts = _on_device(np.append(self.q_start, self.rows), self.device)
             self.positions = _on_device(np.arange(self.rows) - np.repeat(self.q_start - (k - q), q), self.device)
-        self._lists: dict = {}
+        self._lists, self._plans = {}, {}
 
     def _tiles(self, count: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
         """(sequence, which) of every tile of `count` rows or keys a sequence."""
@@ -256,49 +300,77 @@ class PackedSequences:
         return got
 
 
+class _PackedPlan:
+    """One layout of q, k and v over one batch: checked once, its work lists and the kernels' arguments kept."""
+
+    def __init__(self, pack, q, k, v, causal, scale):
+        _check("packed_attention", q=q, k=k, v=v)
+        _attention_shapes("packed_attention", q, k, v)
+        if pack.device != q.device:
+            raise S2GError(f"packed_attention: pack must be PackedSequences on {q.device}")
+        if q.shape[0] < pack.rows or k.shape[0] < pack.key_rows:
+            raise S2GError(f"packed_attention: the layout needs {pack.rows} queries and {pack.key_rows} keys, got {q.shape[0]} and {k.shape[0]}")
+        if q.shape[0] * q.shape[1] >= 1 << 30 or k.shape[0] >= 1 << 30:
+            raise S2GError("packed_attention: 2^30 rows or more")
+        (R, H, D), (M, Hk, _) = q.shape, k.shape
+        self.copies = [not _fetchable(x) for x in (q, k, v)]
+        self.pack, self.causal, self.group, self.kv_heads = pack, causal, H // Hk, Hk
+        self.device, self.rows, self.key_rows = q.get_device(), pack.rows, pack.key_rows
+        self.stats = Hk * R * self.group
+        self.fields = (TYPES[q.dtype], H, Hk, D, int(causal), _scale("packed_attention", scale, D), *_strides(q), *_strides(k), *_strides(v))
+        self.size, self.whole = (R, M), R == pack.rows and M == pack.key_rows
+        self.dims = S2GPacked(*self.fields, H * D, D, R, M)
+        self.fwd = ctypes.byref(self.dims)
+        self.q_tiles = pack.query_tiles(self.group, causal)
+        self.q_list = (ptr(self.q_tiles), self.q_tiles.shape[0])
+        self.bwd: dict = {}
+
+    def backward(self, do):
+        """(arguments, key-side lists, floats of workspace) for a gradient laid out like `do`."""
+        key = _layout(do)
+        got = self.bwd.get(key)
+        if got is None:
+            dims = S2GPacked(*self.fields, *_strides(do), *self.size)
+            k_tiles, cut, slots = self.pack.key_tiles(self.group, self.causal, self.kv_heads)
+            got = self.bwd[key] = (ctypes.byref(dims), (ptr(k_tiles), k_tiles.shape[0], ptr(cut), cut.shape[0]),
+                                   get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots))
+        return got
+
+
 class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, pack, causal, scale):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        (R, H, D), (M, Hk, _) = q.shape, k.shape
-        G = H // Hk
-        dims = S2GPacked(TYPES[q.dtype], H, Hk, D, int(causal), scale, *_strides(q), *_strides(k), *_strides(v), H * D, D, R, M)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        out[pack.rows:].zero_()
-        q_tiles = pack.query_tiles(G, causal)
+    def forward(ctx, q, k, v, plan):
+        out = _new(q)
+        if not plan.whole:
+            out[plan.rows:].zero_()
         lse = rest = None
         if any(ctx.needs_input_grad):
-            lse = torch.empty(Hk * R * G, dtype=torch.float32, device=q.device)
+            lse = q.new_empty(2, plan.stats, dtype=torch.float32)         # and room for D
             rest = torch.empty_like(out) if q.dtype != torch.float32 else None
-        if q_tiles.shape[0]:
-            with _device(q):
-                call("s2g_packed_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), ptr(q_tiles), q_tiles.shape[0],
-                     ctypes.byref(dims), stream_ptr())
+        if plan.q_list[1]:
+            _launch(plan.device, "s2g_packed_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(rest), ptr(lse),
+                    *plan.q_list, plan.fwd)
         ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.pack, ctx.how = pack, (causal, scale)
+        ctx.plan = plan
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         q, k, v, out, rest, lse = ctx.saved_tensors
-        pack, (causal, scale) = ctx.pack, ctx.how
-        (R, H, D), (M, Hk, _) = q.shape, k.shape
-        G, dev = H // Hk, q.device
-        do = _rows16(do)
-        dims = S2GPacked(TYPES[q.dtype], H, Hk, D, int(causal), scale, *_strides(q), *_strides(k), *_strides(v), *_strides(do), R, M)
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
-        dq[pack.rows:].zero_()
-        dk[pack.key_rows:].zero_()
-        dv[pack.key_rows:].zero_()
-        q_tiles, (k_tiles, cut, slots) = pack.query_tiles(G, causal), pack.key_tiles(G, causal, Hk)
-        delta = torch.empty(Hk * R * G, dtype=torch.float32, device=dev)
-        work = torch.empty(get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots), dtype=torch.float32, device=dev)
-        with _device(q):
-            call("s2g_packed_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(do), ptr(lse), ptr(delta), ptr(dq), ptr(dk),
-                 ptr(dv), ptr(work) if slots else None, ptr(q_tiles), q_tiles.shape[0], ptr(k_tiles), k_tiles.shape[0], ptr(cut),
-                 cut.shape[0], ctypes.byref(dims), stream_ptr())
-        return dq, dk, dv, None, None, None
+        plan = ctx.plan
+        if do.data_ptr() & 15 or not _fetchable(do):
+            do = _copy(do)
+        dims, lists, floats = plan.backward(do)
+        dq, dk, dv = _new(q), _new(k), _new(v)
+        if not plan.whole:
+            dq[plan.rows:].zero_()
+            dk[plan.key_rows:].zero_()
+            dv[plan.key_rows:].zero_()
+        work = lse.new_empty(floats) if floats else None
+        _launch(plan.device, "s2g_packed_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(rest), do.data_ptr(),
+                lse.data_ptr(), lse.data_ptr() + 4 * plan.stats, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(work), *plan.q_list, *lists, dims)
+        return dq, dk, dv, None
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: PackedSequences, causal: bool = True,
@@ -308,15 +380,19 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Pa
     reading kv head h // (heads / kv heads); dim a multiple of 8 up to 128; scale: 1 / sqrt(dim).  A row that sees no key
     gives zeros; rows behind the last sequence give zeros and have no gradient.  Differentiable in q, k and v, with the
     same bits on every run."""
-    _check("packed_attention", q=q, k=k, v=v)
-    _attention_shapes("packed_attention", q, k, v)
-    if not isinstance(pack, PackedSequences) or pack.device != q.device:
-        raise S2GError(f"packed_attention: pack must be PackedSequences on {q.device}")
-    if q.shape[0] < pack.rows or k.shape[0] < pack.key_rows:
-        raise S2GError(f"packed_attention: the layout needs {pack.rows} queries and {pack.key_rows} keys, got {q.shape[0]} and {k.shape[0]}")
-    if q.shape[0] * q.shape[1] >= 1 << 30 or k.shape[0] >= 1 << 30:
-        raise S2GError("packed_attention: 2^30 rows or more")
-    return PackedAttentionFn.apply(q, k, v, pack, bool(causal), _scale("packed_attention", scale, q.shape[2]))
+    if not isinstance(pack, PackedSequences):
+        raise S2GError("packed_attention: pack must be PackedSequences")
+    try:
+        key = (_layout(q, k, v), causal, scale)
+    except AttributeError:
+        raise S2GError("packed_attention: q, k and v must be GPU tensors") from None
+    plan = pack._plans.get(key)
+    if plan is None:
+        plan = pack._plans[key] = _PackedPlan(pack, q, k, v, bool(causal), scale)
+    copies = [c or x.data_ptr() & 15 for c, x in zip(plan.copies, (q, k, v))]
+    if any(copies):                                    # rows that cannot be fetched in 16-byte units, or do not start so
+        return packed_attention(*(_copy(x) if c else x for c, x in zip(copies, (q, k, v))), pack, causal, scale)
+    return PackedAttentionFn.apply(q, k, v, plan)
 
 
 # ---------------------------------------------------------------------------------------------------------- paged cache
@@ -326,6 +402,8 @@ class PagedBatch:
     new; the new tokens of all sequences lie one after another, `rows` in all.  table, lengths and starts live on the
     device and may be rewritten there between launches (a captured decoding loop does `batch.lengths.add_(1)`), up to
     max_length tokens a sequence; what the host knows is max_new, max_length and rows."""
+
+    __slots__ = ("table", "lengths", "starts", "sequences", "rows", "max_new", "max_length", "_length", "_new", "_cuts", "_plans")
 
     def __init__(self, table, lengths: Sequence[int], new_lengths: Sequence[int], max_length: Optional[int] = None, device=None):
         n, c = np.asarray(new_lengths, dtype=np.int64).reshape(-1), np.asarray(lengths, dtype=np.int64).reshape(-1)
@@ -345,9 +423,12 @@ class PagedBatch:
         self.lengths, self.starts = _on_device(c, dev), _on_device(np.append(0, np.cumsum(n)), dev)
         self.sequences, self.rows, self.max_new = n.size, int(n.sum()), int(n.max())
         self.max_length = int(c.max()) if max_length is None else int(max_length)
-        self._length, self._new, self._cuts = c, n, {}
+        self._length, self._new, self._cuts, self._plans = c, n, {}, {}
         if self.max_length < c.max():
             raise S2GError("PagedBatch: max_length is below a length")
+
+    def pointers(self) -> Tuple[int, int, int]:
+        return self.table.data_ptr(), self.lengths.data_ptr(), self.starts.data_ptr()
 
 
 def _pool(what: str, keys: torch.Tensor, values: torch.Tensor) -> Tuple[int, int, int]:
@@ -373,8 +454,40 @@ def _batch(what: str, batch: PagedBatch, q: torch.Tensor, keys: torch.Tensor) ->
 
 
 def _no_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise S2GError(f"{what} serves: it has no gradient (call it under torch.no_grad())")
+
+
+def _plan_of(batch, what, how, make, *tensors):
+    """The batch's plan for tensors laid out like these, made (and they checked) when they first come."""
+    if not isinstance(batch, PagedBatch):
+        raise S2GError(f"{what}: batch must be a PagedBatch")
+    try:
+        key = (what, how, _layout(*tensors))
+    except AttributeError:
+        raise S2GError(f"{what}: needs GPU tensors") from None
+    got = batch._plans.get(key)
+    if got is None:
+        got = batch._plans[key] = make(batch, how, *tensors)
+    return got
+
+
+class _AppendPlan:
+    def __init__(self, batch, how, q, k, v, keys, values, frequencies):
+        what = "append_rotary"
+        _check(what, q=q, k=k, v=v, keys=keys, values=values)
+        if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or q.shape[1] == 0:
+            raise S2GError(f"{what}: q must be [tokens, heads, dim], k and v [tokens, kv heads, dim]")
+        page_ld, token_ld, head_ld = _pool(what, keys, values)
+        if tuple(keys.shape[2:]) != tuple(k.shape[1:]) or k.shape[1] == 0:
+            raise S2GError(f"{what}: pages hold heads {tuple(keys.shape[2:])}, k has {tuple(k.shape[1:])}")
+        _batch(what, batch, q, keys)
+        self.copy = any(x.stride(2) != 1 for x in (q, k, v))
+        self.device, self.whole = q.get_device(), q.shape[0] == batch.rows
+        dims = _rotary_dims(q, k, v, _frequencies(what, frequencies, q.get_device(), q.shape[2]), bool(how[0]), float(how[1]), False)
+        paged = S2GPaged(sequences=batch.sequences, page_size=keys.shape[1], pages=keys.shape[0], table_cols=batch.table.shape[1],
+                         max_new=batch.max_new, page_ld=page_ld, token_ld=token_ld, head_ld=head_ld)
+        self.args, self.paged = ctypes.byref(dims), ctypes.byref(paged)
 
 
 def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
@@ -383,24 +496,17 @@ def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch
     by the tokens' positions in their sequences, k and v written to their pages (keys, values: [pages, page size, kv heads,
     dim], in place), the turned q returned.  A token whose position has no page is not written.  Rows of q behind the
     batch's come back as zeros.  No two sequences may own a page that both write to."""
-    _check("append_rotary", q=q, k=k, v=v, keys=keys, values=values)
     _no_grad("append_rotary", q, k, v, keys, values)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or q.shape[1] == 0:
-        raise S2GError("append_rotary: q must be [tokens, heads, dim], k and v [tokens, kv heads, dim]")
-    page_ld, token_ld, head_ld = _pool("append_rotary", keys, values)
-    if tuple(keys.shape[2:]) != tuple(k.shape[1:]) or k.shape[1] == 0:
-        raise S2GError(f"append_rotary: pages hold heads {tuple(keys.shape[2:])}, k has {tuple(k.shape[1:])}")
-    _batch("append_rotary", batch, q, keys)
-    q, k, v = _dense(q), _dense(k), _dense(v)
-    dims = _rotary_dims("append_rotary", q, k, v, frequencies, interleaved, multiplier, False)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out[batch.rows:].zero_()
+    plan = _plan_of(batch, "append_rotary", (interleaved, multiplier), _AppendPlan, q, k, v, keys, values, frequencies)
+    if plan.copy:
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        plan = _plan_of(batch, "append_rotary", (interleaved, multiplier), _AppendPlan, q, k, v, keys, values, frequencies)
+    out = _new(q)
+    if not plan.whole:
+        out[batch.rows:].zero_()
     if batch.rows:
-        paged = S2GPaged(sequences=batch.sequences, page_size=keys.shape[1], pages=keys.shape[0], table_cols=batch.table.shape[1],
-                         max_new=batch.max_new, page_ld=page_ld, token_ld=token_ld, head_ld=head_ld)
-        with _device(q):
-            call("s2g_rotary_append", ptr(q), ptr(k), ptr(v), ptr(frequencies), ptr(out), ptr(keys), ptr(values), ptr(batch.table),
-                 ptr(batch.lengths), ptr(batch.starts), ctypes.byref(dims), ctypes.byref(paged), stream_ptr())
+        _launch(plan.device, "s2g_rotary_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), frequencies.data_ptr(), out.data_ptr(),
+                keys.data_ptr(), values.data_ptr(), *batch.pointers(), plan.args, plan.paged)
     return out
 
 
@@ -438,37 +544,52 @@ def _cut(batch: PagedBatch, Hk: int, G: int, D: int, size: int) -> Tuple[bool, i
     return got
 
 
+class _PagedPlan:
+    """One layout of q and of the pool for one batch: checked once, cut into parts, the kernel's arguments kept."""
+
+    def __init__(self, batch, how, q, keys, values):
+        causal, scale = how
+        what = "paged_attention"
+        _check(what, q=q, keys=keys, values=values)
+        page_ld, token_ld, head_ld = _pool(what, keys, values)
+        if q.dim() != 3 or q.shape[2] != keys.shape[3]:
+            raise S2GError(f"{what}: q must be [tokens, heads, {keys.shape[3]}]")
+        (R, H, D), Hk = q.shape, keys.shape[2]
+        _attention_heads(what, H, Hk, D)
+        unit = 16 // q.element_size()
+        if any(s % unit for s in (page_ld, token_ld, head_ld)) or max(token_ld, head_ld) >= 1 << 22:
+            raise S2GError(f"{what}: pages must be strided by multiples of 16 bytes")
+        _batch(what, batch, q, keys)
+        if R * H >= 1 << 30:
+            raise S2GError(f"{what}: 2^30 rows or more")
+        by_rows, part_keys, parts = _cut(batch, Hk, H // Hk, D, q.element_size())
+        self.copy, self.device, self.whole = not _fetchable(q), q.get_device(), R == batch.rows
+        dims = S2GPaged(TYPES[q.dtype], batch.sequences, H, Hk, D, int(bool(causal)), keys.shape[1], keys.shape[0], batch.table.shape[1],
+                        batch.max_new, batch.max_length, part_keys, parts, int(by_rows), _scale(what, scale, D), R, *_strides(q),
+                        page_ld, token_ld, head_ld)
+        self.args = ctypes.byref(dims)
+        self.floats = 0 if self.copy or not batch.rows else get().s2g_paged_attention_workspace(self.args)
+
+
 def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, batch: PagedBatch, causal: bool = True,
                     scale: Optional[float] = None) -> torch.Tensor:
     """Attention of a batch's new tokens (q [tokens, heads, dim]) over what its sequences hold in the cache: query i of n
     new tokens of a sequence of m sees keys j <= m - n + i (causal) or all m.  One token or thousands per sequence, mixed
     at will; types, heads and scale as in packed_attention.  A page number outside the pool is a page whose keys are not
     there; a query without keys gives zeros, and so do rows of q behind the batch's."""
-    _check("paged_attention", q=q, keys=keys, values=values)
     _no_grad("paged_attention", q, keys, values)
-    page_ld, token_ld, head_ld = _pool("paged_attention", keys, values)
-    if q.dim() != 3 or q.shape[2] != keys.shape[3]:
-        raise S2GError(f"paged_attention: q must be [tokens, heads, {keys.shape[3]}]")
-    (R, H, D), Hk = q.shape, keys.shape[2]
-    _attention_heads("paged_attention", H, Hk, D)
-    unit = 16 // q.element_size()
-    if any(s % unit for s in (page_ld, token_ld, head_ld)) or keys.data_ptr() % 16 or values.data_ptr() % 16 or max(token_ld, head_ld) >= 1 << 22:
-        raise S2GError("paged_attention: pages must start, and be strided, at multiples of 16 bytes")
-    _batch("paged_attention", batch, q, keys)
-    s = _scale("paged_attention", scale, D)
-    if R * H >= 1 << 30:
-        raise S2GError("paged_attention: 2^30 rows or more")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out[batch.rows:].zero_()
+    plan = _plan_of(batch, "paged_attention", (causal, scale), _PagedPlan, q, keys, values)
+    if plan.copy or q.data_ptr() & 15:
+        return paged_attention(_copy(q), keys, values, batch, causal, scale)
+    if (keys.data_ptr() | values.data_ptr()) & 15:
+        raise S2GError("paged_attention: pages must start at multiples of 16 bytes")
+    out = _new(q)
+    if not plan.whole:
+        out[batch.rows:].zero_()
     if batch.rows:
-        q = _rows16(q)
-        by_rows, part_keys, parts = _cut(batch, Hk, H // Hk, D, q.element_size())
-        dims = S2GPaged(TYPES[q.dtype], batch.sequences, H, Hk, D, int(causal), keys.shape[1], keys.shape[0], batch.table.shape[1],
-                        batch.max_new, batch.max_length, part_keys, parts, int(by_rows), s, R, *_strides(q), page_ld, token_ld, head_ld)
-        work = torch.empty(max(0, get().s2g_paged_attention_workspace(ctypes.byref(dims))), dtype=torch.float32, device=q.device)
-        with _device(q):
-            call("s2g_paged_attention", ptr(q), ptr(keys), ptr(values), ptr(batch.table), ptr(batch.lengths), ptr(batch.starts),
-                 ptr(out), ptr(work) if parts > 1 else None, ctypes.byref(dims), stream_ptr())
+        work = q.new_empty(plan.floats, dtype=torch.float32) if plan.floats else None
+        _launch(plan.device, "s2g_paged_attention", q.data_ptr(), keys.data_ptr(), values.data_ptr(), *batch.pointers(), out.data_ptr(), ptr(work),
+                plan.args)
     return out
 
 
