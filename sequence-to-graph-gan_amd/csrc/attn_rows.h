@@ -2,11 +2,12 @@
 #pragma once
 #include "frag.h"
 
+// DP: the feature width the kernels are compiled for; rows in LDS are a power of two of 16-byte chunks, four at least
 template <typename T, int DP>
 struct Shape {
-  static constexpr int PITCH = DP == 96 ? 128 : DP;
-  static constexpr int KT = sizeof(T) == 2 ? 64 : 32;        // keys (rows, in the key-side backward pass) per LDS tile
-  static constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  static constexpr int PITCH = DP == 96 ? 128 : DP == 16 && sizeof(T) == 2 ? 32 : DP;
+  static constexpr int KT = sizeof(T) == 2 || DP == 16 ? 64 : 32;      // keys (rows, in the key-side backward pass) per LDS tile
+  static constexpr int KS = DP / 16, DB = (DP + 31) / 32, KB = KT / 32;
   static constexpr int AHEAD = 2;
   typedef Tile<T, PITCH, KT, 4> LT;
 };
@@ -28,14 +29,22 @@ __device__ __forceinline__ void fetch_rows(char* lds, const T* p, long ld, int D
   for (int i = 0; i < LT::NI; ++i) load_to_lds(b, to + (i * 4 + wave) * 1024, off[i]);
 }
 
-// 8 elements of a row straight from memory: zeros beyond the row's D elements or where !ok
+// 8 elements of a row straight from memory: zeros beyond the row's D elements or where !ok.  The loads are unconditional (of
+// the row's beginning where there is nothing to load; the row itself always exists), so that many are on their way at once.
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::v8 row8(const T* p, int at, int D, bool ok) {
-  if (sizeof(T) == 2 || at + 8 <= D) return ok && at < D ? load8(p + at) : zero8<T>();
-  typename Vec<T>::v8 r = zero8<T>();              // fp32 rows come in fours
-  if (ok && at < D) {
+  typename Vec<T>::v8 r;
+  if constexpr (sizeof(T) == 2) {
+    r = load8(p + (at < D ? at : 0));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = p[at + j];
+    for (int j = 0; j < 8; ++j) r[j] = ok && at < D ? r[j] : (T)0.0f;
+  } else {                                          // fp32 rows come in fours
+    const fx4 a = *reinterpret_cast<const fx4*>(p + (at < D ? at : 0)), b = *reinterpret_cast<const fx4*>(p + (at + 4 < D ? at + 4 : 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r[j] = ok && at < D ? a[j] : 0.0f;
+      r[j + 4] = ok && at + 4 < D ? b[j] : 0.0f;
+    }
   }
   return r;
 }

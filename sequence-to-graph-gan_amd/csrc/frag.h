@@ -146,7 +146,8 @@ struct Tile {
       return (fx8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
-  // contraction across rows: column 32 d + lane % 32, rows 16 s + 4 half + {0..3, 8..11}
+  // contraction across rows: column 32 d + lane % 32 (of a 16-column tile: columns 16 .. 31 repeat 0 .. 15, nobody takes
+  // them), rows 16 s + 4 half + {0..3, 8..11}
   static __device__ __forceinline__ typename Vec<T>::v8 across(const char* lds, int d, int s, int lane) {
     const int half = lane >> 5;
     if constexpr (ES == 2) {
@@ -161,7 +162,7 @@ struct Tile {
       }
       return u.v;
     } else {
-      const int col = 32 * d + (lane & 31);
+      const int col = (32 * d + (lane & 31)) % PITCH;
       fx8 v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -33,7 +33,8 @@ struct PackedDims {
 
 // F<T, width>(...) for the feature width that holds dm.D
 #define PER_DIM(F, T, ...)                          \
-  (dm.D <= 32   ? F<T, 32>(__VA_ARGS__)             \
+  (dm.D <= 16   ? F<T, 16>(__VA_ARGS__)             \
+   : dm.D <= 32 ? F<T, 32>(__VA_ARGS__)             \
    : dm.D <= 64 ? F<T, 64>(__VA_ARGS__)             \
    : dm.D <= 96 ? F<T, 96>(__VA_ARGS__)             \
                 : F<T, 128>(__VA_ARGS__))

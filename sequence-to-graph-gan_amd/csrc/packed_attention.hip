@@ -140,19 +140,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 
   v8 q[S::KS], g[S::KS];
   float dl = 0.0f;
+  {
+    v8 y[S::KS], x[S::KS];
+    const bool few = sizeof(T) == 2 && w_lo < FEW_KEYS;
 #pragma unroll
-  for (int s = 0; s < S::KS; ++s) {
-    const int at = 16 * s + 8 * half;
-    q[s] = row8(qp, at, dm.D, live);
-    g[s] = row8(gp, at, dm.D, live);
-    const v8 y = row8(out + orow, at, dm.D, live);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)y[j], dl);
-    if (sizeof(T) == 2 && w_lo < FEW_KEYS) {
-      const v8 x = row8(rest + orow, at, dm.D, live && last < FEW_KEYS);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)x[j], dl);
+    for (int s = 0; s < S::KS; ++s) {
+      const int at = 16 * s + 8 * half;
+      q[s] = row8(qp, at, dm.D, live);
+      g[s] = row8(gp, at, dm.D, live);
+      y[s] = row8(out + orow, at, dm.D, live);
     }
+    if (few)
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) x[s] = row8(rest + orow, 16 * s + 8 * half, dm.D, live && last < FEW_KEYS);
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)y[s][j], dl);
+    if (few)
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dl = fmaf((float)g[s][j], (float)x[s][j], dl);
   }
   dl = both_sum(dl);
   const float L = live ? lse[lrow] : INFINITY, c = dm.scale * LOG2E;
