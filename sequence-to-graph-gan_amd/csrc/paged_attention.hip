@@ -8,7 +8,7 @@
 // of 32 keys of its own through LDS without ever waiting for the others, and the waves join at the end.  Chunks of new
 // tokens are bound by the products: a workgroup takes 128 rows, its waves share tiles of 64 keys.  Either way a long
 // axis is cut into parts of part_keys keys so that few rows still fill the chip; parts leave (O, m, l) in 32 bits and
-// s2g_k_paged_join adds them in order.  A sequence with a single part is written at once.
+// s2g_k_paged_join_few / _many add them in order.  A sequence with a single part is written at once.
 //
 // Lengths and pages come from device memory (a captured decoding loop updates them there), so nothing read from it is
 // trusted: lengths are cut to what the table covers, a page number outside the pool is a page that is not there.
@@ -257,20 +257,66 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
   }
 }
 
-// WAVES waves per row (4 where there are many parts, else 1 and four rows to a workgroup): each brings its share of the
-// parts to the row's maximum, eight at a time (a loop of single loads would wait for memory at every part), and the waves'
-// sums are added in order.
-template <typename T, int WAVES>
-__global__ __launch_bounds__(256) void s2g_k_paged_join(const float* __restrict__ ws, const int* __restrict__ lens,
-                                                        const int* __restrict__ starts, T* __restrict__ out, int tile_rows,
-                                                        PagedDims dm) {
-  __shared__ float sum[4][132];
-  const int lane = threadIdx.x & 63, id = uniform(threadIdx.x >> 6), wave = id % WAVES;
-  const int kvh = blockIdx.x % dm.Hk, row = blockIdx.x / dm.Hk * (4 / WAVES) + id / WAVES, s = blockIdx.z;
-  const PagedSeq sq = paged_seq(lens, starts, s, dm);
-  const int seen = row < sq.rows ? keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm) : 0;   // as the row's workgroup saw it
+// The parts of a row brought to its maximum and added.  Up to 32 parts: half a wave to a row, lane p of the half holding
+// part p's factor, each lane four features.
+template <typename T>
+__global__ __launch_bounds__(256) void s2g_k_paged_join_few(const float* __restrict__ ws, const int* __restrict__ lens,
+                                                            const int* __restrict__ starts, T* __restrict__ out, int tile_rows,
+                                                            PagedDims dm) {
+  const int l32 = threadIdx.x & 31, kvh = blockIdx.x % dm.Hk, row = blockIdx.x / dm.Hk * 8 + (threadIdx.x >> 5);
+  const PagedSeq sq = paged_seq(lens, starts, blockIdx.z, dm);
+  if (row >= sq.rows) return;
+  const int seen = keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm);     // as the row's workgroup saw it
   const int parts = (seen + dm.part_keys - 1) / dm.part_keys;
-  if (parts <= 1) return;                       // all waves of the row, and of the workgroup where they share one
+  if (parts <= 1) return;
+  const Joined j = workspace(const_cast<float*>(ws), dm);
+  const long at = ws_row(sq, kvh, row, dm) * dm.parts;
+  const float* sums = j.sums + at * dm.D;
+  const int p0 = min(l32, parts - 1), d = min(4 * l32, dm.D - 4);
+  const float2 ml = *reinterpret_cast<const float2*>(j.ml + 2 * (at + p0));
+  fx4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  fx4 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const fx4*>(sums + (long)min(i, parts - 1) * dm.D + d);
+  float m = ml.x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f((ml.x - m) * dm.scale * LOG2E);
+  float l = l32 < parts ? ml.y * f : 0.0f;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) l += __shfl_xor(l, o);
+  for (int p = 0; p < parts; p += 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = __shfl(f, p + i, 32);
+      if (p + i < parts) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = fmaf(x[i][k], w, a[k]);
+      }
+      x[i] = *reinterpret_cast<const fx4*>(sums + (long)min(p + 4 + i, parts - 1) * dm.D + d);
+    }
+  }
+  if (4 * l32 >= dm.D) return;
+  const int tk = divide(row, dm.by);
+  typename Vec<T>::v4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = (T)(l == 0.0f ? 0.0f : a[k] / l);
+  *reinterpret_cast<typename Vec<T>::v4*>(out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + row - tk * dm.by.G) * dm.D + d) = v;
+}
+
+// Many parts: a workgroup to a row, the parts dealt to its four waves, eight loads of each on their way at a time (a loop of
+// single loads would wait for memory at every part), the waves' sums added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void s2g_k_paged_join_many(const float* __restrict__ ws, const int* __restrict__ lens,
+                                                             const int* __restrict__ starts, T* __restrict__ out, int tile_rows,
+                                                             PagedDims dm) {
+  __shared__ float sum[4][132];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % dm.Hk, row = blockIdx.x / dm.Hk;
+  const PagedSeq sq = paged_seq(lens, starts, blockIdx.z, dm);
+  const int seen = row < sq.rows ? keys_seen(sq, row / tile_rows * tile_rows + tile_rows - 1, dm) : 0;
+  const int parts = (seen + dm.part_keys - 1) / dm.part_keys;
+  if (parts <= 1) return;                       // the whole workgroup
   const Joined j = workspace(const_cast<float*>(ws), dm);
   const long at = ws_row(sq, kvh, row, dm) * dm.parts;
   const float* ml = j.ml + 2 * at;
@@ -282,11 +328,11 @@ __global__ __launch_bounds__(256) void s2g_k_paged_join(const float* __restrict_
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
   const int f0 = min(lane, dm.D - 1), f1 = min(lane + 64, dm.D - 1);
   float l = 0.0f, a0 = 0.0f, a1 = 0.0f;
-  for (int p0 = wave; p0 < parts; p0 += 8 * WAVES) {
+  for (int p0 = wave; p0 < parts; p0 += 32) {
     float mp[8], lp[8], x0[8], x1[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int p = min(p0 + WAVES * i, parts - 1);
+      const int p = min(p0 + 4 * i, parts - 1);
       mp[i] = ml[2 * p];
       lp[i] = ml[2 * p + 1];
       x0[i] = sums[(long)p * dm.D + f0];
@@ -294,23 +340,21 @@ __global__ __launch_bounds__(256) void s2g_k_paged_join(const float* __restrict_
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (p0 + WAVES * i < parts) {
+      if (p0 + 4 * i < parts) {
         const float f = mp[i] == m ? 1.0f : __builtin_amdgcn_exp2f((mp[i] - m) * c);
         l = fmaf(lp[i], f, l);
         a0 = fmaf(x0[i], f, a0);
         a1 = fmaf(x1[i], f, a1);
       }
   }
-  if constexpr (WAVES > 1) {
-    sum[wave][lane] = a0;
-    sum[wave][lane + 64] = a1;
-    if (lane == 0) sum[wave][128] = l;
-    __syncthreads();
-    if (wave != 0) return;
-    a0 = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
-    a1 = (sum[0][lane + 64] + sum[1][lane + 64]) + (sum[2][lane + 64] + sum[3][lane + 64]);
-    l = (sum[0][128] + sum[1][128]) + (sum[2][128] + sum[3][128]);
-  }
+  sum[wave][lane] = a0;
+  sum[wave][lane + 64] = a1;
+  if (lane == 0) sum[wave][128] = l;
+  __syncthreads();
+  if (wave != 0) return;
+  a0 = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+  a1 = (sum[0][lane + 64] + sum[1][lane + 64]) + (sum[2][lane + 64] + sum[3][lane + 64]);
+  l = (sum[0][128] + sum[1][128]) + (sum[2][128] + sum[3][128]);
   const int tk = divide(row, dm.by);
   T* o = out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + row - tk * dm.by.G) * dm.D;
   if (lane < dm.D) o[lane] = (T)(l == 0.0f ? 0.0f : a0 / l);
@@ -336,10 +380,10 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   }
-  if (dm.parts > 16)
-    hipLaunchKernelGGL((s2g_k_paged_join<T, 4>), dim3((unsigned)dm.Hk * dm.max_rows, 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
+  if (dm.parts > 32)
+    hipLaunchKernelGGL(s2g_k_paged_join_many<T>, dim3((unsigned)dm.Hk * dm.max_rows, 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
   else if (dm.parts > 1)
-    hipLaunchKernelGGL((s2g_k_paged_join<T, 1>), dim3((unsigned)dm.Hk * ((dm.max_rows + 3) / 4), 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
+    hipLaunchKernelGGL(s2g_k_paged_join_few<T>, dim3((unsigned)dm.Hk * ((dm.max_rows + 7) / 8), 1, dm.n), dim3(256), 0, st, ws, lens, starts, (T*)out, tile_rows, dm);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
