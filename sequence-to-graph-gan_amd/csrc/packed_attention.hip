@@ -190,29 +190,43 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     const int k0 = t * S::KT;
     if (k0 > w_hi) continue;
     const bool edge = k0 + S::KT - 1 > w_lo;
+    // 32 keys at a time, 2^x beside the products of dP, dS beside those of the next keys' S
+    fx16 st = zero16(), next;
+    products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(kt, lane & 31, i, half); },
+                                 [&](int i, const v8& a) { st = mma(a, q[i], st); }, [](int) {});
 #pragma unroll
     for (int b = 0; b < S::KB; ++b) {
-      fx16 st = zero16(), dp = zero16();
+      fx16 dp = zero16();
+      products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(vt, 32 * b + (lane & 31), i, half); },
+                                   [&](int i, const v8& a) { dp = mma(a, g[i], dp); },
+                                   [&](int i) {
 #pragma unroll
-      for (int s = 0; s < S::KS; ++s) st = mma(LT::along(kt, 32 * b + (lane & 31), s, half), q[s], st);
-#pragma unroll
-      for (int s = 0; s < S::KS; ++s) dp = mma(LT::along(vt, 32 * b + (lane & 31), s, half), g[s], dp);
+                                     for (int e = 16 * i / S::KS; e < 16 * (i + 1) / S::KS; ++e) st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -L));
+                                   });
       // a row that sees one key only has D = dP there, to the last bit: its scores have no gradient
       if (b == 0 && k0 == 0 && last == 0) dl = dp[0];
+      const auto slope = [&](int i) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], c, -L)) * (dp[i] - dl);
+        for (int e = 16 * i / S::KS; e < 16 * (i + 1) / S::KS; ++e) st[e] *= dp[e] - dl;
+      };
+      if (b + 1 < S::KB) {
+        next = zero16();
+        products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(kt, 32 * (b + 1) + (lane & 31), i, half); },
+                                     [&](int i, const v8& a) { next = mma(a, q[i], next); }, slope);
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::KS; ++i) slope(i);
+      }
       if (edge) {
-        const int at = hidden(last - k0 - 4 * half);
+        const int at = hidden(last - k0 - 32 * b - 4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * b + reg_row(i) > at) st[i] = 0.0f;
+          if (reg_row(i) > at) st[i] = 0.0f;
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const v8 ds = operand<T>(st, s);
-#pragma unroll
-        for (int d = 0; d < S::DB; ++d) dq[d] = mma(LT::across(kt, d, 2 * b + s, lane), ds, dq[d]);
-      }
+      const v8 ds[2] = {operand<T>(st, 0), operand<T>(st, 1)};
+      products<T, 2 * S::DB, S::AHEAD>([&](int i) { return LT::across(kt, i % S::DB, 2 * b + i / S::DB, lane); },
+                                       [&](int i, const v8& a) { dq[i % S::DB] = mma(a, ds[i / S::DB], dq[i % S::DB]); }, [](int) {});
+      st = next;
     }
   }
   if (live && half == 0) delta[lrow] = dl;
