@@ -67,6 +67,32 @@ __device__ __forceinline__ void store_rows(U* p, const fx16* acc, float f, int D
     }
 }
 
+// acc += f x row, in the layout of a transposed result, row by row: the slow way, for tiles that products cannot take
+template <typename T, int DB>
+__device__ __forceinline__ void add_row(fx16* acc, float f, const T* p, int D, int half) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = 32 * d + 8 * g + 4 * half;
+      const typename Vec<T>::v4 x = *reinterpret_cast<const typename Vec<T>::v4*>(p + (at < D ? at : 0));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[d][4 * g + j] = fmaf(f, at < D ? (float)x[j] : 0.0f, acc[d][4 * g + j]);
+      __builtin_amdgcn_sched_barrier(0);              // one load at a time: its registers are the main loop's
+    }
+}
+// the dot product of a row with operands held in registers, this half's share of it
+template <typename T, int KS>
+__device__ __forceinline__ float dot_row(const typename Vec<T>::v8* a, const T* p, int D, int half) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    s = dot8(a[i], row8(p, 16 * i + 8 * half, D, true), s);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return s;
+}
+
 // fp16 weights below 2^-14 lose bits, and a long row's weights are that small: there all of them are taken 2^RAISE times
 // as large (the sums alike, so it cancels), as much as the largest term, 2^SLACK, leaves room for.
 template <typename T> struct Weights { static constexpr float RAISE = 0.0f, SLACK = 8.0f; };
@@ -81,13 +107,14 @@ struct Rows {
   v8 q[S::KS];
   fx16 o[S::DB];
   float m, l, c, slack;
+  bool tainted;              // a tile with hidden keys held an infinity or a NaN in V: o is not to be used (repair)
 
   __device__ __forceinline__ void begin(const T* qp, int D, bool live, int half, float scale) {
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) q[s] = row8(qp, 16 * s + 8 * half, D, live);
 #pragma unroll
     for (int d = 0; d < S::DB; ++d) o[d] = zero16();
-    m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c;
+    m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c, tainted = false;
   }
   // S^T = K Q^T of KB blocks of 32 keys: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's
   // own registers and one exchange between the halves
@@ -106,6 +133,7 @@ struct Rows {
                                       unsigned long long absent, int lane) {
     const int half = lane >> 5;
     if (edge) {
+      tainted = tainted || not_finite<T>(vt, 32 * KB * S::PITCH * (int)sizeof(T), lane);
       const int at = hidden(last - 4 * half);
 #pragma unroll
       for (int b = 0; b < KB; ++b)
@@ -168,6 +196,16 @@ struct Rows {
     fx16 st[KB];
     scores<KB>(st, kt, lane, [](int) {});
     add<KB, false>(st, nullptr, nullptr, vt, edge, last, absent, lane);
+  }
+  // One key of o made anew: each row adds its own keys only, whatever the others hold.
+  __device__ __forceinline__ void repair(const T* kp, const T* vp, bool sees, int D, int half) {
+    const float s = dot_row<T, S::KS>(q, kp, D, half);
+    const float w = __builtin_amdgcn_exp2f(fmaf(both_sum(s), c, Weights<T>::RAISE - (m == -INFINITY ? 0.0f : m * c)));
+    if (sees) add_row<T, S::DB>(o, w, vp, D, half);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < S::DB; ++d) o[d] = zero16();
   }
   // log2 of the row's sum of exponentials, given the sum over both halves
   __device__ __forceinline__ float log_sum(float sum) const { return fmaf(m, c, __builtin_amdgcn_logf(sum)) - Weights<T>::RAISE; }

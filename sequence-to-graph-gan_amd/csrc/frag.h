@@ -11,6 +11,7 @@
 // read in that same order (Tile::across).
 #pragma once
 #include "s2g_common.h"
+#include <type_traits>
 
 typedef float fx16 __attribute__((ext_vector_type(16)));
 typedef float fx8 __attribute__((ext_vector_type(8)));
@@ -222,6 +223,28 @@ __device__ __forceinline__ void products(L load, U use, B beside) {
       beside(i);
     }
   }
+}
+
+// Whether `bytes` (a multiple of 1024) of LDS hold an infinity or a NaN; the same in all lanes.  A product takes 0 x NaN for
+// NaN, so where a tile holds one, what a row (or key) does not see has to be kept from it some other way.
+template <typename T>
+__device__ __forceinline__ bool not_finite(const char* lds, int bytes, int lane) {
+  constexpr unsigned EXP = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, _Float16>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr unsigned ONE = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u;
+  unsigned any = 0;
+  for (int at = lane * 16; at < bytes; at += 1024) {
+    const ix4 x = *reinterpret_cast<const ix4*>(lds + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= ((unsigned)x[i] & EXP) + ONE;      // an exponent of ones carries into the sign
+  }
+  return __any(any & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u));
+}
+// sum over 8 elements, in fp32
+template <typename V>
+__device__ __forceinline__ float dot8(const V& a, const V& b, float s) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s = fmaf((float)a[j], (float)b[j], s);
+  return s;
 }
 
 // wave-uniform values: tells the compiler to keep them in scalar registers

@@ -15,7 +15,88 @@
 // b / Hk: with 8 kv heads each XCD (workgroups are dealt to the 8 XCDs in turn) keeps to one head's K and V.
 #include "attn_rows.h"
 #include "packed_attention.h"
-#include <type_traits>
+
+// ------------------------------------------------------------------------------------------------- infinities and NaN
+// A product takes 0 x NaN for NaN, so a tile that holds one, and a row (key) that does not see it, cannot go through the
+// matrix unit together.  Where a tile with hidden pairs holds one, a wave makes its 32 rows (keys) anew: pair by pair,
+// straight from memory, 16 features at a time, and only the pairs that see each other.  Functions of their own, never
+// inlined: their registers would be the main loops' (query side 297 -> 330 us).
+template <typename T, int N>
+__device__ __forceinline__ float slow_dot(const T* a, const T* b, int D, int half) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int i = 0; i < N; ++i) s = dot8(row8(a, 16 * i + 8 * half, D, true), row8(b, 16 * i + 8 * half, D, true), s);
+  return both_sum(s);
+}
+template <typename T>
+__device__ __forceinline__ void slow_add(float* acc, float f, const T* p, int from, int D) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int at = from + 4 * g;
+    const typename Vec<T>::v4 x = *reinterpret_cast<const typename Vec<T>::v4*>(p + (at < D ? at : 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[4 * g + j] = fmaf(f, (float)x[j], acc[4 * g + j]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void slow_store(T* p, const float* acc, float f, int from, int D, bool ok) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (ok && from + j < D) p[from + j] = (T)(acc[j] * f);
+}
+// rows of a wave: O = sum over the keys 0 .. last of 2^(c s - base) V, times f
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int keys, int last, float c,
+                                                   float base, float f, T* out, T* rest, int D, bool live) {
+  const int half = (threadIdx.x >> 5) & 1;
+  for (int from = 16 * half; from < DP + 16 * half; from += 32) {                // both halves take every turn: their dots are one
+    float acc[16] = {};
+    for (int key = 0; key < keys; ++key) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -base));
+      if (key <= last) slow_add(acc, w, v + key * ldv, from, D);
+    }
+    slow_store(out, acc, f, from, D, live);
+    if (rest) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[j] = acc[j] * f - (float)(T)(acc[j] * f);
+      slow_store(rest, acc, 1.0f, from, D, live);
+    }
+  }
+}
+// dQ of a wave's rows
+template <typename T, int DP>
+__device__ __attribute__((noinline)) void slow_dq(const T* q, const T* g, const T* k, long ldk, const T* v, long ldv, int keys, int last,
+                                                  float c, float scale, float L, float delta, T* dq, int D, bool live) {
+  const int half = (threadIdx.x >> 5) & 1;
+  for (int from = 16 * half; from < DP + 16 * half; from += 32) {
+    float acc[16] = {};
+    for (int key = 0; key < keys; ++key) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -L));
+      const float ds = last == 0 ? 0.0f : p * (slow_dot<T, DP / 16>(g, v + key * ldv, D, half) - delta);
+      if (key <= last) slow_add(acc, ds, k + key * ldk, from, D);
+    }
+    slow_store(dq, acc, scale, from, D, live);
+  }
+}
+// dK (which 0) or dV (1) of a wave's keys, over the rows lo .. hi of their kv head
+template <typename T, int DP, typename U>
+__device__ __attribute__((noinline)) void slow_key(int which, const T* k, const T* v, const T* Q, const T* dO, const float* lse,
+                                                   const float* delta, int lo, int hi, int first, float c, float f, U* to, bool live,
+                                                   int D, DivBy by, long ldq, long hq, long ldo, long ho) {
+  const int half = (threadIdx.x >> 5) & 1;
+  for (int from = 16 * half; from < DP + 16 * half; from += 32) {
+    float acc[16] = {};
+    for (int r = lo; r < hi; ++r) {
+      const int tk = divide(r, by), h = r - tk * by.G;
+      const T* q = Q + tk * ldq + h * hq;
+      const T* g = dO + tk * ldo + h * ho;
+      const float p = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(k, q, D, half), c, -lse[r]));
+      const float ds = p * (slow_dot<T, DP / 16>(v, g, D, half) - delta[r]);
+      if (r >= first) slow_add(acc, which ? p : ds, which ? g : q, from, D);
+    }
+    slow_store(to, acc, f, from, D, live);
+  }
+}
 
 #define FEW_KEYS 128
 
@@ -91,6 +172,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   }
   const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l;
   const long orow = (qrow * dm.H + head) * dm.D;
+  // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
+  if (lse && live && half == 0)
+    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
+  if (r.tainted) {
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, r.c, (r.m == -INFINITY ? 0.0f : r.m * r.c) - Weights<T>::RAISE, f,
+                    out + orow, sizeof(T) == 2 && rest ? rest + orow : nullptr, dm.D, live);
+    return;
+  }
   store_rows<T, S::DB>(out + orow, r.o, f, dm.D, half, live);
   // what rounding took from O: with it the backward pass has D = dO . O nearly exactly where dP - D is a small difference.
   // Only rows of few keys need it: of n like keys, D's error is 1 / sqrt(n) of what rounding dS adds.  (Without it dQ and dK
@@ -102,9 +191,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
       for (int i = 0; i < 16; ++i) r.o[d][i] = r.o[d][i] * f - (float)(T)(r.o[d][i] * f);
     store_rows<T, S::DB>(rest + orow, r.o, 1.0f, dm.D, half, live && last < FEW_KEYS);
   }
-  // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
-  if (lse && live && half == 0)
-    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
 }
 
 // ------------------------------------------------------------------------------------------------- backward, query side
@@ -169,6 +255,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   int ko[LT::NI], vo[LT::NI];
   tile_offsets<LT, T>(ko, dm.ldk, dm.D, wave, lane);
   tile_offsets<LT, T>(vo, dm.ldv, dm.D, wave, lane);
+  bool tainted = false;            // a tile with hidden keys held an infinity or a NaN in K
   fx16 dq[S::DB];
 #pragma unroll
   for (int d = 0; d < S::DB; ++d) dq[d] = zero16();
@@ -218,6 +305,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
         for (int i = 0; i < S::KS; ++i) slope(i);
       }
       if (edge) {
+        tainted = tainted || not_finite<T>(kt + 32 * b * S::PITCH * (int)sizeof(T), 32 * S::PITCH * (int)sizeof(T), lane);
         const int at = hidden(last - k0 - 32 * b - 4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -230,6 +318,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     }
   }
   if (live && half == 0) delta[lrow] = dl;
+  if (tainted) {
+    slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
+    return;
+  }
   store_rows<T, S::DB>(dQ + orow, dq, dm.scale, dm.D, half, live);
 }
 
@@ -249,6 +341,7 @@ struct KeySums {
   typedef typename Vec<T>::v8 v8;
   v8 k[S::KS], v[S::KS];
   fx16 dv[S::DB], dk[S::DB];
+  bool tainted;                // a tile with rows that do not see some key held an infinity or a NaN
 
   __device__ __forceinline__ void begin(const T* kp, const T* vp, int D, bool live, int half) {
 #pragma unroll
@@ -260,12 +353,14 @@ struct KeySums {
     for (int d = 0; d < S::DB; ++d) {
       dv[d] = zero16();
       dk[d] = zero16();
+      tainted = false;
     }
   }
   // a tile of rows: Q, dO, (L, D); edge: some of them do not see some of the wave's keys (`first`: the first that sees this
   // lane's, counted from the tile's first)
   __device__ __forceinline__ void step(const char* qt, const char* gt, const float* sl, float c, bool edge, int first, int lane) {
     const int half = lane >> 5, col = lane & 31;
+    if (edge) tainted = tainted || not_finite<T>(qt, 2 * LT::BYTES, lane);        // Q and dO, side by side
 #pragma unroll
     for (int b = 0; b < S::KB; ++b) {
       fx16 p = zero16(), ds = zero16();
@@ -360,10 +455,28 @@ struct KeyWork {
       }
     }
   }
+  // where this lane's key's dK (second 0) or dV (1) goes
+  template <typename T>
+  __device__ __forceinline__ T* row_of(T* out, const PackedDims& dm) const { return out + (krow * dm.Hk + kvh) * dm.D; }
+  __device__ __forceinline__ float* slot_of(float* partial, int second, int group, int lane, const PackedDims& dm) const {
+    return partial + (((long)w.slot * dm.Hk + kvh) * 256 + 128 * second + 32 * group + (lane & 31)) * dm.D;
+  }
   template <typename T, int DB>
   __device__ __forceinline__ void store(T* out, float* partial, int second, const fx16* acc, float f, int group, int lane, const PackedDims& dm) const {
-    if (w.slot < 0) store_rows<T, DB>(out + (krow * dm.Hk + kvh) * dm.D, acc, f, dm.D, lane >> 5, live);
-    else store_rows<T, DB>(partial + (((long)w.slot * dm.Hk + kvh) * 256 + 128 * second + 32 * group + (lane & 31)) * dm.D, acc, f, dm.D, lane >> 5, live);
+    if (w.slot < 0) store_rows<T, DB>(row_of(out, dm), acc, f, dm.D, lane >> 5, live);
+    else store_rows<T, DB>(slot_of(partial, second, group, lane, dm), acc, f, dm.D, lane >> 5, live);
+  }
+  template <typename T, int DP>
+  __device__ __forceinline__ void slow(int second, const T* Q, const T* K, const T* V, const T* dO, const float* lse, const float* delta,
+                                       T* out, float* partial, int rows_per_tile, int group, int lane, const PackedDims& dm) const {
+    const T* k = K + krow * dm.ldk + kvh * dm.hk;
+    const T* v = V + krow * dm.ldv + kvh * dm.hv;
+    const T* q = Q + (long)w.q_start * dm.ldq + kvh * dm.by.G * dm.hq;
+    const T* g = dO + (long)w.q_start * dm.ldo + kvh * dm.by.G * dm.ho;
+    const int lo = t0 * rows_per_tile, hi = min(rows, t1 * rows_per_tile);
+    const float c = dm.scale * LOG2E, f = second ? 1.0f : dm.scale;
+    if (w.slot < 0) slow_key<T, DP>(second, k, v, q, g, lse + lrow, delta + lrow, lo, hi, first, c, f, row_of(out, dm), live, dm.D, dm.by, dm.ldq, dm.hq, dm.ldo, dm.ho);
+    else slow_key<T, DP>(second, k, v, q, g, lse + lrow, delta + lrow, lo, hi, first, c, f, slot_of(partial, second, group, lane, dm), live, dm.D, dm.by, dm.ldq, dm.hq, dm.ldo, dm.ho);
   }
 };
 
@@ -412,6 +525,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     if (r0 + S::KT <= kw.w_lo) continue;                              // none of these rows sees this wave's keys
     sums.step(qt, qt + LT::BYTES, sl, c, kw.ragged || r0 < kw.w_hi, kw.first - r0, lane);
   }
+  if (sums.tainted) {
+    kw.slow<T, DP>(0, Q, K, V, dO, lse, delta, dK, partial, S::KT, wave, lane, dm);
+    kw.slow<T, DP>(1, Q, K, V, dO, lse, delta, dV, partial, S::KT, wave, lane, dm);
+    return;
+  }
   kw.store<T, S::DB>(dK, partial, 0, sums.dk, dm.scale, wave, lane, dm);
   kw.store<T, S::DB>(dV, partial, 1, sums.dv, 1.0f, wave, lane, dm);
 }
@@ -432,12 +550,14 @@ struct PairSums {
   static constexpr float RAISE = 14.0f, LOWER = 1.0f / 16384.0f;
   v8 k[S::KS];                                     // K of the first four, V of the others
   fx16 sum[S::DB];
+  bool tainted;                                    // a tile with rows that do not see some key held an infinity or a NaN
 
   __device__ __forceinline__ void begin(const T* p, int D, bool live, int half) {
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) k[s] = row8(p, 16 * s + 8 * half, D, live);
 #pragma unroll
     for (int d = 0; d < S::DB; ++d) sum[d] = zero16();
+    tainted = false;
   }
   template <typename B>
   __device__ __forceinline__ void rows_by_keys(const char* tile, int b, fx16& to, int lane, B beside) const {
@@ -483,6 +603,7 @@ struct PairSums {
   // a tile of rows: P to `share` ([block][unit][lane] of 16 bytes), dV^T += dO^T P
   __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, fx4* share, float c, bool edge, int first, int lane) {
     fx16 p, next;
+    if (edge) tainted = tainted || not_finite<T>(gt, LT::BYTES, lane);
     rows_by_keys(qt, 0, p, lane, [](int) {});
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
@@ -505,6 +626,7 @@ struct PairSums {
   // the same rows, P taken from `share`: dK^T += Q^T dS
   __device__ __forceinline__ void slopes(const char* qt, const char* gt, const float* D, const fx4* share, bool edge, int first, int lane) {
     fx16 ds, next;
+    if (edge) tainted = tainted || not_finite<T>(qt, LT::BYTES, lane);
     rows_by_keys(gt, 0, ds, lane, [](int) {});
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
@@ -586,13 +708,14 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
       else sums.slopes(qt, qt + LT::BYTES, st + ROWS, share, edge, kw.first - r0, lane);
     }
   };
-  if (wave < 4) {
-    turns(std::true_type{});
-    kw.store<T, DB>(dV, partial, 1, sums.sum, P::LOWER, group, lane, dm);
-  } else {
-    turns(std::false_type{});
-    kw.store<T, DB>(dK, partial, 0, sums.sum, dm.scale, group, lane, dm);
+  if (wave < 4) turns(std::true_type{});
+  else turns(std::false_type{});
+  if (sums.tainted) {
+    kw.slow<T, DP>(wave < 4, Q, K, V, dO, lse, delta, wave < 4 ? dV : dK, partial, ROWS, group, lane, dm);
+    return;
   }
+  if (wave < 4) kw.store<T, DB>(dV, partial, 1, sums.sum, P::LOWER, group, lane, dm);
+  else kw.store<T, DB>(dK, partial, 0, sums.sum, dm.scale, group, lane, dm);
 }
 
 // one cut tile (its entry's row_lo: the number of its slots) and kv head: blockIdx.y / 4 0 dK, 1 dV, and 32 of its keys

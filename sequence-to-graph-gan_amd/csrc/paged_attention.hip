@@ -63,6 +63,18 @@ __device__ __forceinline__ void page_offsets(int* off, int wave, int lane, const
   }
 }
 
+// keys lo .. hi of a wave's rows, key by key (Rows::repair)
+template <typename R, typename T>
+__device__ __forceinline__ void repair_tile(R& r, const int* table, int lo, int hi, int last, const T* keys, const T* values, int half,
+                                            const PagedDims& dm) {
+  for (int key = lo; key < hi; ++key) {
+    const int page = uniform(table[key >> dm.page_shift]);
+    if (!in_pool(page, dm)) continue;
+    const long at = page * dm.page_ld + (key & ((1 << dm.page_shift) - 1)) * dm.ld;
+    r.repair(keys + at, values + at, key <= last, dm.D, half);
+  }
+}
+
 // The part that the i-th workgroup of a sequence takes: turned by one from sequence to sequence.  Workgroups are dealt to
 // the XCDs and their engines in turn, so the parts that short sequences lack would otherwise all fall to the same ones
 // (64 sequences of 300 to 8200 tokens in 8 parts: 300 us, turned 250).
@@ -140,6 +152,11 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
       next = page_of(table, k0 + 64 * NW + (lane & 31), hi, dm);
     }
     r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
+  }
+  if (r.tainted) {
+    r.clear();
+    for (k0 = lo + 32 * wave; k0 < hi; k0 += 32 * NW)
+      repair_tile(r, table, k0, min(k0 + 32, hi), last, kb, vb, half, dm);
   }
   // ---- the waves' results joined: maxima and sums through LDS, then the scaled O
   float* ml = reinterpret_cast<float*>(lds);                   // [NW][32] (m, l)
@@ -242,6 +259,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
     if (k0 > w_hi) continue;
     const bool edge = k0 + S::KT - 1 > min(w_lo, hi - 1);
     r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, absent, lane);
+  }
+  if (r.tainted) {
+    r.clear();
+    repair_tile(r, table, lo, hi, last, kb, vb, half, dm);
   }
   const float l = both_sum(r.l);
   if (alone) {

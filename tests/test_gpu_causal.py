@@ -112,6 +112,68 @@ def test_packed_attention_views_and_rows_behind(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (4, 1, 64), (8, 2, 128), (3, 1, 96)], ids=str)
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_packed_attention_hidden_values(dtype, shape, what):
+    """An infinity or NaN in K and V of token 150 reaches no row before it; one in Q and dO of rows before 70 reaches the
+    gradient of no key that they do not see.  The neighbours in the tile are the plain result."""
+    import transformer as M
+    H, Hk, D = shape
+    g, n = gen(17), [20, 237, 33]
+    pack = M.PackedSequences(n, DEV)
+    q, k, v, do = (rand(g, sum(n), h, D, dtype=dtype) for h in (H, Hk, Hk, H))
+    at, last = 20 + 150, 20 + 150
+    kb, vb = k.clone(), v.clone()
+    vb[at, :, 3] = what
+    for keys in (kb, kb.clone()):
+        if keys is not kb:
+            keys[at + 1] = what                    # and in K of the next
+        leaves = [x.detach().requires_grad_() for x in (q, keys, vb)]
+        out = M.packed_attention(*leaves, pack)
+        dq = torch.autograd.grad(out, leaves[0], do)[0]
+        want = ref.packed(q[20:last], k[20:last], v[20:last], [150], [150], True, 1 / math.sqrt(D), do[20:last])
+        ref.within(out[20:last].detach(), want[0], "out before")
+        ref.within(dq[20:last], want[1], "dq before")
+        assert not torch.isfinite(out[at, :, 3]).any()
+        for part in (slice(0, 20), slice(257, 290)):
+            m = part.stop - part.start
+            want = ref.packed(q[part], k[part], v[part], [m], [m], True, 1 / math.sqrt(D), do[part])
+            ref.within(out[part].detach(), want[0], "other sequences")
+            ref.within(dq[part], want[1], "other sequences")
+    for dirty in ("q", "do"):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        d = do.clone()
+        if dirty == "q":
+            with torch.no_grad():
+                leaves[0][20 + 60:20 + 70] = what
+        else:
+            d[20 + 60:20 + 70] = what
+        dk, dv = torch.autograd.grad(M.packed_attention(*leaves, pack), leaves[1:], d)
+        want = ref.packed(q[20:257], k[20:257], v[20:257], [237], [237], True, 1 / math.sqrt(D), do[20:257])
+        for got, w, which in ((dk, want[2], "dk"), (dv, want[3], "dv")):
+            ref.within(got[20 + 70:257], [x[70:] for x in w], f"{dirty} {which} behind")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (4, 1, 64), (8, 2, 128)], ids=str)
+def test_paged_attention_hidden_values(dtype, shape):
+    """The same for new tokens over a cache: a NaN in V of a later one of the chunk reaches no earlier one."""
+    import transformer as M
+    H, Hk, D = shape
+    g, page = gen(18), 16
+    for n, c in ((4, 700), (90, 333), (200, 200)):
+        keys, values, table = cache_of(g, [c, 40], page, Hk, D, dtype)
+        q = rand(g, n + 1, H, D, dtype=dtype)
+        bad = values.clone()
+        at = c - 2
+        bad[table[0, at // page].long(), at % page, :, 1] = math.nan
+        got = M.paged_attention(q, keys, bad, M.PagedBatch(table, [c, 40], [n, 1]))
+        check_paged(q[:n - 2], keys, values, table[:1], [c - 2], [n - 2], True, 1 / math.sqrt(D), got[:n - 2])
+        check_paged(q[n:], keys, values, table[1:], [40], [1], True, 1 / math.sqrt(D), got[n:])
+        assert torch.isnan(got[n - 2:n, :, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 def test_packed_attention_of_one_key(dtype, shape):
     """A row that sees a single key returns its value, and its scores have no gradient: zeros, not small numbers."""
