@@ -150,7 +150,7 @@ struct S2GLstm64Stack {    // mirrors include/s2g.h
 
 // SPLIT (two layers only): a third group of 256 threads takes layer 1's input product W_ih1 x_t + b off the cell
 // group's hands one tick ahead (through LDS), and the cell group runs two ticks behind layer 0: three waves per SIMD
-// with 32 packed FMAs each per tick instead of two with 32 and 64.
+// with 32 pairs of FMAs each per tick instead of two with 32 and 64.
 template <int NL, bool TOK, bool SPLIT>
 __global__ __launch_bounds__(X_G * (NL + (SPLIT ? 1 : 0))) void s2g_k_lstm64_stack_fwd(S2GLstm64Stack a,
                                                                                        const int* __restrict__ lengths,
@@ -451,7 +451,7 @@ __device__ __forceinline__ void x_slice_fma_t(const f2 (&w01)[16], const f2 (&w2
 
 // Three groups of 256 threads: the top layer; a producer that turns the top layer's gate gradients of the previous
 // tick into W_ih1^T delta1_t (64 values through LDS); the lower layer's cell group two ticks behind the top layer
-// (three waves per SIMD with 32 packed FMAs each per tick instead of two with 32 and 64).
+// (three waves per SIMD with 32 pairs of FMAs each per tick instead of two with 32 and 64).
 extern "C" __global__ __launch_bounds__(3 * X_G) void s2g_k_lstm64_stack_bwd(S2GLstm64StackBwd a,
                                                                              const int* __restrict__ lengths, int T) {
   __shared__ __attribute__((aligned(16))) float ds[2][2][X_G];     // [group][buffer][gate row]

@@ -11,11 +11,11 @@
 //   waves 4..7 t = len-i     dy  = mask * (W_ih1^T delta1_t)                      -> LDS
 //   waves 2,3  t = len+1-i   dh0 = dy + W_hh0^T delta0_{t+1}                      -> cell backward -> delta0_t
 // Cell waves: lane = (unit group g of 4 units, slice s of 8): it accumulates the 4 outputs
-// k = 4g + ((s&3) ^ q), q = 0..3, over gate rows 25s..25s+24 (100 weights in registers, packed
-// pairs -> 50 v_pk_fma_f32 per step; the delta slice comes from LDS in 7 16-byte reads).  A quad
+// k = 4g + ((s&3) ^ q), q = 0..3, over gate rows 25s..25s+24 (100 weights in registers, in
+// pairs -> 100 v_fma_f32 per step; the delta slice comes from LDS in 7 16-byte reads).  A quad
 // reduce-scatter (3 DPP adds, no selects thanks to the per-lane slot order) and one row shift
 // leave the total of unit 4g+s in lanes s < 4, which run the cell backward of that unit.
-// Projection waves: lane = (unit pair p, slice s of 8), 2 outputs x 25 rows -> 25 v_pk_fma_f32
+// Projection waves: lane = (unit pair p, slice s of 8), 2 outputs x 25 rows -> 50 v_fma_f32
 // and 3 DPP adds.  Every weight gradient is a batched GEMM over the saved delta afterwards.
 // Saved activations are prefetched by UNCONDITIONAL loads from clamped addresses (lstm_fwd.hip).
 #include "s2g_common.h"
@@ -418,7 +418,7 @@ extern "C" __global__ __launch_bounds__(BWD_THREADS) void s2g_k_lstm2_bwd2(
             if (!top) hb += dybuf[(t & 1) * 64 + uc];
             const float cprev = (t > 0) ? rc[(j + 1) % PFD].x : 0.0f;   // slot of the next iteration = step t-1
             const float cdprev = (t > 0) ? rcd[(j + 1) % PFD] : 0.0f;
-            // Second-order cell backward, two gates per packed instruction.  With s = gate derivative
+            // Second-order cell backward, two gates at a time.  With s = gate derivative
             // factors, X' = gate tangents, (Hd, Cd) = adjoints of the tangent states:
             //   tcb = Hd (od - 2 go tc cd) + hb go                  (adjoint of tanh c)
             //   cbt = cb + tcb (1 - tc^2)

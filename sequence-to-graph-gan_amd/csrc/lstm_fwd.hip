@@ -13,10 +13,10 @@
 //   waves 2,3  t = tau-2    a1 = p1 + W_hh1 h1_{t-1}        -> gates, c1, h1_t
 // (wave i sits on SIMD i%4: every SIMD gets one cell wave and one projection wave).
 // Cell waves: lane = (unit u, half s); it holds the 4 gate rows of u over columns 25s..25s+24 in
-// 100 registers, as packed pairs -> 50 v_pk_fma_f32 per step, the state slice coming from LDS in
+// 100 registers, as pairs -> 100 v_fma_f32 per step, the state slice coming from LDS in
 // 7 16-byte reads.  A 2-lane reduce-scatter (2 DPP adds) leaves gates (i,f) in lane s=0 and
 // (g,o) in lane s=1; each lane activates and stores its pair, lane 1 fetches (i,f) by DPP and
-// advances the cell.  Projection waves: lane = (unit, quarter s) with 13 columns, 26 v_pk_fma_f32
+// advances the cell.  Projection waves: lane = (unit, quarter s) with 13 columns, 52 v_fma_f32
 // and a 4-lane reduce-scatter (3 DPP adds) that leaves gate s in lane s.
 // Per-step inputs are prefetched PF steps ahead into a register ring by UNCONDITIONAL loads from
 // clamped addresses (a load under a branch makes the compiler drain vmcnt to 0 at the join: one
