@@ -390,8 +390,8 @@ int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const 
  * the strides below (page_size a power of two, 16 .. 65536); table [sequences, table_cols] int32: the page of tokens
  * c page_size .. of a sequence; lengths [sequences] int32: tokens in the cache, the new ones among them; starts
  * [sequences + 1] int32: rows of Q.  Query i of n new tokens sees keys j <= length - n + i (causal) or all.  lengths,
- * table and starts are read on the device (a captured graph may update them): a length is cut to what the table and
- * parts * part_keys cover, a page number outside [0, pages) is a page whose keys are absent.  max_new, max_length: upper
+ * table and starts are read on the device (a captured graph may update them): keys beyond what the table and
+ * parts * part_keys cover are absent, and so are those of a page number outside [0, pages).  max_new, max_length: upper
  * bounds known to the host.  Keys are cut into `parts` of part_keys (a multiple of 128); by_rows: 128 rows per workgroup
  * (chunks) instead of 32 (single tokens).  work: s2g_paged_attention_workspace(dims) floats. */
 typedef struct S2GPaged {

@@ -42,10 +42,11 @@ extern "C" int s2g_launch_rotary(int, const void*, const void*, const void*, con
 
 static inline int elem_size(int type) { return type == 0 ? 4 : 2; }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// heads of D elements, 16-byte units throughout, a tile's offsets within 31 bits
-static bool wide_rows(long ld, long hd, int D, int es) {
+// heads of D elements, 16-byte units throughout, the offsets of a tile of rows (of G heads side by side) within 31 bits
+static bool wide_rows(long ld, long hd, int D, int es, int G = 1) {
   const int u = 16 / es;
-  return ld >= 0 && hd >= 0 && ld % u == 0 && hd % u == 0 && D % u == 0 && ld < (1L << 22) && hd < (1L << 22);
+  return ld >= 0 && hd >= 0 && ld % u == 0 && hd % u == 0 && D % u == 0 && ld < (1L << 22) && hd < (1L << 22) &&
+         (64 * ld + G * hd) * es < 0x7ffffe00L;
 }
 
 static int packed_dims(const S2GPacked* a, PackedDims* d) {
@@ -53,8 +54,8 @@ static int packed_dims(const S2GPacked* a, PackedDims* d) {
   if (a->dim <= 0 || a->dim > 128 || a->dim % 8 || !(a->scale > 0.0f) || !(a->scale < INFINITY)) return -1;
   if (a->q_rows < 0 || a->k_rows < 0 || a->q_rows * a->heads >= (1L << 30) || a->k_rows >= (1L << 30)) return -1;
   const int es = elem_size(a->type), G = a->heads / a->kv_heads;
-  if (G > 128 || !wide_rows(a->q_ld, a->q_hd, a->dim, es) || !wide_rows(a->k_ld, a->k_hd, a->dim, es) ||
-      !wide_rows(a->v_ld, a->v_hd, a->dim, es) || !wide_rows(a->do_ld, a->do_hd, a->dim, es))
+  if (G > 128 || !wide_rows(a->q_ld, a->q_hd, a->dim, es, G) || !wide_rows(a->k_ld, a->k_hd, a->dim, es) ||
+      !wide_rows(a->v_ld, a->v_hd, a->dim, es) || !wide_rows(a->do_ld, a->do_hd, a->dim, es, G))
     return -1;
   *d = PackedDims{a->heads, a->kv_heads, a->dim, a->causal != 0, div_by(G), a->q_ld, a->q_hd, a->k_ld, a->k_hd, a->v_ld, a->v_hd,
                   a->do_ld, a->do_hd, a->q_rows, a->k_rows, a->scale};

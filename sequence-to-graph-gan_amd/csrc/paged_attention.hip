@@ -11,19 +11,22 @@
 // s2g_k_paged_join_few / _many add them in order.  A sequence with a single part is written at once.
 //
 // Lengths and pages come from device memory (a captured decoding loop updates them there), so nothing read from it is
-// trusted: lengths are cut to what the table covers, a page number outside the pool is a page that is not there.
+// trusted: keys beyond what the table covers are not there, a page number outside the pool is a page that is not there.
 #include "attn_rows.h"
 #include "paged_attention.h"
 
 struct PagedSeq {
   int n, len, start, rows;
+  int first;                         // position of the first query: it sees keys up to itself
 };
 __device__ __forceinline__ PagedSeq paged_seq(const int* lens, const int* starts, int s, const PagedDims& dm) {
   PagedSeq q;
   const int a = min(max(uniform(starts[s]), 0), (int)dm.q_rows), b = min(max(uniform(starts[s + 1]), a), (int)dm.q_rows);
   q.start = a;
   q.n = b - a;
-  q.len = (int)min((long)max(uniform(lens[s]), 0), (long)dm.cols << dm.page_shift);
+  const int len = min(max(uniform(lens[s]), 0), 1 << 30);
+  q.first = len - q.n;
+  q.len = (int)min((long)len, (long)dm.cols << dm.page_shift);
   q.len = min(q.len, dm.part_keys * dm.parts);
   q.rows = min(q.n * dm.by.G, dm.max_rows);
   return q;
@@ -31,7 +34,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const int* lens, const int* starts
 // keys that the rows [row0, row0 + count) of a sequence see, at most
 __device__ __forceinline__ int keys_seen(const PagedSeq& q, int row, const PagedDims& dm) {
   if (!dm.causal) return q.len;
-  return max(0, min(q.len, divide(min(row, q.rows - 1), dm.by) + q.len - q.n + 1));
+  return max(0, min(q.len, divide(min(row, q.rows - 1), dm.by) + q.first + 1));
 }
 
 // What the table says of key `key`'s page.  The load is unconditional (of a key that exists, or the first) and is looked
@@ -121,7 +124,7 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
   const int row = tile * 32 + (lane & 31), rr = min(row, sq.rows - 1);
   const bool live = row < sq.rows;
   const int tok = divide(rr, dm.by), head = kvh * dm.by.G + rr - tok * dm.by.G;
-  const int last = live ? (dm.causal ? sq.len - sq.n + tok : sq.len - 1) : -1;
+  const int last = live ? (dm.causal ? min(sq.first + tok, sq.len - 1) : sq.len - 1) : -1;
   const int w_lo = keys_seen(sq, tile * 32, dm) - 1;           // every row sees the keys up to here
   table += (long)s * dm.cols;
   const T* kb = keys + kvh * dm.hd;
@@ -227,7 +230,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
   const int w_row = tile * 128 + 32 * wave, row = w_row + (lane & 31), rr = min(row, sq.rows - 1);
   const bool live = row < sq.rows;
   const int tok = divide(rr, dm.by), head = kvh * dm.by.G + rr - tok * dm.by.G;
-  const int last = live ? (dm.causal ? sq.len - sq.n + tok : sq.len - 1) : -1;
+  const int last = live ? (dm.causal ? min(sq.first + tok, sq.len - 1) : sq.len - 1) : -1;
   const int w_lo = keys_seen(sq, w_row, dm) - 1, w_hi = w_row < sq.rows ? keys_seen(sq, w_row + 31, dm) - 1 : -1;
   table += (long)s * dm.cols;
   const T* kb = keys + kvh * dm.hd;

@@ -67,10 +67,11 @@ __global__ __launch_bounds__(256) void s2g_k_rotary(const T* __restrict__ q, con
     const int s = blockIdx.y, a = min(max(starts[s], 0), (int)dm.rows), b = min(max(starts[s + 1], a), (int)dm.rows);
     const int n = min(b - a, dm.max_new), t = blockIdx.x * dm.tokens;
     if (t >= n) return;
-    len = (int)min((long)max(lens[s], 0), (long)dm.cols << dm.page_shift);
+    const int all = min(max(lens[s], 0), 1 << 30);
+    len = (int)min((long)all, (long)dm.cols << dm.page_shift);            // positions from there on have no page
     count = min(dm.tokens, n - t);
     row0 = a + t;
-    pos0 = len - (b - a) + t;
+    pos0 = all - (b - a) + t;
     table += (long)s * dm.cols;
   } else {
     const long first = (long)blockIdx.x * dm.tokens;

@@ -48,11 +48,13 @@ def _strides(x: torch.Tensor) -> Tuple[int, int]:
     return (x.stride(0) if x.shape[0] > 1 else x.shape[1] * h), h
 
 
-def _fetchable(x: torch.Tensor) -> bool:
-    """Rows that the kernels can fetch in 16-byte units, as far as their strides go."""
+def _fetchable(x: torch.Tensor, group: int = 1) -> bool:
+    """Rows that the kernels can fetch in 16-byte units, 64 of them (of `group` heads each, side by side) within 31 bits of
+    each other, as far as their strides go."""
     unit = 16 // x.element_size()
     t, h = _strides(x)
-    return x.stride(2) == 1 and t % unit == 0 and h % unit == 0 and max(t, h) < 1 << 22
+    return (x.stride(2) == 1 and t % unit == 0 and h % unit == 0 and max(t, h) < 1 << 22
+            and (64 * t + group * h) * x.element_size() < 0x7ffffe00)
 
 
 def _once(backward):
@@ -221,6 +223,67 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
 
 # ----------------------------------------------------------------------------------------------------- packed sequences
+class _WorkLists:
+    """The kernels' work lists for a batch of sequences, made when they are first used."""
+
+    def __init__(self, q_len: np.ndarray, k_len: np.ndarray, device):
+        self.q_len, self.k_len, self.device = q_len, k_len, device
+        self.q_start, self.k_start = np.cumsum(q_len) - q_len, np.cumsum(k_len) - k_len
+        self.kept: dict = {}
+
+    def _tiles(self, count: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
+        """(sequence, which) of every tile of `count` rows or keys a sequence."""
+        n = -(-count // TILE)
+        return np.repeat(np.arange(n.size), n), np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
+
+    def _list(self, seq, tile, row_lo, row_hi, slot) -> torch.Tensor:
+        entry = np.empty((seq.size, 8), dtype=np.int32)
+        for i, column in enumerate((self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile, row_lo, row_hi, slot)):
+            entry[:, i] = column
+        return _on_device(entry, self.device)
+
+    def query_tiles(self, group: int, causal: bool) -> torch.Tensor:
+        """Work list of the query side for `group` query heads to a kv head: the longest first, so that what remains at the
+        end of the launch is short."""
+        got = self.kept.get((group, causal))
+        if got is None:
+            count = self.q_len * group
+            seq, tile = self._tiles(count)
+            work = self.k_len[seq]
+            if causal:
+                last = (np.minimum((tile + 1) * TILE, count[seq]) - 1) // group
+                work = np.minimum(work, last + 1 + (self.k_len - self.q_len)[seq])
+            order = np.argsort(-work, kind="stable")
+            got = self.kept[group, causal] = self._list(seq[order], tile[order], 0, 0, -1)
+        return got
+
+    def key_tiles(self, group: int, causal: bool, kv_heads: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
+        """Work list of the key side, the tiles that are cut, and how many slots they need.  A tile is as much work as it has
+        rows; none is left with more than half of what falls to a compute unit, but 512 rows are not worth a slot."""
+        got = self.kept.get((group, causal, kv_heads))
+        if got is None:
+            seq, tile = self._tiles(self.k_len)
+            rows = (self.q_len * group)[seq]
+            first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // TILE * TILE if causal else np.zeros_like(rows)
+            work = np.maximum(0, rows - first)
+            most = max(512, -(-int(work.sum()) * kv_heads // 512 // TILE) * TILE)
+            parts = np.maximum(1, -(-work // most))
+            each = -(-work // parts // TILE) * TILE                      # whole tiles of rows
+            of = np.repeat(np.arange(parts.size), parts)
+            nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
+            lo = np.minimum(first[of] + nth * each[of], rows[of])
+            hi = np.minimum(lo + each[of], rows[of])
+            is_cut = parts[of] > 1
+            slot = np.where(is_cut, np.cumsum(is_cut) - 1, -1)
+            order = np.argsort(lo - hi, kind="stable")
+            cut = np.flatnonzero(parts > 1)
+            start = np.cumsum(parts) - parts
+            got = self.kept[group, causal, kv_heads] = (
+                self._list(seq[of][order], tile[of][order], np.where(is_cut, lo, 0)[order], np.where(is_cut, hi, rows[of])[order], slot[order]),
+                self._list(seq[cut], tile[cut], parts[cut], 0, slot[start[cut]]), int(is_cut.sum()))
+        return got
+
+
 class PackedSequences:
     """The layout of a batch of sequences that lie one after another: `lengths` tokens each (zeros allowed), and
     `key_lengths` keys each where those differ (the newest tokens of longer sequences: query i of n sees the first
@@ -239,65 +302,11 @@ class PackedSequences:
             raise S2GError("PackedSequences: needs a GPU device")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self.q_len, self.k_len = q, k
-        self.q_start, self.k_start = np.cumsum(q) - q, np.cumsum(k) - k
         self.rows, self.key_rows = int(q.sum()), int(k.sum())
         with torch.cuda.device(self.device):
-            self.starts = _on_device(np.append(self.q_start, self.rows), self.device)
-            self.positions = _on_device(np.arange(self.rows) - np.repeat(self.q_start - (k - q), q), self.device)
-        self._lists, self._plans = {}, {}
-
-    def _tiles(self, count: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
-        """(sequence, which) of every tile of `count` rows or keys a sequence."""
-        n = -(-count // TILE)
-        return np.repeat(np.arange(n.size), n), np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
-
-    def _list(self, seq, tile, row_lo, row_hi, slot) -> torch.Tensor:
-        entry = np.empty((seq.size, 8), dtype=np.int32)
-        for i, column in enumerate((self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile, row_lo, row_hi, slot)):
-            entry[:, i] = column
-        return _on_device(entry, self.device)
-
-    def query_tiles(self, group: int, causal: bool) -> torch.Tensor:
-        """Work list of the query side for `group` query heads to a kv head: the longest first, so that what remains at the
-        end of the launch is short."""
-        got = self._lists.get((group, causal))
-        if got is None:
-            count = self.q_len * group
-            seq, tile = self._tiles(count)
-            work = self.k_len[seq]
-            if causal:
-                last = (np.minimum((tile + 1) * TILE, count[seq]) - 1) // group
-                work = np.minimum(work, last + 1 + (self.k_len - self.q_len)[seq])
-            order = np.argsort(-work, kind="stable")
-            got = self._lists[group, causal] = self._list(seq[order], tile[order], 0, 0, -1)
-        return got
-
-    def key_tiles(self, group: int, causal: bool, kv_heads: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
-        """Work list of the key side, the tiles that are cut, and how many slots they need.  A tile is as much work as it has
-        rows; none is left with more than half of what falls to a compute unit, but 512 rows are not worth a slot."""
-        got = self._lists.get((group, causal, kv_heads))
-        if got is None:
-            seq, tile = self._tiles(self.k_len)
-            rows = (self.q_len * group)[seq]
-            first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // TILE * TILE if causal else np.zeros_like(rows)
-            work = np.maximum(0, rows - first)
-            most = max(512, -(-int(work.sum()) * kv_heads // 512 // TILE) * TILE)
-            parts = np.maximum(1, -(-work // most))
-            each = -(-work // parts // TILE) * TILE                      # whole tiles of rows
-            of = np.repeat(np.arange(parts.size), parts)
-            nth = np.arange(of.size) - np.repeat(np.cumsum(parts) - parts, parts)
-            lo = np.minimum(first[of] + nth * each[of], rows[of])
-            hi = np.minimum(lo + each[of], rows[of])
-            is_cut = parts[of] > 1
-            slot = np.where(is_cut, np.cumsum(is_cut) - 1, -1)
-            order = np.argsort(lo - hi, kind="stable")
-            cut = np.flatnonzero(parts > 1)
-            start = np.cumsum(parts) - parts
-            got = self._lists[group, causal, kv_heads] = (
-                self._list(seq[of][order], tile[of][order], np.where(is_cut, lo, 0)[order], np.where(is_cut, hi, rows[of])[order], slot[order]),
-                self._list(seq[cut], tile[cut], parts[cut], 0, slot[start[cut]]), int(is_cut.sum()))
-        return got
+            self.starts = _on_device(np.append(0, np.cumsum(q)), self.device)
+            self.positions = _on_device(np.arange(self.rows) - np.repeat(np.cumsum(q) - k, q), self.device)
+        self._work, self._plans = _WorkLists(q, k, self.device), {}
 
 
 class _PackedPlan:
@@ -313,15 +322,15 @@ class _PackedPlan:
         if q.shape[0] * q.shape[1] >= 1 << 30 or k.shape[0] >= 1 << 30:
             raise S2GError("packed_attention: 2^30 rows or more")
         (R, H, D), (M, Hk, _) = q.shape, k.shape
-        self.copies = [not _fetchable(x) for x in (q, k, v)]
-        self.pack, self.causal, self.group, self.kv_heads = pack, causal, H // Hk, Hk
+        self.copies = [not _fetchable(q, H // Hk), not _fetchable(k), not _fetchable(v)]
+        self.work, self.causal, self.group, self.kv_heads = pack._work, causal, H // Hk, Hk
         self.device, self.rows, self.key_rows = q.get_device(), pack.rows, pack.key_rows
         self.stats = Hk * R * self.group
         self.fields = (TYPES[q.dtype], H, Hk, D, int(causal), _scale("packed_attention", scale, D), *_strides(q), *_strides(k), *_strides(v))
         self.size, self.whole = (R, M), R == pack.rows and M == pack.key_rows
         self.dims = S2GPacked(*self.fields, H * D, D, R, M)
         self.fwd = ctypes.byref(self.dims)
-        self.q_tiles = pack.query_tiles(self.group, causal)
+        self.q_tiles = self.work.query_tiles(self.group, causal)
         self.q_list = (ptr(self.q_tiles), self.q_tiles.shape[0])
         self.bwd: dict = {}
 
@@ -331,7 +340,7 @@ class _PackedPlan:
         got = self.bwd.get(key)
         if got is None:
             dims = S2GPacked(*self.fields, *_strides(do), *self.size)
-            k_tiles, cut, slots = self.pack.key_tiles(self.group, self.causal, self.kv_heads)
+            k_tiles, cut, slots = self.work.key_tiles(self.group, self.causal, self.kv_heads)
             got = self.bwd[key] = (ctypes.byref(dims), (ptr(k_tiles), k_tiles.shape[0], ptr(cut), cut.shape[0]),
                                    get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots))
         return got
@@ -359,7 +368,7 @@ class PackedAttentionFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, out, rest, lse = ctx.saved_tensors
         plan = ctx.plan
-        if do.data_ptr() & 15 or not _fetchable(do):
+        if do.data_ptr() & 15 or not _fetchable(do, plan.group):
             do = _copy(do)
         dims, lists, floats = plan.backward(do)
         dq, dk, dv = _new(q), _new(k), _new(v)
@@ -575,8 +584,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, b
                     scale: Optional[float] = None) -> torch.Tensor:
     """Attention of a batch's new tokens (q [tokens, heads, dim]) over what its sequences hold in the cache: query i of n
     new tokens of a sequence of m sees keys j <= m - n + i (causal) or all m.  One token or thousands per sequence, mixed
-    at will; types, heads and scale as in packed_attention.  A page number outside the pool is a page whose keys are not
-    there; a query without keys gives zeros, and so do rows of q behind the batch's."""
+    at will; types, heads and scale as in packed_attention.  A page number outside the pool, or a position that the table does
+    not cover, is a key that is not there; a query without keys gives zeros, and so do rows of q behind the batch's."""
     _no_grad("paged_attention", q, keys, values)
     plan = _plan_of(batch, "paged_attention", (causal, scale), _PagedPlan, q, keys, values)
     if plan.copy or q.data_ptr() & 15:

@@ -73,6 +73,9 @@ def test_c_entry_points_refuse():
         assert l.s2g_packed_attention_fwd(p, p, p, p, None, None, p, 1, packed(**change), None) == -1, change
         assert l.s2g_packed_attention_bwd(p, p, p, p, p, p, p, p, p, p, p, None, p, 1, p, 1, None, 0, packed(**change), None) == -1, change
         assert l.s2g_packed_attention_bwd_workspace(packed(**change), 2) == -1, change
+    wide = dict(heads=256, kv_heads=2, type=0)              # 128 heads of a group, too far apart for 31 bits
+    assert l.s2g_packed_attention_fwd(p, p, p, p, None, None, p, 1, packed(**wide, q_hd=(1 << 22) - 4, q_ld=64), None) == -1
+    assert l.s2g_packed_attention_bwd_workspace(packed(**wide, do_hd=(1 << 22) - 4, do_ld=64), 1) == -1
     for i in (0, 1, 2, 3, 6):
         args = [p, p, p, p, None, None, p]
         args[i] = None
@@ -188,10 +191,7 @@ def test_key_tiles_cover_every_row_once():
     old, causal._on_device = causal._on_device, lambda values, device: torch.from_numpy(np.array(values, dtype=np.int32))
     try:
         for q, k in (([5000, 1, 130], None), ([3], [900]), ([700, 0, 40], [100, 300, 2048]), ([1] * 200, None)):
-            pack = object.__new__(causal.PackedSequences)
-            pack.q_len, pack.k_len = np.array(q), np.array(k or q)
-            pack.q_start, pack.k_start = np.cumsum(pack.q_len) - pack.q_len, np.cumsum(pack.k_len) - pack.k_len
-            pack.device, pack._lists = "cpu", {}
+            pack = causal._WorkLists(np.array(q), np.array(k or q), "cpu")
             for group, heads, is_causal in ((1, 1, True), (8, 2, True), (3, 1, False)):
                 tiles, cut, slots = pack.key_tiles(group, is_causal, heads)
                 spans, used = {}, []

@@ -98,6 +98,12 @@ def test_packed_attention_views_and_rows_behind(dtype):
         for name_, got, w in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), ref.packed(*live, n, n, True, 1 / math.sqrt(D), do[:sum(n)])):
             ref.within(got[:sum(n)], w, f"{what} {name_}")
             assert (got[sum(n):] == 0).all(), f"{what} {name_} behind the last sequence"
+    # heads so far apart that 64 rows of a group pass 31 bits: copied
+    far = torch.empty(12, 1 << 22, dtype=dtype, device=DEV)[:, :rows * 8].view(12, rows, 8).transpose(0, 1)
+    q, k = rand(g, rows, 12, 8, dtype=dtype), rand(g, rows, 1, 8, dtype=dtype)
+    far.copy_(q)
+    a, b = (M.packed_attention(x, k, k, pack) for x in (far, q))
+    assert torch.equal(a[:sum(n)], b[:sum(n)])
     # one key head broadcast to two: the gradient of the shared one is the sum
     one = rand(g, rows, 1, D, dtype=dtype)
     q = views["projection"][0].detach()
@@ -219,6 +225,32 @@ def test_packed_attention_gradient_against_differences(dtype):
     assert abs(along - difference) <= slack + 1e-6 * size, (along, difference, slack)
 
 
+def test_layouts_are_freed_with_their_batch():
+    """A batch's layout, plans and device lists go when it goes, without the cycle collector; a graph of it that still
+    waits for its backward pass keeps what it needs."""
+    import gc
+    import weakref
+    import transformer as M
+    g = gen(14)
+    gc.collect()
+    gc.disable()
+    try:
+        q = rand(g, 50, 2, 32).requires_grad_()
+        pack = M.PackedSequences([20, 30], DEV)
+        out = M.packed_attention(q, q, q, pack)
+        gone = weakref.ref(pack)
+        del pack
+        assert gone() is None
+        out.sum().backward()
+        assert torch.isfinite(q.grad).all()
+        first = M.packed_attention(q, q, q, M.PackedSequences([50], DEV))
+        (one,) = torch.autograd.grad(first.sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError):
+            one.sum().backward()                   # once differentiable
+    finally:
+        gc.enable()
+
+
 def test_packed_attention_captured():
     """Forward and backward in a graph, replayed with new inputs between eager work, on a stream of their own."""
     import transformer as M
@@ -331,6 +363,39 @@ def test_paged_attention_absent_pages(dtype):
                     (w,) = ref.head(q[r + t:r + t + 1, h], k[seen][:, h // 2], v[seen][:, h // 2], 0, False, 1 / math.sqrt(D), dtype)
                     ref.within(got[r + t:r + t + 1, h], w, f"sequence {i} token {t} head {h}")
             r += n
+
+
+def test_paged_lengths_on_the_device():
+    """Lengths rewritten on the device: beyond the table's pages there are no keys and nothing is written, below the number
+    of new tokens the first of them see nothing, negative ones are empty."""
+    import transformer as M
+    g, (H, Hk, D), page, dtype = gen(15), (4, 2, 64), 16, torch.bfloat16
+    for n in (3, 100):
+        context = [120, 120, 120]
+        keys, values, table = cache_of(g, context, page, Hk, D, dtype)           # 8 pages: 128 tokens each
+        batch = M.PagedBatch(table, context, [n] * 3, max_length=128)
+        batch.lengths.copy_(torch.tensor([128 + 2, 2, -7], dtype=torch.int32))
+        q, k, v = (rand(g, 3 * n, h, D, dtype=dtype) for h in (H, Hk, Hk))
+        got = M.paged_attention(q, keys, values, batch)
+        ka, va = rows_of(keys, table[0], 128), rows_of(values, table[0], 128)
+        for h in range(H):
+            (w,) = ref.head(q[:n, h], ka[:, h // 2], va[:, h // 2], 130 - n, True, 1 / math.sqrt(D), dtype)
+            ref.within(got[:n, h], w, "beyond the table")
+            (w,) = ref.head(q[2 * n - 2:2 * n, h], rows_of(keys, table[1], 2)[:, h // 2], rows_of(values, table[1], 2)[:, h // 2], 0, True,
+                            1 / math.sqrt(D), dtype)
+            ref.within(got[2 * n - 2:2 * n, h], w, "short")
+        assert (got[n:2 * n - 2] == 0).all() and (got[2 * n:] == 0).all()
+        freq, _ = M.rotary_frequencies(D, device=DEV)
+        before = keys.clone()
+        M.append_rotary(q, k, v, keys, values, batch, freq)
+        same = torch.ones(keys.shape[:2], dtype=torch.bool, device=DEV)
+        for row, positions in ((0, range(130 - n, 128)), (1, range(2))):
+            for p in positions:
+                at = (table[row, p // page].long(), p % page)
+                same[at] = False
+                source = p - (130 - n) if row == 0 else n + (n - 2) + p
+                assert torch.equal(values[at], v[source])
+        assert torch.equal(keys[same], before[same])
 
 
 def test_paged_attention_pool_beyond_32_bits():
