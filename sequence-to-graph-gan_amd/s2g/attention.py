@@ -148,10 +148,11 @@ class LinearActFn(torch.autograd.Function):
         if not x.is_cuda:
             raise S2GError("CustomTransformerEncoderLayer needs GPU tensors (MI355X-only implementation, no CPU path)")
         K, N = x.shape[-1], W.shape[0]
-        M = x.numel() // K
+        M = math.prod(x.shape[:-1])
         xc, Wc, bc = x.contiguous().float().view(M, K), W.contiguous().float(), b.contiguous().float()
         y = torch.empty(M, N, device=x.device)
-        ops.linear_fwd(xc, Wc, bc, y, act=act)
+        if M:
+            ops.linear_fwd(xc, Wc, bc, y, act=act)
         ctx.save_for_backward(xc, Wc, y)
         ctx.act, ctx.lead = act, tuple(x.shape[:-1])
         return y.view(*ctx.lead, N)
@@ -163,6 +164,8 @@ class LinearActFn(torch.autograd.Function):
         M, K = xc.shape
         N = Wc.shape[0]
         dy = dy.contiguous().float().view(M, N)
+        if not M:
+            return dy.new_zeros(*ctx.lead, K), torch.zeros_like(Wc), dy.new_zeros(N), None
         if ctx.act == 2:
             dy = dy.clone()
             call("s2g_relu_bwd", ptr(y), ptr(dy), dy.numel(), stream_ptr())

@@ -143,7 +143,7 @@ def test_cpu_tensors_are_refused():
     for bad in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=4, base=0.0), dict(rotary_dim=4, factor=0.0), dict(rotary_dim=4, scaling="other")):
         with pytest.raises(S2GError):
             M.rotary_frequencies(**bad, device="cpu")
-    for bad in ((5, 2, None), (8, 3, 2), (8, 4, 3), (8, 4, 0)):
+    for bad in ((5, 2, None), (8, 3, 2), (8, 4, 3), (8, 4, 0), (24, 2, 1), (272, 2, 2), (64, 2, 2, 34), (2064, 258, 2), (16, 2, 1, 4, False, 1e4, None, 1.0, 64, torch.float64)):
         with pytest.raises(S2GError):
             M.GroupedQueryAttention(*bad)
 
@@ -180,6 +180,28 @@ def test_cache_bookkeeping():
                 causal.PagedKVCache(*bad, device="cpu")
         with pytest.raises(S2GError):
             causal.PagedKVCache(4, 16, 2, 32, dtype=torch.float64, device="cpu")
+    finally:
+        causal.PagedBatch = whole
+
+
+def test_cache_refusals_change_nothing():
+    """A batch that cannot be made leaves the cache as it was; pages a sequence does not own yet are no pages."""
+    from s2g import causal
+    from s2g.lib import S2GError
+
+    def refuse(*args, **kw):
+        raise S2GError("refused")
+    whole, causal.PagedBatch = causal.PagedBatch, refuse
+    try:
+        cache = causal.PagedKVCache(6, 16, 2, 32, device="cpu")
+        a, b = cache.add(), cache.add()
+        with pytest.raises(S2GError):
+            cache.extend([a, b], [17, 3])
+        assert cache.free_pages == 6 and cache.length(a) == 0
+        causal.PagedBatch = lambda table, lengths, new, device=None: table
+        table = cache.extend([a, b], [33, 3])
+        assert (table[1, 1:] == -1).all() and len({*table[0].tolist(), int(table[1, 0])}) == 4 and cache.free_pages == 2
+        assert (cache.extend([a], [0])[0] == table[0]).all() and cache.extend([cache.add()], [0]).tolist() == [[-1]]
     finally:
         causal.PagedBatch = whole
 

@@ -577,6 +577,100 @@ def test_other_stream():
     assert torch.equal(got, want)
 
 
+def test_batch_dropped_while_another_stream_reads_it():
+    """A batch that goes while a launch on a side stream still waits: its lists are not handed to the next ones."""
+    import transformer as M
+    g, n = gen(32), [700, 10, 300]
+    q, k, v = (rand(g, sum(n), h, 64, dtype=torch.bfloat16) for h in (4, 2, 2))
+    want = M.packed_attention(q, k, v, M.PackedSequences(n, DEV))
+    keys, values, table = cache_of(g, [90, 40], 16, 2, 64, torch.bfloat16)
+    one = M.paged_attention(q[:2], keys, values, M.PagedBatch(table, [90, 40], [1, 1]))
+    big = torch.empty(1 << 26, device=DEV)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        pack, batch = M.PackedSequences(n, DEV), M.PagedBatch(table.clone(), [90, 40], [1, 1])
+        lists = pack._work.query_tiles(2, True)
+        held = {t.data_ptr() for t in (lists, batch.lengths, batch.starts, batch.table)}
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                big.zero_()                                    # the launches below wait for these
+            got, two = M.packed_attention(q, k, v, pack), M.paged_attention(q[:2], keys, values, batch)
+        del pack, batch, lists
+        new = [torch.full((m,), 1, dtype=torch.int32, device=DEV) for m in (2, 3, 64, 96, 128) for _ in range(4)]
+        waiting = not side.query()
+        assert not waiting or not held & {t.data_ptr() for t in new}
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(two, one)
+
+
+def test_saved_tensors_laid_out_anew():
+    """Hooks on saved tensors may hand back the same values with other strides."""
+    import transformer as M
+    g, n, T = gen(33), [70, 0, 200], 290
+    for dtype in (torch.bfloat16, torch.float32):
+        qkv = rand(g, T, 8, 64, dtype=dtype).requires_grad_()
+        do = rand(g, T, 4, 64, dtype=dtype)
+        pack = M.PackedSequences(n, DEV)
+
+        def run():
+            return torch.autograd.grad(M.packed_attention(*qkv.split([4, 2, 2], 1), pack), qkv, do)[0]
+        want = run()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.to(DEV)):
+            got = run()
+        assert torch.equal(got, want)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)):
+            got = run()
+        assert torch.equal(got, want)
+
+
+def test_arguments_go_by_value():
+    """A scale held in a tensor is read at every call; what the host has checked cannot be replaced."""
+    import transformer as M
+    from s2g.lib import S2GError
+    g = gen(34)
+    q = rand(g, 20, 2, 32)
+    pack = M.PackedSequences([20], DEV)
+    keys, values, table = cache_of(g, [40], 16, 2, 32, torch.float32)
+    batch = M.PagedBatch(table, [40], [20])
+    scale = torch.tensor(0.5)
+    first = M.packed_attention(q, q, q, pack, scale=scale), M.paged_attention(q, keys, values, batch, scale=scale)
+    scale.fill_(0.125)
+    again = M.packed_attention(q, q, q, pack, scale=scale), M.paged_attention(q, keys, values, batch, scale=scale)
+    want = M.packed_attention(q, q, q, pack, scale=0.125), M.paged_attention(q, keys, values, batch, scale=0.125)
+    for f, a, w in zip(first, again, want):
+        assert torch.equal(a, w) and not torch.equal(f, w)
+    for name in ("table", "rows", "max_length"):
+        with pytest.raises(S2GError):
+            setattr(batch, name, getattr(batch, name))
+    with pytest.raises(S2GError):
+        pack.rows = 10
+
+
+@pytest.mark.parametrize("queries,keys", [([0, 0], [3, 0]), ([5, 0], [0, 0]), ([0], [0])])
+def test_packed_attention_without_queries_or_keys(queries, keys):
+    import transformer as M
+    pack = M.PackedSequences(queries, DEV, keys)
+    for spare in (0, 2):
+        q, k, v = (torch.full((r + spare, h, 32), math.nan, device=DEV, requires_grad=True)
+                   for r, h in ((sum(queries), 4), (sum(keys), 2), (sum(keys), 2)))
+        out = M.packed_attention(q, k, v, pack)
+        out.sum().backward()
+        assert all(bool((x == 0).all()) for x in (out, q.grad, k.grad, v.grad))
+
+
+def test_module_without_tokens():
+    import transformer as M
+    net = M.GroupedQueryAttention(64, 4, 2).to(DEV)
+    x = torch.zeros(0, 64, device=DEV, requires_grad=True)
+    y = net(x, M.PackedSequences([0, 0], DEV))
+    assert y.shape == (0, 64)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and all(bool((p.grad == 0).all()) for p in net.parameters())
+    cache = net.new_cache(2, page_size=16)
+    assert net.step(x.detach(), cache, cache.extend([cache.add()], [0])).shape == (0, 64)
+
+
 def test_refusals_on_gpu_tensors():
     import transformer as M
     from s2g.lib import S2GError
@@ -588,7 +682,7 @@ def test_refusals_on_gpu_tensors():
         with pytest.raises(S2GError):
             M.packed_attention(*bad, pack)
     ok = x(4, 2, 32)
-    for scale in (0.0, -1.0, math.nan, math.inf):
+    for scale in (0.0, -1.0, math.nan, math.inf, 1e31, 1e-31):
         with pytest.raises(S2GError):
             M.packed_attention(ok, ok, ok, pack, scale=scale)
     table = torch.zeros(1, 2, dtype=torch.int32, device=DEV)

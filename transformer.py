@@ -161,24 +161,32 @@ class GroupedQueryAttention(nn.Module):
         self.head_dim = embed_size // num_heads
         if self.head_dim * num_heads != embed_size or self.num_kv_heads <= 0 or num_heads % self.num_kv_heads:
             raise S2GError("GroupedQueryAttention: heads must divide the embedding size, kv heads the heads")
+        if self.head_dim % 8 or self.head_dim > 128 or num_heads // self.num_kv_heads > 128:
+            raise S2GError("GroupedQueryAttention: heads of 8, 16, .. 128 features, at most 128 of them to a kv head")
+        if rotary_dim is not None and rotary_dim > self.head_dim:
+            raise S2GError(f"GroupedQueryAttention: {rotary_dim} rotary features in heads of {self.head_dim}")
+        if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise S2GError(f"GroupedQueryAttention: float32, bfloat16 or float16, got {dtype}")
         self.interleaved, self.dtype = interleaved, dtype
         self.in_proj = nn.Linear(embed_size, (num_heads + 2 * self.num_kv_heads) * self.head_dim)
         self.fc_out = nn.Linear(embed_size, embed_size)
-        self._frequencies, self.multiplier = rotary_frequencies(self.head_dim if rotary_dim is None else rotary_dim, base, scaling,
-                                                                factor, original_length, device="cpu")
+        frequencies, self.multiplier = rotary_frequencies(self.head_dim if rotary_dim is None else rotary_dim, base, scaling,
+                                                          factor, original_length, device="cpu")
+        self._frequencies = {frequencies.device: frequencies}
 
     def _turns(self, device):
-        # float64 whatever the module's parameters are cast to
-        if self._frequencies.device != device:
-            self._frequencies = self._frequencies.to(device)
-        return self._frequencies
+        # float64 whatever the module's parameters are cast to, one copy on every device it has run on
+        got = self._frequencies.get(device)
+        if got is None:
+            got = self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
+        return got
 
     def _project(self, x):
         qkv = LinearActFn.apply(x, self.in_proj.weight, self.in_proj.bias, 0).to(self.dtype)
-        return qkv.view(x.shape[0], -1, self.head_dim).split([self.num_heads, self.num_kv_heads, self.num_kv_heads], 1)
+        return qkv.view(x.shape[0], self.num_heads + 2 * self.num_kv_heads, self.head_dim).split([self.num_heads, self.num_kv_heads, self.num_kv_heads], 1)
 
     def _out(self, y):
-        return LinearActFn.apply(y.reshape(y.shape[0], -1).float(), self.fc_out.weight, self.fc_out.bias, 0)
+        return LinearActFn.apply(y.reshape(y.shape[0], self.num_heads * self.head_dim).float(), self.fc_out.weight, self.fc_out.bias, 0)
 
     def forward(self, x, pack):
         """x [tokens, embed_size], the sequences of `pack` one after another."""
