@@ -98,11 +98,11 @@ __device__ __attribute__((noinline)) void slow_key(int which, const T* k, const 
   }
 }
 
-// Rounding dS to 16 bits adds as much to dQ and dK as rounding those results does (1.44 times the error, all told), and more
-// where a row's few slopes, which add up to zero, nearly cancel (1.5 to 1.9 times, over short sequences).  So for rows that
-// see at most this many keys the products take what rounding left, too: 1.05 to 1.25 times, over long sequences 1.3.  They
-// are the first rows of a long sequence or all of short ones; it costs 3 % of a training step on sequences up to 4096 and
-// 5 us of 80 on 96 of up to 203 tokens (12 heads of 64).
+// Rounding dS and P to 16 bits adds as much to dQ, dK and dV as rounding those results does (1.44 times the error, all
+// told), and more where a row's few slopes, which add up to zero, nearly cancel (1.5 to 1.9 times, over short sequences).
+// So for rows that see at most this many keys the products of the backward pass take what rounding left, too: 1.05 to 1.25
+// times, over long sequences 1.3.  They are the first rows of a long sequence or all of short ones; it costs 3 % of a
+// training step on sequences up to 4096 and 9 us of 80 on 96 of up to 203 tokens (12 heads of 64).
 #define FEW_KEYS 128
 template <typename T>
 __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
@@ -415,10 +415,12 @@ struct KeySums {
         for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
       }
       if (sizeof(T) == 2 && __builtin_expect(few, 0)) {
-        const fx16 z = left_by_rounding<T>(ds);
+        const fx16 y = left_by_rounding<T>(p), z = left_by_rounding<T>(ds);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const v8 zt = operand<T>(z, s);
+          const v8 yt = operand<T>(y, s), zt = operand<T>(z, s);
+#pragma unroll
+          for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), yt, dv[d]);
 #pragma unroll
           for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), zt, dk[d]);
         }
@@ -632,7 +634,7 @@ struct PairSums {
     }
   }
   // a tile of rows: P to `share` ([block][unit][lane] of 16 bytes), dV^T += dO^T P
-  __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, fx4* share, float c, bool edge, int first, int lane) {
+  __device__ __forceinline__ void weights(const char* qt, const char* gt, const float* L, fx4* share, float c, bool few, bool edge, int first, int lane) {
     fx16 p, next;
     if (edge) tainted = tainted || not_finite<T>(gt, LT::BYTES, lane);
     rows_by_keys(qt, 0, p, lane, [](int) {});
@@ -651,6 +653,11 @@ struct PairSums {
       give(share + b * UNITS * 64, p, lane);
       const v8 x[2] = {operand<T>(p, 0), operand<T>(p, 1)};
       add(gt, b, x, lane);
+      if (__builtin_expect(few, 0)) {
+        const fx16 y = left_by_rounding<T>(p);
+        const v8 x[2] = {operand<T>(y, 0), operand<T>(y, 1)};
+        add(gt, b, x, lane);
+      }
       p = next;
     }
   }
@@ -740,7 +747,7 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
       const float* st = stats + place * 2 * ROWS;
       fx4* share = shares + ((mine & 1) * 4 + group) * P::SHARE;
       const bool edge = kw.ragged || r0 < kw.w_hi;
-      if constexpr (first_four.value) sums.weights(qt, qt + LT::BYTES, st, share, c, edge, kw.first - r0, lane);
+      if constexpr (first_four.value) sums.weights(qt, qt + LT::BYTES, st, share, c, r0 < kw.few, edge, kw.first - r0, lane);
       else sums.slopes(qt, qt + LT::BYTES, st + ROWS, share, r0 < kw.few, edge, kw.first - r0, lane);
     }
   };
