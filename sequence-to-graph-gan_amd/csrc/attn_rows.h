@@ -10,6 +10,41 @@ struct Shape {
   static constexpr int KS = DP / 16, DB = (DP + 31) / 32, KB = KT / 32;
   static constexpr int AHEAD = 2;
   typedef Tile<T, PITCH, KT, 4> LT;
+  typedef typename Vec<T>::v8 v8;
+  // Sums over rows (keys) of 16 fp32 features: a 32 x 32 step would fill half of its result for nothing, so the same
+  // operands go through v_mfma_f32_16x16x1_4b, four 16 x 16 products at once: columns 0 .. 15 and 16 .. 31 with the lower
+  // half's contraction slots, and again with the upper half's, which whole() adds at the end.
+  static constexpr bool NARROW = sizeof(T) == 4 && DP == 16;
+  static __device__ __forceinline__ fx16 sum(const v8& a, const v8& b, fx16 c) {
+    if constexpr (NARROW) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x1f32(a[j], b[j], c, 0, 0, 0);
+      return c;
+    } else {
+      return mma(a, b, c);
+    }
+  }
+  // Register i of lane l: column l % 16 of block i / 4, feature 4 (l / 16) + i % 4; made the 32 x 32 result it stands for
+  static __device__ __forceinline__ void whole(fx16* c, int lane) {
+    if constexpr (NARROW) {
+      fx16 r = zero16();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = (lane & 15) + 16 * (2 * (i >> 2) + (lane >> 5)), j = i & 3;
+        const float x = __shfl(c[0][j] + c[0][8 + j], from), y = __shfl(c[0][4 + j] + c[0][12 + j], from);
+        r[i] = lane & 16 ? y : x;
+      }
+      c[0] = r;
+    }
+  }
+  // sums times a factor of every column (lane l: column l % 32)
+  static __device__ __forceinline__ void scaled(fx16* c, float f, int lane) {
+    const float x = NARROW ? __shfl(f, lane & 15) : f, y = NARROW ? __shfl(f, 16 + (lane & 15)) : f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[d][i] *= i & 4 ? y : x;
+  }
 };
 
 // Offsets of this lane's chunks of a tile whose rows lie `ld` elements apart, and the buffer over the tile's rows
@@ -162,10 +197,7 @@ struct Rows {
       const float mn = fmaxf(m, mx), a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       l *= a;
-#pragma unroll
-      for (int d = 0; d < S::DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+      S::scaled(o, a, lane);
     }
     const float base = (m == -INFINITY ? 0.0f : m * c) - Weights<T>::RAISE;
     v8 p[2 * KB];
@@ -189,7 +221,7 @@ struct Rows {
     }
     // O^T += V^T P^T, the weights straight from the registers they are in
     products<T, 2 * KB * S::DB, S::AHEAD>([&](int i) { return LT::across(vt, i % S::DB, i / S::DB, lane); },
-                                [&](int i, const v8& a) { o[i % S::DB] = mma(a, p[i / S::DB], o[i % S::DB]); }, [](int) {});
+                                [&](int i, const v8& a) { o[i % S::DB] = S::sum(a, p[i / S::DB], o[i % S::DB]); }, [](int) {});
   }
   template <int KB>
   __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {

@@ -120,7 +120,7 @@ __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
 // workgroups share a compute unit and one's 2^x stand beside the other's products.  Bound by the matrix units, and at long
 // prompts by power: 8191 + 1025 + 5000 bf16 tokens, 32 query and 8 kv heads of 128, 740 us, 1030 TFLOP/s, the units busy
 // 53 % of the time at 1.63 GHz (one 8192^3 product of the library: 1140 TFLOP/s).  64 fp32 sequences up to 512, 4 heads of
-// 16: 32 us, by the exact fp32 matrix instructions (151 TFLOP/s) and the 2^x, as many as there are products of 16.
+// 16: 27 us (query side of the gradient 36), by the longest sequences' chain of products and 2^x rather than by either's rate.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ out,
@@ -190,6 +190,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     turn(t, std::integral_constant<int, 0>{});
     if (t + 1 < nt) turn(t + 1, std::integral_constant<int, 1>{});
   }
+  S::whole(r.o, lane);
   const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l;
   const long orow = (qrow * dm.H + head) * dm.D;
   // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
@@ -335,12 +336,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
       }
       const v8 ds[2] = {operand<T>(st, 0), operand<T>(st, 1)};
       products<T, 2 * S::DB, S::AHEAD>([&](int i) { return LT::across(kt, i % S::DB, 2 * b + i / S::DB, lane); },
-                                       [&](int i, const v8& a) { dq[i % S::DB] = mma(a, ds[i / S::DB], dq[i % S::DB]); }, [](int) {});
+                                       [&](int i, const v8& a) { dq[i % S::DB] = S::sum(a, ds[i / S::DB], dq[i % S::DB]); }, [](int) {});
       if (sizeof(T) == 2 && __builtin_expect(w_lo < FEW_KEYS, 0)) {
         const fx16 z = left_by_rounding<T>(st);
         const v8 ds[2] = {operand<T>(z, 0), operand<T>(z, 1)};
         products<T, 2 * S::DB, S::AHEAD>([&](int i) { return LT::across(kt, i % S::DB, 2 * b + i / S::DB, lane); },
-                                         [&](int i, const v8& a) { dq[i % S::DB] = mma(a, ds[i / S::DB], dq[i % S::DB]); }, [](int) {});
+                                         [&](int i, const v8& a) { dq[i % S::DB] = S::sum(a, ds[i / S::DB], dq[i % S::DB]); }, [](int) {});
       }
       st = next;
     }
@@ -350,6 +351,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
     return;
   }
+  S::whole(dq, lane);
   store_rows<T, S::DB>(dQ + orow, dq, dm.scale, dm.D, half, live);
 }
 
@@ -361,7 +363,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 //
 // Four products (S, dP, dK, dV).  8 bf16 sequences up to 4096, 16 query and 4 kv heads of 128: 473 us, 867 TFLOP/s, and 15 us
 // for the sums of cut tiles.  96 fp16 sequences up to 203, 12 heads of 64: 37 us.  64 fp32 sequences up to 512, 4 heads of
-// 16: 48 us.
+// 16: 40 us, as long with a third workgroup to a compute unit: by the longest chain of row tiles.
 //
 // Two forms.  Up to 64 16-bit features, and in fp32, a wave takes 32 keys.  Beyond, the sums of dK and dV of 32 keys with
 // their K and V leave room for only one wave to a SIMD, which keeps the matrix unit idle while it makes P and dS; so there
@@ -421,9 +423,9 @@ struct KeySums {
       for (int s = 0; s < 2; ++s) {
         const v8 pt = operand<T>(p, s), dt = operand<T>(ds, s);
 #pragma unroll
-        for (int d = 0; d < S::DB; ++d) dv[d] = mma(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
+        for (int d = 0; d < S::DB; ++d) dv[d] = S::sum(LT::across(gt, d, 2 * b + s, lane), pt, dv[d]);
 #pragma unroll
-        for (int d = 0; d < S::DB; ++d) dk[d] = mma(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
+        for (int d = 0; d < S::DB; ++d) dk[d] = S::sum(LT::across(qt, d, 2 * b + s, lane), dt, dk[d]);
       }
       if (sizeof(T) == 2 && __builtin_expect(few, 0)) {
         const fx16 y = left_by_rounding<T>(p), z = left_by_rounding<T>(ds);
@@ -574,6 +576,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     kw.slow<T, DP>(1, Q, K, V, dO, lse, delta, dV, partial, S::KT, wave, lane, dm);
     return;
   }
+  S::whole(sums.dk, lane);
+  S::whole(sums.dv, lane);
   kw.store<T, S::DB>(dK, partial, 0, sums.dk, dm.scale, wave, lane, dm);
   kw.store<T, S::DB>(dV, partial, 1, sums.dv, 1.0f, wave, lane, dm);
 }

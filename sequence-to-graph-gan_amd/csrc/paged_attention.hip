@@ -161,6 +161,7 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
     }
     r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
   }
+  Shape<T, DP>::whole(r.o, lane);
   if (r.tainted) {
     r.clear();
     for (k0 = lo + 32 * wave; k0 < hi; k0 += 32 * NW)
@@ -268,6 +269,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
     const bool edge = k0 + S::KT - 1 > min(w_lo, hi - 1);
     r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, absent, lane);
   }
+  S::whole(r.o, lane);
   if (r.tainted) {
     r.clear();
     repair_tile(r, table, lo, hi, last, kb, vb, half, dm);
