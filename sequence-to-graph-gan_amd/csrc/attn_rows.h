@@ -13,7 +13,8 @@ struct Shape {
   typedef typename Vec<T>::v8 v8;
   // Sums over rows (keys) of 16 fp32 features: a 32 x 32 step would fill half of its result for nothing, so the same
   // operands go through v_mfma_f32_16x16x1_4b, four 16 x 16 products at once: columns 0 .. 15 and 16 .. 31 with the lower
-  // half's contraction slots, and again with the upper half's, which whole() adds at the end.
+  // half's contraction slots, and again with the upper half's, which whole() adds at the end.  (Training on 64 sequences up
+  // to 512, 4 heads: 122 -> 102 us.)
   static constexpr bool NARROW = sizeof(T) == 4 && DP == 16;
   static __device__ __forceinline__ fx16 sum(const v8& a, const v8& b, fx16 c) {
     if constexpr (NARROW) {
@@ -102,30 +103,32 @@ __device__ __forceinline__ void store_rows(U* p, const fx16* acc, float f, int D
     }
 }
 
-// acc += f x row, in the layout of a transposed result, row by row: the slow way, for tiles that products cannot take
-template <typename T, int DB>
-__device__ __forceinline__ void add_row(fx16* acc, float f, const T* p, int D, int half) {
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int at = 32 * d + 8 * g + 4 * half;
-      const typename Vec<T>::v4 x = *reinterpret_cast<const typename Vec<T>::v4*>(p + (at < D ? at : 0));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[d][4 * g + j] = fmaf(f, at < D ? (float)x[j] : 0.0f, acc[d][4 * g + j]);
-      __builtin_amdgcn_sched_barrier(0);              // one load at a time: its registers are the main loop's
-    }
-}
-// the dot product of a row with operands held in registers, this half's share of it
-template <typename T, int KS>
-__device__ __forceinline__ float dot_row(const typename Vec<T>::v8* a, const T* p, int D, int half) {
+// Infinities and NaN.  A product takes 0 x NaN for NaN, so a tile that holds one, and a row (key) that does not see it, cannot
+// go through the matrix unit together.  Where a tile with hidden pairs holds one, a wave makes its 32 rows (keys) anew: pair
+// by pair, straight from memory, 16 features at a time, and only the pairs that see each other.  Functions of their own,
+// never inlined: their registers would be the main loops' (packed attention, query side of the gradient: 297 -> 330 us).
+template <typename T, int N>
+__device__ __forceinline__ float slow_dot(const T* a, const T* b, int D, int half) {
   float s = 0.0f;
+#pragma unroll 1
+  for (int i = 0; i < N; ++i) s = dot8(row8(a, 16 * i + 8 * half, D, true), row8(b, 16 * i + 8 * half, D, true), s);
+  return both_sum(s);
+}
+template <typename T>
+__device__ __forceinline__ void slow_add(float* acc, float f, const T* p, int from, int D) {
 #pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    s = dot8(a[i], row8(p, 16 * i + 8 * half, D, true), s);
-    __builtin_amdgcn_sched_barrier(0);
+  for (int g = 0; g < 4; ++g) {
+    const int at = from + 4 * g;
+    const typename Vec<T>::v4 x = *reinterpret_cast<const typename Vec<T>::v4*>(p + (at < D ? at : 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[4 * g + j] = fmaf(f, (float)x[j], acc[4 * g + j]);
   }
-  return s;
+}
+template <typename T>
+__device__ __forceinline__ void slow_store(T* p, const float* acc, float f, int from, int D, bool ok) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (ok && from + j < D) p[from + j] = (T)(acc[j] * f);
 }
 
 // fp16 weights below 2^-14 lose bits, and a long row's weights are that small: there all of them are taken 2^RAISE times
@@ -142,7 +145,7 @@ struct Rows {
   v8 q[S::KS];
   fx16 o[S::DB];
   float m, l, c, slack;
-  bool tainted;              // a tile with hidden keys held an infinity or a NaN in V: o is not to be used (repair)
+  bool tainted;              // a tile with hidden keys held an infinity or a NaN in V: o is not to be used (slow_out, slow_pages)
 
   __device__ __forceinline__ void begin(const T* qp, int D, bool live, int half, float scale) {
 #pragma unroll
@@ -199,12 +202,12 @@ struct Rows {
       l *= a;
       S::scaled(o, a, lane);
     }
-    const float base = (m == -INFINITY ? 0.0f : m * c) - Weights<T>::RAISE;
+    const float low = base();
     v8 p[2 * KB];
     const auto weigh = [&](int e) {                      // two weights; four pairs make an operand
       const int b = e >> 3, i = 2 * (e & 7);
-      st[b][i] = __builtin_amdgcn_exp2f(fmaf(st[b][i], c, -base));
-      st[b][i + 1] = __builtin_amdgcn_exp2f(fmaf(st[b][i + 1], c, -base));
+      st[b][i] = __builtin_amdgcn_exp2f(fmaf(st[b][i], c, -low));
+      st[b][i + 1] = __builtin_amdgcn_exp2f(fmaf(st[b][i + 1], c, -low));
       p[e >> 2][i & 7] = (T)st[b][i];
       p[e >> 2][(i & 7) + 1] = (T)st[b][i + 1];
       l = add_two(l, p[e >> 2], st[b], i);
@@ -229,16 +232,8 @@ struct Rows {
     scores<KB>(st, kt, lane, [](int) {});
     add<KB, false>(st, nullptr, nullptr, vt, edge, last, absent, lane);
   }
-  // One key of o made anew: each row adds its own keys only, whatever the others hold.
-  __device__ __forceinline__ void repair(const T* kp, const T* vp, bool sees, int D, int half) {
-    const float s = dot_row<T, S::KS>(q, kp, D, half);
-    const float w = __builtin_amdgcn_exp2f(fmaf(both_sum(s), c, Weights<T>::RAISE - (m == -INFINITY ? 0.0f : m * c)));
-    if (sees) add_row<T, S::DB>(o, w, vp, D, half);
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int d = 0; d < S::DB; ++d) o[d] = zero16();
-  }
+  // what weigh() takes from a score (times c) to make a weight
+  __device__ __forceinline__ float base() const { return (m == -INFINITY ? 0.0f : m * c) - Weights<T>::RAISE; }
   // log2 of the row's sum of exponentials, given the sum over both halves
   __device__ __forceinline__ float log_sum(float sum) const { return fmaf(m, c, __builtin_amdgcn_logf(sum)) - Weights<T>::RAISE; }
 

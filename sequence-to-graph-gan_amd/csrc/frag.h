@@ -184,9 +184,10 @@ __device__ __forceinline__ ix4 buffer_of(const void* p, int bytes) {
 #define OUT_OF_BUFFER 0x7fffff00       // an offset beyond every buffer made here
 // 16 bytes per lane to consecutive LDS from `lds` on (an LDS byte address).  In assembly because the compiler, which
 // cannot tell the tile being filled from the one being read, waits for the loads of the builtin before every transposed
-// read: the next tile would never be in flight.  No register is written; wait_loads() is the wait.
+// read: the next tile would never be in flight.  No register is written; wait_loads() is the wait.  The compiler does not look
+// into the assembly for hazards: five wait states (the move and the s_nop) after whatever vector instruction wrote `b`.
 __device__ __forceinline__ void load_to_lds(ix4 b, unsigned lds, int lane_offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(lane_offset), "s"(b) : "memory", "m0");
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {

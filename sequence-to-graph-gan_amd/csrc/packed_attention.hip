@@ -16,34 +16,6 @@
 #include "attn_rows.h"
 #include "packed_attention.h"
 
-// ------------------------------------------------------------------------------------------------- infinities and NaN
-// A product takes 0 x NaN for NaN, so a tile that holds one, and a row (key) that does not see it, cannot go through the
-// matrix unit together.  Where a tile with hidden pairs holds one, a wave makes its 32 rows (keys) anew: pair by pair,
-// straight from memory, 16 features at a time, and only the pairs that see each other.  Functions of their own, never
-// inlined: their registers would be the main loops' (query side 297 -> 330 us).
-template <typename T, int N>
-__device__ __forceinline__ float slow_dot(const T* a, const T* b, int D, int half) {
-  float s = 0.0f;
-#pragma unroll 1
-  for (int i = 0; i < N; ++i) s = dot8(row8(a, 16 * i + 8 * half, D, true), row8(b, 16 * i + 8 * half, D, true), s);
-  return both_sum(s);
-}
-template <typename T>
-__device__ __forceinline__ void slow_add(float* acc, float f, const T* p, int from, int D) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int at = from + 4 * g;
-    const typename Vec<T>::v4 x = *reinterpret_cast<const typename Vec<T>::v4*>(p + (at < D ? at : 0));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[4 * g + j] = fmaf(f, (float)x[j], acc[4 * g + j]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void slow_store(T* p, const float* acc, float f, int from, int D, bool ok) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (ok && from + j < D) p[from + j] = (T)(acc[j] * f);
-}
 // rows of a wave: O = sum over the keys 0 .. last of 2^(c s - base) V, times f
 template <typename T, int DP>
 __device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int keys, int last, float c,
@@ -197,7 +169,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   if (lse && live && half == 0)
     lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
   if (r.tainted) {
-    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, r.c, (r.m == -INFINITY ? 0.0f : r.m * r.c) - Weights<T>::RAISE, f,
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, r.c, r.base(), f,
                     out + orow, sizeof(T) == 2 && rest ? rest + orow : nullptr, dm.D, live);
     return;
   }

@@ -48,18 +48,25 @@ __device__ __forceinline__ int page_of(const int* table, int key, int len, const
   return table[key < len ? key >> dm.page_shift : 0];
 }
 __device__ __forceinline__ bool in_pool(int page, const PagedDims& dm) { return (unsigned)page < (unsigned)dm.pages; }
-// One tile of KT keys from k0 on: wave instruction after wave instruction, each within one page (whose 16 tokens or more
-// it never crosses).  Keys beyond the length and of absent pages come as zeros.
+// One tile of keys from k0 on, and of values behind it: wave instruction after wave instruction, each within one page (whose
+// 16 tokens or more it never crosses).  Keys beyond the length and of absent pages come as zeros.  Where a page's rows lie is
+// made by the vector unit, lane l for key k0 + l, all of a tile at once, and read from there: made for one instruction after
+// another by the scalar unit it is a wave's longest path (chunks over 16001 tokens of 128 bf16: 176 scalar operations a tile).
 template <typename LT, int WAVES, typename T>
-__device__ __forceinline__ void fetch_pages(char* lds, const T* pool, int page, int k0, int len, const int* off, int wave,
-                                            const PagedDims& dm) {
-  const unsigned to = lds_address(lds);
+__device__ __forceinline__ void fetch_pages(char* lds, const T* keys, const T* values, int page, int k0, int len, const int* off,
+                                            int wave, int lane, const PagedDims& dm) {
+  const unsigned to = lds_address(lds), ld = (unsigned)dm.ld * (unsigned)sizeof(T), units = (unsigned)((dm.page_ld * (long)sizeof(T)) >> 4);
+  const int key = k0 + lane, n = min(LT::RPI, len - key);
+  const unsigned long at = (((unsigned long)(unsigned)page * units) << 4) + ((unsigned)key & ((1u << dm.page_shift) - 1u)) * ld;
+  const int bytes = in_pool(page, dm) && n > 0 ? (n - 1) * (int)ld + dm.D * (int)sizeof(T) : 0;       // 0: nothing is touched
+  const int lo = (int)(unsigned)at, hi = (int)(unsigned)(at >> 32);
 #pragma unroll
   for (int i = 0; i < LT::NI; ++i) {
-    const int r = (i * WAVES + wave) * LT::RPI, pg = __builtin_amdgcn_readlane(page, r);
-    const int n = in_pool(pg, dm) ? max(0, min(LT::RPI, len - (k0 + r))) : 0, in = (k0 + r) & ((1 << dm.page_shift) - 1);
-    const T* p = pool + pg * dm.page_ld + in * dm.ld;                    // not touched if n is 0
-    load_to_lds(buffer_of(p, n > 0 ? (int)(((n - 1) * dm.ld + dm.D) * (long)sizeof(T)) : 0), to + (i * WAVES + wave) * 1024, off[i]);
+    const int r = (i * WAVES + wave) * LT::RPI;
+    const unsigned long row = (unsigned long)(unsigned)__builtin_amdgcn_readlane(lo, r) | (unsigned long)(unsigned)__builtin_amdgcn_readlane(hi, r) << 32;
+    const int b = __builtin_amdgcn_readlane(bytes, r);
+    load_to_lds(buffer_of(reinterpret_cast<const char*>(keys) + row, b), to + (i * WAVES + wave) * 1024, off[i]);
+    load_to_lds(buffer_of(reinterpret_cast<const char*>(values) + row, b), to + LT::BYTES + (i * WAVES + wave) * 1024, off[i]);
   }
 }
 template <typename LT, typename T>
@@ -71,15 +78,23 @@ __device__ __forceinline__ void page_offsets(int* off, int wave, int lane, const
   }
 }
 
-// keys lo .. hi of a wave's rows, key by key (Rows::repair)
-template <typename R, typename T>
-__device__ __forceinline__ void repair_tile(R& r, const int* table, int lo, int hi, int last, const T* keys, const T* values, int half,
-                                            const PagedDims& dm) {
-  for (int key = lo; key < hi; ++key) {
-    const int page = uniform(table[key >> dm.page_shift]);
-    if (!in_pool(page, dm)) continue;
-    const long at = page * dm.page_ld + (key & ((1 << dm.page_shift) - 1)) * dm.ld;
-    r.repair(keys + at, values + at, key <= last, dm.D, half);
+// rows of a wave: O = sum over their keys among lo .. lo + 31, lo + step .., up to hi, of 2^(c s - base) V, times f
+template <typename T, int DP, typename U>
+__device__ __attribute__((noinline)) void slow_pages(const T* q, const T* keys, const T* values, const int* table, int lo, int step, int hi,
+                                                     int last, float c, float base, float f, U* to, bool live, int D, int page_shift,
+                                                     int pages, long page_ld, long ld) {
+  const int half = (threadIdx.x >> 5) & 1;
+  for (int from = 16 * half; from < DP + 16 * half; from += 32) {                // both halves take every turn: their dots are one
+    float acc[16] = {};
+    for (int k0 = lo; k0 < hi; k0 += step)
+      for (int key = k0; key < min(k0 + 32, hi); ++key) {
+        const int page = uniform(table[key >> page_shift]);
+        if ((unsigned)page >= (unsigned)pages) continue;
+        const long at = page * page_ld + (key & ((1 << page_shift) - 1)) * ld;
+        const float w = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, keys + at, D, half), c, -base));
+        if (key <= last) slow_add(acc, w, values + at, from, D);
+      }
+    slow_store(to, acc, f, from, D, live);
   }
 }
 
@@ -143,11 +158,11 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
   int k0 = lo + 32 * wave;
   Rows<T, DP> r;
   if (k0 < hi) {
-    fetch_pages<LT, 1>(mine, kb, page, k0, hi, off, 0, dm);
-    fetch_pages<LT, 1>(mine + LT::BYTES, vb, page, k0, hi, off, 0, dm);
+    fetch_pages<LT, 1>(mine, kb, vb, page, k0, hi, off, 0, lane, dm);
   }
   int next = page_of(table, k0 + 32 * NW + (lane & 31), hi, dm);
-  r.begin(Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq, dm.D, live, half, dm.scale);
+  const T* qp = Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq;
+  r.begin(qp, dm.D, live, half, dm.scale);
   for (int t = 0; k0 < hi; ++t, k0 += 32 * NW) {
     const char* kt = mine + (t & 1) * 2 * LT::BYTES;
     wait_loads();
@@ -155,18 +170,12 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
     page = next;
     if (k0 + 32 * NW < hi) {
       char* nx = mine + ((t + 1) & 1) * 2 * LT::BYTES;
-      fetch_pages<LT, 1>(nx, kb, page, k0 + 32 * NW, hi, off, 0, dm);
-      fetch_pages<LT, 1>(nx + LT::BYTES, vb, page, k0 + 32 * NW, hi, off, 0, dm);
+      fetch_pages<LT, 1>(nx, kb, vb, page, k0 + 32 * NW, hi, off, 0, lane, dm);
       next = page_of(table, k0 + 64 * NW + (lane & 31), hi, dm);
     }
     r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
   }
   Shape<T, DP>::whole(r.o, lane);
-  if (r.tainted) {
-    r.clear();
-    for (k0 = lo + 32 * wave; k0 < hi; k0 += 32 * NW)
-      repair_tile(r, table, k0, min(k0 + 32, hi), last, kb, vb, half, dm);
-  }
   // ---- the waves' results joined: maxima and sums through LDS, then the scaled O
   float* ml = reinterpret_cast<float*>(lds);                   // [NW][32] (m, l)
   const float l = both_sum(r.l);
@@ -187,7 +196,12 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
   const float f = r.m == m ? 1.0f : __builtin_amdgcn_exp2f((r.m - m) * r.c);
   constexpr int PAD = 32 * DB + 4;                             // floats per row
   float* os = reinterpret_cast<float*>(lds) + NW * 64;
-  store_rows<T, DB>(os + (wave * 32 + (lane & 31)) * PAD, r.o, alone ? (sum == 0.0f ? 0.0f : f / sum) : f, 32 * DB, half, true);
+  float* mine_o = os + (wave * 32 + (lane & 31)) * PAD;
+  const float scaled = alone ? (sum == 0.0f ? 0.0f : f / sum) : f;
+  if (r.tainted)
+    slow_pages<T, DP>(qp, kb, vb, table, lo + 32 * wave, 32 * NW, hi, last, r.c, r.base(), scaled, mine_o, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+  else
+    store_rows<T, DB>(mine_o, r.o, scaled, 32 * DB, half, true);
   const Joined j = workspace(ws, dm);
   if (!alone && wave == 0 && half == 0 && live) {
     float* p = j.ml + (ws_row(sq, kvh, row, dm) * dm.parts + part) * 2;
@@ -225,7 +239,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(blockIdx.x / dm.Hk, s + tile, dm.parts);
+  const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.x / dm.Hk, s = blockIdx.z, part = part_of(blockIdx.y, s, dm.parts);
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
   if (tile * 128 >= sq.rows) return;
   const int seen = keys_seen(sq, tile * 128 + 127, dm);
@@ -247,12 +261,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
   const int kl = lane & (S::KT - 1);
   int k0 = lo, page = page_of(table, k0 + kl, hi, dm);
   if (k0 < hi) {
-    fetch_pages<LT, 4>(lds, kb, page, k0, hi, off, wave, dm);
-    fetch_pages<LT, 4>(lds + LT::BYTES, vb, page, k0, hi, off, wave, dm);
+    fetch_pages<LT, 4>(lds, kb, vb, page, k0, hi, off, wave, lane, dm);
   }
   int next = page_of(table, k0 + S::KT + kl, hi, dm);
   Rows<T, DP> r;
-  r.begin(Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq, dm.D, live, half, dm.scale);
+  const T* qp = Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq;
+  r.begin(qp, dm.D, live, half, dm.scale);
   for (int t = 0; k0 < hi; ++t, k0 += S::KT) {
     const char* kt = lds + (t & 1) * 2 * LT::BYTES;
     wait_loads();
@@ -260,9 +274,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
     page = next;
     __syncthreads();
     if (k0 + S::KT < hi) {
-      char* nx = lds + ((t + 1) & 1) * 2 * LT::BYTES;
-      fetch_pages<LT, 4>(nx, kb, page, k0 + S::KT, hi, off, wave, dm);
-      fetch_pages<LT, 4>(nx + LT::BYTES, vb, page, k0 + S::KT, hi, off, wave, dm);
+      fetch_pages<LT, 4>(lds + ((t + 1) & 1) * 2 * LT::BYTES, kb, vb, page, k0 + S::KT, hi, off, wave, lane, dm);
       next = page_of(table, k0 + 2 * S::KT + kl, hi, dm);
     }
     if (k0 > w_hi) continue;
@@ -270,17 +282,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
     r.template step<S::KB>(kt, kt + LT::BYTES, edge, min(last, hi - 1) - k0, absent, lane);
   }
   S::whole(r.o, lane);
-  if (r.tainted) {
-    r.clear();
-    repair_tile(r, table, lo, hi, last, kb, vb, half, dm);
-  }
   const float l = both_sum(r.l);
   if (alone) {
-    store_rows<T, S::DB>(out + (((long)sq.start + tok) * dm.H + head) * dm.D, r.o, l == 0.0f ? 0.0f : 1.0f / l, dm.D, half, live);
+    T* to = out + (((long)sq.start + tok) * dm.H + head) * dm.D;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, hi, last, r.c, r.base(), f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+    else store_rows<T, S::DB>(to, r.o, f, dm.D, half, live);
   } else {
     const Joined j = workspace(ws, dm);
     const long at = ws_row(sq, kvh, rr, dm) * dm.parts + part;
-    store_rows<T, S::DB>(j.sums + at * dm.D, r.o, 1.0f, dm.D, half, live);
+    float* to = j.sums + at * dm.D;
+    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, hi, last, r.c, r.base(), 1.0f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+    else store_rows<T, S::DB>(to, r.o, 1.0f, dm.D, half, live);
     if (live && half == 0) {
       j.ml[2 * at] = r.m;
       j.ml[2 * at + 1] = l;
@@ -403,7 +416,7 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     const auto kernel = s2g_k_paged_attn_rows<T, DP>;
     const int bytes = 4 * Shape<T, DP>::LT::BYTES;
     if (s2g_lds_cap(rcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)dm.Hk * tiles, dm.parts, dm.n), dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   } else {
     const auto kernel = s2g_k_paged_attn_keys<T, DP>;
     typedef KeyTiles<T, DP> KT;
