@@ -109,6 +109,8 @@ static int paged_dims(const S2GPaged* a, PagedDims* d) {
   if (shift < 0 || a->pages <= 0 || a->table_cols <= 0 || (long)a->table_cols * a->page_size >= (1L << 30) || G > 128) return -1;
   if (a->q_rows <= 0 || a->q_rows * a->heads >= (1L << 30) || a->max_new <= 0 || a->max_new > a->q_rows || a->max_length < 0) return -1;
   if (!wide_rows(a->q_ld, a->q_hd, a->dim, es) || !wide_rows(a->token_ld, a->head_ld, a->dim, es) || a->page_ld % (16 / es) || a->page_ld < 0) return -1;
+  // a page's offset is its number times 32 bits of 16-byte units, a token's within its page has 32 bits
+  if (a->page_ld >= (1L << 36) / es || a->page_size * a->token_ld * es >= (1L << 32)) return -1;
   if (a->part_keys <= 0 || a->part_keys % 128 || a->parts <= 0 || (long)a->part_keys * a->parts < a->max_length || a->parts > 4096 ||
       (long)a->part_keys * a->parts >= (1L << 31))
     return -1;

@@ -605,7 +605,9 @@ class _PagedPlan:
         _attention_heads(what, H, Hk, D)
         unit = 16 // q.element_size()
         if any(s % unit for s in (page_ld, token_ld, head_ld)) or max(token_ld, head_ld) >= 1 << 22:
-            raise S2GError(f"{what}: pages must be strided by multiples of 16 bytes")
+            raise S2GError(f"{what}: pages must be strided by multiples of 16 bytes, tokens by less than 2^22 elements")
+        if page_ld * q.element_size() >= 1 << 36 or keys.shape[1] * token_ld * q.element_size() >= 1 << 32:
+            raise S2GError(f"{what}: a page must span less than 4 GiB, and the next begin within 64")
         _batch(what, batch, q, keys)
         if R * H >= 1 << 30:
             raise S2GError(f"{what}: 2^30 rows or more")

@@ -90,7 +90,7 @@ def test_c_entry_points_refuse():
     for change in BAD_HEADS + [dict(sequences=0), dict(sequences=65536), dict(page_size=8), dict(page_size=24), dict(page_size=1 << 17),
                                dict(pages=0), dict(table_cols=0), dict(table_cols=1 << 26), dict(max_new=0), dict(max_new=3),
                                dict(part_keys=0), dict(part_keys=100), dict(parts=0), dict(parts=5000), dict(max_length=600), dict(token_ld=3),
-                               dict(head_ld=1), dict(page_ld=5)]:
+                               dict(head_ld=1), dict(page_ld=5), dict(page_ld=1 << 35), dict(page_size=65536, token_ld=1 << 15)]:
         assert l.s2g_paged_attention(p, p, p, p, p, p, p, p, paged(**change), None) == -1, change
         assert l.s2g_paged_attention_workspace(paged(**change)) == -1, change
     for i in range(7):
