@@ -387,8 +387,8 @@ int s2g_packed_attention_bwd(const void* Q, const void* K, const void* V, const 
                              int n_cut_tiles, const S2GPacked* dims, void* stream);
 
 /* ---- attention of new tokens over a paged cache (paged_attention).  keys, values [pages, page_size, kv_heads, dim] with
- * the strides below (page_size a power of two, 16 .. 65536; page_size * token_ld below 4 GiB, page_ld below 64); table [sequences, table_cols] int32: the page of tokens
- * c page_size .. of a sequence; lengths [sequences] int32: tokens in the cache, the new ones among them; starts
+ * the strides below (page_size a power of two, 16 .. 65536; page_size * token_ld below 4 GiB, page_ld below 64); table
+ * [sequences, table_cols] int32: the page of tokens c page_size .. of a sequence; lengths [sequences] int32: tokens in the cache, the new ones among them; starts
  * [sequences + 1] int32: rows of Q.  Query i of n new tokens sees keys j <= length - n + i (causal) or all.  lengths,
  * table and starts are read on the device (a captured graph may update them): keys beyond what the table and
  * parts * part_keys cover are absent, and so are those of a page number outside [0, pages).  max_new, max_length: upper

@@ -5,7 +5,10 @@ constructor arguments, parameter names (in_proj_weight [3E, 3E], in_proj_bias, f
 including the unusual ones (the fused projection of concat(q, k, v), the finite -1e3 fill, the
 tril(diagonal=1) "causal" mask, scaling by sqrt(embed_size), the padding mask that fills the non-pad keys,
 batch_first=True meaning "transpose first").  All arithmetic of MaskedMultiheadAttention runs in libs2g
-kernels (include/s2g.h: s2g_attention_fwd / _bwd and the fp32 MFMA GEMM); it needs GPU tensors."""
+kernels (include/s2g.h: s2g_attention_fwd / _bwd and the fp32 MFMA GEMM); it needs GPU tensors.
+
+Beyond the reference, for causal models over the same sequences: rotary positions, attention over packed sequences with
+grouped heads, a paged key/value cache and attention over it (s2g/causal.py), and GroupedQueryAttention, which uses them."""
 import math
 import os
 import sys
