@@ -57,12 +57,12 @@ __device__ __forceinline__ void tile_offsets(int* off, long ld, int D, int wave,
     off[i] = c * 16 < D * (int)sizeof(T) ? (int)(LT::row_of(i, wave, lane) * ld * (long)sizeof(T)) + c * 16 : OUT_OF_BUFFER;
   }
 }
-template <typename LT, typename T>
+template <typename LT, typename T, int WAVES = 4>
 __device__ __forceinline__ void fetch_rows(char* lds, const T* p, long ld, int D, int rows, const int* off, int wave) {
   const ix4 b = buffer_of(p, rows > 0 ? (int)(((rows - 1) * ld + D) * (long)sizeof(T)) : 0);
   const unsigned to = lds_address(lds);
 #pragma unroll
-  for (int i = 0; i < LT::NI; ++i) load_to_lds(b, to + (i * 4 + wave) * 1024, off[i]);
+  for (int i = 0; i < LT::NI; ++i) load_to_lds(b, to + (i * WAVES + wave) * 1024, off[i]);
 }
 
 // 8 elements of a row straight from memory: zeros beyond the row's D elements or where !ok.  The loads are unconditional (of
@@ -247,3 +247,70 @@ struct Rows {
   static __device__ __forceinline__ float add_two(float l, hx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
   static __device__ __forceinline__ float add_two(float l, fx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
 };
+
+// A wave's own tiles of 32 keys (K and V, twice), and what joins the waves of a workgroup
+template <typename T, int DP>
+struct WaveTiles {
+  typedef Shape<T, DP> S;
+  typedef Tile<T, S::PITCH, 32, 1> LT;
+  static constexpr int NW = 16 * LT::BYTES <= 131072 ? 4 : 2;
+  static constexpr int PAD = 32 * S::DB + 4;                   // floats of a row of sums
+  static constexpr int TILES = 4 * NW * LT::BYTES, JOIN = NW * (64 + 32 * PAD) * (int)sizeof(float);
+  static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
+};
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const fx4& a) {
+  typename Vec<T>::v4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (T)a[i];
+  *reinterpret_cast<typename Vec<T>::v4*>(p) = v;
+}
+// 32 rows' sums of every wave (float [wave][row][PAD] in LDS) added; store(row, feature, four of them)
+template <typename T, int DP, typename Store>
+__device__ __forceinline__ void add_waves(const float* os, int rows, int D, Store store) {
+  typedef WaveTiles<T, DP> W;
+  const int n4 = D >> 2, count = rows * n4;
+  for (int e = threadIdx.x; e < count; e += 64 * W::NW) {
+    const int y = e / n4, d = (e - y * n4) * 4;
+    fx4 a = *reinterpret_cast<const fx4*>(os + y * W::PAD + d);
+#pragma unroll
+    for (int w = 1; w < W::NW; ++w) {
+      const fx4 b = *reinterpret_cast<const fx4*>(os + (w * 32 + y) * W::PAD + d);
+      a[0] += b[0]; a[1] += b[1]; a[2] += b[2]; a[3] += b[3];
+    }
+    store(y, d, a);
+  }
+}
+// The running softmaxes of 32 rows, each wave's over its own keys, joined: maxima and sums through LDS, then O scaled to the
+// common maximum (and by its sum if `divided`).  slow(f, to): a wave's O times f made anew; statistics(m, sum): of this lane's row.
+template <typename T, int DP, typename Slow, typename Statistics, typename Store>
+__device__ __forceinline__ void join_waves(char* lds, Rows<T, DP>& r, int rows, bool divided, int D, int wave, int lane, Slow slow,
+                                           Statistics statistics, Store store) {
+  typedef WaveTiles<T, DP> W;
+  const int half = lane >> 5;
+  float* ml = reinterpret_cast<float*>(lds);                   // [wave][row] (m, l)
+  const float l = both_sum(r.l);
+  Shape<T, DP>::whole(r.o, lane);
+  __syncthreads();
+  if (half == 0) {
+    ml[(wave * 32 + lane) * 2] = r.m;
+    ml[(wave * 32 + lane) * 2 + 1] = l;
+  }
+  __syncthreads();
+  float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W::NW; ++w) m = fmaxf(m, ml[(w * 32 + (lane & 31)) * 2]);
+#pragma unroll
+  for (int w = 0; w < W::NW; ++w) {
+    const float mw = ml[(w * 32 + (lane & 31)) * 2];
+    sum += ml[(w * 32 + (lane & 31)) * 2 + 1] * (mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * r.c));
+  }
+  const float f = r.m == m ? 1.0f : __builtin_amdgcn_exp2f((r.m - m) * r.c), scaled = divided ? (sum == 0.0f ? 0.0f : f / sum) : f;
+  float* os = ml + W::NW * 64;
+  float* mine = os + (wave * 32 + (lane & 31)) * W::PAD;
+  if (r.tainted) slow(scaled, mine);
+  else store_rows<T, Shape<T, DP>::DB>(mine, r.o, scaled, 32 * Shape<T, DP>::DB, half, true);
+  if (wave == 0 && half == 0) statistics(m, sum);
+  __syncthreads();
+  add_waves<T, DP>(os, rows, D, store);
+}

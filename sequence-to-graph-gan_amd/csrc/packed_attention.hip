@@ -16,17 +16,18 @@
 #include "attn_rows.h"
 #include "packed_attention.h"
 
-// rows of a wave: O = sum over the keys 0 .. last of 2^(c s - base) V, times f
-template <typename T, int DP>
-__device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int keys, int last, float c,
-                                                   float base, float f, T* out, T* rest, int D, bool live) {
+// rows of a wave: O = sum over their keys among lo .. lo + 31, lo + step .., up to `keys`, of 2^(c s - base) V, times f
+template <typename T, int DP, typename U>
+__device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int lo, int step, int keys,
+                                                   int last, float c, float base, float f, U* out, T* rest, int D, bool live) {
   const int half = (threadIdx.x >> 5) & 1;
   for (int from = 16 * half; from < DP + 16 * half; from += 32) {                // both halves take every turn: their dots are one
     float acc[16] = {};
-    for (int key = 0; key < keys; ++key) {
-      const float w = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -base));
-      if (key <= last) slow_add(acc, w, v + key * ldv, from, D);
-    }
+    for (int k0 = lo; k0 < keys; k0 += step)
+      for (int key = k0; key < min(k0 + 32, keys); ++key) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -base));
+        if (key <= last) slow_add(acc, w, v + key * ldv, from, D);
+      }
     slow_store(out, acc, f, from, D, live);
     if (rest) {
 #pragma unroll
@@ -35,18 +36,19 @@ __device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long 
     }
   }
 }
-// dQ of a wave's rows
-template <typename T, int DP>
-__device__ __attribute__((noinline)) void slow_dq(const T* q, const T* g, const T* k, long ldk, const T* v, long ldv, int keys, int last,
-                                                  float c, float scale, float L, float delta, T* dq, int D, bool live) {
+// dQ of a wave's rows over the same keys
+template <typename T, int DP, typename U>
+__device__ __attribute__((noinline)) void slow_dq(const T* q, const T* g, const T* k, long ldk, const T* v, long ldv, int lo, int step,
+                                                  int keys, int last, float c, float scale, float L, float delta, U* dq, int D, bool live) {
   const int half = (threadIdx.x >> 5) & 1;
   for (int from = 16 * half; from < DP + 16 * half; from += 32) {
     float acc[16] = {};
-    for (int key = 0; key < keys; ++key) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -L));
-      const float ds = last == 0 ? 0.0f : p * (slow_dot<T, DP / 16>(g, v + key * ldv, D, half) - delta);
-      if (key <= last) slow_add(acc, ds, k + key * ldk, from, D);
-    }
+    for (int k0 = lo; k0 < keys; k0 += step)
+      for (int key = k0; key < min(k0 + 32, keys); ++key) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -L));
+        const float ds = last == 0 ? 0.0f : p * (slow_dot<T, DP / 16>(g, v + key * ldv, D, half) - delta);
+        if (key <= last) slow_add(acc, ds, k + key * ldk, from, D);
+      }
     slow_store(dq, acc, scale, from, D, live);
   }
 }
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   if (lse && live && half == 0)
     lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
   if (r.tainted) {
-    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, r.c, r.base(), f,
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 0, 32, w_hi + 1, last, r.c, r.base(), f,
                     out + orow, sizeof(T) == 2 && rest ? rest + orow : nullptr, dm.D, live);
     return;
   }
@@ -186,24 +188,88 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   }
 }
 
+// The same for few tiles, which would leave most compute units idle: 32 rows to a workgroup (blockIdx.y: which of the tile's
+// 128), every wave over 32-key tiles of its own, joined at the end as in the paged cache's single tokens.  4444 fp16 tokens,
+// 3 / 1 heads of 128: 85 -> 61 us; 1000 bf16 tokens, 8 heads of 128: 25 -> 15; 8 fp32 sequences up to 722, 2 heads of 96:
+// 90 -> 50.  (few_tiles() says when.)
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn_fwd_few(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ out, T* __restrict__ rest,
+    float* __restrict__ lse, const PackedTile* __restrict__ tiles, PackedDims dm) {
+  typedef WaveTiles<T, DP> WT;
+  typedef typename WT::LT LT;
+  constexpr int NW = WT::NW;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int kvh = blockIdx.x % dm.Hk;
+  const PackedTile w = tiles[blockIdx.x / dm.Hk];
+  const int rows = w.q_len * dm.by.G, row0 = w.tile * 128 + 32 * blockIdx.y;
+  if (row0 >= rows) return;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int row = row0 + (lane & 31);
+  const bool live = row < rows;
+  const int tok = divide(min(row, rows - 1), dm.by), head = kvh * dm.by.G + (min(row, rows - 1) - tok * dm.by.G);
+  const T* qp = Q + ((long)w.q_start + tok) * dm.ldq + head * dm.hq;
+  const T* kp = K + (long)w.k_start * dm.ldk + kvh * dm.hk;
+  const T* vp = V + (long)w.k_start * dm.ldv + kvh * dm.hv;
+  const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
+  const int last = live ? min(w.k_len - 1, tok + shift) : -1;
+  const int w_lo = min(w.k_len - 1, divide(row0, dm.by) + shift);
+  const int hi = max(0, min(w.k_len, divide(min(row0 + 31, rows - 1), dm.by) + shift + 1));       // the keys that some row sees
+  int ko[LT::NI], vo[LT::NI];
+  tile_offsets<LT, T>(ko, dm.ldk, dm.D, 0, lane);
+  tile_offsets<LT, T>(vo, dm.ldv, dm.D, 0, lane);
+  char* mine = lds + wave * 4 * LT::BYTES;
+  const auto fetch = [&](int k0, int t) {
+    fetch_rows<LT, T, 1>(mine + (t & 1) * 2 * LT::BYTES, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(32, w.k_len - k0), ko, 0);
+    fetch_rows<LT, T, 1>(mine + (t & 1) * 2 * LT::BYTES + LT::BYTES, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(32, w.k_len - k0), vo, 0);
+  };
+  if (32 * wave < hi) fetch(32 * wave, 0);
+  Rows<T, DP> r;
+  r.begin(qp, dm.D, live, half, dm.scale);
+  for (int t = 0, k0 = 32 * wave; k0 < hi; ++t, k0 += 32 * NW) {
+    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
+    wait_loads();
+    if (k0 + 32 * NW < hi) fetch(k0 + 32 * NW, t + 1);
+    r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > w_lo, last - k0, 0, lane);
+  }
+  const auto slow = [&](float f, float* to) {
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 32 * wave, 32 * NW, hi, last, r.c, r.base(), f, to, (T*)nullptr, dm.D, true);
+  };
+  const auto statistics = [&](float m, float sum) {
+    if (lse && live)
+      lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = sum == 0.0f ? INFINITY : fmaf(m, r.c, __builtin_amdgcn_logf(sum)) - Weights<T>::RAISE;
+  };
+  join_waves<T, DP>(lds, r, min(32, rows - row0), true, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
+    const int tk = divide(row0 + y, dm.by);
+    const long at = (((long)w.q_start + tk) * dm.H + kvh * dm.by.G + row0 + y - tk * dm.by.G) * dm.D + d;
+    put4(out + at, a);
+    if (sizeof(T) == 2 && rest && min(w.k_len - 1, tk + shift) < FEW_KEYS)
+      put4(rest + at, (fx4){a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]});
+  });
+}
+
 // ------------------------------------------------------------------------------------------------- backward, query side
 // D of every row, and dQ: lanes are rows, as in the forward pass.  Three products (S, dP, dQ) to the forward's two.  8 bf16
 // sequences up to 4096, 16 query and 4 kv heads of 128: 297 us, 1035 TFLOP/s.  Making dQ here and not with atomics from the
-// key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
+// key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.  FEW: few tiles, as in
+// s2g_k_packed_attn_fwd_few (4444 fp16 tokens, 3 / 1 heads of 128: 96 -> 74 us).
+template <typename T, int DP, bool FEW>
+__global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || sizeof(T) == 4 ? 1 : 2) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, const T* __restrict__ out,
                                                                const T* __restrict__ rest, const T* __restrict__ dO, const float* __restrict__ lse,
                                                                float* __restrict__ delta, T* __restrict__ dQ,
                                                                const PackedTile* __restrict__ tiles, PackedDims dm) {
   typedef Shape<T, DP> S;
-  typedef typename S::LT LT;
+  typedef WaveTiles<T, DP> WT;
+  typedef typename std::conditional<FEW, typename WT::LT, typename S::LT>::type LT;
+  constexpr int KT = FEW ? 32 : S::KT, KB = KT / 32, STEP = FEW ? 32 * WT::NW : KT, LOADERS = FEW ? 1 : 4;
   typedef typename Vec<T>::v8 v8;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int kvh = blockIdx.x % dm.Hk;
   const PackedTile w = tiles[blockIdx.x / dm.Hk];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
-  const int rows = w.q_len * dm.by.G, row = w.tile * 128 + 32 * wave + (lane & 31);
+  const int rows = w.q_len * dm.by.G, row0 = w.tile * 128 + 32 * (FEW ? (int)blockIdx.y : wave), row = row0 + (lane & 31);
+  if (FEW && row0 >= rows) return;
   const bool live = row < rows;
   const int tok = divide(min(row, rows - 1), dm.by), head = kvh * dm.by.G + (min(row, rows - 1) - tok * dm.by.G);
   const long qrow = (long)w.q_start + tok, orow = (qrow * dm.H + head) * dm.D, lrow = ((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row;
@@ -214,10 +280,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 
   const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
   const int last = live ? min(w.k_len - 1, tok + shift) : -1;
-  const int w_lo = min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave, rows - 1), dm.by) + shift);
-  const int w_hi = w.tile * 128 + 32 * wave < rows ? min(w.k_len - 1, divide(min(w.tile * 128 + 32 * wave + 31, rows - 1), dm.by) + shift) : -1;
-  const int b_hi = min(w.k_len - 1, divide(min(w.tile * 128 + 127, rows - 1), dm.by) + shift);
-  const int nt = b_hi < 0 ? 0 : b_hi / S::KT + 1;
+  const int w_lo = min(w.k_len - 1, divide(min(row0, rows - 1), dm.by) + shift);
+  const int w_hi = row0 < rows ? min(w.k_len - 1, divide(min(row0 + 31, rows - 1), dm.by) + shift) : -1;
+  const int b_hi = FEW ? w_hi : min(w.k_len - 1, divide(min(w.tile * 128 + 127, rows - 1), dm.by) + shift);
+  const int first = FEW ? 32 * wave : 0;                         // this wave's first tile of keys
 
   v8 q[S::KS], g[S::KS];
   float dl = 0.0f;
@@ -248,36 +314,34 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   const float L = live ? lse[lrow] : INFINITY, c = dm.scale * LOG2E;
 
   int ko[LT::NI], vo[LT::NI];
-  tile_offsets<LT, T>(ko, dm.ldk, dm.D, wave, lane);
-  tile_offsets<LT, T>(vo, dm.ldv, dm.D, wave, lane);
+  tile_offsets<LT, T>(ko, dm.ldk, dm.D, FEW ? 0 : wave, lane);
+  tile_offsets<LT, T>(vo, dm.ldv, dm.D, FEW ? 0 : wave, lane);
   bool tainted = false;            // a tile with hidden keys held an infinity or a NaN in K
   fx16 dq[S::DB];
 #pragma unroll
   for (int d = 0; d < S::DB; ++d) dq[d] = zero16();
-  if (nt > 0) {
-    fetch_rows<LT>(lds, kp, dm.ldk, dm.D, min(S::KT, w.k_len), ko, wave);
-    fetch_rows<LT>(lds + LT::BYTES, vp, dm.ldv, dm.D, min(S::KT, w.k_len), vo, wave);
-  }
-  for (int t = 0; t < nt; ++t) {
-    char* kt = lds + (t & 1) * 2 * LT::BYTES;
+  char* mine = lds + (FEW ? wave * 4 * LT::BYTES : 0);
+  const auto fetch = [&](int k0, int t) {
+    char* to = mine + (t & 1) * 2 * LT::BYTES;
+    const int n = min(KT, w.k_len - k0);
+    fetch_rows<LT, T, LOADERS>(to, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, n, ko, FEW ? 0 : wave);
+    fetch_rows<LT, T, LOADERS>(to + LT::BYTES, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, n, vo, FEW ? 0 : wave);
+  };
+  if (first <= b_hi) fetch(first, 0);
+  for (int t = 0, k0 = first; k0 <= b_hi; ++t, k0 += STEP) {
+    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
     const char* vt = kt + LT::BYTES;
     wait_loads();
-    __syncthreads();
-    if (t + 1 < nt) {
-      char* nx = lds + ((t + 1) & 1) * 2 * LT::BYTES;
-      const int k1 = (t + 1) * S::KT, n = min(S::KT, w.k_len - k1);
-      fetch_rows<LT>(nx, kp + (long)k1 * dm.ldk, dm.ldk, dm.D, n, ko, wave);
-      fetch_rows<LT>(nx + LT::BYTES, vp + (long)k1 * dm.ldv, dm.ldv, dm.D, n, vo, wave);
-    }
-    const int k0 = t * S::KT;
+    if (!FEW) __syncthreads();
+    if (k0 + STEP <= b_hi) fetch(k0 + STEP, t + 1);
     if (k0 > w_hi) continue;
-    const bool edge = k0 + S::KT - 1 > w_lo;
+    const bool edge = k0 + KT - 1 > w_lo;
     // 32 keys at a time, 2^x beside the products of dP, dS beside those of the next keys' S
     fx16 st = zero16(), next;
     products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(kt, lane & 31, i, half); },
                                  [&](int i, const v8& a) { st = mma(a, q[i], st); }, [](int) {});
 #pragma unroll
-    for (int b = 0; b < S::KB; ++b) {
+    for (int b = 0; b < KB; ++b) {
       fx16 dp = zero16();
       products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(vt, 32 * b + (lane & 31), i, half); },
                                    [&](int i, const v8& a) { dp = mma(a, g[i], dp); },
@@ -291,7 +355,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 #pragma unroll
         for (int e = 16 * i / S::KS; e < 16 * (i + 1) / S::KS; ++e) st[e] *= dp[e] - dl;
       };
-      if (b + 1 < S::KB) {
+      if (b + 1 < KB) {
         next = zero16();
         products<T, S::KS, S::AHEAD>([&](int i) { return LT::along(kt, 32 * (b + 1) + (lane & 31), i, half); },
                                      [&](int i, const v8& a) { next = mma(a, q[i], next); }, slope);
@@ -318,13 +382,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
       st = next;
     }
   }
-  if (live && half == 0) delta[lrow] = dl;
-  if (tainted) {
-    slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
-    return;
+  if (live && half == 0 && (!FEW || wave == 0)) delta[lrow] = dl;          // (the first wave has seen the first key)
+  if constexpr (FEW) {
+    S::whole(dq, lane);
+    __syncthreads();
+    float* os = reinterpret_cast<float*>(lds);
+    float* to = os + (wave * 32 + (lane & 31)) * WT::PAD;
+    if (tainted) slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, first, STEP, w_hi + 1, last, c, dm.scale, L, dl, to, dm.D, true);
+    else store_rows<T, S::DB>(to, dq, dm.scale, 32 * S::DB, half, true);
+    __syncthreads();
+    add_waves<T, DP>(os, min(32, rows - row0), dm.D, [&](int y, int d, const fx4& a) {
+      const int tk = divide(row0 + y, dm.by);
+      put4(dQ + (((long)w.q_start + tk) * dm.H + kvh * dm.by.G + row0 + y - tk * dm.by.G) * dm.D + d, a);
+    });
+  } else {
+    if (tainted) {
+      slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, 0, 32, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
+      return;
+    }
+    S::whole(dq, lane);
+    store_rows<T, S::DB>(dQ + orow, dq, dm.scale, dm.D, half, live);
   }
-  S::whole(dq, lane);
-  store_rows<T, S::DB>(dQ + orow, dq, dm.scale, dm.D, half, live);
 }
 
 // --------------------------------------------------------------------------------------------------- backward, key side
@@ -776,14 +854,26 @@ __global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __rest
 }
 
 // ----------------------------------------------------------------------------------------------------------------- host
+// Whether 128-row tiles are too few for 256 compute units, so that 32 rows to a workgroup and keys dealt to its waves, at less
+// a rate, end sooner.  Measured with tiles / with the keys dealt, forward and query side of the gradient (us):
+// bf16, 8 heads of 128, 1000 tokens (64 tiles) 25 + 29 / 15 + 19; 2000 (128) 43 + 49 / 40 + 49; 16 / 4 heads of 64, 1500 (192) 19 +
+// 22 / 18 + 23; 32 / 8 of 128, 700 (176) 20 + 25 / 29 + 37.  fp32, whose products take eight times as long: 4 heads of 16, 8 x 512
+// tokens (128) 20 + 24 / 12 + 14; 16 x 512 (256) 20 + 25 / 17 + 22; 64 up to 512 (700) 26 + 35 / 27 + 40.
+template <typename T>
+static bool few_tiles(int nt, const PackedDims& dm) { return (long)nt * dm.Hk <= (sizeof(T) == 4 ? 256 : 128); }
+
 template <typename T, int DP>
 static int launch_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
                       const PackedDims& dm, hipStream_t st) {
-  const int bytes = 4 * Shape<T, DP>::LT::BYTES;
-  static S2GLdsCap cap;
-  const auto kernel = s2g_k_packed_attn_fwd<T, DP>;
-  if (s2g_lds_cap(cap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)nt * dm.Hk), dim3(256), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
+  static S2GLdsCap cap, few_cap;
+  const auto launch = [&](auto kernel, S2GLdsCap& c, dim3 grid, int threads, int bytes) {
+    if (s2g_lds_cap(c, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
+    return 0;
+  };
+  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
+                                      : launch(s2g_k_packed_attn_fwd<T, DP>, cap, dim3((unsigned)nt * dm.Hk), 256, 4 * Shape<T, DP>::LT::BYTES);
+  if (rc != 0) return rc;
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 template <typename T, int DP>
@@ -792,21 +882,24 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
                       const PackedTile* kt, int nkt, const PackedTile* cut, int ncut, const PackedDims& dm, hipStream_t st) {
   typedef typename Shape<T, DP>::LT LT;
   constexpr bool PAIR = sizeof(T) == 2 && DP > 64;
-  const int qb = 4 * LT::BYTES;
-  static S2GLdsCap qcap, kcap;
-  const auto kq = s2g_k_packed_attn_bwd_q<T, DP>;
-  if (s2g_lds_cap(qcap, reinterpret_cast<const void*>(kq), qb) != 0) return -2;
+  static S2GLdsCap qcap, few_cap, kcap;
+  const auto query_side = [&](auto kq, S2GLdsCap& c, dim3 grid, int threads, int bytes) {
+    if (s2g_lds_cap(c, reinterpret_cast<const void*>(kq), bytes) != 0) return -2;
+    if (nqt > 0)
+      hipLaunchKernelGGL(kq, grid, dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out, (const T*)rest,
+                         (const T*)dO, lse, delta, (T*)dQ, qt, dm);
+    return 0;
+  };
   const auto key_side = [&](auto kk, int threads, int bytes) {
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kk), bytes) != 0) return -2;
-    if (nqt > 0)
-      hipLaunchKernelGGL(kq, dim3((unsigned)nqt * dm.Hk), dim3(256), qb, st, (const T*)Q, (const T*)K, (const T*)V, (const T*)out,
-                         (const T*)rest, (const T*)dO, lse, delta, (T*)dQ, qt, dm);
     if (nkt > 0)
       hipLaunchKernelGGL(kk, dim3((unsigned)nkt * dm.Hk), dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V,
                          (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
     return 0;
   };
-  int rc;
+  int rc = few_tiles<T>(nqt, dm) ? query_side(s2g_k_packed_attn_bwd_q<T, DP, true>, few_cap, dim3((unsigned)nqt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
+                                 : query_side(s2g_k_packed_attn_bwd_q<T, DP, false>, qcap, dim3((unsigned)nqt * dm.Hk), 256, 4 * LT::BYTES);
+  if (rc != 0) return rc;
   if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, PairSums<T, DP>::BYTES);
   else rc = key_side(s2g_k_packed_attn_bwd_kv<T, DP>, 256, 4 * LT::BYTES + 4 * Shape<T, DP>::KT * (int)sizeof(float));
   if (rc != 0) return rc;

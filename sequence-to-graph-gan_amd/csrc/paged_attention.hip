@@ -120,20 +120,12 @@ __device__ __forceinline__ long ws_row(const PagedSeq& q, int kvh, int row, cons
 
 // --------------------------------------------------------------------------------------------------------- single tokens
 template <typename T, int DP>
-struct KeyTiles {                                              // tiles of 32 keys, one wave's own
-  static constexpr int PITCH = Shape<T, DP>::PITCH;
-  typedef Tile<T, PITCH, 32, 1> LT;
-  static constexpr int NW = 16 * LT::BYTES <= 131072 ? 4 : 2;  // K and V, twice, per wave
-  static constexpr int BYTES = 4 * NW * LT::BYTES;
-};
-
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_keys(
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_keys(
     const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
-  typedef KeyTiles<T, DP> KT;
+  typedef WaveTiles<T, DP> KT;
   typedef typename KT::LT LT;
-  constexpr int NW = KT::NW, DB = Shape<T, DP>::DB;
+  constexpr int NW = KT::NW;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(blockIdx.x / dm.Hk, s + tile, dm.parts);
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
@@ -177,60 +169,26 @@ __global__ __launch_bounds__(64 * (KeyTiles<T, DP>::NW)) void s2g_k_paged_attn_k
     }
     r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
   }
-  Shape<T, DP>::whole(r.o, lane);
-  // ---- the waves' results joined: maxima and sums through LDS, then the scaled O
-  float* ml = reinterpret_cast<float*>(lds);                   // [NW][32] (m, l)
-  const float l = both_sum(r.l);
-  __syncthreads();
-  if (half == 0) {
-    ml[(wave * 32 + lane) * 2] = r.m;
-    ml[(wave * 32 + lane) * 2 + 1] = l;
-  }
-  __syncthreads();
-  float m = -INFINITY, sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[(w * 32 + (lane & 31)) * 2]);
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const float mw = ml[(w * 32 + (lane & 31)) * 2];
-    sum += ml[(w * 32 + (lane & 31)) * 2 + 1] * (mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * r.c));
-  }
-  const float f = r.m == m ? 1.0f : __builtin_amdgcn_exp2f((r.m - m) * r.c);
-  constexpr int PAD = 32 * DB + 4;                             // floats per row
-  float* os = reinterpret_cast<float*>(lds) + NW * 64;
-  float* mine_o = os + (wave * 32 + (lane & 31)) * PAD;
-  const float scaled = alone ? (sum == 0.0f ? 0.0f : f / sum) : f;
-  if (r.tainted)
-    slow_pages<T, DP>(qp, kb, vb, table, lo + 32 * wave, 32 * NW, hi, last, r.c, r.base(), scaled, mine_o, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
-  else
-    store_rows<T, DB>(mine_o, r.o, scaled, 32 * DB, half, true);
   const Joined j = workspace(ws, dm);
-  if (!alone && wave == 0 && half == 0 && live) {
-    float* p = j.ml + (ws_row(sq, kvh, row, dm) * dm.parts + part) * 2;
-    p[0] = m;
-    p[1] = sum;
-  }
-  __syncthreads();
-  const int n4 = dm.D >> 2, count = min(32, sq.rows - tile * 32) * n4;
-  for (int e = threadIdx.x; e < count; e += 64 * NW) {
-    const int y = e / n4, d = (e - y * n4) * 4;
-    fx4 a = *reinterpret_cast<const fx4*>(os + y * PAD + d);
-#pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      const fx4 b = *reinterpret_cast<const fx4*>(os + (w * 32 + y) * PAD + d);
-      a[0] += b[0]; a[1] += b[1]; a[2] += b[2]; a[3] += b[3];
+  const auto slow = [&](float f, float* to) {
+    slow_pages<T, DP>(qp, kb, vb, table, lo + 32 * wave, 32 * NW, hi, last, r.c, r.base(), f, to, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+  };
+  const auto statistics = [&](float m, float sum) {
+    if (!alone && live) {
+      float* p = j.ml + (ws_row(sq, kvh, row, dm) * dm.parts + part) * 2;
+      p[0] = m;
+      p[1] = sum;
     }
+  };
+  join_waves<T, DP>(lds, r, min(32, sq.rows - tile * 32), alone, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
     const int ry = tile * 32 + y;
     if (alone) {
       const int tk = divide(ry, dm.by);
-      typename Vec<T>::v4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (T)a[i];
-      *reinterpret_cast<typename Vec<T>::v4*>(out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + ry - tk * dm.by.G) * dm.D + d) = v;
+      put4(out + (((long)sq.start + tk) * dm.H + kvh * dm.by.G + ry - tk * dm.by.G) * dm.D + d, a);
     } else {
       *reinterpret_cast<fx4*>(j.sums + (ws_row(sq, kvh, ry, dm) * dm.parts + part) * dm.D + d) = a;
     }
-  }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------- chunks
@@ -421,7 +379,7 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     hipLaunchKernelGGL(kernel, dim3((unsigned)dm.Hk * tiles, dm.parts, dm.n), dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   } else {
     const auto kernel = s2g_k_paged_attn_keys<T, DP>;
-    typedef KeyTiles<T, DP> KT;
+    typedef WaveTiles<T, DP> KT;
     const int join = KT::NW * (64 + 32 * (32 * Shape<T, DP>::DB + 4)) * (int)sizeof(float), bytes = KT::BYTES > join ? KT::BYTES : join;
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);

@@ -280,16 +280,20 @@ class _WorkLists:
             got = self.kept[group, causal] = self._list(seq[order], tile[order], 0, 0, -1)
         return got
 
-    def key_tiles(self, group: int, causal: bool, kv_heads: int) -> Tuple[torch.Tensor, torch.Tensor, int]:
+    def key_tiles(self, group: int, causal: bool, kv_heads: int, exact: bool = False) -> Tuple[torch.Tensor, torch.Tensor, int]:
         """Work list of the key side, the tiles that are cut, and how many slots they need.  A tile is as much work as it has
-        rows; none is left with more than half of what falls to a compute unit, but 512 rows are not worth a slot."""
-        got = self.kept.get((group, causal, kv_heads))
+        rows; none is left with more than half of what falls to a compute unit, but 256 rows are not worth a slot.  exact:
+        fp32, whose products take eight times as long: 128 rows, but all that falls to a compute unit, where several tiles
+        overlap.  (Kernel and sum, us.  16 / 4 bf16 heads of 64, 4 x 500 tokens, at least 128 / 256 / 512 rows: 28 / 28 / 39; 12 /
+        1 fp16 heads of 64, 96 up to 203: 38 / 39 / 42; 8 bf16 heads of 128, 1000: 36 / 29 / 32; 2 fp32 heads of 96, 8 up to 722:
+        49 / 76 / 124.)"""
+        got = self.kept.get((group, causal, kv_heads, exact))
         if got is None:
             seq, tile = self._tiles(self.k_len)
             rows = (self.q_len * group)[seq]
             first = np.maximum(0, tile * TILE - (self.k_len - self.q_len)[seq]) * group // TILE * TILE if causal else np.zeros_like(rows)
             work = np.maximum(0, rows - first)
-            most = max(512, -(-int(work.sum()) * kv_heads // 512 // TILE) * TILE)
+            most = max(128 if exact else 256, -(-int(work.sum()) * kv_heads // (256 if exact else 512) // TILE) * TILE)
             parts = np.maximum(1, -(-work // most))
             each = -(-work // parts // TILE) * TILE                      # whole tiles of rows
             of = np.repeat(np.arange(parts.size), parts)
@@ -301,7 +305,7 @@ class _WorkLists:
             order = np.argsort(lo - hi, kind="stable")
             cut = np.flatnonzero(parts > 1)
             start = np.cumsum(parts) - parts
-            got = self.kept[group, causal, kv_heads] = (
+            got = self.kept[group, causal, kv_heads, exact] = (
                 self._list(seq[of][order], tile[of][order], np.where(is_cut, lo, 0)[order], np.where(is_cut, hi, rows[of])[order], slot[order]),
                 self._list(seq[cut], tile[cut], parts[cut], 0, slot[start[cut]]), int(is_cut.sum()))
         return got
@@ -363,7 +367,7 @@ class _PackedPlan:
         got = self.bwd.get(key)
         if got is None:
             dims = S2GPacked(*self.fields, *_strides(q), *_strides(k), *_strides(v), *_strides(do), *self.size)
-            k_tiles, cut, slots = self.work.key_tiles(self.group, self.causal, self.kv_heads)
+            k_tiles, cut, slots = self.work.key_tiles(self.group, self.causal, self.kv_heads, self.fields[0] == 0)
             got = self.bwd[key] = (ctypes.byref(dims), (ptr(k_tiles), k_tiles.shape[0], ptr(cut), cut.shape[0]),
                                    get().s2g_packed_attention_bwd_workspace(ctypes.byref(dims), slots), (self.q_tiles, k_tiles, cut))
         return got
