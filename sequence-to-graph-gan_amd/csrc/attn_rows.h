@@ -248,14 +248,16 @@ struct Rows {
   static __device__ __forceinline__ float add_two(float l, fx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
 };
 
-// A wave's own tiles of 32 keys (K and V, twice), and what joins the waves of a workgroup
-template <typename T, int DP>
+// A wave's own tiles of 32 keys (K and V, twice), and what joins the waves of a workgroup.  Rows of 512 bytes leave room for
+// two waves, or, if FOUR are wanted all the same, for one tile of each, which is filled again once it has been read (ONCE).
+template <typename T, int DP, bool FOUR>
 struct WaveTiles {
   typedef Shape<T, DP> S;
   typedef Tile<T, S::PITCH, 32, 1> LT;
-  static constexpr int NW = 16 * LT::BYTES <= 131072 ? 4 : 2;
+  static constexpr bool WIDE = 16 * LT::BYTES > 131072, ONCE = WIDE && FOUR;
+  static constexpr int NW = WIDE && !FOUR ? 2 : 4;
   static constexpr int PAD = 32 * S::DB + 4;                   // floats of a row of sums
-  static constexpr int TILES = 4 * NW * LT::BYTES, JOIN = NW * (64 + 32 * PAD) * (int)sizeof(float);
+  static constexpr int TILES = (ONCE ? 2 : 4) * NW * LT::BYTES, JOIN = NW * (64 + 32 * PAD) * (int)sizeof(float);
   static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
 };
 template <typename T>
@@ -266,9 +268,8 @@ __device__ __forceinline__ void put4(T* p, const fx4& a) {
   *reinterpret_cast<typename Vec<T>::v4*>(p) = v;
 }
 // 32 rows' sums of every wave (float [wave][row][PAD] in LDS) added; store(row, feature, four of them)
-template <typename T, int DP, typename Store>
+template <typename W, typename Store>
 __device__ __forceinline__ void add_waves(const float* os, int rows, int D, Store store) {
-  typedef WaveTiles<T, DP> W;
   const int n4 = D >> 2, count = rows * n4;
   for (int e = threadIdx.x; e < count; e += 64 * W::NW) {
     const int y = e / n4, d = (e - y * n4) * 4;
@@ -283,10 +284,9 @@ __device__ __forceinline__ void add_waves(const float* os, int rows, int D, Stor
 }
 // The running softmaxes of 32 rows, each wave's over its own keys, joined: maxima and sums through LDS, then O scaled to the
 // common maximum (and by its sum if `divided`).  slow(f, to): a wave's O times f made anew; statistics(m, sum): of this lane's row.
-template <typename T, int DP, typename Slow, typename Statistics, typename Store>
+template <typename W, typename T, int DP, typename Slow, typename Statistics, typename Store>
 __device__ __forceinline__ void join_waves(char* lds, Rows<T, DP>& r, int rows, bool divided, int D, int wave, int lane, Slow slow,
                                            Statistics statistics, Store store) {
-  typedef WaveTiles<T, DP> W;
   const int half = lane >> 5;
   float* ml = reinterpret_cast<float*>(lds);                   // [wave][row] (m, l)
   const float l = both_sum(r.l);
@@ -312,5 +312,5 @@ __device__ __forceinline__ void join_waves(char* lds, Rows<T, DP>& r, int rows, 
   else store_rows<T, Shape<T, DP>::DB>(mine, r.o, scaled, 32 * Shape<T, DP>::DB, half, true);
   if (wave == 0 && half == 0) statistics(m, sum);
   __syncthreads();
-  add_waves<T, DP>(os, rows, D, store);
+  add_waves<W>(os, rows, D, store);
 }

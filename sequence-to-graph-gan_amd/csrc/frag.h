@@ -193,6 +193,12 @@ __device__ __forceinline__ void load_to_lds(ix4 b, unsigned lds, int lane_offset
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return __builtin_amdgcn_readfirstlane((int)(unsigned long)(const __attribute__((address_space(3))) void*)p);
 }
+// this wave's LDS reads are done: what they read may be filled again
+__device__ __forceinline__ void wait_reads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
 // this wave's loads have arrived, and its LDS reads are done (the next loads may take the place of what they read).  The
 // builtin, not assembly: the compiler then knows that its own loads have arrived too, and waits no second time in the loop.
 __device__ __forceinline__ void wait_loads() {

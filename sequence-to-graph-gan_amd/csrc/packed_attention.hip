@@ -191,12 +191,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 // The same for few tiles, which would leave most compute units idle: 32 rows to a workgroup (blockIdx.y: which of the tile's
 // 128), every wave over 32-key tiles of its own, joined at the end as in the paged cache's single tokens.  4444 fp16 tokens,
 // 3 / 1 heads of 128: 85 -> 61 us; 1000 bf16 tokens, 8 heads of 128: 25 -> 15; 8 fp32 sequences up to 722, 2 heads of 96:
-// 90 -> 50.  (few_tiles() says when.)
+// 90 -> 30.  (few_tiles() says when.)
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn_fwd_few(
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP, true>::NW)) void s2g_k_packed_attn_fwd_few(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ out, T* __restrict__ rest,
     float* __restrict__ lse, const PackedTile* __restrict__ tiles, PackedDims dm) {
-  typedef WaveTiles<T, DP> WT;
+  typedef WaveTiles<T, DP, true> WT;
   typedef typename WT::LT LT;
   constexpr int NW = WT::NW;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -218,19 +218,35 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
   int ko[LT::NI], vo[LT::NI];
   tile_offsets<LT, T>(ko, dm.ldk, dm.D, 0, lane);
   tile_offsets<LT, T>(vo, dm.ldv, dm.D, 0, lane);
-  char* mine = lds + wave * 4 * LT::BYTES;
-  const auto fetch = [&](int k0, int t) {
-    fetch_rows<LT, T, 1>(mine + (t & 1) * 2 * LT::BYTES, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(32, w.k_len - k0), ko, 0);
-    fetch_rows<LT, T, 1>(mine + (t & 1) * 2 * LT::BYTES + LT::BYTES, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(32, w.k_len - k0), vo, 0);
-  };
-  if (32 * wave < hi) fetch(32 * wave, 0);
+  char* mine = lds + wave * (WT::ONCE ? 2 : 4) * LT::BYTES;
+  const auto fetch_k = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(32, w.k_len - k0), ko, 0); };
+  const auto fetch_v = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(32, w.k_len - k0), vo, 0); };
+  if (32 * wave < hi) {
+    fetch_k(32 * wave, mine);
+    fetch_v(32 * wave, mine + LT::BYTES);
+  }
   Rows<T, DP> r;
   r.begin(qp, dm.D, live, half, dm.scale);
   for (int t = 0, k0 = 32 * wave; k0 < hi; ++t, k0 += 32 * NW) {
-    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
+    char* kt = mine + (WT::ONCE ? 0 : (t & 1) * 2 * LT::BYTES);
+    const bool edge = k0 + 31 > w_lo, more = k0 + 32 * NW < hi;
     wait_loads();
-    if (k0 + 32 * NW < hi) fetch(k0 + 32 * NW, t + 1);
-    r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > w_lo, last - k0, 0, lane);
+    if constexpr (WT::ONCE) {
+      fx16 st;
+      r.template scores<1>(&st, kt, lane, [](int) {});
+      wait_reads();
+      if (more) fetch_k(k0 + 32 * NW, kt);
+      r.template add<1, false>(&st, nullptr, nullptr, kt + LT::BYTES, edge, last - k0, 0, lane);
+      wait_reads();
+      if (more) fetch_v(k0 + 32 * NW, kt + LT::BYTES);
+    } else {
+      if (more) {
+        char* to = mine + ((t + 1) & 1) * 2 * LT::BYTES;
+        fetch_k(k0 + 32 * NW, to);
+        fetch_v(k0 + 32 * NW, to + LT::BYTES);
+      }
+      r.template step<1>(kt, kt + LT::BYTES, edge, last - k0, 0, lane);
+    }
   }
   const auto slow = [&](float f, float* to) {
     slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 32 * wave, 32 * NW, hi, last, r.c, r.base(), f, to, (T*)nullptr, dm.D, true);
@@ -239,7 +255,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
     if (lse && live)
       lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = sum == 0.0f ? INFINITY : fmaf(m, r.c, __builtin_amdgcn_logf(sum)) - Weights<T>::RAISE;
   };
-  join_waves<T, DP>(lds, r, min(32, rows - row0), true, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
+  join_waves<WT>(lds, r, min(32, rows - row0), true, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
     const int tk = divide(row0 + y, dm.by);
     const long at = (((long)w.q_start + tk) * dm.H + kvh * dm.by.G + row0 + y - tk * dm.by.G) * dm.D + d;
     put4(out + at, a);
@@ -254,15 +270,16 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
 // key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.  FEW: few tiles, as in
 // s2g_k_packed_attn_fwd_few (4444 fp16 tokens, 3 / 1 heads of 128: 96 -> 74 us).
 template <typename T, int DP, bool FEW>
-__global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || sizeof(T) == 4 ? 1 : 2) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW || sizeof(T) == 4 ? 1 : 2) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, const T* __restrict__ out,
                                                                const T* __restrict__ rest, const T* __restrict__ dO, const float* __restrict__ lse,
                                                                float* __restrict__ delta, T* __restrict__ dQ,
                                                                const PackedTile* __restrict__ tiles, PackedDims dm) {
   typedef Shape<T, DP> S;
-  typedef WaveTiles<T, DP> WT;
+  typedef WaveTiles<T, DP, true> WT;
   typedef typename std::conditional<FEW, typename WT::LT, typename S::LT>::type LT;
   constexpr int KT = FEW ? 32 : S::KT, KB = KT / 32, STEP = FEW ? 32 * WT::NW : KT, LOADERS = FEW ? 1 : 4;
+  constexpr bool ONCE = FEW && WT::ONCE;
   typedef typename Vec<T>::v8 v8;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int kvh = blockIdx.x % dm.Hk;
@@ -320,20 +337,28 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
   fx16 dq[S::DB];
 #pragma unroll
   for (int d = 0; d < S::DB; ++d) dq[d] = zero16();
-  char* mine = lds + (FEW ? wave * 4 * LT::BYTES : 0);
-  const auto fetch = [&](int k0, int t) {
-    char* to = mine + (t & 1) * 2 * LT::BYTES;
-    const int n = min(KT, w.k_len - k0);
-    fetch_rows<LT, T, LOADERS>(to, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, n, ko, FEW ? 0 : wave);
-    fetch_rows<LT, T, LOADERS>(to + LT::BYTES, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, n, vo, FEW ? 0 : wave);
+  char* mine = lds + (FEW ? wave * (ONCE ? 2 : 4) * LT::BYTES : 0);
+  const auto place = [&](int t) { return mine + (ONCE ? 0 : (t & 1) * 2 * LT::BYTES); };
+  const auto fetch_k = [&](int k0, int t) {
+    fetch_rows<LT, T, LOADERS>(place(t), kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(KT, w.k_len - k0), ko, FEW ? 0 : wave);
   };
-  if (first <= b_hi) fetch(first, 0);
+  const auto fetch_v = [&](int k0, int t) {
+    fetch_rows<LT, T, LOADERS>(place(t) + LT::BYTES, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(KT, w.k_len - k0), vo, FEW ? 0 : wave);
+  };
+  if (first <= b_hi) {
+    fetch_k(first, 0);
+    fetch_v(first, 0);
+  }
   for (int t = 0, k0 = first; k0 <= b_hi; ++t, k0 += STEP) {
-    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
+    const char* kt = place(t);
     const char* vt = kt + LT::BYTES;
+    const bool more = k0 + STEP <= b_hi;
     wait_loads();
     if (!FEW) __syncthreads();
-    if (k0 + STEP <= b_hi) fetch(k0 + STEP, t + 1);
+    if (!ONCE && more) {
+      fetch_k(k0 + STEP, t + 1);
+      fetch_v(k0 + STEP, t + 1);
+    }
     if (k0 > w_hi) continue;
     const bool edge = k0 + KT - 1 > w_lo;
     // 32 keys at a time, 2^x beside the products of dP, dS beside those of the next keys' S
@@ -349,6 +374,10 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
 #pragma unroll
                                      for (int e = 16 * i / S::KS; e < 16 * (i + 1) / S::KS; ++e) st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -L));
                                    });
+      if constexpr (ONCE) {
+        wait_reads();
+        if (more) fetch_v(k0 + STEP, 0);
+      }
       // a row that sees one key only has D = dP there, to the last bit: its scores have no gradient
       if (b == 0 && k0 == 0 && last == 0) dl = dp[0];
       const auto slope = [&](int i) {
@@ -381,6 +410,10 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
       }
       st = next;
     }
+    if constexpr (ONCE) {
+      wait_reads();
+      if (more) fetch_k(k0 + STEP, 0);
+    }
   }
   if (live && half == 0 && (!FEW || wave == 0)) delta[lrow] = dl;          // (the first wave has seen the first key)
   if constexpr (FEW) {
@@ -391,7 +424,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
     if (tainted) slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, first, STEP, w_hi + 1, last, c, dm.scale, L, dl, to, dm.D, true);
     else store_rows<T, S::DB>(to, dq, dm.scale, 32 * S::DB, half, true);
     __syncthreads();
-    add_waves<T, DP>(os, min(32, rows - row0), dm.D, [&](int y, int d, const fx4& a) {
+    add_waves<WT>(os, min(32, rows - row0), dm.D, [&](int y, int d, const fx4& a) {
       const int tk = divide(row0 + y, dm.by);
       put4(dQ + (((long)w.q_start + tk) * dm.H + kvh * dm.by.G + row0 + y - tk * dm.by.G) * dm.D + d, a);
     });
@@ -857,10 +890,11 @@ __global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __rest
 // Whether 128-row tiles are too few for 256 compute units, so that 32 rows to a workgroup and keys dealt to its waves, at less
 // a rate, end sooner.  Measured with tiles / with the keys dealt, forward and query side of the gradient (us):
 // bf16, 8 heads of 128, 1000 tokens (64 tiles) 25 + 29 / 15 + 19; 2000 (128) 43 + 49 / 40 + 49; 16 / 4 heads of 64, 1500 (192) 19 +
-// 22 / 18 + 23; 32 / 8 of 128, 700 (176) 20 + 25 / 29 + 37.  fp32, whose products take eight times as long: 4 heads of 16, 8 x 512
-// tokens (128) 20 + 24 / 12 + 14; 16 x 512 (256) 20 + 25 / 17 + 22; 64 up to 512 (700) 26 + 35 / 27 + 40.
+// 22 / 18 + 23; 32 / 8 of 128, 700 (176) 20 + 25 / 29 + 37.  fp32, whose products take eight times as long: 8 / 4 heads of 128,
+// 2630 tokens (168) 386 + 564 / 189 + 277; twice those (336) 394 + 568 / 323 + 474; 4 heads of 32, 8 x 1500 (384) 84 + 110 / 60 + 81;
+// 32 x 500 (512) 35 + 47 / 40 + 55; 4 of 16, 64 up to 512 (700) 26 + 35 / 27 + 40.
 template <typename T>
-static bool few_tiles(int nt, const PackedDims& dm) { return (long)nt * dm.Hk <= (sizeof(T) == 4 ? 256 : 128); }
+static bool few_tiles(int nt, const PackedDims& dm) { return (long)nt * dm.Hk <= (sizeof(T) == 4 ? 384 : 128); }
 
 template <typename T, int DP>
 static int launch_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
@@ -871,7 +905,7 @@ static int launch_fwd(const void* Q, const void* K, const void* V, void* out, vo
     hipLaunchKernelGGL(kernel, grid, dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
     return 0;
   };
-  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
+  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP, true>::NW, WaveTiles<T, DP, true>::BYTES)
                                       : launch(s2g_k_packed_attn_fwd<T, DP>, cap, dim3((unsigned)nt * dm.Hk), 256, 4 * Shape<T, DP>::LT::BYTES);
   if (rc != 0) return rc;
   return hipGetLastError() == hipSuccess ? 0 : -2;
@@ -897,7 +931,7 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
                          (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
     return 0;
   };
-  int rc = few_tiles<T>(nqt, dm) ? query_side(s2g_k_packed_attn_bwd_q<T, DP, true>, few_cap, dim3((unsigned)nqt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
+  int rc = few_tiles<T>(nqt, dm) ? query_side(s2g_k_packed_attn_bwd_q<T, DP, true>, few_cap, dim3((unsigned)nqt * dm.Hk, 4), 64 * WaveTiles<T, DP, true>::NW, WaveTiles<T, DP, true>::BYTES)
                                  : query_side(s2g_k_packed_attn_bwd_q<T, DP, false>, qcap, dim3((unsigned)nqt * dm.Hk), 256, 4 * LT::BYTES);
   if (rc != 0) return rc;
   if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, PairSums<T, DP>::BYTES);

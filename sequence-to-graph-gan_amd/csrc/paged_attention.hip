@@ -120,10 +120,10 @@ __device__ __forceinline__ long ws_row(const PagedSeq& q, int kvh, int row, cons
 
 // --------------------------------------------------------------------------------------------------------- single tokens
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_keys(
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP, false>::NW)) void s2g_k_paged_attn_keys(
     const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
-  typedef WaveTiles<T, DP> KT;
+  typedef WaveTiles<T, DP, false> KT;
   typedef typename KT::LT LT;
   constexpr int NW = KT::NW;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_
       p[1] = sum;
     }
   };
-  join_waves<T, DP>(lds, r, min(32, sq.rows - tile * 32), alone, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
+  join_waves<KT>(lds, r, min(32, sq.rows - tile * 32), alone, dm.D, wave, lane, slow, statistics, [&](int y, int d, const fx4& a) {
     const int ry = tile * 32 + y;
     if (alone) {
       const int tk = divide(ry, dm.by);
@@ -379,7 +379,7 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     hipLaunchKernelGGL(kernel, dim3((unsigned)dm.Hk * tiles, dm.parts, dm.n), dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   } else {
     const auto kernel = s2g_k_paged_attn_keys<T, DP>;
-    typedef WaveTiles<T, DP> KT;
+    typedef WaveTiles<T, DP, false> KT;
     const int join = KT::NW * (64 + 32 * (32 * Shape<T, DP>::DB + 4)) * (int)sizeof(float), bytes = KT::BYTES > join ? KT::BYTES : join;
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);

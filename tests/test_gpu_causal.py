@@ -33,7 +33,7 @@ LENGTHS = [
 
 
 # Few 128-row tiles are worked on 32 rows at a time, many 128: short sequences behind the tested ones make them many
-MANY = [5] * 260
+MANY = [5] * 400
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
