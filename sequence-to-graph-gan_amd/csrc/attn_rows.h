@@ -248,14 +248,15 @@ struct Rows {
   static __device__ __forceinline__ float add_two(float l, fx8, const fx16& st, int i) { return l + st[i] + st[i + 1]; }
 };
 
-// A wave's own tiles of 32 keys (K and V, twice), and what joins the waves of a workgroup.  Rows of 512 bytes leave room for
-// two waves, or, if FOUR are wanted all the same, for one tile of each, which is filled again once it has been read (ONCE).
-template <typename T, int DP, bool FOUR>
+// A wave's own tiles of 32 keys (K and V, twice), and what joins the waves of a workgroup.  Four waves' rows of 512 bytes leave
+// room for one tile of each only, which is filled again as it has been read (ONCE): two waves with two tiles of each leave half
+// the matrix units idle (one fp32 token of 32 sequences of 4000, 32 / 8 heads of 128: 379 -> 268 us).
+template <typename T, int DP>
 struct WaveTiles {
   typedef Shape<T, DP> S;
-  typedef Tile<T, S::PITCH, 32, 1> LT;
-  static constexpr bool WIDE = 16 * LT::BYTES > 131072, ONCE = WIDE && FOUR;
-  static constexpr int NW = WIDE && !FOUR ? 2 : 4;
+  static constexpr int KEYS = 32, KB = KEYS / 32, NW = 4;
+  typedef Tile<T, S::PITCH, KEYS, 1> LT;
+  static constexpr bool ONCE = 4 * NW * LT::BYTES > 131072;
   static constexpr int PAD = 32 * S::DB + 4;                   // floats of a row of sums
   static constexpr int TILES = (ONCE ? 2 : 4) * NW * LT::BYTES, JOIN = NW * (64 + 32 * PAD) * (int)sizeof(float);
   static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;

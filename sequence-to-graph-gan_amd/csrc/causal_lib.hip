@@ -3,6 +3,7 @@
 #include "paged_attention.h"
 #include "rotary.h"
 #include <math.h>
+#include <algorithm>
 #include <initializer_list>
 
 // mirror include/s2g.h
@@ -115,7 +116,8 @@ static int paged_dims(const S2GPaged* a, PagedDims* d) {
       (long)a->part_keys * a->parts >= (1L << 31))
     return -1;
   *d = PagedDims{a->sequences, a->heads, a->kv_heads, a->dim, a->causal != 0, div_by(G), shift, a->table_cols, a->pages,
-                 a->q_ld, a->q_hd, a->page_ld, a->token_ld, a->head_ld, a->q_rows, a->max_new * G, a->part_keys, a->parts, a->scale};
+                 a->q_ld, a->q_hd, a->page_ld, a->token_ld, a->head_ld, a->q_rows, a->max_new * G, a->part_keys, a->parts, a->scale,
+                 (int)(a->head_ld > 0 ? std::max(1L, 128 / (a->head_ld * es)) : 1)};
   return 0;
 }
 

@@ -16,15 +16,15 @@
 #include "attn_rows.h"
 #include "packed_attention.h"
 
-// rows of a wave: O = sum over their keys among lo .. lo + 31, lo + step .., up to `keys`, of 2^(c s - base) V, times f
+// rows of a wave: O = sum over their keys among lo .. lo + width - 1, lo + step .., up to `keys`, of 2^(c s - base) V, times f
 template <typename T, int DP, typename U>
-__device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int lo, int step, int keys,
-                                                   int last, float c, float base, float f, U* out, T* rest, int D, bool live) {
+__device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long ldk, const T* v, long ldv, int lo, int width, int step,
+                                                   int keys, int last, float c, float base, float f, U* out, T* rest, int D, bool live) {
   const int half = (threadIdx.x >> 5) & 1;
   for (int from = 16 * half; from < DP + 16 * half; from += 32) {                // both halves take every turn: their dots are one
     float acc[16] = {};
     for (int k0 = lo; k0 < keys; k0 += step)
-      for (int key = k0; key < min(k0 + 32, keys); ++key) {
+      for (int key = k0; key < min(k0 + width, keys); ++key) {
         const float w = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -base));
         if (key <= last) slow_add(acc, w, v + key * ldv, from, D);
       }
@@ -38,13 +38,13 @@ __device__ __attribute__((noinline)) void slow_out(const T* q, const T* k, long 
 }
 // dQ of a wave's rows over the same keys
 template <typename T, int DP, typename U>
-__device__ __attribute__((noinline)) void slow_dq(const T* q, const T* g, const T* k, long ldk, const T* v, long ldv, int lo, int step,
-                                                  int keys, int last, float c, float scale, float L, float delta, U* dq, int D, bool live) {
+__device__ __attribute__((noinline)) void slow_dq(const T* q, const T* g, const T* k, long ldk, const T* v, long ldv, int lo, int width,
+                                                  int step, int keys, int last, float c, float scale, float L, float delta, U* dq, int D, bool live) {
   const int half = (threadIdx.x >> 5) & 1;
   for (int from = 16 * half; from < DP + 16 * half; from += 32) {
     float acc[16] = {};
     for (int k0 = lo; k0 < keys; k0 += step)
-      for (int key = k0; key < min(k0 + 32, keys); ++key) {
+      for (int key = k0; key < min(k0 + width, keys); ++key) {
         const float p = __builtin_amdgcn_exp2f(fmaf(slow_dot<T, DP / 16>(q, k + key * ldk, D, half), c, -L));
         const float ds = last == 0 ? 0.0f : p * (slow_dot<T, DP / 16>(g, v + key * ldv, D, half) - delta);
         if (key <= last) slow_add(acc, ds, k + key * ldk, from, D);
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   if (lse && live && half == 0)
     lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
   if (r.tainted) {
-    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 0, 32, w_hi + 1, last, r.c, r.base(), f,
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 0, 32, 32, w_hi + 1, last, r.c, r.base(), f,
                     out + orow, sizeof(T) == 2 && rest ? rest + orow : nullptr, dm.D, live);
     return;
   }
@@ -193,12 +193,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 // 3 / 1 heads of 128: 85 -> 61 us; 1000 bf16 tokens, 8 heads of 128: 25 -> 15; 8 fp32 sequences up to 722, 2 heads of 96:
 // 90 -> 30.  (few_tiles() says when.)
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (WaveTiles<T, DP, true>::NW)) void s2g_k_packed_attn_fwd_few(
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn_fwd_few(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ out, T* __restrict__ rest,
     float* __restrict__ lse, const PackedTile* __restrict__ tiles, PackedDims dm) {
-  typedef WaveTiles<T, DP, true> WT;
+  typedef WaveTiles<T, DP> WT;
   typedef typename WT::LT LT;
-  constexpr int NW = WT::NW;
+  constexpr int STEP = WT::KEYS * WT::NW;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int kvh = blockIdx.x % dm.Hk;
   const PackedTile w = tiles[blockIdx.x / dm.Hk];
@@ -219,37 +219,38 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP, true>::NW)) void s2g_k_packe
   tile_offsets<LT, T>(ko, dm.ldk, dm.D, 0, lane);
   tile_offsets<LT, T>(vo, dm.ldv, dm.D, 0, lane);
   char* mine = lds + wave * (WT::ONCE ? 2 : 4) * LT::BYTES;
-  const auto fetch_k = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(32, w.k_len - k0), ko, 0); };
-  const auto fetch_v = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(32, w.k_len - k0), vo, 0); };
-  if (32 * wave < hi) {
-    fetch_k(32 * wave, mine);
-    fetch_v(32 * wave, mine + LT::BYTES);
+  const auto fetch_k = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, kp + (long)k0 * dm.ldk, dm.ldk, dm.D, min(WT::KEYS, w.k_len - k0), ko, 0); };
+  const auto fetch_v = [&](int k0, char* to) { fetch_rows<LT, T, 1>(to, vp + (long)k0 * dm.ldv, dm.ldv, dm.D, min(WT::KEYS, w.k_len - k0), vo, 0); };
+  const int first = WT::KEYS * wave;
+  if (first < hi) {
+    fetch_k(first, mine);
+    fetch_v(first, mine + LT::BYTES);
   }
   Rows<T, DP> r;
   r.begin(qp, dm.D, live, half, dm.scale);
-  for (int t = 0, k0 = 32 * wave; k0 < hi; ++t, k0 += 32 * NW) {
+  for (int t = 0, k0 = first; k0 < hi; ++t, k0 += STEP) {
     char* kt = mine + (WT::ONCE ? 0 : (t & 1) * 2 * LT::BYTES);
-    const bool edge = k0 + 31 > w_lo, more = k0 + 32 * NW < hi;
+    const bool edge = k0 + WT::KEYS - 1 > w_lo, more = k0 + STEP < hi;
     wait_loads();
     if constexpr (WT::ONCE) {
-      fx16 st;
-      r.template scores<1>(&st, kt, lane, [](int) {});
+      fx16 st[WT::KB];
+      r.template scores<WT::KB>(st, kt, lane, [](int) {});
       wait_reads();
-      if (more) fetch_k(k0 + 32 * NW, kt);
-      r.template add<1, false>(&st, nullptr, nullptr, kt + LT::BYTES, edge, last - k0, 0, lane);
+      if (more) fetch_k(k0 + STEP, kt);
+      r.template add<WT::KB, false>(st, nullptr, nullptr, kt + LT::BYTES, edge, last - k0, 0, lane);
       wait_reads();
-      if (more) fetch_v(k0 + 32 * NW, kt + LT::BYTES);
+      if (more) fetch_v(k0 + STEP, kt + LT::BYTES);
     } else {
       if (more) {
         char* to = mine + ((t + 1) & 1) * 2 * LT::BYTES;
-        fetch_k(k0 + 32 * NW, to);
-        fetch_v(k0 + 32 * NW, to + LT::BYTES);
+        fetch_k(k0 + STEP, to);
+        fetch_v(k0 + STEP, to + LT::BYTES);
       }
-      r.template step<1>(kt, kt + LT::BYTES, edge, last - k0, 0, lane);
+      r.template step<WT::KB>(kt, kt + LT::BYTES, edge, last - k0, 0, lane);
     }
   }
   const auto slow = [&](float f, float* to) {
-    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 32 * wave, 32 * NW, hi, last, r.c, r.base(), f, to, (T*)nullptr, dm.D, true);
+    slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, first, WT::KEYS, STEP, hi, last, r.c, r.base(), f, to, (T*)nullptr, dm.D, true);
   };
   const auto statistics = [&](float m, float sum) {
     if (lse && live)
@@ -270,15 +271,15 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP, true>::NW)) void s2g_k_packe
 // key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.  FEW: few tiles, as in
 // s2g_k_packed_attn_fwd_few (4444 fp16 tokens, 3 / 1 heads of 128: 96 -> 74 us).
 template <typename T, int DP, bool FEW>
-__global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW || sizeof(T) == 4 ? 1 : 2) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || sizeof(T) == 4 ? 1 : 2) void s2g_k_packed_attn_bwd_q(const T* __restrict__ Q, const T* __restrict__ K,
                                                                const T* __restrict__ V, const T* __restrict__ out,
                                                                const T* __restrict__ rest, const T* __restrict__ dO, const float* __restrict__ lse,
                                                                float* __restrict__ delta, T* __restrict__ dQ,
                                                                const PackedTile* __restrict__ tiles, PackedDims dm) {
   typedef Shape<T, DP> S;
-  typedef WaveTiles<T, DP, true> WT;
+  typedef WaveTiles<T, DP> WT;
   typedef typename std::conditional<FEW, typename WT::LT, typename S::LT>::type LT;
-  constexpr int KT = FEW ? 32 : S::KT, KB = KT / 32, STEP = FEW ? 32 * WT::NW : KT, LOADERS = FEW ? 1 : 4;
+  constexpr int KT = FEW ? WT::KEYS : S::KT, KB = KT / 32, STEP = FEW ? KT * WT::NW : KT, LOADERS = FEW ? 1 : 4;
   constexpr bool ONCE = FEW && WT::ONCE;
   typedef typename Vec<T>::v8 v8;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW 
   const int w_lo = min(w.k_len - 1, divide(min(row0, rows - 1), dm.by) + shift);
   const int w_hi = row0 < rows ? min(w.k_len - 1, divide(min(row0 + 31, rows - 1), dm.by) + shift) : -1;
   const int b_hi = FEW ? w_hi : min(w.k_len - 1, divide(min(w.tile * 128 + 127, rows - 1), dm.by) + shift);
-  const int first = FEW ? 32 * wave : 0;                         // this wave's first tile of keys
+  const int first = FEW ? KT * wave : 0;                         // this wave's first tile of keys
 
   v8 q[S::KS], g[S::KS];
   float dl = 0.0f;
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW 
 #pragma unroll
                                      for (int e = 16 * i / S::KS; e < 16 * (i + 1) / S::KS; ++e) st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -L));
                                    });
-      if constexpr (ONCE) {
+      if constexpr (ONCE) {                       // (32 keys)
         wait_reads();
         if (more) fetch_v(k0 + STEP, 0);
       }
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW 
     __syncthreads();
     float* os = reinterpret_cast<float*>(lds);
     float* to = os + (wave * 32 + (lane & 31)) * WT::PAD;
-    if (tainted) slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, first, STEP, w_hi + 1, last, c, dm.scale, L, dl, to, dm.D, true);
+    if (tainted) slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, first, KT, STEP, w_hi + 1, last, c, dm.scale, L, dl, to, dm.D, true);
     else store_rows<T, S::DB>(to, dq, dm.scale, 32 * S::DB, half, true);
     __syncthreads();
     add_waves<WT>(os, min(32, rows - row0), dm.D, [&](int y, int d, const fx4& a) {
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP, true>::NW) : 256, FEW 
     });
   } else {
     if (tainted) {
-      slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, 0, 32, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
+      slow_dq<T, DP>(qp, gp, kp, dm.ldk, vp, dm.ldv, 0, 32, 32, w_hi + 1, last, c, dm.scale, L, dl, dQ + orow, dm.D, live);
       return;
     }
     S::whole(dq, lane);
@@ -905,7 +906,7 @@ static int launch_fwd(const void* Q, const void* K, const void* V, void* out, vo
     hipLaunchKernelGGL(kernel, grid, dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
     return 0;
   };
-  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP, true>::NW, WaveTiles<T, DP, true>::BYTES)
+  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
                                       : launch(s2g_k_packed_attn_fwd<T, DP>, cap, dim3((unsigned)nt * dm.Hk), 256, 4 * Shape<T, DP>::LT::BYTES);
   if (rc != 0) return rc;
   return hipGetLastError() == hipSuccess ? 0 : -2;
@@ -931,7 +932,7 @@ static int launch_bwd(const void* Q, const void* K, const void* V, const void* o
                          (const T*)dO, lse, delta, (T*)dK, (T*)dV, partial, kt, dm);
     return 0;
   };
-  int rc = few_tiles<T>(nqt, dm) ? query_side(s2g_k_packed_attn_bwd_q<T, DP, true>, few_cap, dim3((unsigned)nqt * dm.Hk, 4), 64 * WaveTiles<T, DP, true>::NW, WaveTiles<T, DP, true>::BYTES)
+  int rc = few_tiles<T>(nqt, dm) ? query_side(s2g_k_packed_attn_bwd_q<T, DP, true>, few_cap, dim3((unsigned)nqt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
                                  : query_side(s2g_k_packed_attn_bwd_q<T, DP, false>, qcap, dim3((unsigned)nqt * dm.Hk), 256, 4 * LT::BYTES);
   if (rc != 0) return rc;
   if constexpr (PAIR) rc = key_side(s2g_k_packed_attn_bwd_kv2<T, DP>, 512, PairSums<T, DP>::BYTES);

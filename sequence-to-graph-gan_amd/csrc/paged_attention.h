@@ -12,4 +12,5 @@ struct PagedDims {
   int max_rows;                      // rows (token, head of the group) of the longest chunk
   int part_keys, parts;              // keys per part of a sequence, parts of the longest one
   float scale;
+  int line_heads;                    // heads of a token that share 128 bytes of the cache
 };

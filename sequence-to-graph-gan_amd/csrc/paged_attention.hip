@@ -54,7 +54,7 @@ __device__ __forceinline__ bool in_pool(int page, const PagedDims& dm) { return 
 // 16 tokens or more it never crosses).  Keys beyond the length and of absent pages come as zeros.  Where a page's rows lie is
 // made by the vector unit, lane l for key k0 + l, all of a tile at once, and read from there: made for one instruction after
 // another by the scalar unit it is a wave's longest path (chunks over 16001 tokens of 128 bf16: 176 scalar operations a tile).
-template <typename LT, int WAVES, typename T>
+template <typename LT, int WAVES, bool KEYS = true, bool VALUES = true, typename T>
 __device__ __forceinline__ void fetch_pages(char* lds, const T* keys, const T* values, int page, int k0, int len, const int* off,
                                             int wave, int lane, const PagedDims& dm) {
   const unsigned to = lds_address(lds), ld = (unsigned)dm.ld * (unsigned)sizeof(T), units = (unsigned)((dm.page_ld * (long)sizeof(T)) >> 4);
@@ -67,8 +67,8 @@ __device__ __forceinline__ void fetch_pages(char* lds, const T* keys, const T* v
     const int r = (i * WAVES + wave) * LT::RPI;
     const unsigned long row = (unsigned long)(unsigned)__builtin_amdgcn_readlane(lo, r) | (unsigned long)(unsigned)__builtin_amdgcn_readlane(hi, r) << 32;
     const int b = __builtin_amdgcn_readlane(bytes, r);
-    load_to_lds(buffer_of(reinterpret_cast<const char*>(keys) + row, b), to + (i * WAVES + wave) * 1024, off[i]);
-    load_to_lds(buffer_of(reinterpret_cast<const char*>(values) + row, b), to + LT::BYTES + (i * WAVES + wave) * 1024, off[i]);
+    if constexpr (KEYS) load_to_lds(buffer_of(reinterpret_cast<const char*>(keys) + row, b), to + (i * WAVES + wave) * 1024, off[i]);
+    if constexpr (VALUES) load_to_lds(buffer_of(reinterpret_cast<const char*>(values) + row, b), to + LT::BYTES + (i * WAVES + wave) * 1024, off[i]);
   }
 }
 template <typename LT, typename T>
@@ -80,16 +80,16 @@ __device__ __forceinline__ void page_offsets(int* off, int wave, int lane, const
   }
 }
 
-// rows of a wave: O = sum over their keys among lo .. lo + 31, lo + step .., up to hi, of 2^(c s - base) V, times f
+// rows of a wave: O = sum over their keys among lo .. lo + width - 1, lo + step .., up to hi, of 2^(c s - base) V, times f
 template <typename T, int DP, typename U>
-__device__ __attribute__((noinline)) void slow_pages(const T* q, const T* keys, const T* values, const int* table, int lo, int step, int hi,
+__device__ __attribute__((noinline)) void slow_pages(const T* q, const T* keys, const T* values, const int* table, int lo, int width, int step, int hi,
                                                      int last, float c, float base, float f, U* to, bool live, int D, int page_shift,
                                                      int pages, long page_ld, long ld) {
   const int half = (threadIdx.x >> 5) & 1;
   for (int from = 16 * half; from < DP + 16 * half; from += 32) {                // both halves take every turn: their dots are one
     float acc[16] = {};
     for (int k0 = lo; k0 < hi; k0 += step)
-      for (int key = k0; key < min(k0 + 32, hi); ++key) {
+      for (int key = k0; key < min(k0 + width, hi); ++key) {
         const int page = uniform(table[key >> page_shift]);
         if ((unsigned)page >= (unsigned)pages) continue;
         const long at = page * page_ld + (key & ((1 << page_shift) - 1)) * ld;
@@ -104,6 +104,14 @@ __device__ __attribute__((noinline)) void slow_pages(const T* q, const T* keys, 
 // the XCDs and their engines in turn, so the parts that short sequences lack would otherwise all fall to the same ones
 // (64 sequences of 300 to 8200 tokens in 8 parts: 300 us, turned 250).
 __device__ __forceinline__ int part_of(int i, int by, int parts) { return (i + by) % parts; }
+
+// The order of a sequence's (part, kv head) pairs, heads fastest.  Workgroups are dealt to the 8 XCDs in turn, so neighbouring
+// heads would be read by different caches, and where several share a 128-byte line each would fetch it whole (one token of 64
+// sequences of 8000, 8 heads of 16 bf16: 162 us, so 93; 4000, of 32: 82, so 46): such heads lie 8 apart.
+__device__ __forceinline__ int shared_lines(int b, int blocks, int line_heads) {
+  const int all = 8 * line_heads, r = b % all;
+  return line_heads == 1 || b - r + all > blocks ? b : b - r + r % 8 * line_heads + r / 8;
+}
 
 // Where a row's result goes: the output if its sequence has one part, else part `part` of the workspace
 // ([row of all kv heads][part][D] sums, then [row][part] (m, l)).
@@ -120,14 +128,15 @@ __device__ __forceinline__ long ws_row(const PagedSeq& q, int kvh, int row, cons
 
 // --------------------------------------------------------------------------------------------------------- single tokens
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * (WaveTiles<T, DP, false>::NW)) void s2g_k_paged_attn_keys(
+__global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_keys(
     const T* __restrict__ Q, const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ starts, T* __restrict__ out, float* __restrict__ ws, PagedDims dm) {
-  typedef WaveTiles<T, DP, false> KT;
+  typedef WaveTiles<T, DP> KT;
   typedef typename KT::LT LT;
-  constexpr int NW = KT::NW;
+  constexpr int KEYS = KT::KEYS, STEP = KEYS * KT::NW;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int kvh = blockIdx.x % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(blockIdx.x / dm.Hk, s + tile, dm.parts);
+  const int pair = shared_lines(blockIdx.x, gridDim.x, dm.line_heads);
+  const int kvh = pair % dm.Hk, tile = blockIdx.y, s = blockIdx.z, part = part_of(pair / dm.Hk, s + tile, dm.parts);
   const PagedSeq sq = paged_seq(lens, starts, s, dm);
   if (tile * 32 >= sq.rows) return;
   const int seen = keys_seen(sq, tile * 32 + 31, dm);
@@ -146,32 +155,40 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP, false>::NW)) void s2g_k_page
 
   int off[LT::NI];
   page_offsets<LT, T>(off, 0, lane, dm);
-  char* mine = lds + wave * 4 * LT::BYTES;
-  // tiles lo + 32 (wave + NW t), the pages of the one after next on their way with the next
-  int page = page_of(table, lo + 32 * wave + (lane & 31), hi, dm);
-  int k0 = lo + 32 * wave;
+  char* mine = lds + wave * (KT::ONCE ? 2 : 4) * LT::BYTES;
+  // tiles lo + KEYS wave + STEP t, the pages of the one after next on their way with the next
+  int k0 = lo + KEYS * wave;
+  const int at = lane & (KEYS - 1);
+  int page = page_of(table, k0 + at, hi, dm);
   Rows<T, DP> r;
-  if (k0 < hi) {
-    fetch_pages<LT, 1>(mine, kb, vb, page, k0, hi, off, 0, lane, dm);
-  }
-  int next = page_of(table, k0 + 32 * NW + (lane & 31), hi, dm);
+  if (k0 < hi) fetch_pages<LT, 1>(mine, kb, vb, page, k0, hi, off, 0, lane, dm);
+  int next = page_of(table, k0 + STEP + at, hi, dm);
   const T* qp = Q + ((long)sq.start + tok) * dm.ldq + head * dm.hq;
   r.begin(qp, dm.D, live, half, dm.scale);
-  for (int t = 0; k0 < hi; ++t, k0 += 32 * NW) {
-    const char* kt = mine + (t & 1) * 2 * LT::BYTES;
+  for (int t = 0; k0 < hi; ++t, k0 += STEP) {
+    char* kt = mine + (KT::ONCE ? 0 : (t & 1) * 2 * LT::BYTES);
     wait_loads();
-    const unsigned absent = (unsigned)__ballot(!in_pool(page, dm) && k0 + (lane & 31) < hi);
+    const unsigned long long gone = __ballot(!in_pool(page, dm) && k0 + at < hi), absent = KEYS == 32 ? (unsigned)gone : gone;
     page = next;
-    if (k0 + 32 * NW < hi) {
-      char* nx = mine + ((t + 1) & 1) * 2 * LT::BYTES;
-      fetch_pages<LT, 1>(nx, kb, vb, page, k0 + 32 * NW, hi, off, 0, lane, dm);
-      next = page_of(table, k0 + 64 * NW + (lane & 31), hi, dm);
+    const bool edge = k0 + KEYS - 1 > min(w_lo, hi - 1), more = k0 + STEP < hi;
+    const int end = min(last, hi - 1) - k0;
+    if constexpr (KT::ONCE) {
+      fx16 st[KT::KB];
+      r.template scores<KT::KB>(st, kt, lane, [](int) {});
+      wait_reads();
+      if (more) fetch_pages<LT, 1, true, false>(kt, kb, vb, page, k0 + STEP, hi, off, 0, lane, dm);
+      r.template add<KT::KB, false>(st, nullptr, nullptr, kt + LT::BYTES, edge, end, absent, lane);
+      wait_reads();
+      if (more) fetch_pages<LT, 1, false, true>(kt, kb, vb, page, k0 + STEP, hi, off, 0, lane, dm);
+    } else {
+      if (more) fetch_pages<LT, 1>(mine + ((t + 1) & 1) * 2 * LT::BYTES, kb, vb, page, k0 + STEP, hi, off, 0, lane, dm);
     }
-    r.template step<1>(kt, kt + LT::BYTES, k0 + 31 > min(w_lo, hi - 1), min(last, hi - 1) - k0, absent, lane);
+    if (more) next = page_of(table, k0 + 2 * STEP + at, hi, dm);
+    if constexpr (!KT::ONCE) r.template step<KT::KB>(kt, kt + LT::BYTES, edge, end, absent, lane);
   }
   const Joined j = workspace(ws, dm);
   const auto slow = [&](float f, float* to) {
-    slow_pages<T, DP>(qp, kb, vb, table, lo + 32 * wave, 32 * NW, hi, last, r.c, r.base(), f, to, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+    slow_pages<T, DP>(qp, kb, vb, table, lo + KT::KEYS * wave, KT::KEYS, STEP, hi, last, r.c, r.base(), f, to, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
   };
   const auto statistics = [&](float m, float sum) {
     if (!alone && live) {
@@ -246,13 +263,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_paged_attn_
   if (alone) {
     T* to = out + (((long)sq.start + tok) * dm.H + head) * dm.D;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, hi, last, r.c, r.base(), f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, 32, hi, last, r.c, r.base(), f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
     else store_rows<T, S::DB>(to, r.o, f, dm.D, half, live);
   } else {
     const Joined j = workspace(ws, dm);
     const long at = ws_row(sq, kvh, rr, dm) * dm.parts + part;
     float* to = j.sums + at * dm.D;
-    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, hi, last, r.c, r.base(), 1.0f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
+    if (r.tainted) slow_pages<T, DP>(qp, kb, vb, table, lo, 32, 32, hi, last, r.c, r.base(), 1.0f, to, live, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);
     else store_rows<T, S::DB>(to, r.o, 1.0f, dm.D, half, live);
     if (live && half == 0) {
       j.ml[2 * at] = r.m;
@@ -379,7 +396,7 @@ static int launch_paged(const void* Q, const void* keys, const void* values, con
     hipLaunchKernelGGL(kernel, dim3((unsigned)dm.Hk * tiles, dm.parts, dm.n), dim3(256), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
   } else {
     const auto kernel = s2g_k_paged_attn_keys<T, DP>;
-    typedef WaveTiles<T, DP, false> KT;
+    typedef WaveTiles<T, DP> KT;
     const int join = KT::NW * (64 + 32 * (32 * Shape<T, DP>::DB + 4)) * (int)sizeof(float), bytes = KT::BYTES > join ? KT::BYTES : join;
     if (s2g_lds_cap(kcap, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * KT::NW), bytes, st, (const T*)Q, (const T*)keys, (const T*)values, table, lens, starts, (T*)out, ws, dm);
