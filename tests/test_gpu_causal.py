@@ -366,6 +366,19 @@ def test_paged_attention(dtype, shape, case):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(8, 8, 16), (16, 8, 8), (6, 6, 24), (10, 5, 32), (3, 3, 40)], ids=str)
+def test_paged_attention_of_narrow_heads(dtype, shape):
+    """Heads that share 128 bytes of the cache are worked on in an order of their own: every (part, head) once."""
+    import transformer as M
+    H, Hk, D = shape
+    g, context, new = gen(19), [3000, 1, 700], [1, 1, 1]
+    keys, values, table = cache_of(g, context, 16, Hk, D, dtype)
+    q = rand(g, 3, H, D, dtype=dtype)
+    got = M.paged_attention(q, keys, values, M.PagedBatch(table, context, new))
+    check_paged(q, keys, values, table, context, new, True, 1 / math.sqrt(D), got)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
 def test_paged_attention_absent_pages(dtype):
     """A page number outside the pool: its keys are not there; a sequence of such pages gives zeros."""
     import transformer as M
