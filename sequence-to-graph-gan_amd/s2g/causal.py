@@ -330,8 +330,8 @@ class PackedSequences(_Fixed):
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
         self.rows, self.key_rows = int(q.sum()), int(k.sum())
         with torch.cuda.device(self.device):
-            self.starts = _on_device(np.append(0, np.cumsum(q)), self.device)
-            self.positions = _on_device(np.arange(self.rows) - np.repeat(np.cumsum(q) - k, q), self.device)
+            both = _on_device(np.concatenate(([0], np.cumsum(q), np.arange(self.rows) - np.repeat(np.cumsum(q) - k, q))), self.device)
+        self.starts, self.positions = both[:q.size + 1], both[q.size + 1:]
         self._work, self._plans = _WorkLists(q, k, self.device, torch.cuda.current_stream(self.device)), {}
 
 
@@ -464,11 +464,14 @@ class PagedBatch(_Fixed):
         dev = table.device if table.is_cuda else torch.device(device or "cuda")
         if dev.type != "cuda":
             raise S2GError("PagedBatch: needs a GPU device")
-        _no_capture()
-        self.table = table.to(dev).contiguous()
-        dev = self.device = self.table.device
+        # one copy to the device: a step of serving makes a batch
+        columns = table.shape[1]
+        host = [c, [0], np.cumsum(n)] + ([] if table.is_cuda else [table.numpy().reshape(-1)])
+        buffer = _on_device(np.concatenate(host), dev)
+        dev = self.device = buffer.device
+        self.lengths, self.starts = buffer[:n.size], buffer[n.size:2 * n.size + 1]
+        self.table = table.contiguous() if table.is_cuda else buffer[2 * n.size + 1:].view(n.size, columns)
         self.stream = torch.cuda.current_stream(dev)
-        self.lengths, self.starts = _on_device(c, dev), _on_device(np.append(0, np.cumsum(n)), dev)
         self.sequences, self.rows, self.max_new = n.size, int(n.sum()), int(n.max())
         self.max_length = int(c.max()) if max_length is None else int(max_length)
         self._length, self._new, self._cuts, self._plans = c, n, {}, {}
