@@ -77,6 +77,8 @@ __device__ __attribute__((noinline)) void slow_key(int which, const T* k, const 
 // So for rows that see at most this many keys the products of the backward pass take what rounding left, too: 1.05 to 1.25
 // times, over long sequences 1.3.  They are the first rows of a long sequence or all of short ones; it costs 3 % of a
 // training step on sequences up to 4096 and 9 us of 80 on 96 of up to 203 tokens (12 heads of 64).
+// fp16 slopes are not raised as the weights are: how large they get is up to dO and V, so nothing says how far they may be.
+// Those below 2^-14 lose bits, like dO, dQ, dK and dV of that size themselves: fp16 training scales its loss.
 #define FEW_KEYS 128
 template <typename T>
 __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
