@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .lib import S2GError, S2GPacked, S2GPaged, S2GRotary, call, get
-from .ops import ptr, stream_ptr
+from .ops import cur_stream, ptr, stream_ptr
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 TILE = 128                       # rows, or keys, of one workgroup
@@ -116,12 +116,23 @@ def _on_device(values, device) -> torch.Tensor:
     return torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32)).to(device)
 
 
+def _stream(device: int) -> torch.cuda.Stream:
+    """A device's current stream."""
+    return cur_stream() if device == torch._C._cuda_getDevice() else torch.cuda.current_stream(device)
+
+
+def _hold(device: int, *tensors: torch.Tensor) -> None:
+    """Tensors that a launch on the current stream reads: their memory is not given away before it is done, whichever stream
+    they were made on and whenever they go (0.3 us each)."""
+    stream = _stream(device)
+    for t in tensors:
+        t.record_stream(stream)
+
+
 def _lend(owner, *tensors: torch.Tensor) -> None:
-    """A batch's own tensors, read by a launch on another stream than owner.stream, on which they were made: their memory is
-    not given away before that launch is done, whenever the batch goes."""
+    """The same for a batch's own tensors, which were made on owner.stream."""
     if torch._C._cuda_getCurrentRawStream(owner.device.index) != owner.stream.cuda_stream:
-        for t in tensors:
-            t.record_stream(torch.cuda.current_stream(owner.device))
+        _hold(owner.device.index, *tensors)
 
 
 class _Fixed:
@@ -205,6 +216,7 @@ def _turn(q, k, positions, frequencies, interleaved, multiplier, backward):
         return _turn(_dense(q), None if k is None else _dense(k), positions, frequencies, interleaved, multiplier, backward)
     qo, ko = _new(q), None if k is None else _new(k)
     if plan.rows:
+        _hold(plan.device, positions, frequencies)         # a batch's and a module's own, which may go before the launch is done
         _launch(plan.device, "s2g_rotary", q.data_ptr(), ptr(k), positions.data_ptr(), frequencies.data_ptr(), qo.data_ptr(), ptr(ko), plan.args)
     return qo, ko
 
@@ -559,6 +571,7 @@ def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch
     if not plan.whole:
         out[batch.rows:].zero_()
     if batch.rows:
+        _hold(plan.device, frequencies)
         _launch(plan.device, "s2g_rotary_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), frequencies.data_ptr(), out.data_ptr(),
                 keys.data_ptr(), values.data_ptr(), *batch.pointers(), plan.args, plan.paged)
     return out

@@ -234,3 +234,32 @@ def test_key_tiles_cover_every_row_once():
                     assert all(a[1] == b[0] for a, b in zip(parts, parts[1:])) and (parts[-1][1] == rows or first >= rows)
     finally:
         causal._on_device = old
+
+
+class Watched(torch.Tensor):
+    """Says on which streams it has been recorded."""
+
+    def record_stream(self, stream):
+        self.streams.append(stream)
+
+
+def watched(x):
+    x = x.as_subclass(Watched)
+    x.streams = []
+    return x
+
+
+def test_rotary_holds_positions_and_frequencies(monkeypatch):
+    """What a launch reads of a batch (or of a module) that may go before the launch is done is kept from the allocator on the
+    launch's stream, in the gradient too."""
+    from s2g import causal
+    monkeypatch.setattr(causal, "_launch", lambda *args: None)
+    monkeypatch.setattr(causal, "_stream", lambda device: "the current one", raising=False)
+    q, k = torch.randn(6, 2, 8, requires_grad=True), torch.randn(6, 1, 8, requires_grad=True)
+    positions, frequencies = watched(torch.arange(6, dtype=torch.int32)), watched(torch.rand(4, dtype=torch.float64))
+    causal._turn(q.detach(), None, positions, frequencies, False, 1.0, False)
+    assert positions.streams == frequencies.streams == ["the current one"]
+    out = causal.RotaryFn.apply(q, k, positions, frequencies, True, 1.0)
+    assert positions.streams == frequencies.streams == ["the current one"] * 2
+    torch.autograd.grad(out, (q, k), [torch.ones_like(x) for x in out])
+    assert positions.streams == frequencies.streams == ["the current one"] * 3

@@ -748,3 +748,40 @@ def test_refusals_on_gpu_tensors():
                  (x(4, 2, 16), None, pos, freq), (x(4, 1, 300), None, pos, freq)):
         with pytest.raises(S2GError):
             M.apply_rotary(*args)
+
+
+def test_positions_and_frequencies_dropped_while_another_stream_reads_them():
+    """The same for the positions of a batch and the frequencies of a module, which the rotation reads: forward without a graph,
+    and the gradient's launch, which outlives the graph that held them."""
+    import transformer as M
+    g, n = gen(35), [700, 10, 300]
+    q, k = (rand(g, sum(n), h, 64, dtype=torch.bfloat16).requires_grad_() for h in (4, 2))
+    d = [rand(g, sum(n), h, 64, dtype=torch.bfloat16) for h in (4, 2)]
+    freq, _ = M.rotary_frequencies(64, device=DEV)
+    keys, values, table = cache_of(g, [90, 40], 16, 2, 64, torch.bfloat16)
+    new = [x.detach()[:2] for x in (q, k, k)]
+
+    def turned(pack, freq, batch):
+        out = M.apply_rotary(q, k, pack.positions, freq)
+        return [*(x.detach() for x in out), *torch.autograd.grad(out, (q, k), d),
+                *M.apply_rotary(q.detach(), k.detach(), pack.positions, freq),
+                M.append_rotary(*new, keys, values, batch, freq)]
+
+    want = turned(M.PackedSequences(n, DEV), freq, M.PagedBatch(table, [90, 40], [1, 1]))
+    big = torch.empty(1 << 26, device=DEV)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        pack, mine, batch = M.PackedSequences(n, DEV), freq.clone(), M.PagedBatch(table.clone(), [90, 40], [1, 1])
+        held = {pack.starts.data_ptr(), mine.data_ptr()}                # positions lie behind the starts
+        rows = sum(n) + len(n) + 1
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                big.zero_()                                            # the launches below wait for these
+            got = turned(pack, mine, batch)
+        del pack, mine, batch
+        fresh = [torch.full((m,), 7, dtype=t, device=DEV) for m, t in ((rows, torch.int32), (32, torch.float64)) for _ in range(4)]
+        waiting = not side.query()
+        assert not waiting or not held & {t.data_ptr() for t in fresh}
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
