@@ -9,6 +9,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .lib import S2GError, S2GPacked, S2GPaged, S2GRotary, call, get
@@ -57,11 +58,19 @@ def _fetchable(x: torch.Tensor, group: int = 1) -> bool:
             and (64 * t + group * h) * x.element_size() < 0x7ffffe00)
 
 
+def _no_tangent(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels write new tensors through their addresses: a forward-mode tangent would be lost without a word, also where
+    no gradient is asked for."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise S2GError(f"{what}: no forward-mode derivative (a tensor carries a tangent)")
+
+
 def _once(backward):
     """once_differentiable, whose bookkeeping (10 us a call) is needed only where a graph of the gradient is being made."""
     slow = once_differentiable(backward)
 
     def choose(ctx, *grads):
+        _no_tangent("gradient of a causal operator", *grads)
         return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return choose
 
@@ -244,6 +253,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     None, fp32 / bf16 / fp16 with any strides; positions int32 [tokens]; pairs are features (2i, 2i + 1) if interleaved,
     else (i, i + len(frequencies)).  Returns new tensors; differentiable in q and k."""
     _check("apply_rotary", q=q, k=k)
+    _no_tangent("apply_rotary", q, k, frequencies)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise S2GError("apply_rotary: q and k must be [tokens, heads, dim] with the same tokens and dim")
     if q.shape[1] == 0 or q.shape[2] == 0 or (k is not None and k.shape[1] == 0):
@@ -439,6 +449,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Pa
     same bits on every run."""
     if not isinstance(pack, PackedSequences):
         raise S2GError("packed_attention: pack must be PackedSequences")
+    _no_tangent("packed_attention", q, k, v)
     causal, scale = bool(causal), None if scale is None else float(scale)
     try:
         key = (_layout(q, k, v), causal, scale)
@@ -519,6 +530,7 @@ def _batch(what: str, batch: PagedBatch, q: torch.Tensor, keys: torch.Tensor) ->
 
 
 def _no_grad(what: str, *tensors: torch.Tensor) -> None:
+    _no_tangent(what, *tensors)
     if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise S2GError(f"{what} serves: it has no gradient (call it under torch.no_grad())")
 
@@ -562,6 +574,7 @@ def append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch
     dim], in place), the turned q returned.  A token whose position has no page is not written.  Rows of q behind the
     batch's come back as zeros.  No two sequences may own a page that both write to."""
     _no_grad("append_rotary", q, k, v, keys, values)
+    _no_tangent("append_rotary", frequencies)
     how = (bool(interleaved), float(multiplier))
     plan = _plan_of(batch, "append_rotary", how, _AppendPlan, q, k, v, keys, values, frequencies)
     if plan.copy:

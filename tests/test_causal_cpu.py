@@ -263,3 +263,35 @@ def test_rotary_holds_positions_and_frequencies(monkeypatch):
     assert positions.streams == frequencies.streams == ["the current one"] * 2
     torch.autograd.grad(out, (q, k), [torch.ones_like(x) for x in out])
     assert positions.streams == frequencies.streams == ["the current one"] * 3
+
+
+def test_tangents_are_refused(monkeypatch):
+    """The operators have no forward-mode derivative: a tensor that carries a tangent is turned down, whatever the gradient mode,
+    where it would come back without it; so is one that reaches a gradient."""
+    import transformer as M
+    from s2g import causal
+    from s2g.lib import S2GError
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(causal, "_launch", lambda *args: None)
+    monkeypatch.setattr(causal, "_check", lambda *args, **tensors: None)
+    monkeypatch.setattr(causal, "_stream", lambda device: None)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, stream: None)
+    x = torch.randn(4, 2, 32)
+    pool, positions = torch.zeros(2, 16, 2, 32), torch.arange(4, dtype=torch.int32)
+    freq, _ = M.rotary_frequencies(32, device="cpu")
+    batch, pack = object.__new__(M.PagedBatch), object.__new__(M.PackedSequences)
+    out = M.apply_rotary(x.clone().requires_grad_(), None, positions, freq)[0]
+    with forward_ad.dual_level():
+        dual, dual_pool = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(pool, torch.ones_like(pool))
+        turns = forward_ad.make_dual(freq, torch.ones_like(freq))
+        calls = [lambda: M.apply_rotary(x, None, positions, turns), lambda: M.append_rotary(x, x, x, pool, pool, batch, turns),
+                 lambda: M.apply_rotary(dual, None, positions, freq), lambda: M.apply_rotary(x, dual, positions, freq),
+                 lambda: M.packed_attention(dual, x, x, pack), lambda: M.packed_attention(x, x, dual, pack),
+                 lambda: M.append_rotary(dual, x, x, pool, pool, batch, freq), lambda: M.append_rotary(x, x, x, pool, dual_pool, batch, freq),
+                 lambda: M.paged_attention(dual, pool, pool, batch), lambda: M.paged_attention(x, dual_pool, pool, batch),
+                 lambda: torch.autograd.grad(out, out.grad_fn.next_functions[0][0].variable, dual, retain_graph=True)]
+        for call in calls:
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(S2GError, match="tangent"):
+                    call()
+        M.apply_rotary(x, None, positions, freq)           # without one: as ever, inside a level too

@@ -785,3 +785,23 @@ def test_positions_and_frequencies_dropped_while_another_stream_reads_them():
         assert not waiting or not held & {t.data_ptr() for t in fresh}
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tangents_are_refused_on_gpu_tensors():
+    import transformer as M
+    from s2g.lib import S2GError
+    from torch.autograd import forward_ad
+    g = gen(36)
+    x, pack = rand(g, 20, 2, 32), M.PackedSequences([20], DEV)
+    keys, values, table = cache_of(g, [40], 16, 2, 32, torch.float32)
+    batch, (freq, _) = M.PagedBatch(table, [40], [20]), M.rotary_frequencies(32, device=DEV)
+    leaf = x.clone().requires_grad_()
+    out, want = M.packed_attention(leaf, x, x, pack), M.packed_attention(x, x, x, pack)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: M.apply_rotary(dual, None, pack.positions, freq), lambda: M.packed_attention(x, dual, x, pack),
+                     lambda: M.append_rotary(x, dual, x, keys, values, batch, freq), lambda: M.paged_attention(dual, keys, values, batch),
+                     lambda: torch.autograd.grad(out, leaf, dual)):
+            with pytest.raises(S2GError, match="tangent"):
+                call()
+        assert torch.equal(M.packed_attention(x, x, x, pack), want)
