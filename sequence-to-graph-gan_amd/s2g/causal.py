@@ -119,6 +119,12 @@ def _no_capture() -> None:
         raise S2GError("a batch layout cannot be made inside a graph capture: use it once before")
 
 
+# What batches, caches and modules keep is made outside inference mode, whichever mode its first call runs in: autograd saves no
+# inference tensor, and training steps may come later.
+_lasting = torch.inference_mode(False)
+
+
+@_lasting
 def _on_device(values, device) -> torch.Tensor:
     """An int32 device copy of host integers, complete on return (any stream may use it)."""
     _no_capture()
@@ -155,6 +161,7 @@ class _Fixed:
 
 
 # ---------------------------------------------------------------------------------------------------------------- rotary
+@_lasting
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
                        original_length: int = 4096, device="cuda") -> Tuple[torch.Tensor, float]:
     """(frequencies [rotary_dim / 2] in radians per position, float64; multiplier) for apply_rotary.
@@ -341,6 +348,7 @@ class PackedSequences(_Fixed):
     its sequence's keys.  Made once per batch, and kept for forward and backward; the work lists of a grouping of heads
     are laid out when it is first used.  A captured graph reads them on every replay: keep the batch as long as the graph."""
 
+    @_lasting
     def __init__(self, lengths: Sequence[int], device="cuda", key_lengths: Optional[Sequence[int]] = None):
         q = np.asarray(lengths, dtype=np.int64).reshape(-1)
         k = q if key_lengths is None else np.asarray(key_lengths, dtype=np.int64).reshape(-1)
@@ -476,6 +484,7 @@ class PagedBatch(_Fixed):
 
     __slots__ = ("device", "stream", "table", "lengths", "starts", "sequences", "rows", "max_new", "max_length", "_length", "_new", "_cuts", "_plans")
 
+    @_lasting
     def __init__(self, table, lengths: Sequence[int], new_lengths: Sequence[int], max_length: Optional[int] = None, device=None):
         n, c = np.asarray(new_lengths, dtype=np.int64).reshape(-1), np.asarray(lengths, dtype=np.int64).reshape(-1)
         if n.shape != c.shape or n.size == 0 or n.size > 65535 or n.min() < 0 or (c < n).any() or c.max() >= 1 << 30 or n.sum() >= 1 << 30:
@@ -680,6 +689,7 @@ class PagedKVCache:
     """Keys and values of many sequences in pages of one pool: `keys`, `values` [pages, page size, kv heads, dim].
     Sequences come and go on the host; `extend` reserves room for new tokens and says where they lie."""
 
+    @_lasting
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype=torch.float32, device="cuda"):
         if num_pages <= 0 or page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
             raise S2GError("PagedKVCache: needs pages, of a power of two of tokens, 16 to 65536")

@@ -295,3 +295,19 @@ def test_tangents_are_refused(monkeypatch):
                 with mode(), pytest.raises(S2GError, match="tangent"):
                     call()
         M.apply_rotary(x, None, positions, freq)           # without one: as ever, inside a level too
+
+
+def test_what_a_module_and_a_batch_keep_is_no_inference_tensor(monkeypatch):
+    """Made while torch.inference_mode() is on, they are used by training steps later: autograd could not save them."""
+    import transformer as M
+    from s2g import causal
+    monkeypatch.setattr(causal, "_no_capture", lambda *args: None)
+    net = M.GroupedQueryAttention(64, 4, 2)
+    with torch.inference_mode():
+        made = [causal._on_device([1, 2, 3], "cpu"), net._turns(torch.device("meta")), M.rotary_frequencies(8, device="cpu")[0],
+                *M.GroupedQueryAttention(64, 4, 2)._frequencies.values()]
+        cache = causal.PagedKVCache(2, 16, 2, 32, device="cpu")
+    assert not any(x.is_inference() for x in made + [cache.keys, cache.values])
+    positions, q = made[0], torch.randn(3, 2, 8, requires_grad=True)
+    (q * positions[:, None, None]).sum().backward()        # saved for it
+    assert q.grad is not None

@@ -805,3 +805,24 @@ def test_tangents_are_refused_on_gpu_tensors():
             with pytest.raises(S2GError, match="tangent"):
                 call()
         assert torch.equal(M.packed_attention(x, x, x, pack), want)
+
+
+def test_inference_mode_before_training():
+    """A module, a batch and a cache first used under inference_mode train and are written to afterwards."""
+    import transformer as M
+    torch.manual_seed(4)
+    net = M.GroupedQueryAttention(64, 4, 2, dtype=torch.bfloat16).to(DEV)
+    x = rand(gen(37), 30, 64)
+    with torch.inference_mode():
+        pack = M.PackedSequences([20, 10], DEV)
+        first = net(x, pack)
+        cache = net.new_cache(4, page_size=16)
+        batch = cache.extend([cache.add()], [20])
+        net.step(x[:20], cache, batch)
+    y = net(x, pack)
+    assert torch.equal(y, first)
+    y.square().mean().backward()
+    assert all(bool(torch.isfinite(p.grad).all()) for p in net.parameters())
+    batch.lengths.add_(0)
+    cache.keys[0].zero_()
+    assert not any(t.is_inference() for t in (pack.positions, pack.starts, batch.lengths, batch.starts, batch.table))

@@ -181,7 +181,8 @@ class GroupedQueryAttention(nn.Module):
         # float64 whatever the module's parameters are cast to, one copy on every device it has run on
         got = self._frequencies.get(device)
         if got is None:
-            got = self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
+            with torch.inference_mode(False):          # training steps save it, whatever mode the first call runs in
+                got = self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
         return got
 
     def _project(self, x):
