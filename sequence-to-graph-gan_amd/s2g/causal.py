@@ -114,9 +114,9 @@ def _scale(what: str, scale: Optional[float], D: int) -> float:
     return s
 
 
-def _no_capture() -> None:
+def _no_capture(what: str = "a batch layout") -> None:
     if torch.cuda.is_current_stream_capturing():
-        raise S2GError("a batch layout cannot be made inside a graph capture: use it once before")
+        raise S2GError(f"{what} cannot be made inside a graph capture: use it once before")
 
 
 # What batches, caches and modules keep is made outside inference mode, whichever mode its first call runs in: autograd saves no
@@ -129,6 +129,13 @@ def _on_device(values, device) -> torch.Tensor:
     """An int32 device copy of host integers, complete on return (any stream may use it)."""
     _no_capture()
     return torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32)).to(device)
+
+
+@_lasting
+def lasting_copy(what: str, x: torch.Tensor, device) -> torch.Tensor:
+    """x on `device`, for its owner to keep."""
+    _no_capture(what)
+    return x.to(device)
 
 
 def _stream(device: int) -> torch.cuda.Stream:
@@ -291,6 +298,8 @@ class _WorkLists:
         entry = np.empty((seq.size, 8), dtype=np.int32)
         for i, column in enumerate((self.q_start[seq], self.q_len[seq], self.k_start[seq], self.k_len[seq], tile, row_lo, row_hi, slot)):
             entry[:, i] = column
+        if self.stream is not None:
+            _no_capture()                                  # asked of the caller's stream: the batch's own is not being captured
         with torch.cuda.stream(self.stream):
             return _on_device(entry, self.device)
 

@@ -311,3 +311,36 @@ def test_what_a_module_and_a_batch_keep_is_no_inference_tensor(monkeypatch):
     positions, q = made[0], torch.randn(3, 2, 8, requires_grad=True)
     (q * positions[:, None, None]).sum().backward()        # saved for it
     assert q.grad is not None
+
+
+def test_layouts_are_refused_inside_a_capture(monkeypatch):
+    """Asked of the stream that the call is on, not of the one that the batch was made on, which is not being captured."""
+    import contextlib
+    import numpy as np
+    import transformer as M
+    from s2g import causal
+    from s2g.lib import S2GError
+    current, made = ["the captured stream"], []
+
+    @contextlib.contextmanager
+    def stream(to):
+        before, current[0] = current[0], to
+        try:
+            yield
+        finally:
+            current[0] = before
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == "the captured stream")
+    monkeypatch.setattr(torch, "from_numpy", lambda x: made.append(x) or torch.zeros(x.shape, dtype=torch.int32))
+    lists = causal._WorkLists(np.array([300]), np.array([300]), "cpu", "the batch's stream")
+    for make in (lambda: lists.query_tiles(2, True), lambda: lists.key_tiles(2, True, 1)):
+        with pytest.raises(S2GError, match="capture"):
+            make()
+    net = M.GroupedQueryAttention(64, 4, 2)
+    with pytest.raises(S2GError, match="capture"):
+        net._turns(torch.device("meta"))
+    assert not made and not lists.kept
+    current[0] = "another stream"
+    kept = lists.query_tiles(2, True), lists.key_tiles(2, True, 1), net._turns(torch.device("meta"))
+    current[0] = "the captured stream"
+    assert kept[0] is lists.query_tiles(2, True) and kept[1] is lists.key_tiles(2, True, 1) and kept[2] is net._turns(torch.device("meta"))

@@ -826,3 +826,29 @@ def test_inference_mode_before_training():
     batch.lengths.add_(0)
     cache.keys[0].zero_()
     assert not any(t.is_inference() for t in (pack.positions, pack.starts, batch.lengths, batch.starts, batch.table))
+
+
+def test_first_use_inside_a_capture_is_refused():
+    """A batch, or a module's copy of the frequencies, that would be made inside a capture raises; the capture goes on."""
+    import transformer as M
+    from s2g.lib import S2GError
+    g = gen(38)
+    q, pack = rand(g, 30, 2, 32), M.PackedSequences([30], DEV)
+    leaf = q.clone().requires_grad_()
+    warm = M.PackedSequences([30], DEV)
+    M.packed_attention(leaf, q, q, warm)                   # forward only
+    net, x = M.GroupedQueryAttention(64, 2).to(DEV), rand(g, 30, 64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: M.packed_attention(q, q, q, pack), lambda: M.PackedSequences([30], DEV), lambda: M.PagedBatch([[0]], [3], [1]),
+                     lambda: net._turns(x.device), lambda: torch.autograd.grad(M.packed_attention(leaf, q, q, warm), leaf, q)):
+            with pytest.raises(S2GError, match="capture"):
+                call()
+        held = M.packed_attention(q, q, q, warm)
+    want = M.packed_attention(q, q, q, pack)
+    for _ in range(2):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+    net(x, pack)

@@ -22,8 +22,8 @@ if _PKG not in sys.path:
 
 from s2g import ops  # noqa: E402
 from s2g.attention import AddLayerNormFn, LinearActFn, MulMaskFn, MultiheadAttentionFn, dropout_multiplier  # noqa: E402
-from s2g.causal import (PackedSequences, PagedBatch, PagedKVCache, append_rotary, apply_rotary, packed_attention,  # noqa: E402,F401
-                        paged_attention, rotary_frequencies)
+from s2g.causal import (PackedSequences, PagedBatch, PagedKVCache, append_rotary, apply_rotary, lasting_copy,  # noqa: E402,F401
+                        packed_attention, paged_attention, rotary_frequencies)
 from s2g.lib import S2GError  # noqa: E402
 
 
@@ -181,8 +181,8 @@ class GroupedQueryAttention(nn.Module):
         # float64 whatever the module's parameters are cast to, one copy on every device it has run on
         got = self._frequencies.get(device)
         if got is None:
-            with torch.inference_mode(False):          # training steps save it, whatever mode the first call runs in
-                got = self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
+            got = self._frequencies[device] = lasting_copy("GroupedQueryAttention: a copy of the frequencies",
+                                                           self._frequencies[torch.device("cpu")], device)
         return got
 
     def _project(self, x):
