@@ -89,7 +89,7 @@ def _layout(*tensors) -> tuple:
 
 
 def _dense(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(2) == 1 else x.contiguous()
+    return x if x.stride(2) == 1 else _copy(x)      # contiguous() keeps the strides of empty tensors
 
 
 def _attention_shapes(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:

@@ -344,3 +344,18 @@ def test_layouts_are_refused_inside_a_capture(monkeypatch):
     kept = lists.query_tiles(2, True), lists.key_tiles(2, True, 1), net._turns(torch.device("meta"))
     current[0] = "the captured stream"
     assert kept[0] is lists.query_tiles(2, True) and kept[1] is lists.key_tiles(2, True, 1) and kept[2] is net._turns(torch.device("meta"))
+
+
+@pytest.mark.parametrize("q", [torch.empty(0, 32, 4).transpose(1, 2), torch.ones(3, 2, 5)[:, :, ::5], torch.ones(3, 4, 4).transpose(1, 2)], ids=["empty", "narrow", "dense copy"])
+def test_turn_of_layouts_that_count_as_contiguous(q, monkeypatch):
+    """No tokens, or one feature: contiguous() hands such a tensor back with whatever last stride it has."""
+    from s2g import causal
+    launched = []
+    monkeypatch.setattr(causal, "_launch", lambda device, name, *args: launched.append(name))
+    monkeypatch.setattr(causal, "_hold", lambda *args: None)
+    if q.shape[0] == 3 and q.shape[2] == 1:
+        q = q.as_strided(q.shape, (10, 5, 5))
+    assert q.stride(2) != 1
+    positions = torch.zeros(q.shape[0], dtype=torch.int32)
+    out, none = causal._turn(q, None, positions, torch.zeros(q.shape[2] // 2, dtype=torch.float64), False, 1.0, False)
+    assert out.shape == q.shape and out.stride(2) == 1 and none is None and len(launched) == (q.shape[0] > 0)

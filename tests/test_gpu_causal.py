@@ -852,3 +852,17 @@ def test_first_use_inside_a_capture_is_refused():
         torch.cuda.synchronize()
         assert torch.equal(held, want)
     net(x, pack)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+def test_rotary_without_tokens_or_with_one_feature_in_any_layout(dtype):
+    import transformer as M
+    freq, _ = M.rotary_frequencies(32, device=DEV)
+    q = torch.empty(0, 32, 4, dtype=dtype, device=DEV).transpose(1, 2).requires_grad_()
+    out, _ = M.apply_rotary(q, None, torch.zeros(0, dtype=torch.int32, device=DEV), freq)
+    out.sum().backward()
+    assert out.shape == q.grad.shape == (0, 4, 32)
+    wide = rand(gen(39), 7, 3, 5, dtype=dtype)
+    one = wide.as_strided((7, 3, 1), (15, 5, 3))
+    out, _ = M.apply_rotary(one, None, torch.zeros(7, dtype=torch.int32, device=DEV), freq[:0])
+    assert torch.equal(out, wide[:, :, :1])
