@@ -387,6 +387,8 @@ class _PackedPlan:
         if q.shape[0] * q.shape[1] >= 1 << 30 or k.shape[0] >= 1 << 30:
             raise S2GError("packed_attention: 2^30 rows or more")
         (R, H, D), (M, Hk, _) = q.shape, k.shape
+        if H * D >= 1 << 22:                           # no layout of the output's gradient could be fetched
+            raise S2GError("packed_attention: tokens of q have 2^22 elements or more")
         self.copies = [not _fetchable(q, H // Hk), not _fetchable(k), not _fetchable(v)]
         self.strides = (q.stride(), k.stride(), v.stride())
         self.work, self.causal, self.group, self.kv_heads = pack._work, causal, H // Hk, Hk
@@ -664,6 +666,8 @@ class _PagedPlan:
             raise S2GError(f"{what}: 2^30 rows or more")
         by_rows, part_keys, parts = _cut(batch, Hk, H // Hk, D, q.element_size())
         self.copy, self.device, self.whole = not _fetchable(q), q.get_device(), R == batch.rows
+        if H * D >= 1 << 22 and self.copy:             # a copy's tokens would be as far apart
+            raise S2GError(f"{what}: tokens of q have 2^22 elements or more")
         dims = S2GPaged(TYPES[q.dtype], batch.sequences, H, Hk, D, int(causal), keys.shape[1], keys.shape[0], batch.table.shape[1],
                         batch.max_new, batch.max_length, part_keys, parts, int(by_rows), _scale(what, scale, D), R, *_strides(q),
                         page_ld, token_ld, head_ld)

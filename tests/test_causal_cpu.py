@@ -359,3 +359,28 @@ def test_turn_of_layouts_that_count_as_contiguous(q, monkeypatch):
     positions = torch.zeros(q.shape[0], dtype=torch.int32)
     out, none = causal._turn(q, None, positions, torch.zeros(q.shape[2] // 2, dtype=torch.float64), False, 1.0, False)
     assert out.shape == q.shape and out.stride(2) == 1 and none is None and len(launched) == (q.shape[0] > 0)
+
+
+def test_rows_that_no_copy_makes_fetchable_are_refused(monkeypatch):
+    """Tokens of 2^22 elements or more, whichever way they are laid out: refused, not copied over and over."""
+    import types
+    import transformer as M
+    from s2g import causal
+    from s2g.lib import S2GError
+    monkeypatch.setattr(causal, "_check", lambda *args, **tensors: None)
+    tiles = torch.zeros(1, 8, dtype=torch.int32)
+    pack = object.__new__(M.PackedSequences)
+    for name, value in dict(device=torch.device("cpu"), rows=1, key_rows=1, _plans={}, _work=types.SimpleNamespace(query_tiles=lambda *a: tiles)).items():
+        setattr(pack, name, value)
+    q, k = torch.zeros(1, 32768, 128, dtype=torch.float16), torch.zeros(1, 256, 128, dtype=torch.float16)
+    wide = torch.zeros(1, 32768, 128, dtype=torch.float16)
+    for args in ((q, k, k), (q.transpose(1, 2).contiguous().transpose(1, 2), k, k), (wide, wide, wide)):
+        with pytest.raises(S2GError, match="2\\^22"):
+            M.packed_attention(*args, pack)
+    batch = object.__new__(M.PagedBatch)
+    for name, value in dict(device=torch.device("cpu"), table=torch.zeros(1, 1, dtype=torch.int32), rows=1, max_length=1, max_new=1, sequences=1,
+                            _length=torch.ones(1).numpy(), _new=torch.ones(1).numpy(), _plans={}, _cuts={}).items():
+        setattr(batch, name, value)
+    pool = torch.zeros(1, 16, 256, 128, dtype=torch.float16)
+    with pytest.raises(S2GError, match="2\\^22"):
+        M.paged_attention(q, pool, pool, batch)

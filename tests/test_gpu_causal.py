@@ -866,3 +866,19 @@ def test_rotary_without_tokens_or_with_one_feature_in_any_layout(dtype):
     one = wide.as_strided((7, 3, 1), (15, 5, 3))
     out, _ = M.apply_rotary(one, None, torch.zeros(7, dtype=torch.int32, device=DEV), freq[:0])
     assert torch.equal(out, wide[:, :, :1])
+
+
+def test_tokens_too_wide_are_refused():
+    import transformer as M
+    from s2g.lib import S2GError
+    g, t = gen(40), torch.float16
+    q, k = rand(g, 1, 32768, 128, dtype=t), rand(g, 1, 256, 128, dtype=t)
+    pack = M.PackedSequences([1], DEV)
+    for args in ((q, k, k), (q.transpose(1, 2).contiguous().transpose(1, 2), k, k), (q, q, q), (q[:, :1].expand(1, 32768, 128), k, k)):
+        with pytest.raises(S2GError, match="2\\^22"):
+            M.packed_attention(*args, pack)
+    with pytest.raises(S2GError, match="2\\^22"):
+        M.paged_attention(q, k.expand(16, 256, 128)[None].contiguous(), k.expand(16, 256, 128)[None].contiguous(), M.PagedBatch([[0]], [1], [1]))
+    pool = k.expand(16, 256, 128)[None].contiguous()
+    got = M.paged_attention(q[:, :1].expand(1, 32768, 128), pool, pool, M.PagedBatch([[0]], [1], [1]))        # a broadcast one can be fetched
+    assert torch.equal(got, k.repeat_interleave(128, 1))                                                     # (one key: its value)
