@@ -77,8 +77,9 @@ __device__ __attribute__((noinline)) void slow_key(int which, const T* k, const 
 // So for rows that see at most this many keys the products of the backward pass take what rounding left, too: 1.05 to 1.25
 // times, over long sequences 1.3.  They are the first rows of a long sequence or all of short ones; it costs 3 % of a
 // training step on sequences up to 4096 and 9 us of 80 on 96 of up to 203 tokens (12 heads of 64).
-// fp16 slopes are not raised as the weights are: how large they get is up to dO and V, so nothing says how far they may be.
-// Those below 2^-14 lose bits, like dO, dQ, dK and dV of that size themselves: fp16 training scales its loss.
+// fp16 slopes are not raised as the weights are (by 2^11 in the forward pass, by 2^14 on the key side): how large they get is
+// up to dO and V, so nothing says how far they may be.  Those below 2^-14 lose bits, like dO, dQ, dK and dV of that size
+// themselves: fp16 training scales its loss.
 #define FEW_KEYS 128
 template <typename T>
 __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
@@ -459,6 +460,9 @@ struct KeySums {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
   typedef typename Vec<T>::v8 v8;
+  // fp16 weights below 2^-14 lose bits, and a long row's are that small: the products of dV take them 2^14 times as large, as in
+  // PairSums (of 90000 like keys, dV off by 2^-8.8 of itself without it; 8 sequences up to 4096, 16 / 4 heads of 64: 299 -> 307 us).
+  static constexpr float RAISE = std::is_same<T, _Float16>::value ? 16384.0f : 1.0f;
   v8 k[S::KS], v[S::KS];
   fx16 dv[S::DB], dk[S::DB];
   bool tainted;                // a tile with rows that do not see some key held an infinity or a NaN
@@ -497,6 +501,7 @@ struct KeySums {
           const int i = 4 * g + j;
           p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -L[j]));
           ds[i] = p[i] * (ds[i] - D[j]);
+          if constexpr (RAISE != 1.0f) p[i] *= RAISE;
         }
       }
       if (edge) {
@@ -665,7 +670,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   S::whole(sums.dk, lane);
   S::whole(sums.dv, lane);
   kw.store<T, S::DB>(dK, partial, 0, sums.dk, dm.scale, wave, lane, dm);
-  kw.store<T, S::DB>(dV, partial, 1, sums.dv, 1.0f, wave, lane, dm);
+  kw.store<T, S::DB>(dV, partial, 1, sums.dv, 1.0f / sums.RAISE, wave, lane, dm);
 }
 
 // Two waves to 32 keys: wave g of the first four makes S, P and dV, wave 4 + g dP, dS and dK.  P goes from one to the other

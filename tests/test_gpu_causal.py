@@ -882,3 +882,19 @@ def test_tokens_too_wide_are_refused():
     pool = k.expand(16, 256, 128)[None].contiguous()
     got = M.paged_attention(q[:, :1].expand(1, 32768, 128), pool, pool, M.PagedBatch([[0]], [1], [1]))        # a broadcast one can be fetched
     assert torch.equal(got, k.repeat_interleave(128, 1))                                                     # (one key: its value)
+
+
+@pytest.mark.parametrize("dim", [16, 40, 64, 128])
+@pytest.mark.parametrize("queries", [2048, 100], ids=["many", "few"])
+def test_packed_attention_small_weights_in_the_gradient(dim, queries):
+    """fp16 weights below 2^-14, here 1 / 90000 each, reach dV with all their bits.  dO is one, so dV = queries / 90000.
+    Off by half a step of the weight, all of them alike (2^-11), and half a step of the result (2^-11, and its floor); L is off by
+    at most 2^-19 (half a step at 16, as much for the logarithm), 2^x by 2^-21, sums of like weights of 11 bits are exact."""
+    import transformer as M
+    g, m, dt = gen(41), 90000, torch.float16
+    q, do = torch.zeros(queries, 1, dim, dtype=dt, device=DEV), torch.ones(queries, 1, dim, dtype=dt, device=DEV)
+    k, v = (rand(g, m, 1, dim, dtype=dt).requires_grad_() for _ in range(2))
+    out = M.packed_attention(q, k, v, M.PackedSequences([queries], DEV, [m]), causal=False)
+    (dv,) = torch.autograd.grad(out, v, do)
+    want = queries / m
+    assert float((dv.double() - want).abs().max()) <= want * (2.0 ** -10 + 2.0 ** -17) + 2.0 ** -25
