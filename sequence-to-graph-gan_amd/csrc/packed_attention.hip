@@ -561,6 +561,8 @@ struct KeyWork {
   }
   // Q and dO of a tile of rows from r0 on, side by side: the group's heads of a token, then the next token.  Where whole
   // tokens fill the tiles (`off`, made once by offsets()) a tile is fetched as the one before; other groups divide anew.
+  // Behind the last row come its Q again, zeros of dO and an infinite L, so that they weigh nothing: zeros of Q would make NaN of
+  // a key that is minus infinity, whose weight every row that there is takes for zero.
   template <typename LT, typename T>
   __device__ __forceinline__ void offsets(int* off, long ld, long hd, int wave, int lane, const PackedDims& dm) const {
 #pragma unroll
@@ -575,20 +577,21 @@ struct KeyWork {
     const int G = dm.by.G, tok0 = divide(r0, dm.by);
     const ix4 qr = buffer_of(Q + ((long)w.q_start + tok0) * dm.ldq + kvh * G * dm.hq, 0x7ffffe00);
     const ix4 gr = buffer_of(dO + ((long)w.q_start + tok0) * dm.ldo + kvh * G * dm.ho, 0x7ffffe00);
-    if (ROWS % G == 0) {
+    if (ROWS % G == 0 && r0 + ROWS <= rows) {
 #pragma unroll
       for (int i = 0; i < LT::NI; ++i) {
-        const bool ok = LT::row_of(i, wave, lane) < rows - r0;
-        load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? qoff[i] : OUT_OF_BUFFER);
-        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? goff[i] : OUT_OF_BUFFER);
+        load_to_lds(qr, to + (i * WAVES + wave) * 1024, qoff[i]);
+        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, goff[i]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < LT::NI; ++i) {
-        const int r = r0 + LT::row_of(i, wave, lane), tk = divide(r, dm.by), hd = r - tk * G, ch = LT::chunk_of(i, wave, lane) * 16;
-        const bool ok = r < rows && ch < dm.D * (int)sizeof(T);
+        const int at = r0 + LT::row_of(i, wave, lane), r = min(at, rows - 1), tk = divide(r, dm.by), hd = r - tk * G;
+        const int ch = LT::chunk_of(i, wave, lane) * 16;
+        const bool ok = ch < dm.D * (int)sizeof(T);
         load_to_lds(qr, to + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldq + hd * dm.hq) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
-        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024, ok ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
+        load_to_lds(gr, to + LT::BYTES + (i * WAVES + wave) * 1024,
+                    ok && at < rows ? (int)(((tk - tok0) * dm.ldo + hd * dm.ho) * (long)sizeof(T)) + ch : OUT_OF_BUFFER);
       }
     }
   }
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   float st_next = 0.0f;
   const auto stat = [&](int t) {                                      // threads 0 .. 2 KT: L, then D of the tile's rows
     const int r = t * S::KT + (threadIdx.x & (S::KT - 1));
-    st_next = 0.0f;
+    st_next = threadIdx.x < S::KT ? INFINITY : 0.0f;
     if (threadIdx.x < 2 * S::KT && r < kw.rows) st_next = (threadIdx.x < S::KT ? lse : delta)[kw.lrow + r];
   };
   const float c = dm.scale * LOG2E;
@@ -823,7 +826,7 @@ __global__ __launch_bounds__(512, 2) void s2g_k_packed_attn_bwd_kv2(
   float st_next = 0.0f;
   const auto stat = [&](int t) {                                      // threads 0 .. 2 ROWS: RAISE - L, then -LOWER D of the tile's rows
     const int r = t * ROWS + (threadIdx.x & (ROWS - 1));
-    st_next = 0.0f;
+    st_next = threadIdx.x < ROWS ? -INFINITY : 0.0f;
     if (threadIdx.x < 2 * ROWS && r < kw.rows) st_next = threadIdx.x < ROWS ? P::RAISE - lse[kw.lrow + r] : -P::LOWER * delta[kw.lrow + r];
   };
   const float c = dm.scale * LOG2E;

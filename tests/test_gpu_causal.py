@@ -898,3 +898,33 @@ def test_packed_attention_small_weights_in_the_gradient(dim, queries):
     (dv,) = torch.autograd.grad(out, v, do)
     want = queries / m
     assert float((dv.double() - want).abs().max()) <= want * (2.0 ** -10 + 2.0 ** -17) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (4, 2, 32), (3, 1, 64), (8, 2, 128)], ids=str)
+@pytest.mark.parametrize("more", [[], MANY], ids=["few", "many"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_attention_of_a_key_that_no_row_weighs(dtype, shape, more, causal):
+    """A key that is minus infinity in a feature in which all queries are positive: every score of it is minus infinity, every
+    weight zero.  The rest is attention without that key; its own gradients are zeros, whatever stands behind the last row."""
+    import transformer as M
+    H, Hk, D = shape
+    g, n, at = gen(42), [237, 40, 3] + more, 5
+    q, k, v, do = (rand(g, sum(n), h, D, dtype=dtype) for h in (H, Hk, Hk, H))
+    q[..., 1] = q[..., 1].abs() + 1
+    bad = k.clone()
+    bad[at, :, 1] = -math.inf
+    leaves = [x.clone().requires_grad_() for x in (q, bad, v)]
+    out = M.packed_attention(*leaves, M.PackedSequences(n, DEV), causal=causal)
+    dk, dv = torch.autograd.grad(out, leaves[1:], do)
+    assert (dk[at] == 0).all() and (dv[at] == 0).all()
+    # rows before it see the keys up to themselves, rows from it on all of theirs but it
+    rest = lambda x: torch.cat([x[:at], x[at + 1:237]])  # noqa: E731
+    if causal:
+        want = ref.packed(q[:237], *(torch.cat([x[:at], rest(x)]) for x in (k, v)), [at, 237 - at], [at, 236], True, 1 / math.sqrt(D), do[:237])
+        want[2:] = [[torch.cat([x[:at] + x[at:2 * at], x[2 * at:]]) for x in w] for w in want[2:]]
+    else:
+        want = ref.packed(q[:237], rest(k), rest(v), [237], [236], False, 1 / math.sqrt(D), do[:237])
+    ref.within(out[:237].detach(), want[0], "out")
+    ref.within(rest(dk), want[2], "dk")
+    ref.within(rest(dv), want[3], "dv")
