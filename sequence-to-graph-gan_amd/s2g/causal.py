@@ -464,8 +464,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Pa
     """softmax(scale q k^T) v within every sequence of `pack`, row i of n queries and m keys seeing keys j <= i + m - n
     (causal) or all of them.  q [tokens, heads, dim], k and v [keys, kv heads, dim], fp32 / bf16 / fp16, query head h
     reading kv head h // (heads / kv heads); dim a multiple of 8 up to 128; scale: 1 / sqrt(dim).  A row that sees no key
-    gives zeros; rows behind the last sequence give zeros and have no gradient.  Differentiable in q, k and v, with the
-    same bits on every run."""
+    gives zeros and has no gradient, and so does one whose scores are all minus infinity (a softmax of those would be NaN); rows
+    behind the last sequence give zeros and have no gradient.  Differentiable in q, k and v, with the same bits on every run.
+    Sums and softmax are taken in 32 bits; of 16-bit inputs the weights are rounded to their type before they meet v."""
     if not isinstance(pack, PackedSequences):
         raise S2GError("packed_attention: pack must be PackedSequences")
     _no_tangent("packed_attention", q, k, v)
@@ -680,7 +681,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, b
     """Attention of a batch's new tokens (q [tokens, heads, dim]) over what its sequences hold in the cache: query i of n
     new tokens of a sequence of m sees keys j <= m - n + i (causal) or all m.  One token or thousands per sequence, mixed
     at will; types, heads and scale as in packed_attention.  A page number outside the pool, or a position that the table does
-    not cover, is a key that is not there; a query without keys gives zeros, and so do rows of q behind the batch's."""
+    not cover, is a key that is not there; a query without keys gives zeros, and so do one whose scores are all minus infinity
+    and rows of q behind the batch's."""
     _no_grad("paged_attention", q, keys, values)
     causal, scale = bool(causal), None if scale is None else float(scale)
     plan = _plan_of(batch, "paged_attention", (causal, scale), _PagedPlan, q, keys, values)

@@ -928,3 +928,27 @@ def test_packed_attention_of_a_key_that_no_row_weighs(dtype, shape, more, causal
     ref.within(out[:237].detach(), want[0], "out")
     ref.within(rest(dk), want[2], "dk")
     ref.within(rest(dv), want[3], "dv")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 2, 32), (8, 2, 128)], ids=str)
+@pytest.mark.parametrize("more", [[], MANY], ids=["few", "many"])
+def test_rows_of_no_weight_give_zeros(dtype, shape, more):
+    """Scores that are all minus infinity: zeros, as of a row that sees no key, and no gradient of k and v."""
+    import transformer as M
+    H, Hk, D = shape
+    g, n = gen(43), [5, 150, 40] + more
+    q, k, v, do = (rand(g, sum(n), h, D, dtype=dtype) for h in (H, Hk, Hk, H))
+    q[..., 1] = q[..., 1].abs() + 1
+    k[5:155, :, 1] = -math.inf
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = M.packed_attention(*leaves, M.PackedSequences(n, DEV))
+    dk, dv = torch.autograd.grad(out, leaves[1:], do)
+    assert all(bool((x[5:155] == 0).all()) for x in (out, dk, dv))
+    assert all(bool(torch.isfinite(x).all()) and bool((x[155:] != 0).any()) for x in (out, dk, dv))
+    keys, values, table = cache_of(g, [150, 90], 16, Hk, D, dtype)
+    keys[table[0].long(), :, :, 1] = -math.inf
+    for new in ([1, 1], [100, 2]):
+        got = M.paged_attention(q.detach()[:sum(new)], keys, values, M.PagedBatch(table, [150, 90], new))
+        assert (got[:new[0]] == 0).all()
+        check_paged(q.detach()[new[0]:sum(new)], keys, values, table[1:], [90], new[1:], True, 1 / math.sqrt(D), got[new[0]:])
