@@ -3,6 +3,7 @@
 lengths the host knows; every product and reduction runs in libs2g kernels (include/s2g.h)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -26,6 +27,13 @@ def _launch(device: int, name: str, *args) -> None:
     else:
         with torch.cuda.device(device):
             call(name, *args, stream_ptr())
+
+
+def current_device(x: torch.Tensor):
+    """x's device as the current one, for kernels that go to the current device's stream."""
+    if not x.is_cuda or x.get_device() == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(x.get_device())
 
 
 def _check(what: str, **tensors: Optional[torch.Tensor]) -> None:

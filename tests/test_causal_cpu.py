@@ -384,3 +384,38 @@ def test_rows_that_no_copy_makes_fetchable_are_refused(monkeypatch):
     pool = torch.zeros(1, 16, 256, 128, dtype=torch.float16)
     with pytest.raises(S2GError, match="2\\^22"):
         M.paged_attention(q, pool, pool, batch)
+
+
+def test_module_runs_on_its_inputs_device(monkeypatch):
+    """The projections' kernels go to the current device's stream: the module makes that its input's while it runs."""
+    import contextlib
+    import types
+    import transformer as M
+    from s2g import causal
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(to):
+        before, current[0] = current[0], to
+        try:
+            yield
+        finally:
+            current[0] = before
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+
+    class Stop(Exception):
+        pass
+
+    def project(self, x):
+        seen.append(current[0])
+        raise Stop
+    monkeypatch.setattr(M.GroupedQueryAttention, "_project", project)
+    net = M.GroupedQueryAttention(64, 4, 2)
+    for index in (1, 0):
+        x = types.SimpleNamespace(is_cuda=True, get_device=lambda: index, device=torch.device("cuda", index))
+        for call in (lambda: net(x, None), lambda: net.step(x, None, None)):
+            with pytest.raises(Stop):
+                call()
+    assert seen == [1, 1, 0, 0] and current == [0]
+    assert type(causal.current_device(torch.zeros(1))) is contextlib.nullcontext

@@ -22,8 +22,8 @@ if _PKG not in sys.path:
 
 from s2g import ops  # noqa: E402
 from s2g.attention import AddLayerNormFn, LinearActFn, MulMaskFn, MultiheadAttentionFn, dropout_multiplier  # noqa: E402
-from s2g.causal import (PackedSequences, PagedBatch, PagedKVCache, append_rotary, apply_rotary, lasting_copy,  # noqa: E402,F401
-                        packed_attention, paged_attention, rotary_frequencies)
+from s2g.causal import (PackedSequences, PagedBatch, PagedKVCache, append_rotary, apply_rotary, current_device,  # noqa: E402,F401
+                        lasting_copy, packed_attention, paged_attention, rotary_frequencies)
 from s2g.lib import S2GError  # noqa: E402
 
 
@@ -194,9 +194,10 @@ class GroupedQueryAttention(nn.Module):
 
     def forward(self, x, pack):
         """x [tokens, embed_size], the sequences of `pack` one after another."""
-        q, k, v = self._project(x)
-        q, k = apply_rotary(q, k, pack.positions, self._turns(x.device), self.interleaved, self.multiplier)
-        return self._out(packed_attention(q, k, v, pack))
+        with current_device(x):
+            q, k, v = self._project(x)
+            q, k = apply_rotary(q, k, pack.positions, self._turns(x.device), self.interleaved, self.multiplier)
+            return self._out(packed_attention(q, k, v, pack))
 
     def new_cache(self, num_pages, page_size=64):
         return PagedKVCache(num_pages, page_size, self.num_kv_heads, self.head_dim, self.dtype, self.in_proj.weight.device)
@@ -204,6 +205,7 @@ class GroupedQueryAttention(nn.Module):
     @torch.no_grad()
     def step(self, x, cache, batch):
         """The new tokens x [tokens, embed_size] of `batch` (cache.extend) into the cache, and their attention over it."""
-        q, k, v = self._project(x)
-        q = append_rotary(q, k, v, cache.keys, cache.values, batch, self._turns(x.device), self.interleaved, self.multiplier)
-        return self._out(paged_attention(q, cache.keys, cache.values, batch))
+        with current_device(x):
+            q, k, v = self._project(x)
+            q = append_rotary(q, k, v, cache.keys, cache.values, batch, self._turns(x.device), self.interleaved, self.multiplier)
+            return self._out(paged_attention(q, cache.keys, cache.values, batch))
