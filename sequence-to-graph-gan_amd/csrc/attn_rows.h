@@ -166,7 +166,11 @@ struct Rows {
   // Scores st into sums.  edge: some row of the wave does not see all of the keys (`last`: the last one that this lane's
   // row sees, counted from the tile's first); absent: keys (bits) that are not there.  NEXT: the scores of the next tile,
   // kt, are made meanwhile, so that the matrix unit has work while this tile's 2^x are taken.
-  template <int KB, bool NEXT>
+  // The matrix unit takes 16-bit weights, and rounding them to those costs the result as much as its own rounding does: errors of
+  // 2.0e-3 for 1.6e-3 (bf16).  WHOLE: products of what rounding left as well, for kernels in which the unit is idle (single tokens
+  // over a paged cache: 64 sequences of 300 to 8200, 8 heads of 128, 215 -> 216 us; 2 of 131071 and 90001, 2 of 96, 36.8 -> 37.7;
+  // 64 of 8000, 8 of 16, 92 -> 94); where it is the bound (prompts, chunks, training) they would be a third product beside two.
+  template <int KB, bool NEXT, bool WHOLE = false>
   __device__ __forceinline__ void add(fx16* st, fx16* next, const char* kt, const char* vt, bool edge, int last,
                                       unsigned long long absent, int lane) {
     const int half = lane >> 5;
@@ -203,14 +207,21 @@ struct Rows {
       S::scaled(o, a, lane);
     }
     const float low = base();
-    v8 p[2 * KB];
+    constexpr bool LEFT = WHOLE && sizeof(T) == 2;
+    v8 p[2 * KB], left[LEFT ? 2 * KB : 1];
     const auto weigh = [&](int e) {                      // two weights; four pairs make an operand
       const int b = e >> 3, i = 2 * (e & 7);
       st[b][i] = __builtin_amdgcn_exp2f(fmaf(st[b][i], c, -low));
       st[b][i + 1] = __builtin_amdgcn_exp2f(fmaf(st[b][i + 1], c, -low));
       p[e >> 2][i & 7] = (T)st[b][i];
       p[e >> 2][(i & 7) + 1] = (T)st[b][i + 1];
-      l = add_two(l, p[e >> 2], st[b], i);
+      if constexpr (LEFT) {
+        left[e >> 2][i & 7] = (T)(st[b][i] - (float)p[e >> 2][i & 7]);
+        left[e >> 2][(i & 7) + 1] = (T)(st[b][i + 1] - (float)p[e >> 2][(i & 7) + 1]);
+        l += st[b][i] + st[b][i + 1];
+      } else {
+        l = add_two(l, p[e >> 2], st[b], i);
+      }
     };
     constexpr int PAIRS = 8 * KB, N = KB * S::KS;
     if constexpr (NEXT) {
@@ -224,13 +235,16 @@ struct Rows {
     }
     // O^T += V^T P^T, the weights straight from the registers they are in
     products<T, 2 * KB * S::DB, S::AHEAD>([&](int i) { return LT::across(vt, i % S::DB, i / S::DB, lane); },
-                                [&](int i, const v8& a) { o[i % S::DB] = S::sum(a, p[i / S::DB], o[i % S::DB]); }, [](int) {});
+                                [&](int i, const v8& a) {
+                                  o[i % S::DB] = S::sum(a, p[i / S::DB], o[i % S::DB]);
+                                  if constexpr (LEFT) o[i % S::DB] = S::sum(a, left[i / S::DB], o[i % S::DB]);
+                                }, [](int) {});
   }
-  template <int KB>
+  template <int KB, bool WHOLE = false>
   __device__ __forceinline__ void step(const char* kt, const char* vt, bool edge, int last, unsigned long long absent, int lane) {
     fx16 st[KB];
     scores<KB>(st, kt, lane, [](int) {});
-    add<KB, false>(st, nullptr, nullptr, vt, edge, last, absent, lane);
+    add<KB, false, WHOLE>(st, nullptr, nullptr, vt, edge, last, absent, lane);
   }
   // what weigh() takes from a score (times c) to make a weight
   __device__ __forceinline__ float base() const { return (m == -INFINITY ? 0.0f : m * c) - Weights<T>::RAISE; }

@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_
       if (more) fetch_pages<LT, 1>(mine + ((t + 1) & 1) * 2 * LT::BYTES, kb, vb, page, k0 + STEP, hi, off, 0, lane, dm);
     }
     if (more) next = page_of(table, k0 + 2 * STEP + at, hi, dm);
-    if constexpr (!KT::ONCE) r.template step<KT::KB>(kt, kt + LT::BYTES, edge, end, absent, lane);
+    if constexpr (!KT::ONCE) r.template step<KT::KB, true>(kt, kt + LT::BYTES, edge, end, absent, lane);
   }
   const Joined j = workspace(ws, dm);
   const auto slow = [&](float f, float* to) {

@@ -952,3 +952,26 @@ def test_rows_of_no_weight_give_zeros(dtype, shape, more):
         got = M.paged_attention(q.detach()[:sum(new)], keys, values, M.PagedBatch(table, [150, 90], new))
         assert (got[:new[0]] == 0).all()
         check_paged(q.detach()[new[0]:sum(new)], keys, values, table[1:], [90], new[1:], True, 1 / math.sqrt(D), got[new[0]:])
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (8, 2, 64), (16, 4, 128), (6, 2, 96)], ids=str)
+def test_paged_attention_of_single_tokens_keeps_its_weights(dtype, shape):
+    """Single tokens: rounding the weights adds nothing to what rounding the result costs.  Their second half leaves 2^-16 (bf16) of
+    a weight, 2^-7 of a half step; with weights of one half the error is sqrt(2) of the result's own."""
+    import transformer as M
+    H, Hk, D = shape
+    g, context = gen(44), [700, 33, 2900, 5100]
+    keys, values, table = cache_of(g, context, 32, Hk, D, dtype)
+    for new in ([1] * 4, [3, 1, 2, 4]):
+        q = rand(g, sum(new), H, D, dtype=dtype)
+        got = M.paged_attention(q, keys, values, M.PagedBatch(table, context, new))
+        r, off, own = 0, 0.0, 0.0
+        for i, (n, c) in enumerate(zip(new, context)):
+            k, v = rows_of(keys, table[i], c), rows_of(values, table[i], c)
+            for h in range(H):
+                ((value, _),) = ref.head(q[r:r + n, h], k[:, h // (H // Hk)], v[:, h // (H // Hk)], c - n, True, 1 / math.sqrt(D), dtype)
+                off += float((got[r:r + n, h].double() - value).square().sum())
+                own += float((value.to(dtype).double() - value).square().sum())
+            r += n
+        assert off <= 1.02 ** 2 * own, math.sqrt(off / own)
