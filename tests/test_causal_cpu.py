@@ -419,3 +419,20 @@ def test_module_runs_on_its_inputs_device(monkeypatch):
                 call()
     assert seen == [1, 1, 0, 0] and current == [0]
     assert type(causal.current_device(torch.zeros(1))) is contextlib.nullcontext
+
+
+def test_module_loaded_onto_another_device_makes_its_frequencies_anew(monkeypatch):
+    """A module saved whole and loaded with map_location has its copies of the frequencies moved with the rest."""
+    import io
+    import transformer as M
+    from s2g import causal
+    monkeypatch.setattr(causal, "_no_capture", lambda *args: None)
+    net = M.GroupedQueryAttention(64, 4, 2)
+    there = torch.device("meta")
+    net._frequencies[there] = net._frequencies[torch.device("cpu")].clone()          # what map_location="cpu" makes of a device's copy
+    assert net._turns(there).device == there
+    file = io.BytesIO()
+    torch.save(net, file)
+    file.seek(0)
+    again = torch.load(file, weights_only=False)
+    assert torch.equal(again._turns(torch.device("cpu")), net._turns(torch.device("cpu")))

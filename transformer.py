@@ -180,7 +180,7 @@ class GroupedQueryAttention(nn.Module):
     def _turns(self, device):
         # float64 whatever the module's parameters are cast to, one copy on every device it has run on
         got = self._frequencies.get(device)
-        if got is None:
+        if got is None or got.device != device:        # (a module loaded with map_location)
             got = self._frequencies[device] = lasting_copy("GroupedQueryAttention: a copy of the frequencies",
                                                            self._frequencies[torch.device("cpu")], device)
         return got
