@@ -975,3 +975,101 @@ def test_paged_attention_of_single_tokens_keeps_its_weights(dtype, shape):
                 own += float((value.to(dtype).double() - value).square().sum())
             r += n
         assert off <= 1.02 ** 2 * own, math.sqrt(off / own)
+
+
+def test_module_training_captured():
+    """A training pass of the module in a graph: positions and frequencies of another stream, replayed between eager passes; the
+    batch may go after the graph."""
+    import transformer as M
+    torch.manual_seed(5)
+    g = gen(45)
+    net = M.GroupedQueryAttention(64, 4, 2, rotary_dim=8, interleaved=True, dtype=torch.bfloat16).to(DEV)
+    pack = M.PackedSequences([70, 3, 200], DEV)
+    x, do = rand(g, 273, 64), rand(g, 273, 64)
+    params = list(net.parameters())
+
+    def both():
+        y = net(x, pack)
+        return [y.detach(), *torch.autograd.grad(y, params, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for turn in range(3):
+        x.copy_(rand(g, 273, 64))
+        do.copy_(rand(g, 273, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [y.clone() for y in held]
+        for a, b in zip(got, both()):
+            assert torch.equal(a, b), turn
+    del graph, held, pack
+    torch.cuda.synchronize()
+    assert torch.isfinite(net(x, M.PackedSequences([273], DEV))).all()
+
+
+def test_captured_decoding_over_pages_reserved_ahead():
+    """All the tokens to come reserved by one extension, a batch of one token a sequence over its table, lengths advanced in place."""
+    import transformer as M
+    torch.manual_seed(6)
+    g, steps, prompts = gen(46), 40, [20, 5]
+    net = M.GroupedQueryAttention(64, 4, 2, dtype=torch.bfloat16).to(DEV)
+    cache, plain = net.new_cache(16, page_size=16), net.new_cache(16, page_size=16)
+    ids, twins = [cache.add() for _ in prompts], [plain.add() for _ in prompts]
+    x = rand(g, sum(prompts), 64)
+    net.step(x, cache, cache.extend(ids, prompts))
+    net.step(x, plain, plain.extend(twins, prompts))
+    ahead = cache.extend(ids, [steps] * 2)
+    batch = M.PagedBatch(ahead.table, [p + 1 for p in prompts], [1, 1], max_length=max(prompts) + steps)
+    token = rand(g, 2, 64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        net.step(token, cache, batch)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = net.step(token, cache, batch)
+    # two roundings of attention, a mean of values, half a step each, through fc_out's weights
+    through, largest = float(net.fc_out.weight.detach().abs().sum(1).max()), 0.0
+    for i in range(steps):
+        token.copy_(rand(g, 2, 64))
+        with torch.no_grad():
+            largest = max(largest, *(float(net._project(z)[2].abs().max()) for z in (x, token)))
+        graph.replay()
+        want = net.step(token, plain, plain.extend(twins, [1, 1]))
+        assert float((y - want).abs().max()) <= 2 * 2.0 ** -8 * 1.01 * through * largest, i
+        batch.lengths.add_(1)
+
+
+def test_first_calls_of_two_threads():
+    """Two threads that use one batch for the first time, each on a stream of its own."""
+    import threading
+    import transformer as M
+    g, n = gen(47), [500, 30, 77]
+    q, k, v, do = (rand(g, sum(n), h, 64, dtype=torch.bfloat16) for h in (4, 2, 2, 4))
+
+    def both(pack):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = M.packed_attention(*leaves, pack)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+    want = both(M.PackedSequences(n, DEV))
+    for _ in range(5):
+        pack, got, streams = M.PackedSequences(n, DEV), {}, [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+
+        def run(i):
+            with torch.cuda.stream(streams[i]):
+                got[i] = both(pack)
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want))
