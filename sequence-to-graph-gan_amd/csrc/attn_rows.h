@@ -105,8 +105,11 @@ __device__ __forceinline__ void store_rows(U* p, const fx16* acc, float f, int D
 
 // Infinities and NaN.  A product takes 0 x NaN for NaN, so a tile that holds one, and a row (key) that does not see it, cannot
 // go through the matrix unit together.  Where a tile with hidden pairs holds one, a wave makes its 32 rows (keys) anew: pair
-// by pair, straight from memory, 16 features at a time, and only the pairs that see each other.  Functions of their own,
-// never inlined: their registers would be the main loops' (packed attention, query side of the gradient: 297 -> 330 us).
+// by pair, straight from memory, 16 features at a time, and only the pairs that see each other: all of their pairs, those of clean
+// tiles too.  That is slow (8 bf16 sequences up to 4096, 16 / 4 heads of 128: the gradient 0.8 -> 97 ms for one infinity in dO and
+// 242 for all of it, the forward pass 0.2 -> 52 for one value in a hundred tokens; 96 fp16 ones up to 203, 12 heads of 64: 0.06 -> 2.4
+// and 3.3).  Functions of their own, never inlined: their registers would be the main loops' (packed attention, query side of the
+// gradient: 297 -> 330 us).
 template <typename T, int N>
 __device__ __forceinline__ float slow_dot(const T* a, const T* b, int D, int half) {
   float s = 0.0f;

@@ -95,9 +95,10 @@ __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
 // -------------------------------------------------------------------------------------------------------------- forward
 // 128 rows to a workgroup of four waves, 64 keys to a tile; K and V twice in LDS (64 KB at 128 features), so that two
 // workgroups share a compute unit and one's 2^x stand beside the other's products.  Bound by the matrix units, and at long
-// prompts by power: 8191 + 1025 + 5000 bf16 tokens, 32 query and 8 kv heads of 128, 740 us, 1030 TFLOP/s, the units busy
-// 53 % of the time at 1.63 GHz (one 8192^3 product of the library: 1140 TFLOP/s).  64 fp32 sequences up to 512, 4 heads of
-// 16: 27 us (query side of the gradient 36), by the longest sequences' chain of products and 2^x rather than by either's rate.
+// prompts by power: 8191 + 1025 + 5000 bf16 tokens, 32 query and 8 kv heads of 128, 748 us, 1020 TFLOP/s, the units busy half
+// of the time at 1.8 GHz (one 8192^3 product of the library: 1140 TFLOP/s).  64 fp32 sequences up to 512, 4 heads of 16: 28 us
+// (query side of the gradient 38), the units busy 26 (28) % of the time and the waves waiting 40 %.  It is not the longest
+// sequences' chain of products: a quarter of it (s2g_k_packed_attn_fwd_few) takes as long.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ out,
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
 
 // ------------------------------------------------------------------------------------------------- backward, query side
 // D of every row, and dQ: lanes are rows, as in the forward pass.  Three products (S, dP, dQ) to the forward's two.  8 bf16
-// sequences up to 4096, 16 query and 4 kv heads of 128: 297 us, 1035 TFLOP/s.  Making dQ here and not with atomics from the
+// sequences up to 4096, 16 query and 4 kv heads of 128: 302 to 320 us, 1015 to 960 TFLOP/s.  Making dQ here and not with atomics from the
 // key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.  FEW: few tiles, as in
 // s2g_k_packed_attn_fwd_few (4444 fp16 tokens, 3 / 1 heads of 128: 96 -> 74 us).
 template <typename T, int DP, bool FEW>
@@ -448,9 +449,10 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
 // for the chip, the host cuts a tile's rows into ranges, each leaving a 32-bit partial result in a slot of its own that
 // s2g_k_packed_attn_sum adds in a fixed order: no atomics, the same bits every time.
 //
-// Four products (S, dP, dK, dV).  8 bf16 sequences up to 4096, 16 query and 4 kv heads of 128: 473 us, 867 TFLOP/s, and 15 us
-// for the sums of cut tiles.  96 fp16 sequences up to 203, 12 heads of 64: 37 us.  64 fp32 sequences up to 512, 4 heads of
-// 16: 40 us, as long with a third workgroup to a compute unit: by the longest chain of row tiles.
+// Four products (S, dP, dK, dV).  8 bf16 sequences up to 4096, 16 query and 4 kv heads of 128: 485 to 528 us, 845 to 777
+// TFLOP/s, and 15 us for the sums of cut tiles.  96 fp16 sequences up to 203, 12 heads of 64: 33 us and 7.  64 fp32 sequences up
+// to 512, 4 heads of 16: 37 to 40 us, the matrix units busy 35 % of the time and the waves waiting 37 %; as long with a third
+// workgroup to a compute unit.
 //
 // Two forms.  Up to 64 16-bit features, and in fp32, a wave takes 32 keys.  Beyond, the sums of dK and dV of 32 keys with
 // their K and V leave room for only one wave to a SIMD, which keeps the matrix unit idle while it makes P and dS; so there

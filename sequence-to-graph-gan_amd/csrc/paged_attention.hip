@@ -10,12 +10,12 @@
 // axis is cut into parts of part_keys keys so that few rows still fill the chip; parts leave (O, m, l) in 32 bits and
 // s2g_k_paged_join_few / _many add them in order.  A sequence with a single part is written at once.
 //
-// Measured (8 kv heads of 128 bf16, 32 query heads): one token of 64 sequences of 300 to 8200, 210 us and 4 to join, 5.2 TB/s
-// of keys and values (a copy: 4.8); chunks of 512, 301, 777 and 5 new tokens over up to 16001, 337 us and 14 to join, 780
-// TFLOP/s: the matrix units busy 42 % of the time at 2.25 GHz, by the chain of scores, weights and sums of the two waves of a
+// Measured (8 kv heads of 128 bf16, 32 query heads): one token of 64 sequences of 300 to 8200, 213 us and 4 to join, 5.2 TB/s
+// of keys and values (a copy: 4.8); chunks of 512, 301, 777 and 5 new tokens over up to 16001, 349 us with 16 to join (profiled
+// 365 and 16, the matrix units busy 35 % of the time at 2.1 GHz): by the chain of scores, weights and sums of the two waves of a
 // SIMD.  (The packed forward pass hides weights behind the next keys' scores; here the second list of pages which that takes
-// costs more: 388 us for 370.)  One token of 131071 and of 90001 (2 kv heads of 96 fp16): 36 us and 5, 4.7 TB/s.  One token of
-// 777 fp32: 7 us and 4, latency.
+// costs more: 388 us for 370.)  One token of 131071 and of 90001 (2 kv heads of 96 fp16): 37 us and 5, 4.6 TB/s.  One token of
+// 777 fp32: 8 us and 3, latency.
 //
 // Lengths and pages come from device memory (a captured decoding loop updates them there), so nothing read from it is
 // trusted: keys beyond what the table covers are not there, a page number outside the pool is a page that is not there.

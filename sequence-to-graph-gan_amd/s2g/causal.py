@@ -474,7 +474,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Pa
     reading kv head h // (heads / kv heads); dim a multiple of 8 up to 128; scale: 1 / sqrt(dim).  A row that sees no key
     gives zeros and has no gradient, and so does one whose scores are all minus infinity (a softmax of those would be NaN); rows
     behind the last sequence give zeros and have no gradient.  Differentiable in q, k and v, with the same bits on every run.
-    Sums and softmax are taken in 32 bits; of 16-bit inputs the weights are rounded to their type before they meet v."""
+    Sums and softmax are taken in 32 bits; of 16-bit inputs the weights are rounded to their type before they meet v.  A pass
+    that is trained keeps two floats a row of a head and, of 16-bit inputs, a tensor of the output's size beside the output.
+    Infinities and NaN stay with the rows that see them, but rows or keys near one that others do not see are made anew pair by
+    pair, a hundred times as slow (a training step whose gradient has overflowed)."""
     if not isinstance(pack, PackedSequences):
         raise S2GError("packed_attention: pack must be PackedSequences")
     _no_tangent("packed_attention", q, k, v)
@@ -625,7 +628,8 @@ def _cut(batch: PagedBatch, Hk: int, G: int, D: int, size: int) -> Tuple[bool, i
     part; or they come in turn, which takes the whole work and, at the end, about 0.6 of a part.  Beginning and ending cost
     a workgroup about 256 keys' time, a part's sums of 128 rows another 4 to write and to join.  (64 sequences of 300 to 8200
     tokens, 8 kv heads of 128 bf16: parts of 512 / 1024 / 2048 / 8192 keys 253 / 232 / 212 / 236 us.)  From the lengths as
-    they were when the batch was made, and kept with it."""
+    they were when the batch was made, and kept with it.  Of 128 rows it counts one workgroup to a compute unit, as in fp32; of the
+    16-bit ones two fit.  (The parts were swept for single tokens only.)"""
     got = batch._cuts.get((Hk, G, D, size))
     if got is None:
         rows = np.maximum(batch._new, 0) * G
@@ -752,7 +756,9 @@ class PagedKVCache:
 
     def extend(self, sequences: Sequence[int], new_lengths: Sequence[int]) -> PagedBatch:
         """Room for new_lengths[i] more tokens of sequences[i]; the batch of them for append_rotary and paged_attention.
-        Refuses, changing nothing, if the pool has too few pages."""
+        Refuses, changing nothing, if the pool has too few pages.  The batch's layout is copied to the device before it returns,
+        behind what is queued on the stream; a loop that is not to wait reserves all its tokens in one call and makes one
+        PagedBatch over that batch's table, whose lengths it advances on the device."""
         if len(sequences) != len(new_lengths) or len(set(sequences)) != len(sequences) or not sequences or min(new_lengths) < 0:
             raise S2GError("PagedKVCache.extend: needs different sequences, each with its number of new tokens")
         lengths = [self._length[self._known(s)] + int(n) for s, n in zip(sequences, new_lengths)]
