@@ -679,8 +679,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 }
 
 // Two waves to 32 keys: wave g of the first four makes S, P and dV, wave 4 + g dP, dS and dK.  P goes from one to the other
-// through LDS, raised by 2^14.  For bf16 it goes as fp16: half a step is 2^-11 of it, an eighth of what rounding dS to bf16
-// adds; for fp16 that would be as much as rounding dS adds, so there it goes in 32 bits, and a tile is half as many rows.
+// through LDS.  For bf16 it goes as the upper 24 bits of a float: its range, as a key that no row weighs much has weights of any
+// size and dK made of them (as fp16 they would end at 2^-38), and 2^-15 of a weight, a hundredth of what rounding dS to bf16
+// takes (two instructions a weight: 497 -> 510 us).  fp16 has dS in more bits, so there it goes whole, and a tile is half as many
+// rows; the weights are raised by 2^14, as dV's products take them.
 // The first four are a tile ahead, so that neither waits for the other within one.
 template <typename T, int DP>
 struct PairSums {
@@ -689,9 +691,10 @@ struct PairSums {
   static constexpr int BLOCKS = WIDE ? 1 : 2, ROWS = 32 * BLOCKS;
   typedef Tile<T, S::PITCH, ROWS, 8> LT;
   typedef typename Vec<T>::v8 v8;
-  static constexpr int UNITS = WIDE ? 4 : 2, SHARE = BLOCKS * UNITS * 64;      // 16-byte units of P of 32 rows per lane; of a tile
+  static constexpr int UNITS = WIDE ? 4 : 3, SHARE = BLOCKS * UNITS * 64;      // 16-byte units of P of 32 rows per lane; of a tile
   static constexpr int BYTES = 6 * LT::BYTES + 8 * SHARE * 16 + 3 * 2 * ROWS * (int)sizeof(float);
-  static constexpr float RAISE = 14.0f, LOWER = 1.0f / 16384.0f;
+  static_assert(BYTES <= 163840, "LDS");
+  static constexpr float RAISE = WIDE ? 14.0f : 0.0f, LOWER = WIDE ? 1.0f / 16384.0f : 1.0f;
   v8 k[S::KS];                                     // K of the first four, V of the others
   fx16 sum[S::DB];
   bool tainted;                                    // a tile with rows that do not see some key held an infinity or a NaN
@@ -732,16 +735,33 @@ struct PairSums {
 #pragma unroll
       for (int u = 0; u < 4; ++u) share[u * 64 + lane] = (fx4){p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]};
     } else {
+      unsigned w[12];                              // four floats' upper three bytes in three words
 #pragma unroll
-      for (int u = 0; u < 2; ++u) share[u * 64 + lane] = __builtin_bit_cast(fx4, operand<_Float16>(p, u));
+      for (int g = 0; g < 4; ++g) {
+        const unsigned x0 = bits(p[4 * g]), x1 = bits(p[4 * g + 1]), x2 = bits(p[4 * g + 2]), x3 = bits(p[4 * g + 3]);
+        w[3 * g] = __builtin_amdgcn_perm(x1, x0, 0x05030201u);
+        w[3 * g + 1] = __builtin_amdgcn_perm(x2, x1, 0x06050302u);
+        w[3 * g + 2] = __builtin_amdgcn_perm(x3, x2, 0x07060503u);
+      }
+#pragma unroll
+      for (int u = 0; u < 3; ++u)
+        share[u * 64 + lane] = (fx4){flt(w[4 * u]), flt(w[4 * u + 1]), flt(w[4 * u + 2]), flt(w[4 * u + 3])};
     }
   }
+  static __device__ __forceinline__ unsigned bits(float x) { return __builtin_bit_cast(unsigned, x); }
+  static __device__ __forceinline__ float flt(unsigned x) { return __builtin_bit_cast(float, x); }
   // P of register i out of what was given
   static __device__ __forceinline__ float given(const fx4* x, int i) {
     if constexpr (WIDE) return x[i >> 2][i & 3];
     else {
-      const hx8 h = __builtin_bit_cast(hx8, x[i >> 3]);
-      return (float)h[i & 7];
+      const auto w = [&](int k) { const float y = x[k >> 2][k & 3]; return bits(y); };
+      const int k = 3 * (i >> 2);
+      switch (i & 3) {
+        case 0: return flt(w(k) << 8);
+        case 1: return flt(__builtin_amdgcn_perm(w(k + 1), w(k), 0x0504030cu));
+        case 2: return flt(__builtin_amdgcn_perm(w(k + 2), w(k + 1), 0x0403020cu));
+        default: return flt(w(k + 2) & 0xffffff00u);
+      }
     }
   }
   // a tile of rows: P to `share` ([block][unit][lane] of 16 bytes), dV^T += dO^T P
@@ -785,7 +805,7 @@ struct PairSums {
       const auto slope = [&](int g) {
         const fx4 d = *reinterpret_cast<const fx4*>(D + 32 * b + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = fmaf(given(x, i), fmaf(ds[i], LOWER, d[i & 3]), 0.0f);     // v_fma_mix
+        for (int i = 4 * g; i < 4 * g + 4; ++i) ds[i] = given(x, i) * (WIDE ? fmaf(ds[i], LOWER, d[i & 3]) : ds[i] + d[i & 3]);
       };
       if (b + 1 < BLOCKS) rows_by_keys(gt, 1, next, lane, spread(slope));
       else

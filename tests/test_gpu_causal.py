@@ -1073,3 +1073,18 @@ def test_first_calls_of_two_threads():
             t.join()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for i in range(2) for a, b in zip(got[i], want))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(3, 3, 128), (4, 2, 96), (9, 3, 72), (4, 2, 64)], ids=str)
+def test_packed_attention_gradient_of_keys_of_little_weight(dtype, shape):
+    """Scores far apart, weights down to 2^-60 and below: a key that no row weighs much has a small gradient, not a wrong one."""
+    import transformer as M
+    H, Hk, D = shape
+    g, n = gen(48), [126, 216, 5, 40]
+    q, k, v, do = (rand(g, sum(n), h, D, dtype=dtype) for h in (H, Hk, Hk, H))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = M.packed_attention(*leaves, M.PackedSequences(n, DEV), scale=1.0)
+    got = (out.detach(), *torch.autograd.grad(out, leaves, do))
+    for x, w, what in zip(got, ref.packed(*(x.detach() for x in leaves), n, n, True, 1.0, do), ("out", "dq", "dk", "dv")):
+        ref.within(x, w, what)
