@@ -140,7 +140,11 @@ template <typename T> struct Weights { static constexpr float RAISE = 0.0f, SLAC
 template <> struct Weights<_Float16> { static constexpr float RAISE = 11.0f, SLACK = 4.0f; };
 
 // The running softmax of 32 rows of one wave: lane l holds row l % 32 (both halves of the wave; each its own keys).
-template <typename T, int DP>
+// TRAIN: bf16 rows whose sums go into the backward pass.  O is divided by the sum of the rounded weights, whose errors cancel
+// those of a row's few large ones; the weights of the backward pass are not rounded, and by that sum they would be off by half a
+// step all alike: the sum of the weights as they were is kept beside it (8 sequences up to 4096, 16 / 4 heads of 128: 229 -> 239 us;
+// of 64: 128 -> 135).
+template <typename T, int DP, bool TRAIN = false>
 struct Rows {
   typedef Shape<T, DP> S;
   typedef typename S::LT LT;
@@ -148,6 +152,7 @@ struct Rows {
   v8 q[S::KS];
   fx16 o[S::DB];
   float m, l, c, slack;
+  float whole;               // TRAIN: the sum of the weights before they are rounded
   bool tainted;              // a tile with hidden keys held an infinity or a NaN in V: o is not to be used (slow_out, slow_pages)
 
   __device__ __forceinline__ void begin(const T* qp, int D, bool live, int half, float scale) {
@@ -155,7 +160,7 @@ struct Rows {
     for (int s = 0; s < S::KS; ++s) q[s] = row8(qp, 16 * s + 8 * half, D, live);
 #pragma unroll
     for (int d = 0; d < S::DB; ++d) o[d] = zero16();
-    m = -INFINITY, l = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c, tainted = false;
+    m = -INFINITY, l = 0.0f, whole = 0.0f, c = scale * LOG2E, slack = Weights<T>::SLACK / c, tainted = false;
   }
   // S^T = K Q^T of KB blocks of 32 keys: a lane holds one row's scores, so a row's maximum and sum are taken over a lane's
   // own registers and one exchange between the halves
@@ -207,6 +212,7 @@ struct Rows {
       const float mn = fmaxf(m, mx), a = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       l *= a;
+      if constexpr (TRAIN) whole *= a;
       S::scaled(o, a, lane);
     }
     const float low = base();
@@ -224,6 +230,7 @@ struct Rows {
         l += st[b][i] + st[b][i + 1];
       } else {
         l = add_two(l, p[e >> 2], st[b], i);
+        if constexpr (TRAIN) whole += st[b][i] + st[b][i + 1];
       }
     };
     constexpr int PAIRS = 8 * KB, N = KB * S::KS;
@@ -275,7 +282,7 @@ struct WaveTiles {
   typedef Tile<T, S::PITCH, KEYS, 1> LT;
   static constexpr bool ONCE = 4 * NW * LT::BYTES > 131072;
   static constexpr int PAD = 32 * S::DB + 4;                   // floats of a row of sums
-  static constexpr int TILES = (ONCE ? 2 : 4) * NW * LT::BYTES, JOIN = NW * (64 + 32 * PAD) * (int)sizeof(float);
+  static constexpr int TILES = (ONCE ? 2 : 4) * NW * LT::BYTES, JOIN = NW * (96 + 32 * PAD) * (int)sizeof(float);
   static constexpr int BYTES = TILES > JOIN ? TILES : JOIN;
 };
 template <typename T>
@@ -301,34 +308,38 @@ __device__ __forceinline__ void add_waves(const float* os, int rows, int D, Stor
   }
 }
 // The running softmaxes of 32 rows, each wave's over its own keys, joined: maxima and sums through LDS, then O scaled to the
-// common maximum (and by its sum if `divided`).  slow(f, to): a wave's O times f made anew; statistics(m, sum): of this lane's row.
-template <typename W, typename T, int DP, typename Slow, typename Statistics, typename Store>
-__device__ __forceinline__ void join_waves(char* lds, Rows<T, DP>& r, int rows, bool divided, int D, int wave, int lane, Slow slow,
+// common maximum (and by its sum if `divided`).  slow(f, to): a wave's O times f made anew; statistics(m, sum): of this lane's row
+// (TRAIN: of its weights before they are rounded).
+template <typename W, typename T, int DP, bool TRAIN, typename Slow, typename Statistics, typename Store>
+__device__ __forceinline__ void join_waves(char* lds, Rows<T, DP, TRAIN>& r, int rows, bool divided, int D, int wave, int lane, Slow slow,
                                            Statistics statistics, Store store) {
+  constexpr int N = TRAIN ? 3 : 2;
   const int half = lane >> 5;
-  float* ml = reinterpret_cast<float*>(lds);                   // [wave][row] (m, l)
-  const float l = both_sum(r.l);
+  float* ml = reinterpret_cast<float*>(lds);                   // [wave][row] (m, l, TRAIN: whole)
+  const float l = both_sum(r.l), all = TRAIN ? both_sum(r.whole) : 0.0f;
   Shape<T, DP>::whole(r.o, lane);
   __syncthreads();
   if (half == 0) {
-    ml[(wave * 32 + lane) * 2] = r.m;
-    ml[(wave * 32 + lane) * 2 + 1] = l;
+    ml[(wave * 32 + lane) * N] = r.m;
+    ml[(wave * 32 + lane) * N + 1] = l;
+    if (TRAIN) ml[(wave * 32 + lane) * N + 2] = all;
   }
   __syncthreads();
-  float m = -INFINITY, sum = 0.0f;
+  float m = -INFINITY, sum = 0.0f, whole = 0.0f;
 #pragma unroll
-  for (int w = 0; w < W::NW; ++w) m = fmaxf(m, ml[(w * 32 + (lane & 31)) * 2]);
+  for (int w = 0; w < W::NW; ++w) m = fmaxf(m, ml[(w * 32 + (lane & 31)) * N]);
 #pragma unroll
   for (int w = 0; w < W::NW; ++w) {
-    const float mw = ml[(w * 32 + (lane & 31)) * 2];
-    sum += ml[(w * 32 + (lane & 31)) * 2 + 1] * (mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * r.c));
+    const float mw = ml[(w * 32 + (lane & 31)) * N], f = mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * r.c);
+    sum += ml[(w * 32 + (lane & 31)) * N + 1] * f;
+    if (TRAIN) whole += ml[(w * 32 + (lane & 31)) * N + 2] * f;
   }
   const float f = r.m == m ? 1.0f : __builtin_amdgcn_exp2f((r.m - m) * r.c), scaled = divided ? (sum == 0.0f ? 0.0f : f / sum) : f;
-  float* os = ml + W::NW * 64;
+  float* os = ml + W::NW * 32 * N;
   float* mine = os + (wave * 32 + (lane & 31)) * W::PAD;
   if (r.tainted) slow(scaled, mine);
   else store_rows<T, Shape<T, DP>::DB>(mine, r.o, scaled, 32 * Shape<T, DP>::DB, half, true);
-  if (wave == 0 && half == 0) statistics(m, sum);
+  if (wave == 0 && half == 0) statistics(m, TRAIN ? whole : sum);
   __syncthreads();
   add_waves<W>(os, rows, D, store);
 }

@@ -99,7 +99,7 @@ __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
 // of the time at 1.8 GHz (one 8192^3 product of the library: 1140 TFLOP/s).  64 fp32 sequences up to 512, 4 heads of 16: 28 us
 // (query side of the gradient 38), the units busy 26 (28) % of the time and the waves waiting 40 %.  It is not the longest
 // sequences' chain of products: a quarter of it (s2g_k_packed_attn_fwd_few) takes as long.
-template <typename T, int DP>
+template <typename T, int DP, bool TRAIN>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn_fwd(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ out,
                                                              T* __restrict__ rest, float* __restrict__ lse, const PackedTile* __restrict__ tiles,
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
   const T* kp = K + (long)w.k_start * dm.ldk + kvh * dm.hk;
   const T* vp = V + (long)w.k_start * dm.ldv + kvh * dm.hv;
 
-  Rows<T, DP> r;
+  Rows<T, DP, TRAIN> r;
   r.begin(qp, dm.D, live, half, dm.scale);
   // the last key this row sees; of this wave's rows, and of the workgroup's
   const int shift = dm.causal ? w.k_len - w.q_len : 0x40000000;
@@ -169,11 +169,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
     if (t + 1 < nt) turn(t + 1, std::integral_constant<int, 1>{});
   }
   S::whole(r.o, lane);
-  const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l;
+  const float l = both_sum(r.l), f = l == 0.0f ? 0.0f : 1.0f / l, sum = TRAIN ? both_sum(r.whole) : l;
   const long orow = (qrow * dm.H + head) * dm.D;
   // a row that sees no key gives zeros, and L = +inf makes its P zero in the backward pass
   if (lse && live && half == 0)
-    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(l);
+    lse[((long)kvh * dm.q_rows + w.q_start) * dm.by.G + row] = l == 0.0f ? INFINITY : r.log_sum(sum);
   if (r.tainted) {
     slow_out<T, DP>(qp, kp, dm.ldk, vp, dm.ldv, 0, 32, 32, w_hi + 1, last, r.c, r.base(), f,
                     out + orow, sizeof(T) == 2 && rest ? rest + orow : nullptr, dm.D, live);
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void s2g_k_packed_attn
 // 128), every wave over 32-key tiles of its own, joined at the end as in the paged cache's single tokens.  4444 fp16 tokens,
 // 3 / 1 heads of 128: 85 -> 61 us; 1000 bf16 tokens, 8 heads of 128: 25 -> 15; 8 fp32 sequences up to 722, 2 heads of 96:
 // 90 -> 30.  (few_tiles() says when.)
-template <typename T, int DP>
+template <typename T, int DP, bool TRAIN>
 __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn_fwd_few(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ out, T* __restrict__ rest,
     float* __restrict__ lse, const PackedTile* __restrict__ tiles, PackedDims dm) {
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
     fetch_k(first, mine);
     fetch_v(first, mine + LT::BYTES);
   }
-  Rows<T, DP> r;
+  Rows<T, DP, TRAIN> r;
   r.begin(qp, dm.D, live, half, dm.scale);
   for (int t = 0, k0 = first; k0 < hi; ++t, k0 += STEP) {
     char* kt = mine + (WT::ONCE ? 0 : (t & 1) * 2 * LT::BYTES);
@@ -929,19 +929,26 @@ __global__ __launch_bounds__(256) void s2g_k_packed_attn_sum(const float* __rest
 template <typename T>
 static bool few_tiles(int nt, const PackedDims& dm) { return (long)nt * dm.Hk <= (sizeof(T) == 4 ? 384 : 128); }
 
-template <typename T, int DP>
-static int launch_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
-                      const PackedDims& dm, hipStream_t st) {
+template <typename T, int DP, bool TRAIN>
+static int launch_fwd_for(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
+                          const PackedDims& dm, hipStream_t st) {
   static S2GLdsCap cap, few_cap;
   const auto launch = [&](auto kernel, S2GLdsCap& c, dim3 grid, int threads, int bytes) {
     if (s2g_lds_cap(c, reinterpret_cast<const void*>(kernel), bytes) != 0) return -2;
     hipLaunchKernelGGL(kernel, grid, dim3(threads), bytes, st, (const T*)Q, (const T*)K, (const T*)V, (T*)out, (T*)rest, lse, tiles, dm);
     return 0;
   };
-  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
-                                      : launch(s2g_k_packed_attn_fwd<T, DP>, cap, dim3((unsigned)nt * dm.Hk), 256, 4 * Shape<T, DP>::LT::BYTES);
+  const int rc = few_tiles<T>(nt, dm) ? launch(s2g_k_packed_attn_fwd_few<T, DP, TRAIN>, few_cap, dim3((unsigned)nt * dm.Hk, 4), 64 * WaveTiles<T, DP>::NW, WaveTiles<T, DP>::BYTES)
+                                      : launch(s2g_k_packed_attn_fwd<T, DP, TRAIN>, cap, dim3((unsigned)nt * dm.Hk), 256, 4 * Shape<T, DP>::LT::BYTES);
   if (rc != 0) return rc;
   return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+template <typename T, int DP>
+static int launch_fwd(const void* Q, const void* K, const void* V, void* out, void* rest, float* lse, const PackedTile* tiles, int nt,
+                      const PackedDims& dm, hipStream_t st) {
+  if constexpr (std::is_same<T, __bf16>::value)          // fp32 and fp16 sum the weights as they were anyway
+    if (lse) return launch_fwd_for<T, DP, true>(Q, K, V, out, rest, lse, tiles, nt, dm, st);
+  return launch_fwd_for<T, DP, false>(Q, K, V, out, rest, lse, tiles, nt, dm, st);
 }
 template <typename T, int DP>
 static int launch_bwd(const void* Q, const void* K, const void* V, const void* out, const void* rest, const void* dO, const float* lse,

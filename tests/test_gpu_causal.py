@@ -1088,3 +1088,30 @@ def test_packed_attention_gradient_of_keys_of_little_weight(dtype, shape):
     got = (out.detach(), *torch.autograd.grad(out, leaves, do))
     for x, w, what in zip(got, ref.packed(*(x.detach() for x in leaves), n, n, True, 1.0, do), ("out", "dq", "dk", "dv")):
         ref.within(x, w, what)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("more", [[], MANY], ids=["few", "many"])
+def test_packed_attention_statistics_in_32_bits(dtype, dim, more):
+    """One row over each set of keys and dO of ones, so dV is the row's weights.  Scores are whole eighths and exact; the row's
+    statistics and 2^x are off by 2^-17 at |score| < 64 (half steps of score log2(e), of the maximum and of L), what the weights'
+    second half leaves of them by 2^-16, the result by half a step."""
+    import transformer as M
+    g, H = gen(49), 2
+    m = torch.randint(2, 128, (60,), generator=g, device=DEV).tolist()
+    n, keys = [1] * 60 + more, m + more
+    q = torch.randint(-2, 3, (sum(n), H, dim), generator=g, device=DEV) / 2
+    k = torch.randint(-2, 3, (sum(keys), H, dim), generator=g, device=DEV) / 4 * (2 if dim < 64 else 1)
+    q, k = q.to(dtype), k.to(dtype)
+    v = rand(g, sum(keys), H, dim, dtype=dtype).requires_grad_()
+    (dv,) = torch.autograd.grad(M.packed_attention(q, k, v, M.PackedSequences(n, DEV, keys), scale=1.0), v, torch.ones_like(q))
+    at = 0
+    for i, c in enumerate(m):
+        s = torch.einsum("hd,khd->kh", q[i].double().cpu(), k[at:at + c].double().cpu())
+        assert float(s.abs().max()) < 64
+        p = torch.softmax(s, 0)[..., None].to(DEV)
+        bound = p * (ref.U[dtype] * 1.01 + 2.0 ** -15) + ref.FLOOR[dtype]
+        over = ((dv[at:at + c].double() - p).abs() - bound).max()
+        assert float(over) <= 0, (i, float(over))
+        at += c
