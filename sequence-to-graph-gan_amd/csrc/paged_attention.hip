@@ -186,6 +186,15 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_paged_attn_
     if (more) next = page_of(table, k0 + 2 * STEP + at, hi, dm);
     if constexpr (!KT::ONCE) r.template step<KT::KB, true>(kt, kt + LT::BYTES, edge, end, absent, lane);
   }
+  // what rounding left of a weight may be zero, and makes NaN of an infinite value then: such rows are made anew
+  if constexpr (sizeof(T) == 2) {
+    bool none = false;
+#pragma unroll
+    for (int d = 0; d < Shape<T, DP>::DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) none = none || r.o[d][i] != r.o[d][i];
+    r.tainted = r.tainted || __any(none && r.l == r.l);
+  }
   const Joined j = workspace(ws, dm);
   const auto slow = [&](float f, float* to) {
     slow_pages<T, DP>(qp, kb, vb, table, lo + KT::KEYS * wave, KT::KEYS, STEP, hi, last, r.c, r.base(), f, to, true, dm.D, dm.page_shift, dm.pages, dm.page_ld, dm.ld);

@@ -1115,3 +1115,24 @@ def test_packed_attention_statistics_in_32_bits(dtype, dim, more):
         over = ((dv[at:at + c].double() - p).abs() - bound).max()
         assert float(over) <= 0, (i, float(over))
         at += c
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("shape", [(4, 4, 16), (8, 2, 64), (6, 2, 96), (16, 4, 128)], ids=str)
+@pytest.mark.parametrize("what", [math.inf, -math.inf])
+def test_paged_attention_of_an_infinite_value(dtype, shape, what):
+    """An infinity in V of a key that the rows see, and weigh: infinite in its feature, with its sign; the rest as ever."""
+    import transformer as M
+    H, Hk, D = shape
+    g, context = gen(50), [700, 90]
+    keys, values, table = cache_of(g, context, 16, Hk, D, dtype)
+    bad, at = values.clone(), 333
+    bad[table[0, at // 16].long(), at % 16, :, 3] = what
+    rest = torch.arange(D, device=DEV) != 3
+    for new in ([1, 1], [2, 5], [100, 1]):
+        q = rand(g, sum(new), H, D, dtype=dtype)
+        got = M.paged_attention(q, keys, bad, M.PagedBatch(table, context, new))
+        want = M.paged_attention(q, keys, values, M.PagedBatch(table, context, new))
+        assert (got[:new[0], :, 3] == what).all()
+        got[:new[0], :, 3] = want[:new[0], :, 3]
+        check_paged(q, keys, values, table, context, new, True, 1 / math.sqrt(D), got)
