@@ -78,8 +78,8 @@ __device__ __attribute__((noinline)) void slow_key(int which, const T* k, const 
 // times, over long sequences 1.3.  They are the first rows of a long sequence or all of short ones; it costs 3 % of a
 // training step on sequences up to 4096 and 9 us of 80 on 96 of up to 203 tokens (12 heads of 64).
 // fp16 slopes are not raised as the weights are (by 2^11 in the forward pass, by 2^14 on the key side): how large they get is
-// up to dO and V, so nothing says how far they may be.  Those below 2^-14 lose bits, like dO, dQ, dK and dV of that size
-// themselves: fp16 training scales its loss.
+// up to dO and V, so nothing says how far they may be.  Those below 2^-14 lose bits and those beyond 65504 are infinite, like dO,
+// dQ, dK and dV of that size themselves: fp16 training scales its loss.
 #define FEW_KEYS 128
 template <typename T>
 __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
@@ -95,7 +95,7 @@ __device__ __forceinline__ fx16 left_by_rounding(const fx16& x) {
 // -------------------------------------------------------------------------------------------------------------- forward
 // 128 rows to a workgroup of four waves, 64 keys to a tile; K and V twice in LDS (64 KB at 128 features), so that two
 // workgroups share a compute unit and one's 2^x stand beside the other's products.  Bound by the matrix units, and at long
-// prompts by power: 8191 + 1025 + 5000 bf16 tokens, 32 query and 8 kv heads of 128, 748 us, 1020 TFLOP/s, the units busy half
+// prompts by power: 8191 + 1025 + 5000 bf16 tokens, 32 query and 8 kv heads of 128, 748 to 765 us, 1020 to 1000 TFLOP/s, the units busy half
 // of the time at 1.8 GHz (one 8192^3 product of the library: 1140 TFLOP/s).  64 fp32 sequences up to 512, 4 heads of 16: 28 us
 // (query side of the gradient 38), the units busy 26 (28) % of the time and the waves waiting 40 %.  It is not the longest
 // sequences' chain of products: a quarter of it (s2g_k_packed_attn_fwd_few) takes as long.
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(64 * (WaveTiles<T, DP>::NW)) void s2g_k_packed_attn
 
 // ------------------------------------------------------------------------------------------------- backward, query side
 // D of every row, and dQ: lanes are rows, as in the forward pass.  Three products (S, dP, dQ) to the forward's two.  8 bf16
-// sequences up to 4096, 16 query and 4 kv heads of 128: 302 to 320 us, 1015 to 960 TFLOP/s.  Making dQ here and not with atomics from the
+// sequences up to 4096, 16 query and 4 kv heads of 128: 302 to 324 us, 1015 to 950 TFLOP/s.  Making dQ here and not with atomics from the
 // key side costs S and dP twice (two products of seven) and keeps every bit the same from run to run.  FEW: few tiles, as in
 // s2g_k_packed_attn_fwd_few (4444 fp16 tokens, 3 / 1 heads of 128: 96 -> 74 us).
 template <typename T, int DP, bool FEW>
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(FEW ? 64 * (WaveTiles<T, DP>::NW) : 256, FEW || siz
 // for the chip, the host cuts a tile's rows into ranges, each leaving a 32-bit partial result in a slot of its own that
 // s2g_k_packed_attn_sum adds in a fixed order: no atomics, the same bits every time.
 //
-// Four products (S, dP, dK, dV).  8 bf16 sequences up to 4096, 16 query and 4 kv heads of 128: 485 to 528 us, 845 to 777
+// Four products (S, dP, dK, dV).  8 bf16 sequences up to 4096, 16 query and 4 kv heads of 128: 510 to 547 us, 805 to 750
 // TFLOP/s, and 15 us for the sums of cut tiles.  96 fp16 sequences up to 203, 12 heads of 64: 33 us and 7.  64 fp32 sequences up
 // to 512, 4 heads of 16: 37 to 40 us, the matrix units busy 35 % of the time and the waves waiting 37 %; as long with a third
 // workgroup to a compute unit.
